@@ -316,7 +316,7 @@ def _plain_product(s):
     out = [(_rows8(s["x"]) @ w.t()).to(dtype)]
     if s["case"]["grad"]:
         out.append((_rows8(s["d_out"]) @ w).to(dtype))
-        out.append(_columns8(s["d_out"]).t() @ _columns8(s["x"]))
+        out.append((_columns8(s["d_out"]).t() @ _columns8(s["x"])).to(dtype))
     return out
 
 
@@ -345,7 +345,7 @@ def _plain_experts(s):
         dx = room(w.shape[2])
         dx[place[wanted]] = torch.matmul(_rows8(d), w)[wanted]
         out.append(dx.to(dtype))
-        out.append(torch.matmul(_columns8(d).transpose(1, 2).contiguous(), _columns8(x)))
+        out.append(torch.matmul(_columns8(d).transpose(1, 2).contiguous(), _columns8(x)).to(dtype))
     return out
 
 
@@ -382,7 +382,7 @@ def _own_product(s):
     out = [product(s["x"], Blocks(s["wq"], s["ws"]), dtype=dtype)]
     if s["case"]["grad"]:
         out.append(product(s["d_out"], Blocks(s["tq"], s["ts"]), dtype=dtype))
-        out.append(weight_grad(s["d_out"], s["x"]))
+        out.append(weight_grad(s["d_out"], s["x"], dtype=dtype))
     return out
 
 
@@ -394,7 +394,7 @@ def _own_experts(s):
     out = [product(s["x"], Blocks(s["wq"], s["ws"]), plan, gather=True, dtype=dtype)]
     if s["case"]["grad"]:
         out.append(product(s["d_out"], Blocks(s["tq"], s["ts"]), plan, dtype=dtype))
-        out.append(weight_grad(s["d_out"], s["x"], plan, gather=True))
+        out.append(weight_grad(s["d_out"], s["x"], plan, gather=True, dtype=dtype))
     return out
 
 
@@ -539,5 +539,5 @@ def work(case):
         matrices = min(c["experts"], max(1, out_rows))    # of those, the ones that have rows are read
     moved = rows * k * size + matrices * n * k + out_rows * n * size
     if grad:   # incoming gradient and weights again, both gradients written
-        moved += out_rows * n * size + matrices * n * k + out_rows * k * size + 4 * (1 if c["op"] == "product" else c["experts"]) * n * k
+        moved += out_rows * n * size + matrices * n * k + out_rows * k * size + size * (1 if c["op"] == "product" else c["experts"]) * n * k
     return {"bytes": moved, "flops": (6 if grad else 2) * out_rows * n * k}
