@@ -478,6 +478,128 @@ int mint_torn_line_probe(void* staging, size_t staging_bytes, int pairs, int ite
                          int cache_policy, int placement, int per_sector, uint32_t flag_epoch,
                          uint32_t spin_budget, void* counters, void* stream);
 
+/* ---- operators of an expert layer ---------------------------------------------
+ * What stands beside the collectives where experts are spread over ranks: the
+ * router, matrix products in 8-bit floating point with a scale for each block of
+ * 128 numbers, and the combination of the experts' rows, with their gradients.
+ * No counterpart in the reference.  Element strides count elements, strides of
+ * 8-bit matrices bytes; rows and columns of size zero are allowed everywhere and
+ * do nothing. */
+
+typedef enum { MINT_SCORE_SOFTMAX = 0, MINT_SCORE_SIGMOID = 1 } mint_score;
+
+/* Routing of `tokens` rows of logits to `topk` of `experts` experts each.
+ *   s      softmax or sigmoid of a row's logits x
+ *   key    x + bias (softmax), s + bias (sigmoid): what the choice goes by
+ *   kept   of `groups` groups of consecutive experts, the ones whose group_top
+ *          (1 or 2) largest keys have the largest sum; the choice is from these
+ *   chosen (tokens, topk) int32: the largest keys first, the lowest expert
+ *          first among equals
+ *   weights (tokens, topk) f32: scale * s, with `renormalise` divided by the sum
+ *          of the chosen ones' s (0 where that sum is 0)
+ * A logit of -inf masks its expert, and a bias of -inf too: where fewer experts
+ * are left than topk, chosen is -1 and the weight 0.  A NaN ranks above every
+ * number.  At most 1024 experts, 64 of them chosen, 64 groups. */
+typedef struct {
+    uint64_t logits;       /* (tokens, experts) of `dtype`, rows row_stride apart */
+    uint64_t bias;         /* f32 (experts), or 0 */
+    uint64_t weights;      /* f32 (tokens, topk) */
+    uint64_t chosen;       /* int32 (tokens, topk) */
+    int64_t row_stride;
+    uint64_t tokens;
+    uint32_t experts, topk, groups, kept, group_top;
+    int32_t dtype;         /* MINT_F16, MINT_BF16, MINT_F32 */
+    int32_t score;         /* mint_score */
+    int32_t renormalise;
+    float scale;
+    uint32_t reserved;     /* 0 */
+} mint_route_op;
+int mint_route(const mint_route_op* op, void* stream);
+/* The logits' gradient (every element written, rows d_stride apart) from the
+ * weights' (f32); op as for mint_route, whose logits and chosen it reads
+ * (bias, weights, groups, kept and group_top are not looked at: the choice has no
+ * gradient). */
+int mint_route_grad(const mint_route_op* op, uint64_t d_weights, uint64_t d_logits, int64_t d_stride,
+                    void* stream);
+
+/* The pairs (token, choice) in the order of the experts first .. first +
+ * experts - 1, pairs of an expert in their own order:
+ *   offsets int32 (experts + 1): where each expert's begin, and their end
+ *   order   int32 (tokens * topk): the token at each place, -1 behind the end
+ *   slots   int32 (tokens, topk): the place of each pair, -1 if its expert is
+ *           none of these
+ * workspace: mint_assign_workspace(tokens * topk, experts) bytes (may be 0). */
+size_t mint_assign_workspace(uint64_t pairs, uint32_t experts);
+int mint_assign(const void* chosen, uint64_t tokens, uint32_t topk, uint32_t first, uint32_t experts,
+                void* offsets, void* order, void* slots, void* workspace, size_t workspace_bytes,
+                void* stream);
+
+/* Rounding to 8 bits (e4m3) in blocks of 128: with m = max(2^-96, largest
+ * magnitude of the block), scale = m / 448 and q = x * (448 / m) rounded to the
+ * nearest.  q and its strides are multiples of 16 bytes, and its rows are whole
+ * blocks: zeros fill up the last.
+ *   rows8     blocks along a row; the scale of row r, block b is at
+ *             scale[r * s_row + b * s_block]
+ *   columns8  blocks along a column, q turned: (width, q_stride), scale
+ *             (blocks, width).  With `offsets` (int32, experts + 1) the rows of an
+ *             expert begin a new block; with `tokens` (int32, rows) row i is
+ *             x[tokens[i]].  mint_columns8_blocks(rows, experts) blocks at most
+ *   squares8  squares of 128 x 128 of `matrices` matrices; scale
+ *             (matrices, blocks of rows, blocks of depth) */
+int mint_rows8(const void* x, int64_t x_stride, uint64_t rows, uint64_t depth, int dtype, void* q,
+               int64_t q_stride, void* scale, int64_t s_row, int64_t s_block, void* stream);
+size_t mint_columns8_blocks(uint64_t rows, uint32_t experts);
+int mint_columns8(const void* x, int64_t x_stride, uint64_t x_rows, uint64_t width, int dtype,
+                  const void* tokens, uint64_t rows, const void* offsets, uint32_t experts, void* q,
+                  int64_t q_stride, void* scale, void* stream);
+int mint_squares8(const void* w, int64_t w_matrix, int64_t w_stride, uint32_t matrices, uint64_t rows,
+                  uint64_t depth, int dtype, void* q, int64_t q_matrix, int64_t q_stride, void* scale,
+                  void* stream);
+
+/* out = x w^T of two 8-bit matrices, sums in 32 bits.
+ *   MINT_PRODUCT_ROWS      x (x_rows, depth), scales by rows and blocks of the depth; w (cols,
+ *                          depth) with a scale for each square of 128 x 128.  With
+ *                          `offsets` there are `experts` matrices w_matrix bytes apart,
+ *                          rows offsets[e] .. offsets[e + 1] - 1 of out are made with
+ *                          matrix e, and rows behind the last are zeros; with `tokens`
+ *                          row i of out is made from row tokens[i] of x
+ *   MINT_PRODUCT_GRADIENT  both operands as mint_columns8 leaves them: x (rows,
+ *                          depth), w (cols, depth), each with scales by rows and
+ *                          blocks.  With `offsets` (experts' rows among group_rows, as for
+ *                          mint_columns8) there are `experts` results out_matrix
+ *                          elements apart, each the sum over its expert's blocks
+ * Both matrices start at multiples of 16 bytes, and so do their rows; nothing
+ * behind a row's depth is read. */
+typedef enum { MINT_PRODUCT_ROWS = 0, MINT_PRODUCT_GRADIENT = 1 } mint_product_kind;
+typedef struct {
+    int32_t kind;          /* mint_product_kind */
+    int32_t dtype;         /* of out: MINT_F16, MINT_BF16, MINT_F32 */
+    uint64_t x, w;         /* 8-bit matrices */
+    uint64_t sx, sw;       /* f32 scales */
+    uint64_t out;
+    uint64_t tokens;       /* int32 (rows), or 0 */
+    uint64_t offsets;      /* int32 (experts + 1), or 0 */
+    uint64_t rows, cols, depth, x_rows, group_rows;
+    int64_t x_stride, w_stride, w_matrix, out_stride, out_matrix;
+    int64_t sx_row, sx_block;            /* between the scales of consecutive rows, blocks */
+    int64_t sw_matrix, sw_row, sw_block; /* ... of matrices, rows (ROWS: of 128 rows), blocks */
+    uint32_t experts;
+    uint32_t reserved;     /* 0 */
+} mint_product_op;
+int mint_product8(const mint_product_op* op, void* stream);
+
+/* out[t] = sum over j of weights[t, j] * rows[slots[t, j]] (weights 0: all 1), in
+ * 32 bits; a slot outside the rows adds nothing.  The gradients: d_rows of every
+ * row (those that are no token's, from *rows_used (int32) on, are cleared), and
+ * d_weights unless it is 0. */
+int mint_combine(const void* rows, int64_t row_stride, uint64_t n_rows, const void* slots,
+                 const void* weights, uint64_t tokens, uint32_t topk, uint32_t width, void* out,
+                 int64_t out_stride, int dtype, void* stream);
+int mint_combine_grad(const void* d_out, int64_t d_stride, const void* rows, int64_t row_stride,
+                      uint64_t n_rows, const void* slots, const void* weights, const void* rows_used,
+                      uint64_t tokens, uint32_t topk, uint32_t width, void* d_rows, int64_t d_row_stride,
+                      void* d_weights, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,10 @@ CODEC_SRC = os.path.join(_CSRC, "codec.hip")
 FAMILY_SRC = os.path.join(_CSRC, "ring_family.hip")     # compiled once per element type
 HOST_SRC = os.path.join(_CSRC, "host.cpp")              # the extension module _host
 HOST_PATH = os.path.join(_PKG, "_host.so")
+# the expert layer's operators, and the extension module _expert_host that calls them
+EXPERT_SRCS = [os.path.join(_CSRC, f) for f in ("routing.hip", "block8.hip", "combine.hip")]
+EXPERT_HOST_SRC = os.path.join(_CSRC, "expert_host.cpp")
+EXPERT_HOST_PATH = os.path.join(_PKG, "_expert_host.so")
 BUILD_DIR = os.path.join(_PKG, "_build")
 
 MAX_RANKS = 8
@@ -93,6 +97,25 @@ class RingDebug(ctypes.Structure):
                 ("stats", ctypes.c_uint64)]
 
 
+class RouteOp(ctypes.Structure):
+    """``mint_route_op``."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("logits", "bias", "weights", "chosen")] + [
+        ("row_stride", ctypes.c_int64), ("tokens", ctypes.c_uint64)] + [
+        (n, ctypes.c_uint32) for n in ("experts", "topk", "groups", "kept", "group_top")] + [
+        ("dtype", ctypes.c_int32), ("score", ctypes.c_int32), ("renormalise", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
+class ProductOp(ctypes.Structure):
+    """``mint_product_op``."""
+    _fields_ = [("kind", ctypes.c_int32), ("dtype", ctypes.c_int32)] + [
+        (n, ctypes.c_uint64) for n in ("x", "w", "sx", "sw", "out", "tokens", "offsets", "rows", "cols",
+                                       "depth", "x_rows", "group_rows")] + [
+        (n, ctypes.c_int64) for n in ("x_stride", "w_stride", "w_matrix", "out_stride", "out_matrix",
+                                      "sx_row", "sx_block", "sw_matrix", "sw_row", "sw_block")] + [
+        ("experts", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
 # name -> (restype, argtypes); every symbol include/mintccl.h declares
 _vp, _sz, _u64, _u32, _i = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint64,
                             ctypes.c_uint32, ctypes.c_int)
@@ -100,6 +123,7 @@ _ip = ctypes.POINTER(ctypes.c_int)
 _u32p = ctypes.POINTER(ctypes.c_uint32)
 _opp = ctypes.POINTER(RingOp)
 _dbgp = ctypes.POINTER(RingDebug)
+_i64 = ctypes.c_int64
 SYMBOLS = {
     "mint_version": (_i, []),
     "mint_build_flags": (_i, []),
@@ -123,6 +147,18 @@ SYMBOLS = {
     "mint_ring_launch_static": (_i, [_opp, _vp]),
     "mint_static_init": (_i, []),
     "mint_epoch_advance": (_i, [_vp, _vp, _sz, _i, _vp]),
+    "mint_route": (_i, [ctypes.POINTER(RouteOp), _vp]),
+    "mint_route_grad": (_i, [ctypes.POINTER(RouteOp), _u64, _u64, _i64, _vp]),
+    "mint_assign_workspace": (_sz, [_u64, _u32]),
+    "mint_assign": (_i, [_vp, _u64, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mint_rows8": (_i, [_vp, _i64, _u64, _u64, _i, _vp, _i64, _vp, _i64, _i64, _vp]),
+    "mint_columns8_blocks": (_sz, [_u64, _u32]),
+    "mint_columns8": (_i, [_vp, _i64, _u64, _u64, _i, _vp, _u64, _vp, _u32, _vp, _i64, _vp, _vp]),
+    "mint_squares8": (_i, [_vp, _i64, _i64, _u32, _u64, _u64, _i, _vp, _i64, _i64, _vp, _vp]),
+    "mint_product8": (_i, [ctypes.POINTER(ProductOp), _vp]),
+    "mint_combine": (_i, [_vp, _i64, _u64, _vp, _vp, _u64, _u32, _u32, _vp, _i64, _i, _vp]),
+    "mint_combine_grad": (_i, [_vp, _i64, _vp, _i64, _u64, _vp, _vp, _vp, _u64, _u32, _u32, _vp, _i64, _vp,
+                               _i, _vp]),
     "mint_torn_line_probe": (_i, [_vp, _sz, _i, _i, _i, _i, _i, _u32, _u32, _vp, _vp]),
 }
 
@@ -156,8 +192,8 @@ def stores_with_scalar_offset(asm: str) -> list[str]:
     return [line.strip() for line in asm.splitlines() if pat.match(line)]
 
 
-def host_command(out: str) -> list[str]:
-    """The compiler call for the extension module (host code only: g++, the
+def host_command(out: str, source: str = HOST_SRC) -> list[str]:
+    """The compiler call for an extension module (host code only: g++, the
     headers of Python and of the installed torch)."""
     import sysconfig
 
@@ -169,14 +205,14 @@ def host_command(out: str) -> list[str]:
             *[f"-isystem{d}" for d in (os.path.join(base, "include"),
                                        os.path.join(base, "include", "torch", "csrc", "api", "include"),
                                        os.path.join(rocm, "include"), sysconfig.get_paths()["include"])],
-            "-o", out, HOST_SRC, "-L" + os.path.join(base, "lib"),
+            "-o", out, source, "-L" + os.path.join(base, "lib"),
             "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"]
 
 
 def build(verbose: bool = False, defines: tuple[str, ...] = (), so_path: str | None = None) -> str:
     """Compile the HIP sources for gfx950 into ``libmintccl.so`` (in-tree).
 
-    The ring kernels are one translation unit per element type; the seven
+    The ring kernels are one translation unit per element type; the ten
     compilations run side by side and are linked at the end.  ``defines``
     (``-DMINT_RING_STATS``: wait accounting per ring position,
     ``-DMINT_ROW_NOLOAD``: whole blocks of own rows are not loaded - wrong
@@ -189,15 +225,19 @@ def build(verbose: bool = False, defines: tuple[str, ...] = (), so_path: str | N
     units = [(SRC, list(defines), os.path.join(build_dir, "mintccl.o")),
              (CU_SRC, [*PRELOAD_FLAGS, *defines], os.path.join(build_dir, "cu_ring.o")),
              (CODEC_SRC, [*PRELOAD_FLAGS, *defines], os.path.join(build_dir, "codec.o"))]
+    for src in EXPERT_SRCS:
+        units.append((src, list(defines), os.path.join(build_dir, os.path.basename(src)[:-4] + ".o")))
     for dt in range(4):
         units.append((FAMILY_SRC, [f"-DMINT_FAMILY_DT={dt}", *defines],
                       os.path.join(build_dir, f"ring_family_{dt}.o")))
-    host = None
-    if so_path is None:           # (a diagnostic build shares the product's host module)
-        cmd = host_command(os.path.join(build_dir, "_host.so"))
-        if verbose:
-            print(" ".join(cmd))
-        host = subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    hosts = []
+    if so_path is None:           # (a diagnostic build shares the product's host modules)
+        for src, to in ((HOST_SRC, HOST_PATH), (EXPERT_HOST_SRC, EXPERT_HOST_PATH)):
+            cmd = host_command(os.path.join(build_dir, os.path.basename(to)), src)
+            if verbose:
+                print(" ".join(cmd))
+            hosts.append((src, to, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                                                    text=True)))
     procs = []
     for src, defs, obj in units:
         # every unit compiles in a directory of its own: the compiler leaves the
@@ -212,10 +252,10 @@ def build(verbose: bool = False, defines: tuple[str, ...] = (), so_path: str | N
         procs.append((cmd, tmp, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE,
                                                       stderr=subprocess.PIPE, text=True)))
     errors, spilling, hazards = [], [], []
-    if host is not None:
-        text, _ = host.communicate()
-        if host.returncode != 0:
-            errors.append(f"{HOST_SRC}\n{text}")
+    for src, _, proc in hosts:
+        text, _ = proc.communicate()
+        if proc.returncode != 0:
+            errors.append(f"{src}\n{text}")
     for cmd, tmp, obj, proc in procs:
         _, err = proc.communicate()
         if proc.returncode != 0:
@@ -248,8 +288,8 @@ def build(verbose: bool = False, defines: tuple[str, ...] = (), so_path: str | N
     proc = subprocess.run(link, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"hipcc link failed:\n{proc.stderr}")
-    if host is not None:
-        os.replace(os.path.join(build_dir, "_host.so"), HOST_PATH)
+    for _, to, _ in hosts:
+        os.replace(os.path.join(build_dir, os.path.basename(to)), to)
     return out
 
 
@@ -314,6 +354,30 @@ def host():
                                    "mint_ll128_unpack", "mint_ll128_packed_bytes")], check, empty_bytes)
         _host = module
     return _host
+
+
+_experts = None
+#: the entry points that the module of the expert layer's operators calls, in the order of its bind()
+EXPERT_SYMBOLS = ("mint_route", "mint_route_grad", "mint_assign_workspace", "mint_assign", "mint_rows8",
+                  "mint_columns8_blocks", "mint_columns8", "mint_squares8", "mint_product8", "mint_combine",
+                  "mint_combine_grad")
+
+
+def experts():
+    """The native module of the expert layer's operators, bound to the loaded
+    library.  Raises if it has not been built."""
+    global _experts
+    if _experts is None:
+        L = lib()
+        if not os.path.exists(EXPERT_HOST_PATH):
+            raise RuntimeError(f"{EXPERT_HOST_PATH} is missing: run `python -c 'import __graft_entry__ as g; "
+                               "g.build()'` in the repository root. There is no Python fallback.")
+        from . import _expert_host as module
+        if (module.ROUTE_BYTES, module.PRODUCT_BYTES) != (ctypes.sizeof(RouteOp), ctypes.sizeof(ProductOp)):
+            raise RuntimeError(f"{EXPERT_HOST_PATH} was built for other descriptors: rebuild it")
+        module.bind(check, *[ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in EXPERT_SYMBOLS])
+        _experts = module
+    return _experts
 
 
 def empty_bytes(n: int, like):

@@ -1,0 +1,78 @@
+"""Matrix products in 8-bit floating point with a scale for each block of 128.
+
+A block's largest magnitude m (at least 2**-96) gives it the float32 scale m / 448, and
+its numbers x are kept as x * (448 / m) rounded to ``float8_e4m3fn``.  Activations have
+blocks of 128 along their rows, weights squares of 128 x 128, so that a weight
+matrix and its transpose share their scales; for the weights' gradient both
+sides have blocks of 128 rows.  Products and sums are in 32 bits.  With an
+:class:`~mintccl_amd.routing.Assignment` there is a weight matrix for each expert, for
+the rows of that expert.  No counterpart in the reference.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .common import DTYPE_CODE
+from .routing import Assignment
+
+
+class Blocks(NamedTuple):
+    """Numbers in 8 bits and the scales of their blocks."""
+    q: torch.Tensor          #: float8_e4m3fn, rows at multiples of 16 bytes
+    scale: torch.Tensor      #: float32: (rows, blocks), of weights (blocks of rows, blocks), with as many dimensions as q
+
+
+def _code(dtype: torch.dtype | None) -> int | None:
+    if dtype is not None and dtype not in DTYPE_CODE:
+        raise TypeError("products come in float16, bfloat16 or float32")
+    return None if dtype is None else DTYPE_CODE[dtype]
+
+
+def quantise(x: torch.Tensor) -> Blocks:
+    """``x`` (rows, depth) in float32, bfloat16 or float16, rounded to 8 bits in
+    blocks of 128 along its rows."""
+    return Blocks(*_lib.experts().quantise(x))
+
+
+def quantise_weight(w: torch.Tensor) -> Blocks:
+    """``w`` (cols, depth), or (experts, cols, depth), rounded to 8 bits in squares of
+    128 x 128."""
+    return Blocks(*_lib.experts().quantise_weight(w))
+
+
+def transposed(weight: Blocks) -> Blocks:
+    """The weights as the activations' gradient reads them, laid out once:
+    ``product(grad, transposed(weight))`` is the gradient of ``product(x, weight)``."""
+    q = weight.q.view(torch.uint8).transpose(-1, -2)
+    *lead, rows, depth = q.shape
+    room = torch.zeros(*lead, rows, -(-depth // 128) * 128, dtype=torch.uint8, device=q.device)
+    room[..., :depth] = q
+    return Blocks(room.view(weight.q.dtype)[..., :depth], weight.scale.transpose(-1, -2).contiguous())
+
+
+def product(x: torch.Tensor | Blocks, weight: Blocks, plan: Assignment | None = None, *, gather: bool = False,
+            dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``x @ weight.T``, of ``dtype`` (bfloat16 if none is named) or into ``out``.
+
+    ``x`` (rows, depth) is rounded by :func:`quantise` first where it is not
+    :class:`Blocks` yet; ``weight`` (cols, depth).  With ``plan`` the weight is
+    (experts, cols, depth) and the result has a row for each place of the
+    assignment, made with its expert's matrix from that row of ``x`` or, with
+    ``gather``, from the row of ``x`` that belongs to its token; rows that are no
+    expert's are zeros."""
+    q, scale = x if isinstance(x, Blocks) else (x, None)
+    return _lib.experts().product(q, scale, weight.q, weight.scale, None if plan is None else plan.offsets,
+                                  None if plan is None else plan.tokens, gather, _code(dtype), out)
+
+
+def weight_grad(grad: torch.Tensor, x: torch.Tensor, plan: Assignment | None = None, *, gather: bool = False,
+                dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The gradient of the weights of ``product(x, weight, plan, gather=gather)``
+    from its result's ``grad``: ``grad.T @ x``, of ``dtype`` (float32 if none is
+    named), for each expert where there is a ``plan``.  Both sides are rounded to
+    8 bits in blocks of 128 rows (of an expert's 128 rows)."""
+    return _lib.experts().weight_grad(grad, x, None if plan is None else plan.offsets, None if plan is None else plan.tokens,
+                                      gather, _code(dtype))
