@@ -583,9 +583,13 @@ typedef struct {
     int64_t x_stride, w_stride, w_matrix, out_stride, out_matrix;
     int64_t sx_row, sx_block;            /* between the scales of consecutive rows, blocks */
     int64_t sw_matrix, sw_row, sw_block; /* ... of matrices, rows (ROWS: of 128 rows), blocks */
+    uint64_t workspace, workspace_bytes; /* mint_product8_workspace() bytes, 16-byte aligned */
     uint32_t experts;
-    uint32_t reserved;     /* 0 */
+    int32_t x_dtype;       /* MINT_BYTES: x is in 8 bits; ROWS only: MINT_F16, MINT_BF16, MINT_F32: x is
+                              rounded as by mint_rows8 first (x_stride in elements, any
+                              alignment; sx, sx_row and sx_block are not looked at) */
 } mint_product_op;
+size_t mint_product8_workspace(const mint_product_op* op);
 int mint_product8(const mint_product_op* op, void* stream);
 
 /* out[t] = sum over j of weights[t, j] * rows[slots[t, j]] (weights 0: all 1), in

@@ -113,7 +113,8 @@ class ProductOp(ctypes.Structure):
                                        "depth", "x_rows", "group_rows")] + [
         (n, ctypes.c_int64) for n in ("x_stride", "w_stride", "w_matrix", "out_stride", "out_matrix",
                                       "sx_row", "sx_block", "sw_matrix", "sw_row", "sw_block")] + [
-        ("experts", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+        ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64), ("experts", ctypes.c_uint32),
+        ("x_dtype", ctypes.c_int32)]
 
 
 # name -> (restype, argtypes); every symbol include/mintccl.h declares
@@ -155,6 +156,7 @@ SYMBOLS = {
     "mint_columns8_blocks": (_sz, [_u64, _u32]),
     "mint_columns8": (_i, [_vp, _i64, _u64, _u64, _i, _vp, _u64, _vp, _u32, _vp, _i64, _vp, _vp]),
     "mint_squares8": (_i, [_vp, _i64, _i64, _u32, _u64, _u64, _i, _vp, _i64, _i64, _vp, _vp]),
+    "mint_product8_workspace": (_sz, [ctypes.POINTER(ProductOp)]),
     "mint_product8": (_i, [ctypes.POINTER(ProductOp), _vp]),
     "mint_combine": (_i, [_vp, _i64, _u64, _vp, _vp, _u64, _u32, _u32, _vp, _i64, _i, _vp]),
     "mint_combine_grad": (_i, [_vp, _i64, _vp, _i64, _u64, _vp, _vp, _vp, _u64, _u32, _u32, _vp, _i64, _vp,
@@ -359,7 +361,8 @@ def host():
 _experts = None
 #: the entry points that the module of the expert layer's operators calls, in the order of its bind()
 EXPERT_SYMBOLS = ("mint_route", "mint_route_grad", "mint_assign_workspace", "mint_assign", "mint_rows8",
-                  "mint_columns8_blocks", "mint_columns8", "mint_squares8", "mint_product8", "mint_combine",
+                  "mint_columns8_blocks", "mint_columns8", "mint_squares8", "mint_product8_workspace",
+                  "mint_product8", "mint_combine",
                   "mint_combine_grad")
 
 

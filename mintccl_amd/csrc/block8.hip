@@ -40,27 +40,37 @@ struct Tile {
 __device__ __forceinline__ uint32_t row_bound(const Groups& g, uint32_t i) {
     return min((uint32_t)max(g.offsets[i], 0), g.rows);
 }
-// The expert of tile `t`.  `rest`: the rows that are no expert's follow as those of an expert with number
-// g.experts.  Every wavefront looks for itself, 64 experts at a time.
+// The tiles of expert e, how many there are in all, and the expert of tile `t`.  `rest`: the rows that are no
+// expert's follow as those of an expert with number g.experts.  Every wavefront looks for itself, 64 experts at a time.
+__device__ __forceinline__ uint32_t tiles_of(const Groups& g, uint32_t e, uint32_t tile_rows, bool rest, uint32_t& begin, uint32_t& end) {
+    begin = end = 0;
+    if (e < g.experts + rest) {
+        begin = row_bound(g, e);
+        end = max(begin, e < g.experts ? row_bound(g, e + 1) : g.rows);
+    }
+    return (end - begin + tile_rows - 1) / tile_rows;
+}
+__device__ __forceinline__ uint32_t sum_below(uint32_t v) {       // of the lanes up to this one
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t other = (uint32_t)__shfl_up((int)v, d);
+        v += lane_id() >= d ? other : 0u;
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t count_tiles(const Groups& g, uint32_t tile_rows, bool rest) {
+    if (!g.offsets) return (g.rows + tile_rows - 1) / tile_rows;
+    uint32_t mine = 0, begin, end;
+    for (uint32_t e = lane_id(); e < g.experts + rest; e += 64) mine += tiles_of(g, e, tile_rows, rest, begin, end);
+    return (uint32_t)__builtin_amdgcn_readlane((int)sum_below(mine), 63);
+}
 __device__ __forceinline__ Tile find_tile(const Groups& g, uint32_t t, uint32_t tile_rows, bool rest) {
     Tile r = {0, 0, 0, g.rows, true};
     if (!g.offsets) return r;
     uint32_t base = 0;
     for (uint32_t e0 = 0; e0 < g.experts + rest; e0 += 64) {
-        const uint32_t e = e0 + lane_id();
-        uint32_t begin = 0, end = 0;
-        if (e < g.experts + rest) {
-            begin = row_bound(g, e);
-            end = e < g.experts ? row_bound(g, e + 1) : g.rows;
-            end = max(begin, end);
-        }
-        const uint32_t tiles = (end - begin + tile_rows - 1) / tile_rows;
-        uint32_t sum = tiles;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t other = (uint32_t)__shfl_up((int)sum, d);
-            sum += lane_id() >= d ? other : 0u;
-        }
+        uint32_t begin, end;
+        const uint32_t tiles = tiles_of(g, e0 + lane_id(), tile_rows, rest, begin, end), sum = sum_below(tiles);
         const uint64_t behind = __ballot(base + sum > t);
         if (behind) {
             const int at = __builtin_ctzll(behind);
@@ -217,12 +227,16 @@ struct ProductArgs {
     Groups groups;               // experts' rows (or, `along_depth`, experts' blocks of the depth)
     int64_t x_stride, w_stride, w_matrix, out_stride, out_matrix;
     int64_t sx_row, sx_block, sw_matrix, sw_row, sw_block;
-    uint32_t x_rows, rows, cols, depth, col_tiles, row_tiles, out_whole;
+    uint32_t x_rows, rows, cols, depth, col_tiles, row_tiles, out_whole, x_whole;
 };
 
-// Where a row's 16-byte piece lies in its 128 bytes of LDS: turned by the row's number so that the lanes of a
-// wavefront that read the same piece of different rows (16 consecutive ones of x, four times four of the weights) fall on different banks.
-__device__ __forceinline__ uint32_t turn(uint32_t row) { return ((row >> 1) ^ ((row >> 4) << 1)) & 7u; }
+// Where a row's 16-byte piece lies in its 128 bytes of LDS: turned by the row's number, so that the lanes that a 16-byte read
+// serves together (0 - 3, 12 - 15 and 20 - 27 of 32, then the others), each a row, fall on different banks. For that lane groups 0
+// and 1 (2 and 3) read pieces that differ in their lowest bit.
+__device__ __forceinline__ uint32_t turn(uint32_t row) { return (row >> 1) & 7u; }
+// Which column of the result a row of the weights in LDS stands for: of the 64 of a wavefront, the four that a lane
+// gets from each of four matrix instructions lie side by side.
+__device__ __forceinline__ uint32_t column_of(uint32_t row) { return (row & ~63u) | (row << 2 & 0x30u) | (row >> 2 & 0xCu) | (row & 3u); }
 
 __device__ __forceinline__ void to_lds16(const uint8_t* from, uint32_t lds) {
     __builtin_amdgcn_global_load_lds((MINT_GLOBAL const void*)as_global(from), (MINT_LDS void*)(uintptr_t)lds, 16, 0, 0);
@@ -232,8 +246,9 @@ __device__ __forceinline__ void to_lds4(const float* from, uint32_t lds) {
 }
 __device__ __forceinline__ u32x4 lds16(uint32_t at) { return *(MINT_LDS const u32x4*)(uintptr_t)at; }
 __device__ __forceinline__ float lds_float(uint32_t at) { return *(MINT_LDS const float*)(uintptr_t)at; }
-__device__ __forceinline__ i32x8 piece(uint32_t row_at, uint32_t turned, uint32_t part) {
-    const u32x4 a = lds16(row_at + ((2 * part) ^ turned) * 16), b = lds16(row_at + ((2 * part + 1) ^ turned) * 16);
+// a lane's part of 16 rows: two of a row's eight pieces (the same two of both operands: the order of the depth does not matter)
+__device__ __forceinline__ i32x8 piece(uint32_t at0, uint32_t at1) {
+    const u32x4 a = lds16(at0), b = lds16(at1);
     return i32x8{(int)a.x, (int)a.y, (int)a.z, (int)a.w, (int)b.x, (int)b.y, (int)b.z, (int)b.w};
 }
 
@@ -267,19 +282,30 @@ struct Operand<true> {
     }
 };
 
-// A thread block has BM rows and BN columns of the result, a wavefront 64 columns and BM / WM rows.
+// A thread block has BM rows and BN columns of the result, a wavefront 64 columns and BM / WM rows of them.
 // The depth goes by in blocks of 128: while one is multiplied the next one's bytes are on their way into the other half of LDS.
 // The weights are the matrix instruction's first operand, so a lane has four consecutive columns of one row for each,
 // and 16 with the four of a wavefront's columns dealt to the instructions in fours.
 template <int OUT, int BM, int BN, int WM, bool ROWS_W, bool ALONG>
 __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArgs a) {
     using Op = Operand<OUT == DT_F32>;
+    using T = typename Elem<OUT>::type;
     constexpr int WN = BN / 64, WAVES = WM * WN, MT = BM / WM / 16, NT = 4;
     constexpr uint32_t kX = BM * 128, kW = BN * 128, kSx = BM * 4, kSw = ROWS_W ? BN * 4 : 0, kStage = kX + kW + kSx + kSw;
+    static_assert(BM / 64 <= WAVES && BN / 64 <= WAVES, "a wavefront for each 64 scales");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
     const uint32_t base = (uint32_t)(uintptr_t)(MINT_LDS uint8_t*)lds;
-    const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block());
-    const uint32_t row_tile = blockIdx.x / a.col_tiles, n0 = blockIdx.x % a.col_tiles * BN;
+    const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), wm = wave / WN, wn = wave % WN;
+
+    // The hardware deals thread blocks to the eight XCDs in turn: each takes an eighth of the tiles that lie together, in
+    // columns of GROUP row tiles, so that those at work at a time share rows and weights in its L2.
+    constexpr uint32_t GROUP = 4;
+    const uint32_t row_tiles = ALONG ? a.row_tiles * (a.groups.offsets ? a.groups.experts : 1u) : count_tiles(a.groups, BM, true);
+    const uint32_t total = row_tiles * a.col_tiles, xcd = blockIdx.x & 7u, nth = blockIdx.x >> 3;
+    if (nth >= total / 8 + (xcd < total % 8)) return;
+    const uint32_t id = xcd * (total / 8) + min(xcd, total % 8) + nth;
+    const uint32_t group = id / (GROUP * a.col_tiles), in_group = id % (GROUP * a.col_tiles), height = min(GROUP, row_tiles - group * GROUP);
+    const uint32_t row_tile = group * GROUP + in_group % height, n0 = in_group / height * BN;
 
     // which rows, which weights, which part of the depth
     uint32_t expert, m0, m_end, depth0 = 0, depth = a.depth;
@@ -293,15 +319,12 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
                 const uint32_t b = row_bound(a.groups, e), n = row_bound(a.groups, e + 1);
                 before += n > b ? (n - b + 127) / 128 : 0u;
             }
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) before += (uint32_t)__shfl_xor((int)before, d);
             const uint32_t b = row_bound(a.groups, expert), n = row_bound(a.groups, expert + 1);
-            depth0 = __builtin_amdgcn_readfirstlane(before) * 128;
+            depth0 = (uint32_t)__builtin_amdgcn_readlane((int)sum_below(before), 63) * 128;
             depth = n > b ? (n - b + 127) / 128 * 128 : 0u;
         }
     } else {
         const Tile t = find_tile(a.groups, row_tile, BM, true);
-        if (!t.found) return;
         expert = t.expert;
         m0 = t.begin + (row_tile - t.first) * BM;
         m_end = t.end;
@@ -309,39 +332,34 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
     }
     const uint32_t full = depth / 128, steps = (depth + 127) / 128;
 
-    // A wavefront brings 8 rows of 128 bytes with an instruction: the rows it has of x, then of w.
+    // A wavefront brings 8 rows of 128 bytes with an instruction: the rows it has of x, then of the weights.
     constexpr int XI = BM / 8 / WAVES, WI = BN / 8 / WAVES;
     const uint8_t *from_x[XI], *from_w[WI];
+    const float *from_sx = nullptr, *from_sw = nullptr, *sw_block = nullptr;
     const uint32_t sub = lane >> 3, slot = lane & 7u;
     const auto x_row = [&](uint32_t r) MINT_INLINE_LAMBDA {
         uint32_t row = min(m0 + r, m_end ? m_end - 1 : 0u);
         if (!ALONG && a.tokens) row = (uint32_t)a.tokens[row];
         return min(row, a.x_rows - 1);
     };
-    const uint8_t* const w0 = a.w + (ALONG ? 0 : (int64_t)expert * a.w_matrix);
     if (steps) {
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
             const uint32_t r = (wave * XI + i) * 8 + sub;
             from_x[i] = a.x + (int64_t)x_row(r) * a.x_stride + depth0 + ((slot ^ turn(r)) * 16);
         }
+        const uint8_t* const w0 = a.w + (ALONG ? 0 : (int64_t)expert * a.w_matrix);
 #pragma unroll
         for (int i = 0; i < WI; ++i) {
             const uint32_t r = (wave * WI + i) * 8 + sub;
-            from_w[i] = w0 + (int64_t)min(n0 + r, a.cols - 1) * a.w_stride + depth0 + ((slot ^ turn(r)) * 16);
+            from_w[i] = w0 + (int64_t)min(n0 + column_of(r), a.cols - 1) * a.w_stride + depth0 + ((slot ^ turn(r)) * 16);
         }
-    }
-    const float *from_sx = nullptr, *from_sw = nullptr;
-    if (steps) {
         if (wave < BM / 64) from_sx = a.sx + (int64_t)x_row(wave * 64 + lane) * a.sx_row + (int64_t)(depth0 / 128) * a.sx_block;
         if (ROWS_W && wave < BN / 64)
             from_sw = a.sw + (int64_t)min(n0 + wave * 64 + lane, a.cols - 1) * a.sw_row + (int64_t)(depth0 / 128) * a.sw_block;
+        if (!ROWS_W)                         // one number for 128 columns
+            sw_block = a.sw + (int64_t)expert * a.sw_matrix + (int64_t)(min(n0 + wn * 64, a.cols - 1) / 128) * a.sw_row;
     }
-    const float* sw_block = a.sw + (ALONG ? 0 : (int64_t)expert * a.sw_matrix);      // one number for 128 columns
-    const uint32_t wm = wave / WN, wn = wave % WN;
-    if (!ROWS_W) sw_block += (int64_t)((n0 + wn * 64) / 128) * a.sw_row;
-
-    static_assert(BM / 64 <= WAVES && BN / 64 <= WAVES, "a wavefront for each 64 scales");
     const auto bring_scales = [&](uint32_t at) MINT_INLINE_LAMBDA {
         if (wave < BM / 64) {
             to_lds4(from_sx, at + kX + kW + wave * 256);
@@ -352,18 +370,16 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
             from_sw += a.sw_block;
         }
     };
-    const auto bring = [&](uint32_t at) MINT_INLINE_LAMBDA {
-#pragma unroll
-        for (int i = 0; i < XI; ++i) {
-            to_lds16(from_x[i], at + (wave * XI + i) * 1024);
-            from_x[i] += 128;
+    // piece `n` of XI + WI, the scales with the first
+    const auto bring = [&](uint32_t at, int n) MINT_INLINE_LAMBDA {
+        if (n == 0) bring_scales(at);
+        if (n < XI) {
+            to_lds16(from_x[n], at + (wave * XI + n) * 1024);
+            from_x[n] += 128;
+        } else {
+            to_lds16(from_w[n - XI], at + kX + (wave * WI + (n - XI)) * 1024);
+            from_w[n - XI] += 128;
         }
-#pragma unroll
-        for (int i = 0; i < WI; ++i) {
-            to_lds16(from_w[i], at + kX + (wave * WI + i) * 1024);
-            from_w[i] += 128;
-        }
-        bring_scales(at);
     };
     // the last block of a depth that is no multiple of 128: nothing is read behind a row's end
     const auto bring_tail = [&](uint32_t at) MINT_INLINE_LAMBDA {
@@ -393,42 +409,77 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
     const uint32_t r16 = lane & 15u, part = lane >> 4;
-    const uint32_t xr = wm * (BM / WM) + r16, wr = wn * 64 + (r16 >> 2) * 16 + (r16 & 3u);
-    const auto multiply = [&](uint32_t at, float sw) MINT_INLINE_LAMBDA {
+    const uint32_t xr = wm * (BM / WM) + r16, wr = wn * 64 + r16;
+    const uint32_t x_at = xr * 128 + ((part ^ turn(xr)) * 16), w_at = kX + wr * 128 + ((part ^ turn(wr)) * 16);
+    const uint32_t sx_at = kX + kW + xr * 4, sw_at = kX + kW + kSx + (wn * 64 + part * 16) * 4;
+    // The matrix instructions' sums are scaled and added LAG instructions later: the two units work side by side.
+    constexpr int LAG = 3;
+    const auto multiply = [&](uint32_t at, float sw, const auto& meanwhile) MINT_INLINE_LAMBDA {
         f32x4 sw4[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-            if (ROWS_W) sw4[j] = *(MINT_LDS const f32x4*)(uintptr_t)(at + kX + kW + kSx + (wn * 64 + part * 16 + j * 4) * 4);
-        const auto w_piece = [&](int j) MINT_INLINE_LAMBDA { return Op(piece(at + kX + (wr + j * 4) * 128, turn(wr + j * 4), part)); };
-        const Op w[NT] = {w_piece(0), w_piece(1), w_piece(2), w_piece(3)};
+            if (ROWS_W) sw4[j] = *(MINT_LDS const f32x4*)(uintptr_t)(at + sw_at + j * 16);
+        const uint32_t w0 = at + w_at, w1 = at + (w_at ^ 64u), x0 = at + x_at, x1 = at + (x_at ^ 64u);
+        const Op w[NT] = {Op(piece(w0, w1)), Op(piece(w0 + 2048, w1 + 2048)), Op(piece(w0 + 4096, w1 + 4096)), Op(piece(w0 + 6144, w1 + 6144))};
+        Op x(piece(x0, x1));
+        float s[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) s[i] = lds_float(at + sx_at + i * 64) * sw;
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 d[LAG + 1];
+        const auto add = [&](int n) MINT_INLINE_LAMBDA {
+            const int i = n / NT, j = n % NT;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(d[n % (LAG + 1)][k], ROWS_W ? s[i] * sw4[j][k] : s[i], acc[i][j][k]);
+        };
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const uint32_t r = xr + i * 16;
-            const Op x(piece(at + r * 128, turn(r), part));
-            const float s = lds_float(at + kX + kW + r * 4) * sw;
+            // (the next block's loads go out between the products: all at once they would stand in each other's way)
+            constexpr int PIECES = (XI + WI) * 2 / MT;
+#pragma unroll
+            for (int n = 0; n < PIECES; ++n)
+                if (i * PIECES + n < XI + WI) meanwhile(i * PIECES + n);
+            Op next = x;
+            if (i + 1 < MT) next = Op(piece(x0 + (i + 1) * 2048, x1 + (i + 1) * 2048));
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const f32x4 d = Op::multiply(w[j], x);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(d[k], ROWS_W ? s * sw4[j][k] : s, acc[i][j][k]);
+                const int n = i * NT + j;
+                d[n % (LAG + 1)] = Op::multiply(w[j], x);
+                if (n >= LAG) add(n - LAG);
+                __builtin_amdgcn_sched_barrier(0);       // (left alone the compiler puts every sum right behind its instruction)
             }
+            x = next;
         }
+#pragma unroll
+        for (int n = MT * NT - LAG; n < MT * NT; ++n) add(n);
     };
 
     if (steps) {
-        if (full) bring(base);
-        else bring_tail(base);
-        for (uint32_t b = 0; b < steps; ++b) {
-            const uint32_t at = base + (b & 1u) * kStage, other = base + ((b + 1) & 1u) * kStage;
-            const float sw = ROWS_W ? 1.0f : sw_block[(int64_t)b * a.sw_block];
+        uint32_t b = 0, at = base;
+        const auto scale_of = [&]() MINT_INLINE_LAMBDA { return ROWS_W ? 1.0f : sw_block[(int64_t)b * a.sw_block]; };
+        if (full) {
+#pragma unroll
+            for (int n = 0; n < XI + WI; ++n) bring(at, n);
+        } else {
+            bring_tail(at);
+        }
+        for (; b + 1 < full; ++b) {
+            const float sw = scale_of();
+            const uint32_t other = base + base + kStage - at;
             __syncthreads();             // (waits for the loads into LDS too)
-            if (b + 1 < full) bring(other);
-            else if (b + 1 < steps) bring_tail(other);
-            multiply(at, sw);
+            multiply(at, sw, [&](int n) MINT_INLINE_LAMBDA { bring(other, n); });
+            at = other;
+        }
+        for (; b < steps; ++b) {
+            const float sw = scale_of();
+            const uint32_t other = base + base + kStage - at;
+            __syncthreads();
+            if (b + 1 < steps) bring_tail(other);
+            multiply(at, sw, [](int) MINT_INLINE_LAMBDA {});
+            at = other;
         }
     }
 
-    using T = typename Elem<OUT>::type;
     T* const out = static_cast<T*>(a.out) + (ALONG ? (int64_t)expert * a.out_matrix : 0);
     const uint32_t col = n0 + wn * 64 + part * 16;
 #pragma unroll
@@ -446,16 +497,175 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
     }
 }
 
-template <int OUT, bool ROWS_W, bool ALONG>
-int go_product(ProductArgs a, uint32_t matrices, hipStream_t stream) {
-    constexpr int BM = 128, BN = 128, WM = 2;
+// ---- products of few rows ------------------------------------------------------------
+// Bound by reading the weights: 16 MT rows need them once.  A thread block has 16 columns, and its wavefronts every
+// WAVES-th block of the depth, straight from memory into registers: a wavefront asks for AHEAD blocks before
+// it multiplies the first, which is what keeps enough bytes on their way.  The wavefronts' sums are added up in LDS, in
+// their order.  Activations that are not in 8 bits yet (X) are rounded on the way: each thread block does that again, but it is less than
+// another launch takes.
+typedef uint32_t u32x4_near __attribute__((ext_vector_type(4), aligned(4)));
+constexpr int kThinWaves = 8, kThinAhead = 4;
+
+// 32 bytes of a row of 8-bit numbers, `left` of them there
+__device__ __forceinline__ i32x8 eight_bits(const uint8_t* from, int32_t left) {
+    u32x4 v[2] = {};
+    if (left >= 32) {
+        v[0] = *(MINT_GLOBAL const u32x4*)as_global(from);
+        v[1] = *(MINT_GLOBAL const u32x4*)as_global(from + 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < left) v[i / 16][i / 4 % 4] |= (uint32_t)*as_global(from + i) << (i % 4 * 8);
+    }
+    return i32x8{(int)v[0].x, (int)v[0].y, (int)v[0].z, (int)v[0].w, (int)v[1].x, (int)v[1].y, (int)v[1].z, (int)v[1].w};
+}
+
+// X: the activations' type, DT_BYTES if they are in 8 bits
+template <int OUT, int X, int MT>
+__global__ void __launch_bounds__(64 * kThinWaves) thin_kernel(ProductArgs a) {
+    using Op = Operand<OUT == DT_F32>;
+    using T = typename Elem<OUT>::type;
+    constexpr int WAVES = kThinWaves, AHEAD = kThinAhead, BM = 16 * MT;
+    constexpr bool ROUND = X != DT_BYTES;
+    using TX = typename Elem<ROUND ? X : DT_F32>::type;
+    __shared__ float sums[WAVES][BM][17];
+    const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), r16 = lane & 15u, part = lane >> 4;
+    const uint32_t row_tile = blockIdx.x / a.col_tiles, n0 = blockIdx.x % a.col_tiles * 16;
+    const Tile t = find_tile(a.groups, row_tile, BM, true);
+    if (!t.found) return;
+    const uint32_t m0 = t.begin + (row_tile - t.first) * BM, rows = min(t.end - m0, (uint32_t)BM);
+    const uint32_t steps = a.groups.offsets && t.expert == a.groups.experts ? 0u : (a.depth + 127) / 128;
+    const int32_t depth = (int32_t)a.depth;
+
+    f32x4 acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    if (wave < steps) {
+        const uint8_t* const w = a.w + (int64_t)t.expert * a.w_matrix + (int64_t)min(n0 + r16, a.cols - 1) * a.w_stride + part * 32;
+        const float* const sw = a.sw + (int64_t)t.expert * a.sw_matrix + (int64_t)(n0 / 128) * a.sw_row;
+        uint32_t row[MT];
+        bool there[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            there[i] = i * 16 + r16 < rows;
+            row[i] = m0 + min(i * 16 + r16, rows - 1);
+            if (a.tokens) row[i] = (uint32_t)a.tokens[row[i]];
+            row[i] = min(row[i], a.x_rows - 1);
+        }
+        for (uint32_t b0 = wave; b0 < steps; b0 += WAVES * AHEAD) {
+            i32x8 wv[AHEAD];
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const uint32_t b = b0 + u * WAVES;
+                if (b < steps) wv[u] = eight_bits(w + b * 128, depth - (int32_t)(b * 128 + part * 32));
+            }
+#pragma unroll
+            for (int u = 0; u < AHEAD; ++u) {
+                const uint32_t b = b0 + u * WAVES;
+                if (b >= steps) break;
+                const int32_t left = depth - (int32_t)(b * 128 + part * 32);
+                const float s_w = sw[(int64_t)b * a.sw_block];
+                const Op wo(wv[u]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    i32x8 xv = {};
+                    float s = 0.0f;
+                    if constexpr (ROUND) {
+                        float v[32], m = kLeastBlock;
+                        const TX* const from = reinterpret_cast<const TX*>(a.x) + (int64_t)row[i] * a.x_stride + b * 128 + part * 32;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float e[8] = {};
+                            if (there[i]) load_elements<X, 8>(from + k * 8, a.x_whole && left >= k * 8 + 8, left - k * 8, e);
+#pragma unroll
+                            for (int h = 0; h < 8; ++h) {
+                                v[k * 8 + h] = e[h];
+                                m = larger(fabsf(e[h]), m);
+                            }
+                        }
+                        m = larger(__shfl_xor(m, 16), m);
+                        m = larger(__shfl_xor(m, 32), m);
+                        const float r = kLargest8 / m;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) xv[k] = (int)pack8(v[k * 4] * r, v[k * 4 + 1] * r, v[k * 4 + 2] * r, v[k * 4 + 3] * r);
+                        s = m / kLargest8;
+                    } else if (there[i]) {
+                        xv = eight_bits(a.x + (int64_t)row[i] * a.x_stride + b * 128 + part * 32, left);
+                        s = a.sx[(int64_t)row[i] * a.sx_row + (int64_t)b * a.sx_block];
+                    }
+                    const f32x4 d = Op::multiply(wo, Op(xv));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc[i][k] = fmaf(d[k], s * s_w, acc[i][k]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[wave][i * 16 + r16][part * 4 + k] = acc[i][k];
+    __syncthreads();
+    for (uint32_t at = threadIdx.x; at < BM * 16; at += 64 * WAVES) {
+        const uint32_t m = at / 16, n = at % 16;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) sum += sums[i][m][n];
+        if (m < rows && n0 + n < a.cols) *as_global(static_cast<T*>(a.out) + (int64_t)(m0 + m) * a.out_stride + n0 + n) = Elem<OUT>::round(sum);
+    }
+}
+
+// How many tiles of `tile_rows` rows there are at most, and about how many there will be (an expert's last is half full).
+uint64_t most_row_tiles(const ProductArgs& a, uint32_t tile_rows) {
+    return ceil_div(a.rows, tile_rows) + (a.groups.offsets ? (uint64_t)a.groups.experts + 1 : 0);
+}
+template <int OUT, int BM, int BN, int WM, bool ROWS_W, bool ALONG>
+int go_tiles(ProductArgs a, uint32_t matrices, hipStream_t stream) {
     a.col_tiles = (uint32_t)ceil_div(a.cols, BN);
     a.row_tiles = (uint32_t)ceil_div(a.rows, BM);
-    const uint64_t tiles = ALONG ? (uint64_t)a.row_tiles * matrices : a.groups.offsets ? (uint64_t)a.row_tiles + a.groups.experts + 1 : a.row_tiles;
-    const uint64_t blocks = tiles * a.col_tiles;
+    const uint64_t blocks = (ALONG ? (uint64_t)a.row_tiles * matrices : most_row_tiles(a, BM)) * a.col_tiles;
     if (blocks > 0x7FFFFFFFull / (64 * WM * (BN / 64))) return MINT_ERR_TOO_LARGE;
     if (!blocks) return MINT_OK;
-    return Launch<&product_kernel<OUT, BM, BN, WM, ROWS_W, ALONG>>::go((uint32_t)blocks, 64 * WM * (BN / 64), 0, stream, a);
+    return Launch<&product_kernel<OUT, BM, BN, WM, ROWS_W, ALONG>>::go((uint32_t)ceil_div(blocks, 8) * 8, 64 * WM * (BN / 64), 0, stream, a);
+}
+// The tiles whose rounds over the compute units take least: tiles / (those at work at a time), rounded up, times what a round
+// takes for a block of the depth (measured at 8192 x 4096 x 8192, us): 256 x 256 2.04, 128 x 256 1.24, two 128 x 128 1.44.
+template <int OUT, bool ROWS_W, bool ALONG>
+int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
+    const auto rounds = [&](uint32_t bm, uint32_t bn, uint32_t at_a_time) {
+        const uint64_t rows = ALONG ? ceil_div(a.rows, bm) * matrices : ceil_div(a.rows, bm) + (a.groups.offsets ? a.groups.experts / 2 : 0);
+        return (float)ceil_div(rows * ceil_div(a.cols, bn), at_a_time);
+    };
+    const float large = 2.04f * rounds(256, 256, 256), wide = 1.24f * rounds(128, 256, 256), small = 1.44f * rounds(128, 128, 512);
+    if constexpr (OUT != DT_F32) {
+        if (large <= wide && large <= small) return go_tiles<OUT, 256, 256, 2, ROWS_W, ALONG>(a, matrices, stream);
+        if (wide <= small) return go_tiles<OUT, 128, 256, 2, ROWS_W, ALONG>(a, matrices, stream);
+    }
+    return go_tiles<OUT, 128, 128, 2, ROWS_W, ALONG>(a, matrices, stream);
+}
+
+// Few rows: at most 64 for each weight matrix, on the average.
+bool few_rows(uint64_t rows, uint32_t matrices) { return rows <= 64ull * matrices; }
+// ... and so few that the rounding is done on the way
+bool rounded_on_the_way(uint64_t rows, uint32_t matrices) { return rows <= 16ull * matrices; }
+template <int OUT, int X, int MT>
+int go_thin(ProductArgs a, hipStream_t stream) {
+    a.col_tiles = (uint32_t)ceil_div(a.cols, 16);
+    const uint64_t blocks = most_row_tiles(a, 16 * MT) * a.col_tiles;
+    if (blocks > 0x7FFFFFFFull / (64 * kThinWaves)) return MINT_ERR_TOO_LARGE;
+    return Launch<&thin_kernel<OUT, X, MT>>::go((uint32_t)blocks, 64 * kThinWaves, 0, stream, a);
+}
+template <int OUT>
+int go_rows(const ProductArgs& a, int x_dtype, uint32_t matrices, hipStream_t stream) {
+    switch (x_dtype) {
+        case MINT_F16: return go_thin<OUT, DT_F16, 1>(a, stream);
+        case MINT_BF16: return go_thin<OUT, DT_BF16, 1>(a, stream);
+        case MINT_F32: return go_thin<OUT, DT_F32, 1>(a, stream);
+        default: break;
+    }
+    if (a.rows <= 16ull * matrices) return go_thin<OUT, DT_BYTES, 1>(a, stream);
+    if (a.rows <= 32ull * matrices) return go_thin<OUT, DT_BYTES, 2>(a, stream);
+    if (few_rows(a.rows, matrices)) return go_thin<OUT, DT_BYTES, 4>(a, stream);
+    return go_product<OUT, false, false>(a, 1, stream);
 }
 
 bool known(int dtype) { return dtype == MINT_F16 || dtype == MINT_BF16 || dtype == MINT_F32; }
@@ -534,30 +744,60 @@ extern "C" int mint_squares8(const void* w, int64_t w_matrix, int64_t w_stride, 
     }
 }
 
+namespace {
+uint32_t matrices_of(const mint_product_op& op) { return op.offsets ? op.experts : 1; }
+// 8-bit numbers and scales of activations that come as they are, where that takes a launch of its own
+size_t rounded_bytes(const mint_product_op& op) {
+    if (op.kind != MINT_PRODUCT_ROWS || op.x_dtype == MINT_BYTES || rounded_on_the_way(op.rows, matrices_of(op))) return 0;
+    return (size_t)op.x_rows * ceil_div(op.depth, 128) * 132;
+}
+}  // namespace
+
+extern "C" size_t mint_product8_workspace(const mint_product_op* op) { return op ? rounded_bytes(*op) : 0; }
+
 extern "C" int mint_product8(const mint_product_op* op, void* stream) {
     if (!op || !known(op->dtype) || (op->kind != MINT_PRODUCT_ROWS && op->kind != MINT_PRODUCT_GRADIENT)) return MINT_ERR_ARG;
+    const bool along = op->kind == MINT_PRODUCT_GRADIENT, raw = op->x_dtype != MINT_BYTES;
+    if (raw && (along || !known(op->x_dtype))) return MINT_ERR_ARG;
     if (op->rows > kMostRows || op->cols > kMostRows || op->depth > kMostRows || op->x_rows > kMostRows || op->experts > 65535)
         return MINT_ERR_TOO_LARGE;
-    const bool along = op->kind == MINT_PRODUCT_GRADIENT;
     if (op->rows == 0 || op->cols == 0) return MINT_OK;
     if (!op->out || (!op->offsets && op->experts)) return MINT_ERR_ARG;
     // (nothing to multiply: the result is zeros, and neither operand is read)
     const bool some = op->depth != 0;
-    if (some && (!op->x || !op->w || !op->sx || !op->sw || op->x_rows == 0)) return MINT_ERR_ARG;
+    if (some && (!op->x || !op->w || (!raw && !op->sx) || !op->sw || op->x_rows == 0)) return MINT_ERR_ARG;
     if (some && !along && !op->tokens && op->x_rows < op->rows) return MINT_ERR_ARG;
-    if (some && (!aligned_to(reinterpret_cast<void*>(op->x), 16) || !aligned_to(reinterpret_cast<void*>(op->w), 16) || op->x_stride % 16 ||
+    if (some && ((!raw && (!aligned_to(reinterpret_cast<void*>(op->x), 16) || op->x_stride % 16)) || !aligned_to(reinterpret_cast<void*>(op->w), 16) ||
                  op->w_stride % 16 || op->w_matrix % 16))
         return MINT_ERR_ALIGN;
     if (along && op->depth % 128) return MINT_ERR_GEOMETRY;
-    const bool whole = vectors(reinterpret_cast<void*>(op->out), op->out_stride, op->dtype) && op->out_matrix % 8 == 0;
-    const ProductArgs a = {reinterpret_cast<const uint8_t*>(op->x), reinterpret_cast<const uint8_t*>(op->w),
-                           reinterpret_cast<const float*>(op->sx), reinterpret_cast<const float*>(op->sw), reinterpret_cast<void*>(op->out),
-                           reinterpret_cast<const int32_t*>(op->tokens),
-                           {reinterpret_cast<const int32_t*>(op->offsets), op->experts, (uint32_t)(along ? op->group_rows : op->rows)},
-                           op->x_stride, op->w_stride, op->w_matrix, op->out_stride, op->out_matrix, op->sx_row, op->sx_block, op->sw_matrix,
-                           op->sw_row, op->sw_block, (uint32_t)op->x_rows, (uint32_t)op->rows, (uint32_t)op->cols, (uint32_t)op->depth, 0, 0, whole};
+    const size_t need = rounded_bytes(*op);
+    if (need && (op->workspace_bytes < need || !op->workspace)) return MINT_ERR_STAGING;
+    if (need && !aligned_to(reinterpret_cast<void*>(op->workspace), 16)) return MINT_ERR_ALIGN;
     const auto s = static_cast<hipStream_t>(stream);
-    const uint32_t matrices = op->offsets ? op->experts : 1;
+    const bool whole = vectors(reinterpret_cast<void*>(op->out), op->out_stride, op->dtype) && op->out_matrix % 8 == 0;
+    ProductArgs a = {reinterpret_cast<const uint8_t*>(op->x), reinterpret_cast<const uint8_t*>(op->w),
+                     reinterpret_cast<const float*>(op->sx), reinterpret_cast<const float*>(op->sw), reinterpret_cast<void*>(op->out),
+                     reinterpret_cast<const int32_t*>(op->tokens),
+                     {reinterpret_cast<const int32_t*>(op->offsets), op->experts, (uint32_t)(along ? op->group_rows : op->rows)},
+                     op->x_stride, op->w_stride, op->w_matrix, op->out_stride, op->out_matrix, op->sx_row, op->sx_block, op->sw_matrix,
+                     op->sw_row, op->sw_block, (uint32_t)op->x_rows, (uint32_t)op->rows, (uint32_t)op->cols, (uint32_t)op->depth, 0, 0, whole,
+                     raw && vectors(reinterpret_cast<void*>(op->x), op->x_stride, op->x_dtype)};
+    const uint32_t matrices = matrices_of(*op);
+    int x_dtype = op->x_dtype;
+    if (need && some) {
+        const uint64_t per_row = ceil_div(op->depth, 128);
+        auto* const q = reinterpret_cast<uint8_t*>(op->workspace);
+        auto* const scale = reinterpret_cast<float*>(q + op->x_rows * per_row * 128);
+        const int err = mint_rows8(a.x, op->x_stride, op->x_rows, op->depth, x_dtype, q, (int64_t)per_row * 128, scale, 1, (int64_t)op->x_rows, stream);
+        if (err != MINT_OK) return err;
+        a.x = q;
+        a.x_stride = (int64_t)per_row * 128;
+        a.sx = scale;
+        a.sx_row = 1;
+        a.sx_block = (int64_t)op->x_rows;
+    }
+    if (need) x_dtype = MINT_BYTES;
     if (along) {
         switch (op->dtype) {
             case MINT_F16: return go_product<DT_F16, true, true>(a, matrices, s);
@@ -566,8 +806,8 @@ extern "C" int mint_product8(const mint_product_op* op, void* stream) {
         }
     }
     switch (op->dtype) {
-        case MINT_F16: return go_product<DT_F16, false, false>(a, matrices, s);
-        case MINT_BF16: return go_product<DT_BF16, false, false>(a, matrices, s);
-        default: return go_product<DT_F32, false, false>(a, matrices, s);
+        case MINT_F16: return go_rows<DT_F16>(a, x_dtype, matrices, s);
+        case MINT_BF16: return go_rows<DT_BF16>(a, x_dtype, matrices, s);
+        default: return go_rows<DT_F32>(a, x_dtype, matrices, s);
     }
 }

@@ -27,6 +27,7 @@ struct Native {
     decltype(&mint_columns8_blocks) columns8_blocks;
     decltype(&mint_columns8) columns8;
     decltype(&mint_squares8) squares8;
+    decltype(&mint_product8_workspace) product8_workspace;
     decltype(&mint_product8) product8;
     decltype(&mint_combine) combine;
     decltype(&mint_combine_grad) combine_grad;
@@ -320,30 +321,22 @@ void scales_of(const Tensor& s, at::IntArrayRef size, const Tensor& q, const cha
 // the distance of neighbours along `dim`, 0 where there are none
 int64_t apart(const Tensor& t, int64_t dim) { return t.numel() && t.size(dim) > 1 ? t.stride(dim) : 0; }
 
-struct Rows8 {
-    Tensor q, scale;             // q (rows, whole blocks) bytes; scale (blocks, rows)
-};
-Rows8 rounded_rows(const Tensor& x, const OnDevice& on) {
-    const int64_t rows = x.size(0), per_row = blocks(x.size(1));
-    Rows8 r = {empty(x, {rows, per_row * 128}, at::kByte), empty(x, {per_row, rows}, at::kFloat)};
-    const int dtype = code_of(x.scalar_type(), "x");
-    launch("mint_rows8", [&] {
-        return native.rows8(x.data_ptr(), x.stride(0), (uint64_t)rows, (uint64_t)x.size(1), dtype, r.q.data_ptr(), per_row * 128,
-                            r.scale.data_ptr(), 1, rows, on.stream);
-    });
-    return r;
-}
-
 // quantise(x): 8-bit numbers and scales by rows
 PyObject* host_quantise(PyObject*, PyObject* const* list, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         const Args a(list, n, 1);
         const Tensor& x = a.tensor(0, "x");
         rows_of(x, "x");
-        code_of(x.scalar_type(), "x");
+        const int dtype = code_of(x.scalar_type(), "x");
+        const int64_t rows = x.size(0), wide = blocks(x.size(1)) * 128;
         OnDevice on(x.get_device());
-        const Rows8 r = rounded_rows(x, on);
-        return pack({wrap(r.q.view(at::ScalarType::Float8_e4m3fn).narrow(1, 0, x.size(1))), wrap(r.scale.t())});
+        // (scales of a block side by side: products read them for many rows and one block at a time)
+        const Tensor q = empty(x, {rows, wide}, at::kByte), scale = empty(x, {wide / 128, rows}, at::kFloat);
+        launch("mint_rows8", [&] {
+            return native.rows8(x.data_ptr(), x.stride(0), (uint64_t)rows, (uint64_t)x.size(1), dtype, q.data_ptr(), wide, scale.data_ptr(), 1, rows,
+                                on.stream);
+        });
+        return pack({wrap(q.view(at::ScalarType::Float8_e4m3fn).narrow(1, 0, x.size(1))), wrap(scale.t())});
     });
 }
 
@@ -435,21 +428,17 @@ PyObject* host_product(PyObject*, PyObject* const* list, Py_ssize_t n) {
         }
         OnDevice on(x.get_device());
         const Tensor out = given ? a.tensor(8, "out") : empty(x, {rows, cols}, type_of(code));
-        Rows8 r;
+        op.x = address(x);
         if (already) {
             const Tensor& sx = a.tensor(1, "x's scale");
-            op.x = address(x);
+            op.x_dtype = MINT_BYTES;
             op.x_stride = apart(x, 0);
             op.sx = address(sx);
             op.sx_row = sx.stride(0);
             op.sx_block = sx.stride(1);
         } else {
-            r = rounded_rows(x, on);
-            op.x = address(r.q);
-            op.x_stride = r.q.stride(0);
-            op.sx = address(r.scale);
-            op.sx_row = 1;
-            op.sx_block = x.size(0);
+            op.x_dtype = code_of(x.scalar_type(), "x");
+            op.x_stride = x.stride(0);
         }
         op.dtype = (int32_t)code;
         op.w = address(w);
@@ -463,6 +452,11 @@ PyObject* host_product(PyObject*, PyObject* const* list, Py_ssize_t n) {
         op.out_stride = rows > 1 ? out.stride(0) : cols;
         op.sw_row = sw.stride(d - 2);
         op.sw_block = sw.stride(d - 1);
+        Tensor room;
+        if ((op.workspace_bytes = native.product8_workspace(&op))) {
+            room = empty(x, {(int64_t)op.workspace_bytes}, at::kByte);
+            op.workspace = address(room);
+        }
         launch("mint_product8", [&] { return native.product8(&op, on.stream); });
         if (given) return Py_NewRef(list[8]);
         return wrap(out);
@@ -508,6 +502,7 @@ PyObject* host_weight_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
         });
         mint_product_op op = {};
         op.kind = MINT_PRODUCT_GRADIENT;
+        op.x_dtype = MINT_BYTES;
         op.dtype = (int32_t)code;
         op.x = address(dq);
         op.w = address(xq);
@@ -609,13 +604,13 @@ PyObject* host_combine_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
 // bind(check, addresses in the order of Native's)
 PyObject* host_bind(PyObject*, PyObject* const* list, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        const Args a(list, n, 12);
-        void* p[11];
-        for (int i = 0; i < 11; ++i) {
+        constexpr int count = offsetof(Native, check) / sizeof(void*);
+        const Args a(list, n, 1 + count);
+        void* p[count];
+        for (int i = 0; i < count; ++i) {
             p[i] = PyLong_AsVoidPtr(list[1 + i]);
             if (!p[i] && PyErr_Occurred()) throw Raised();
         }
-        static_assert(offsetof(Native, check) == sizeof(p), "addresses one after the other");
         memcpy(&native, p, sizeof(p));
         Py_INCREF(list[0]);
         Py_XSETREF(native.check, list[0]);
