@@ -568,8 +568,9 @@ int mint_squares8(const void* w, int64_t w_matrix, int64_t w_stride, uint32_t ma
  *                          blocks.  With `offsets` (experts' rows among group_rows, as for
  *                          mint_columns8) there are `experts` results out_matrix
  *                          elements apart, each the sum over its expert's blocks
- * Both matrices start at multiples of 16 bytes, and so do their rows; nothing
- * behind a row's depth is read. */
+ * Both matrices start at multiples of 16 bytes, and so do their rows; what lies
+ * behind a row's depth changes nothing (and is not read beyond the 16 bytes that
+ * the row ends in). */
 typedef enum { MINT_PRODUCT_ROWS = 0, MINT_PRODUCT_GRADIENT = 1 } mint_product_kind;
 typedef struct {
     int32_t kind;          /* mint_product_kind */

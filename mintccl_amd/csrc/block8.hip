@@ -24,8 +24,24 @@ __device__ __forceinline__ uint32_t pack8(float a, float b, float c, float d) {
     int v = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, v, true);
 }
-// max |v| of numbers of which one may be a NaN, which then it is
-__device__ __forceinline__ float larger(float a, float b) { return a > b || a != a ? a : b; }
+// Magnitudes are compared as the whole numbers that they are in memory: of a NaN and a number the NaN is larger, and stays.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// the largest of the 16 lanes of a row
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = max(v, dpp<0xB1, 0xf>(v, 0u));
+    v = max(v, dpp<0x4E, 0xf>(v, 0u));
+    v = max(v, dpp<0x141, 0xf>(v, 0u));
+    return max(v, dpp<0x140, 0xf>(v, 0u));
+}
+// 16 lanes' 8 numbers each, a block of 128, in 8 bits; the scale comes back
+__device__ __forceinline__ float round_block(const float (&v)[8], u32x2& q) {
+    uint32_t most = __float_as_uint(kLeastBlock);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, magnitude(v[i]));
+    const float m = __uint_as_float(row_max(most)), r = kLargest8 / m;
+    q = u32x2{pack8(v[0] * r, v[1] * r, v[2] * r, v[3] * r), pack8(v[4] * r, v[5] * r, v[6] * r, v[7] * r)};
+    return m / kLargest8;
+}
 
 // ---- groups of rows --------------------------------------------------------------
 // Rows [offsets[e], offsets[e + 1]) are expert e's; tiles of `rows` rows do not reach over experts.
@@ -68,9 +84,9 @@ __device__ __forceinline__ Tile find_tile(const Groups& g, uint32_t t, uint32_t 
     Tile r = {0, 0, 0, g.rows, true};
     if (!g.offsets) return r;
     uint32_t base = 0;
-    for (uint32_t e0 = 0; e0 < g.experts + rest; e0 += 64) {
+    for (uint32_t e0 = 0; e0 < g.experts; e0 += 64) {
         uint32_t begin, end;
-        const uint32_t tiles = tiles_of(g, e0 + lane_id(), tile_rows, rest, begin, end), sum = sum_below(tiles);
+        const uint32_t tiles = tiles_of(g, e0 + lane_id(), tile_rows, false, begin, end), sum = sum_below(tiles);
         const uint64_t behind = __ballot(base + sum > t);
         if (behind) {
             const int at = __builtin_ctzll(behind);
@@ -82,7 +98,10 @@ __device__ __forceinline__ Tile find_tile(const Groups& g, uint32_t t, uint32_t 
         }
         base += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
     }
-    r.found = false;
+    r.expert = g.experts;
+    r.first = base;
+    r.begin = row_bound(g, g.experts);
+    r.found = rest && t - base < (r.end - r.begin + tile_rows - 1) / tile_rows;
     return r;
 }
 
@@ -103,15 +122,10 @@ __global__ void __launch_bounds__(256) rows8_kernel(RowsArgs a) {
     if (row >= a.rows) return;
     float v[8];
     load_elements<DT, 8>(static_cast<const T*>(a.x) + row * a.x_stride + at, a.whole && at + 8 <= a.depth, (int64_t)a.depth - at, v);
-    float m = kLeastBlock;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = larger(fabsf(v[i]), m);
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) m = larger(__shfl_xor(m, d), m);
-    const float r = kLargest8 / m;
-    const u32x2 w = {pack8(v[0] * r, v[1] * r, v[2] * r, v[3] * r), pack8(v[4] * r, v[5] * r, v[6] * r, v[7] * r)};
-    *(MINT_GLOBAL u32x2*)as_global(a.q + row * a.q_stride + at) = w;
-    if ((threadIdx.x & 15u) == 0) a.scale[row * a.s_row + block * a.s_block] = m / kLargest8;
+    u32x2 q;
+    const float scale = round_block(v, q);
+    *(MINT_GLOBAL u32x2*)as_global(a.q + row * a.q_stride + at) = q;
+    if ((threadIdx.x & 15u) == 0) a.scale[row * a.s_row + block * a.s_block] = scale;
 }
 
 struct ColumnsArgs {
@@ -128,16 +142,16 @@ template <int DT>
 __global__ void __launch_bounds__(256) columns8_kernel(ColumnsArgs a) {
     using T = typename Elem<DT>::type;
     __shared__ __attribute__((aligned(16))) uint8_t turned[64][128 + 16];
-    __shared__ float most[4][64];
+    __shared__ uint32_t most[4][64];
     const uint32_t block = blockIdx.x, c0 = blockIdx.y * 64;
     const Tile t = find_tile(a.groups, block, 128, false);
     if (!t.found) return;
     const uint32_t r0 = t.begin + (block - t.first) * 128;
     const uint32_t vec = threadIdx.x & 7u, first = threadIdx.x >> 3, col = c0 + vec * 8;      // rows first + 32 i
     float v[4][8];
-    float m[8];
+    uint32_t m[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m[j] = kLeastBlock;
+    for (int j = 0; j < 8; ++j) m[j] = __float_as_uint(kLeastBlock);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint32_t row = r0 + first * 4 + i;
@@ -151,19 +165,19 @@ __global__ void __launch_bounds__(256) columns8_kernel(ColumnsArgs a) {
         if (there)
             load_elements<DT, 8>(static_cast<const T*>(a.x) + row * a.x_stride + col, a.whole && col + 8 <= a.width, (int64_t)a.width - col, v[i]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m[j] = larger(fabsf(v[i][j]), m[j]);
+        for (int j = 0; j < 8; ++j) m[j] = max(m[j], magnitude(v[i][j]));
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
 #pragma unroll
-        for (int d = 8; d < 64; d <<= 1) m[j] = larger(__shfl_xor(m[j], d), m[j]);
+        for (int d = 8; d < 64; d <<= 1) m[j] = max(m[j], (uint32_t)__shfl_xor((int)m[j], d));
         if (lane_id() < 8) most[wave_in_block()][vec * 8 + j] = m[j];
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const uint32_t c = vec * 8 + j;
-        const float all = larger(larger(most[0][c], most[1][c]), larger(most[2][c], most[3][c]));
+        const float all = __uint_as_float(max(max(most[0][c], most[1][c]), max(most[2][c], most[3][c])));
         const float r = kLargest8 / all;
         *reinterpret_cast<uint32_t*>(&turned[c][first * 4]) = pack8(v[0][j] * r, v[1][j] * r, v[2][j] * r, v[3][j] * r);
         if (first == 0 && c0 + c < a.width) a.scale[(uint64_t)block * a.width + c0 + c] = all / kLargest8;
@@ -189,10 +203,11 @@ struct SquaresArgs {
 template <int DT>
 __global__ void __launch_bounds__(256) squares8_kernel(SquaresArgs a) {
     using T = typename Elem<DT>::type;
-    __shared__ float most[4];
+    __shared__ uint32_t most[4];
     const uint32_t square = blockIdx.x, matrix = blockIdx.y, r0 = square / a.blocks * 128 + threadIdx.x / 16, at = square % a.blocks * 128 + (threadIdx.x & 15u) * 8;
     const T* const w = static_cast<const T*>(a.w) + matrix * a.w_matrix;
-    float v[8][8], m = kLeastBlock;
+    float v[8][8];
+    uint32_t largest = __float_as_uint(kLeastBlock);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t row = r0 + 16 * i;
@@ -201,13 +216,12 @@ __global__ void __launch_bounds__(256) squares8_kernel(SquaresArgs a) {
         if (row < a.rows)
             load_elements<DT, 8>(w + row * a.w_stride + at, a.whole && at + 8 <= a.depth, (int64_t)a.depth - at, v[i]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m = larger(fabsf(v[i][j]), m);
+        for (int j = 0; j < 8; ++j) largest = max(largest, magnitude(v[i][j]));
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = larger(__shfl_xor(m, d), m);
-    if (lane_id() == 0) most[wave_in_block()] = m;
+    largest = wave_max(largest);
+    if (lane_id() == 0) most[wave_in_block()] = largest;
     __syncthreads();
-    m = larger(larger(most[0], most[1]), larger(most[2], most[3]));
+    const float m = __uint_as_float(max(max(most[0], most[1]), max(most[2], most[3])));
     const float r = kLargest8 / m;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -234,15 +248,29 @@ struct ProductArgs {
 // serves together (0 - 3, 12 - 15 and 20 - 27 of 32, then the others), each a row, fall on different banks. For that lane groups 0
 // and 1 (2 and 3) read pieces that differ in their lowest bit.
 __device__ __forceinline__ uint32_t turn(uint32_t row) { return (row >> 1) & 7u; }
-// Which column of the result a row of the weights in LDS stands for: of the 64 of a wavefront, the four that a lane
-// gets from each of four matrix instructions lie side by side.
-__device__ __forceinline__ uint32_t column_of(uint32_t row) { return (row & ~63u) | (row << 2 & 0x30u) | (row >> 2 & 0xCu) | (row & 3u); }
+// Which column of the result a row of the weights in LDS stands for: a lane gets four consecutive columns of a row from each of
+// four matrix instructions, and those of two lie side by side, so that the four lanes that have a row store 64 bytes together.
+__device__ __forceinline__ uint32_t column_of(uint32_t row) {
+    return (row & ~63u) | (row & 32u) | (row << 1 & 24u) | (row >> 2 & 4u) | (row & 3u);
+}
 
 __device__ __forceinline__ void to_lds16(const uint8_t* from, uint32_t lds) {
     __builtin_amdgcn_global_load_lds((MINT_GLOBAL const void*)as_global(from), (MINT_LDS void*)(uintptr_t)lds, 16, 0, 0);
 }
 __device__ __forceinline__ void to_lds4(const float* from, uint32_t lds) {
     __builtin_amdgcn_global_load_lds((MINT_GLOBAL const void*)as_global(from), (MINT_LDS void*)(uintptr_t)lds, 4, 0, 0);
+}
+// 16 bytes of a row of which the first `left` are there, zeros behind.  (A piece that begins in the row may be read
+// to its end: it is aligned, so it lies in the same page.)
+__device__ __forceinline__ u32x4 piece_of(const uint8_t* from, int32_t left) {
+    u32x4 v = {0, 0, 0, 0};
+    if (left > 0) v = *(MINT_GLOBAL const u32x4*)as_global(from);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int32_t bytes = left - 4 * i;
+        v[i] &= bytes >= 4 ? 0xFFFFFFFFu : bytes <= 0 ? 0u : (1u << 8 * bytes) - 1u;
+    }
+    return v;
 }
 __device__ __forceinline__ u32x4 lds16(uint32_t at) { return *(MINT_LDS const u32x4*)(uintptr_t)at; }
 __device__ __forceinline__ float lds_float(uint32_t at) { return *(MINT_LDS const float*)(uintptr_t)at; }
@@ -284,8 +312,7 @@ struct Operand<true> {
 
 // A thread block has BM rows and BN columns of the result, a wavefront 64 columns and BM / WM rows of them.
 // The depth goes by in blocks of 128: while one is multiplied the next one's bytes are on their way into the other half of LDS.
-// The weights are the matrix instruction's first operand, so a lane has four consecutive columns of one row for each,
-// and 16 with the four of a wavefront's columns dealt to the instructions in fours.
+// The weights are the matrix instruction's first operand, so a lane has consecutive columns of one row of the result (column_of).
 template <int OUT, int BM, int BN, int WM, bool ROWS_W, bool ALONG>
 __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArgs a) {
     using Op = Operand<OUT == DT_F32>;
@@ -381,19 +408,11 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
             from_w[n - XI] += 128;
         }
     };
-    // the last block of a depth that is no multiple of 128: nothing is read behind a row's end
+    // the last block of a depth that is no multiple of 128 (along the rows there is none)
     const auto bring_tail = [&](uint32_t at) MINT_INLINE_LAMBDA {
         const auto guarded = [&](const uint8_t* from, uint32_t r, uint32_t to) MINT_INLINE_LAMBDA {
             const int32_t left = (int32_t)(depth - full * 128) - (int32_t)((slot ^ turn(r)) * 16);
-            u32x4 v = {0, 0, 0, 0};
-            if (left >= 16) {
-                v = *(MINT_GLOBAL const u32x4*)as_global(from);
-            } else if (left > 0) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (i < left) v[i / 4] |= (uint32_t)*as_global(from + i) << (i % 4 * 8);
-            }
-            *(MINT_LDS u32x4*)(uintptr_t)(to + lane * 16) = v;
+            *(MINT_LDS u32x4*)(uintptr_t)(to + lane * 16) = piece_of(from, left);
         };
 #pragma unroll
         for (int i = 0; i < XI; ++i) guarded(from_x[i], (wave * XI + i) * 8 + sub, at + (wave * XI + i) * 1024);
@@ -411,26 +430,25 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
     const uint32_t r16 = lane & 15u, part = lane >> 4;
     const uint32_t xr = wm * (BM / WM) + r16, wr = wn * 64 + r16;
     const uint32_t x_at = xr * 128 + ((part ^ turn(xr)) * 16), w_at = kX + wr * 128 + ((part ^ turn(wr)) * 16);
-    const uint32_t sx_at = kX + kW + xr * 4, sw_at = kX + kW + kSx + (wn * 64 + part * 16) * 4;
+    const uint32_t sx_at = kX + kW + xr * 4, sw_at = kX + kW + kSx + (wn * 64 + part * 8) * 4;
     // The matrix instructions' sums are scaled and added LAG instructions later: the two units work side by side.
     constexpr int LAG = 3;
     const auto multiply = [&](uint32_t at, float sw, const auto& meanwhile) MINT_INLINE_LAMBDA {
         f32x4 sw4[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-            if (ROWS_W) sw4[j] = *(MINT_LDS const f32x4*)(uintptr_t)(at + sw_at + j * 16);
+            if (ROWS_W) sw4[j] = *(MINT_LDS const f32x4*)(uintptr_t)(at + sw_at + (j / 2 * 32 + j % 2 * 4) * 4);
         const uint32_t w0 = at + w_at, w1 = at + (w_at ^ 64u), x0 = at + x_at, x1 = at + (x_at ^ 64u);
         const Op w[NT] = {Op(piece(w0, w1)), Op(piece(w0 + 2048, w1 + 2048)), Op(piece(w0 + 4096, w1 + 4096)), Op(piece(w0 + 6144, w1 + 6144))};
         Op x(piece(x0, x1));
-        float s[MT];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) s[i] = lds_float(at + sx_at + i * 64) * sw;
+        static_assert(LAG <= NT, "sums of this row and the one before");
+        float s[2], next_s = lds_float(at + sx_at);      // of this row of products, and of those whose sums are still to be added
         __builtin_amdgcn_sched_barrier(0);
         f32x4 d[LAG + 1];
         const auto add = [&](int n) MINT_INLINE_LAMBDA {
             const int i = n / NT, j = n % NT;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(d[n % (LAG + 1)][k], ROWS_W ? s[i] * sw4[j][k] : s[i], acc[i][j][k]);
+            for (int k = 0; k < 4; ++k) acc[i][j][k] = fmaf(d[n % (LAG + 1)][k], ROWS_W ? s[i % 2] * sw4[j][k] : s[i % 2], acc[i][j][k]);
         };
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -440,7 +458,11 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
             for (int n = 0; n < PIECES; ++n)
                 if (i * PIECES + n < XI + WI) meanwhile(i * PIECES + n);
             Op next = x;
-            if (i + 1 < MT) next = Op(piece(x0 + (i + 1) * 2048, x1 + (i + 1) * 2048));
+            s[i % 2] = next_s * sw;
+            if (i + 1 < MT) {
+                next = Op(piece(x0 + (i + 1) * 2048, x1 + (i + 1) * 2048));
+                next_s = lds_float(at + sx_at + (i + 1) * 64);
+            }
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int n = i * NT + j;
@@ -457,7 +479,7 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
     if (steps) {
         uint32_t b = 0, at = base;
         const auto scale_of = [&]() MINT_INLINE_LAMBDA { return ROWS_W ? 1.0f : sw_block[(int64_t)b * a.sw_block]; };
-        if (full) {
+        if (ALONG || full) {
 #pragma unroll
             for (int n = 0; n < XI + WI; ++n) bring(at, n);
         } else {
@@ -474,143 +496,161 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
             const float sw = scale_of();
             const uint32_t other = base + base + kStage - at;
             __syncthreads();
-            if (b + 1 < steps) bring_tail(other);
+            if (!ALONG && b + 1 < steps) bring_tail(other);
             multiply(at, sw, [](int) MINT_INLINE_LAMBDA {});
             at = other;
         }
     }
 
     T* const out = static_cast<T*>(a.out) + (ALONG ? (int64_t)expert * a.out_matrix : 0);
-    const uint32_t col = n0 + wn * 64 + part * 16;
+    const uint32_t col = n0 + wn * 64 + part * 8;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const uint32_t row = m0 + xr + i * 16;
-        if (row >= m_end || col >= a.cols) continue;
-        T* const to = out + (int64_t)row * a.out_stride + col;
+        if (row >= m_end) continue;
+        T* const to = out + (int64_t)row * a.out_stride;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = acc[i][h * 2 + k / 4][k % 4];
-            if (col + h * 8 < a.cols) store_elements<OUT, 8>(to + h * 8, a.out_whole && col + h * 8 + 8 <= a.cols, (int64_t)a.cols - (col + h * 8), v);
+            const uint32_t c = col + h * 32;
+            if (c < a.cols) store_elements<OUT, 8>(to + c, a.out_whole && c + 8 <= a.cols, (int64_t)a.cols - c, v);
         }
     }
 }
 
 // ---- products of few rows ------------------------------------------------------------
-// Bound by reading the weights: 16 MT rows need them once.  A thread block has 16 columns, and its wavefronts every
-// WAVES-th block of the depth, straight from memory into registers: a wavefront asks for AHEAD blocks before
-// it multiplies the first, which is what keeps enough bytes on their way.  The wavefronts' sums are added up in LDS, in
-// their order.  Activations that are not in 8 bits yet (X) are rounded on the way: each thread block does that again, but it is less than
-// another launch takes.
-typedef uint32_t u32x4_near __attribute__((ext_vector_type(4), aligned(4)));
-constexpr int kThinWaves = 8, kThinAhead = 4;
+// Bound by reading the weights: 16 MT rows need them once.  A wavefront has 16 columns and every KWAYS-th block of the
+// depth, straight from memory into registers: it asks for AHEAD blocks before it multiplies the first, which is what
+// keeps enough bytes on their way.  The KWAYS wavefronts' sums of a column are added up in LDS, in their order.
+// Activations that are not in 8 bits yet (X) are rounded by the thread block, CHUNK numbers of each row at a time, while the first weights
+// travel, and read from LDS: every thread block does that again, but it takes less than another launch.
+constexpr int kThinWaves = 8;
 
-// 32 bytes of a row of 8-bit numbers, `left` of them there
-__device__ __forceinline__ i32x8 eight_bits(const uint8_t* from, int32_t left) {
-    u32x4 v[2] = {};
-    if (left >= 32) {
-        v[0] = *(MINT_GLOBAL const u32x4*)as_global(from);
-        v[1] = *(MINT_GLOBAL const u32x4*)as_global(from + 16);
-    } else {
+// The 32 bytes that a lane has of a block of a row: 16 from `part` * 16 on, and 16 from there + 64 on (the four lanes of
+// a row read 64 bytes together).
+struct Strip {
+    u32x4 v[2];
+    // `left` bytes of the row from `from` (the lane's first) on
+    __device__ __forceinline__ void load(const uint8_t* from, bool whole, int32_t left) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < left) v[i / 16][i / 4 % 4] |= (uint32_t)*as_global(from + i) << (i % 4 * 8);
+        for (int k = 0; k < 2; ++k) {
+            if (whole) v[k] = *(MINT_GLOBAL const u32x4*)as_global(from + k * 64);
+            else v[k] = piece_of(from + k * 64, left - k * 64);
+        }
     }
-    return i32x8{(int)v[0].x, (int)v[0].y, (int)v[0].z, (int)v[0].w, (int)v[1].x, (int)v[1].y, (int)v[1].z, (int)v[1].w};
-}
+    __device__ __forceinline__ i32x8 bits() const {
+        return i32x8{(int)v[0].x, (int)v[0].y, (int)v[0].z, (int)v[0].w, (int)v[1].x, (int)v[1].y, (int)v[1].z, (int)v[1].w};
+    }
+};
 
 // X: the activations' type, DT_BYTES if they are in 8 bits
-template <int OUT, int X, int MT>
-__global__ void __launch_bounds__(64 * kThinWaves) thin_kernel(ProductArgs a) {
+template <int OUT, int X, int MT, int KWAYS>
+__global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a) {
     using Op = Operand<OUT == DT_F32>;
     using T = typename Elem<OUT>::type;
-    constexpr int WAVES = kThinWaves, AHEAD = kThinAhead, BM = 16 * MT;
     constexpr bool ROUND = X != DT_BYTES;
-    using TX = typename Elem<ROUND ? X : DT_F32>::type;
+    constexpr int WAVES = kThinWaves, BM = 16 * MT, BN = 16 * (WAVES / KWAYS), AHEAD = 4 / MT;
+    constexpr uint32_t CHUNK = 32, XROW = CHUNK * 128 + 16;         // blocks; bytes of a row in LDS
+    static_assert(!ROUND || MT == 1, "rounded rows fit LDS");
     __shared__ float sums[WAVES][BM][17];
+    __shared__ __attribute__((aligned(16))) uint8_t xs[ROUND ? 16 * XROW : 16];
+    __shared__ float xscale[ROUND ? CHUNK : 1][16];
     const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), r16 = lane & 15u, part = lane >> 4;
-    const uint32_t row_tile = blockIdx.x / a.col_tiles, n0 = blockIdx.x % a.col_tiles * 16;
+    const uint32_t way = wave % KWAYS, row_tile = blockIdx.x / a.col_tiles, n0 = blockIdx.x % a.col_tiles * BN, n = n0 + wave / KWAYS * 16;
     const Tile t = find_tile(a.groups, row_tile, BM, true);
     if (!t.found) return;
     const uint32_t m0 = t.begin + (row_tile - t.first) * BM, rows = min(t.end - m0, (uint32_t)BM);
     const uint32_t steps = a.groups.offsets && t.expert == a.groups.experts ? 0u : (a.depth + 127) / 128;
-    const int32_t depth = (int32_t)a.depth;
 
     f32x4 acc[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
-    if (wave < steps) {
-        const uint8_t* const w = a.w + (int64_t)t.expert * a.w_matrix + (int64_t)min(n0 + r16, a.cols - 1) * a.w_stride + part * 32;
-        const float* const sw = a.sw + (int64_t)t.expert * a.sw_matrix + (int64_t)(n0 / 128) * a.sw_row;
-        uint32_t row[MT];
-        bool there[MT];
+    const auto x_row = [&](uint32_t i) MINT_INLINE_LAMBDA {
+        uint32_t row = m0 + min(i, rows - 1);       // (lanes beyond the last row have that one too: what they make is not stored)
+        if (a.tokens) row = (uint32_t)a.tokens[row];
+        return min(row, a.x_rows - 1);
+    };
+    const uint8_t* const w = a.w + (int64_t)t.expert * a.w_matrix + (int64_t)min(n + r16, a.cols - 1) * a.w_stride + part * 16;
+    const float* const sw = a.sw + (int64_t)t.expert * a.sw_matrix + (int64_t)(min(n, a.cols - 1) / 128) * a.sw_row;
+    uint32_t row[MT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            there[i] = i * 16 + r16 < rows;
-            row[i] = m0 + min(i * 16 + r16, rows - 1);
-            if (a.tokens) row[i] = (uint32_t)a.tokens[row[i]];
-            row[i] = min(row[i], a.x_rows - 1);
-        }
-        for (uint32_t b0 = wave; b0 < steps; b0 += WAVES * AHEAD) {
-            i32x8 wv[AHEAD];
+    for (int i = 0; i < MT; ++i) row[i] = ROUND || !steps ? 0u : x_row(i * 16 + r16);
+
+    // blocks of the depth from `first` on, CHUNK of them at most where they are rounded here
+    for (uint32_t first = 0; first < steps; first += CHUNK) {
+        const uint32_t end = ROUND ? min(first + CHUNK, steps) : steps;
+        for (uint32_t b0 = first + way, round = 0; b0 < end || (ROUND && round == 0); b0 += KWAYS * AHEAD, ++round) {
+            Strip wv[AHEAD], xv[AHEAD][MT];
+            float s_x[AHEAD][MT], s_w[AHEAD];
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const uint32_t b = b0 + u * WAVES;
-                if (b < steps) wv[u] = eight_bits(w + b * 128, depth - (int32_t)(b * 128 + part * 32));
+                // (in the place of a block behind the last the first is asked for again, and not multiplied)
+                const uint32_t b = min(b0 + u * KWAYS < end ? b0 + u * KWAYS : b0, end - 1), at = b * 128 + part * 16;
+                const bool whole = b * 128 + 128 <= a.depth;
+                const int32_t left = (int32_t)a.depth - (int32_t)at;
+                wv[u].load(w + b * 128, whole, left);
+                s_w[u] = sw[(int64_t)b * a.sw_block];
+                if constexpr (!ROUND) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        xv[u][i].load(a.x + (int64_t)row[i] * a.x_stride + at, whole, left);
+                        s_x[u][i] = a.sx[(int64_t)row[i] * a.sx_row + (int64_t)b * a.sx_block];
+                    }
+                }
+            }
+            if constexpr (ROUND) {
+                if (round == 0) {
+                    if (first) __syncthreads();          // (all are done with the chunk before)
+                    using TX = typename Elem<X>::type;
+                    const uint32_t blocks = end - first;
+                    for (uint32_t unit = threadIdx.x / 16; unit < rows * blocks; unit += WAVES * 4) {
+                        const uint32_t i = unit / blocks, b = unit % blocks, at = (first + b) * 128 + r16 * 8;
+                        float v[8];
+                        load_elements<X, 8>(reinterpret_cast<const TX*>(a.x) + (int64_t)x_row(i) * a.x_stride + at, a.x_whole && at + 8 <= a.depth,
+                                            (int64_t)a.depth - at, v);
+                        u32x2 q;
+                        const float s = round_block(v, q);
+                        *reinterpret_cast<u32x2*>(xs + i * XROW + b * 128 + r16 * 8) = q;
+                        if (r16 == 0) xscale[b][i] = s;
+                    }
+                    __syncthreads();
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; ++u) {
+                    const uint32_t b = min(b0 + u * KWAYS < end ? b0 + u * KWAYS : b0, end - 1) - first;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) xv[u][0].v[k] = *reinterpret_cast<const u32x4*>(xs + r16 * XROW + b * 128 + part * 16 + k * 64);
+                    s_x[u][0] = xscale[b][r16];
+                }
             }
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const uint32_t b = b0 + u * WAVES;
-                if (b >= steps) break;
-                const int32_t left = depth - (int32_t)(b * 128 + part * 32);
-                const float s_w = sw[(int64_t)b * a.sw_block];
-                const Op wo(wv[u]);
+                if (b0 + u * KWAYS >= end) break;
+                const Op wo(wv[u].bits());
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    i32x8 xv = {};
-                    float s = 0.0f;
-                    if constexpr (ROUND) {
-                        float v[32], m = kLeastBlock;
-                        const TX* const from = reinterpret_cast<const TX*>(a.x) + (int64_t)row[i] * a.x_stride + b * 128 + part * 32;
+                    const f32x4 d = Op::multiply(wo, Op(xv[u][i].bits()));
+                    const float s = s_x[u][i] * s_w[u];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            float e[8] = {};
-                            if (there[i]) load_elements<X, 8>(from + k * 8, a.x_whole && left >= k * 8 + 8, left - k * 8, e);
-#pragma unroll
-                            for (int h = 0; h < 8; ++h) {
-                                v[k * 8 + h] = e[h];
-                                m = larger(fabsf(e[h]), m);
-                            }
-                        }
-                        m = larger(__shfl_xor(m, 16), m);
-                        m = larger(__shfl_xor(m, 32), m);
-                        const float r = kLargest8 / m;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) xv[k] = (int)pack8(v[k * 4] * r, v[k * 4 + 1] * r, v[k * 4 + 2] * r, v[k * 4 + 3] * r);
-                        s = m / kLargest8;
-                    } else if (there[i]) {
-                        xv = eight_bits(a.x + (int64_t)row[i] * a.x_stride + b * 128 + part * 32, left);
-                        s = a.sx[(int64_t)row[i] * a.sx_row + (int64_t)b * a.sx_block];
-                    }
-                    const f32x4 d = Op::multiply(wo, Op(xv));
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[i][k] = fmaf(d[k], s * s_w, acc[i][k]);
+                    for (int k = 0; k < 4; ++k) acc[i][k] = fmaf(d[k], s, acc[i][k]);
                 }
             }
         }
+        if (!ROUND) break;
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) sums[wave][i * 16 + r16][part * 4 + k] = acc[i][k];
     __syncthreads();
-    for (uint32_t at = threadIdx.x; at < BM * 16; at += 64 * WAVES) {
-        const uint32_t m = at / 16, n = at % 16;
+    for (uint32_t at = threadIdx.x; at < BM * BN; at += 64 * WAVES) {
+        const uint32_t m = at / BN, c = at % BN;
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) sum += sums[i][m][n];
-        if (m < rows && n0 + n < a.cols) *as_global(static_cast<T*>(a.out) + (int64_t)(m0 + m) * a.out_stride + n0 + n) = Elem<OUT>::round(sum);
+        for (int i = 0; i < KWAYS; ++i) sum += sums[c / 16 * KWAYS + i][m][c % 16];
+        if (m < rows && n0 + c < a.cols) *as_global(static_cast<T*>(a.out) + (int64_t)(m0 + m) * a.out_stride + n0 + c) = Elem<OUT>::round(sum);
     }
 }
 
@@ -647,12 +687,19 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
 bool few_rows(uint64_t rows, uint32_t matrices) { return rows <= 64ull * matrices; }
 // ... and so few that the rounding is done on the way
 bool rounded_on_the_way(uint64_t rows, uint32_t matrices) { return rows <= 16ull * matrices; }
-template <int OUT, int X, int MT>
-int go_thin(ProductArgs a, hipStream_t stream) {
-    a.col_tiles = (uint32_t)ceil_div(a.cols, 16);
+template <int OUT, int X, int MT, int KWAYS>
+int go_thin_ways(ProductArgs a, hipStream_t stream) {
+    a.col_tiles = (uint32_t)ceil_div(a.cols, 16 * (kThinWaves / KWAYS));
     const uint64_t blocks = most_row_tiles(a, 16 * MT) * a.col_tiles;
     if (blocks > 0x7FFFFFFFull / (64 * kThinWaves)) return MINT_ERR_TOO_LARGE;
-    return Launch<&thin_kernel<OUT, X, MT>>::go((uint32_t)blocks, 64 * kThinWaves, 0, stream, a);
+    return Launch<&thin_kernel<OUT, X, MT, KWAYS>>::go((uint32_t)blocks, 64 * kThinWaves, 0, stream, a);
+}
+// The depth is dealt to eight wavefronts where 16 columns to a thread block leave few of those, else to two.
+template <int OUT, int X, int MT>
+int go_thin(const ProductArgs& a, hipStream_t stream) {
+    const uint64_t blocks = (ceil_div(a.rows, 16 * MT) + (a.groups.offsets ? a.groups.experts / 2 : 0)) * ceil_div(a.cols, 16);
+    if (blocks <= 768) return go_thin_ways<OUT, X, MT, 8>(a, stream);
+    return go_thin_ways<OUT, X, MT, 2>(a, stream);
 }
 template <int OUT>
 int go_rows(const ProductArgs& a, int x_dtype, uint32_t matrices, hipStream_t stream) {
