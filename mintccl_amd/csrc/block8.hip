@@ -67,11 +67,12 @@ __device__ __forceinline__ uint32_t tiles_of(const Groups& g, uint32_t e, uint32
     return (end - begin + tile_rows - 1) / tile_rows;
 }
 __device__ __forceinline__ uint32_t sum_below(uint32_t v) {       // of the lanes up to this one
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t other = (uint32_t)__shfl_up((int)v, d);
-        v += lane_id() >= d ? other : 0u;
-    }
+    v += dpp<0x111, 0xf>(v, 0u);        // row_shr:1, 2, 4, 8
+    v += dpp<0x112, 0xf>(v, 0u);
+    v += dpp<0x114, 0xf>(v, 0u);
+    v += dpp<0x118, 0xf>(v, 0u);
+    v += dpp<0x142, 0xa>(v, 0u);        // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xc>(v, 0u);        // row_bcast:31 into rows 2 and 3
     return v;
 }
 __device__ __forceinline__ uint32_t count_tiles(const Groups& g, uint32_t tile_rows, bool rest) {
@@ -310,17 +311,31 @@ struct Operand<true> {
     }
 };
 
+// All but the N latest of a wavefront's loads are done; then all wavefronts meet.
+template <int N>
+__device__ __forceinline__ void meet() {
+    if constexpr (N == 0) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);
+        compiler_fence();
+        __builtin_amdgcn_s_barrier();
+        compiler_fence();
+    }
+}
+
 // A thread block has BM rows and BN columns of the result, a wavefront 64 columns and BM / WM rows of them.
-// The depth goes by in blocks of 128: while one is multiplied the next one's bytes are on their way into the other half of LDS.
+// The depth goes by in blocks of 128: while one is multiplied the next STAGES - 1 ones' bytes are on their way into LDS.  One ahead
+// is enough where a block's products take longer than its bytes; many are needed where they do not (few tiles, small ones).
 // The weights are the matrix instruction's first operand, so a lane has consecutive columns of one row of the result (column_of).
-template <int OUT, int BM, int BN, int WM, bool ROWS_W, bool ALONG>
+template <int OUT, int BM, int BN, int WM, int STAGES, bool ROWS_W, bool ALONG>
 __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArgs a) {
     using Op = Operand<OUT == DT_F32>;
     using T = typename Elem<OUT>::type;
     constexpr int WN = BN / 64, WAVES = WM * WN, MT = BM / WM / 16, NT = 4;
-    constexpr uint32_t kX = BM * 128, kW = BN * 128, kSx = BM * 4, kSw = ROWS_W ? BN * 4 : 0, kStage = kX + kW + kSx + kSw;
+    constexpr uint32_t kX = BM * 128, kW = BN * 128, kSx = BM * 4, kSw = ROWS_W ? BN * 4 : 256, kStage = kX + kW + kSx + kSw;
     static_assert(BM / 64 <= WAVES && BN / 64 <= WAVES, "a wavefront for each 64 scales");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
     const uint32_t base = (uint32_t)(uintptr_t)(MINT_LDS uint8_t*)lds;
     const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), wm = wave / WN, wn = wave % WN;
 
@@ -362,7 +377,7 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
     // A wavefront brings 8 rows of 128 bytes with an instruction: the rows it has of x, then of the weights.
     constexpr int XI = BM / 8 / WAVES, WI = BN / 8 / WAVES;
     const uint8_t *from_x[XI], *from_w[WI];
-    const float *from_sx = nullptr, *from_sw = nullptr, *sw_block = nullptr;
+    const float *from_sx = nullptr, *from_sw = nullptr;
     const uint32_t sub = lane >> 3, slot = lane & 7u;
     const auto x_row = [&](uint32_t r) MINT_INLINE_LAMBDA {
         uint32_t row = min(m0 + r, m_end ? m_end - 1 : 0u);
@@ -381,19 +396,21 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
             const uint32_t r = (wave * WI + i) * 8 + sub;
             from_w[i] = w0 + (int64_t)min(n0 + column_of(r), a.cols - 1) * a.w_stride + depth0 + ((slot ^ turn(r)) * 16);
         }
-        if (wave < BM / 64) from_sx = a.sx + (int64_t)x_row(wave * 64 + lane) * a.sx_row + (int64_t)(depth0 / 128) * a.sx_block;
-        if (ROWS_W && wave < BN / 64)
-            from_sw = a.sw + (int64_t)min(n0 + wave * 64 + lane, a.cols - 1) * a.sw_row + (int64_t)(depth0 / 128) * a.sw_block;
-        if (!ROWS_W)                         // one number for 128 columns
-            sw_block = a.sw + (int64_t)expert * a.sw_matrix + (int64_t)(min(n0 + wn * 64, a.cols - 1) / 128) * a.sw_row;
+        from_sx = a.sx + (int64_t)x_row(wave % (BM / 64) * 64 + lane) * a.sx_row + (int64_t)(depth0 / 128) * a.sx_block;
+        // (of a weight matrix lane i has the scale of the columns of wavefront i)
+        const uint32_t col = min(n0 + (ROWS_W ? wave % (BN / 64) * 64 + lane : lane * 64), a.cols - 1);
+        from_sw = a.sw + (ROWS_W ? (int64_t)col * a.sw_row + (int64_t)(depth0 / 128) * a.sw_block
+                                 : (int64_t)expert * a.sw_matrix + (int64_t)(col / 128) * a.sw_row);
     }
+    // Where loads are counted (STAGES > 2) all wavefronts have the same number of them under way: some bring scales that others bring too.
+    constexpr int LOADS = XI + WI + 2;
     const auto bring_scales = [&](uint32_t at) MINT_INLINE_LAMBDA {
-        if (wave < BM / 64) {
-            to_lds4(from_sx, at + kX + kW + wave * 256);
+        if (STAGES > 2 || wave < BM / 64) {
+            to_lds4(from_sx, at + kX + kW + wave % (BM / 64) * 256);
             from_sx += a.sx_block;
         }
-        if (ROWS_W && wave < BN / 64) {
-            to_lds4(from_sw, at + kX + kW + kSx + wave * 256);
+        if (STAGES > 2 || (ROWS_W ? wave < BN / 64 : wave == WAVES - 1)) {
+            to_lds4(from_sw, at + kX + kW + kSx + (ROWS_W ? wave % (BN / 64) * 256 : 0));
             from_sw += a.sw_block;
         }
     };
@@ -430,10 +447,10 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
     const uint32_t r16 = lane & 15u, part = lane >> 4;
     const uint32_t xr = wm * (BM / WM) + r16, wr = wn * 64 + r16;
     const uint32_t x_at = xr * 128 + ((part ^ turn(xr)) * 16), w_at = kX + wr * 128 + ((part ^ turn(wr)) * 16);
-    const uint32_t sx_at = kX + kW + xr * 4, sw_at = kX + kW + kSx + (wn * 64 + part * 8) * 4;
+    const uint32_t sx_at = kX + kW + xr * 4, sw_at = kX + kW + kSx + (ROWS_W ? wn * 64 + part * 8 : wn) * 4;
     // The matrix instructions' sums are scaled and added LAG instructions later: the two units work side by side.
     constexpr int LAG = 3;
-    const auto multiply = [&](uint32_t at, float sw, const auto& meanwhile) MINT_INLINE_LAMBDA {
+    const auto multiply = [&](uint32_t at, const auto& meanwhile) MINT_INLINE_LAMBDA {
         f32x4 sw4[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -442,6 +459,7 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
         const Op w[NT] = {Op(piece(w0, w1)), Op(piece(w0 + 2048, w1 + 2048)), Op(piece(w0 + 4096, w1 + 4096)), Op(piece(w0 + 6144, w1 + 6144))};
         Op x(piece(x0, x1));
         static_assert(LAG <= NT, "sums of this row and the one before");
+        const float sw = ROWS_W ? 1.0f : lds_float(at + sw_at);
         float s[2], next_s = lds_float(at + sx_at);      // of this row of products, and of those whose sums are still to be added
         __builtin_amdgcn_sched_barrier(0);
         f32x4 d[LAG + 1];
@@ -453,7 +471,7 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             // (the next block's loads go out between the products: all at once they would stand in each other's way)
-            constexpr int PIECES = (XI + WI) * 2 / MT;
+            constexpr int PIECES = MT > 1 ? ((XI + WI) * 2 + MT - 1) / MT : XI + WI;
 #pragma unroll
             for (int n = 0; n < PIECES; ++n)
                 if (i * PIECES + n < XI + WI) meanwhile(i * PIECES + n);
@@ -477,28 +495,27 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
     };
 
     if (steps) {
-        uint32_t b = 0, at = base;
-        const auto scale_of = [&]() MINT_INLINE_LAMBDA { return ROWS_W ? 1.0f : sw_block[(int64_t)b * a.sw_block]; };
-        if (ALONG || full) {
+        uint32_t b = 0, at = base, ahead = base + (STAGES - 1) * kStage;
+        const auto after = [&](uint32_t stage) MINT_INLINE_LAMBDA { return stage + kStage == base + STAGES * kStage ? base : stage + kStage; };
 #pragma unroll
-            for (int n = 0; n < XI + WI; ++n) bring(at, n);
-        } else {
-            bring_tail(at);
-        }
-        for (; b + 1 < full; ++b) {
-            const float sw = scale_of();
-            const uint32_t other = base + base + kStage - at;
-            __syncthreads();             // (waits for the loads into LDS too)
-            multiply(at, sw, [&](int n) MINT_INLINE_LAMBDA { bring(other, n); });
-            at = other;
+        for (int st = 0; st < STAGES - 1; ++st)
+            if (st < full) {
+#pragma unroll
+                for (int n = 0; n < XI + WI; ++n) bring(base + st * kStage, n);
+            }
+        if (!ALONG && !full) bring_tail(at);
+        for (; b + STAGES - 1 < full; ++b) {
+            meet<(STAGES - 2) * LOADS>();
+            multiply(at, [&](int n) MINT_INLINE_LAMBDA { bring(ahead, n); });
+            at = after(at);
+            ahead = after(ahead);
         }
         for (; b < steps; ++b) {
-            const float sw = scale_of();
-            const uint32_t other = base + base + kStage - at;
-            __syncthreads();
-            if (!ALONG && b + 1 < steps) bring_tail(other);
-            multiply(at, sw, [](int) MINT_INLINE_LAMBDA {});
-            at = other;
+            __syncthreads();             // (waits for the loads into LDS too)
+            const uint32_t next = after(at);
+            if (!ALONG && b + 1 == full && full < steps) bring_tail(next);
+            multiply(at, [](int) MINT_INLINE_LAMBDA {});
+            at = next;
         }
     }
 
@@ -658,33 +675,47 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
 uint64_t most_row_tiles(const ProductArgs& a, uint32_t tile_rows) {
     return ceil_div(a.rows, tile_rows) + (a.groups.offsets ? (uint64_t)a.groups.experts + 1 : 0);
 }
-template <int OUT, int BM, int BN, int WM, bool ROWS_W, bool ALONG>
+template <int OUT, int BM, int BN, int WM, int STAGES, bool ROWS_W, bool ALONG>
 int go_tiles(ProductArgs a, uint32_t matrices, hipStream_t stream) {
     a.col_tiles = (uint32_t)ceil_div(a.cols, BN);
     a.row_tiles = (uint32_t)ceil_div(a.rows, BM);
     const uint64_t blocks = (ALONG ? (uint64_t)a.row_tiles * matrices : most_row_tiles(a, BM)) * a.col_tiles;
     if (blocks > 0x7FFFFFFFull / (64 * WM * (BN / 64))) return MINT_ERR_TOO_LARGE;
     if (!blocks) return MINT_OK;
-    return Launch<&product_kernel<OUT, BM, BN, WM, ROWS_W, ALONG>>::go((uint32_t)ceil_div(blocks, 8) * 8, 64 * WM * (BN / 64), 0, stream, a);
+    return Launch<&product_kernel<OUT, BM, BN, WM, STAGES, ROWS_W, ALONG>>::go((uint32_t)ceil_div(blocks, 8) * 8, 64 * WM * (BN / 64), 0, stream, a);
 }
 // The tiles whose rounds over the compute units take least: tiles / (those at work at a time), rounded up, times what a round
-// takes for a block of the depth (measured at 8192 x 4096 x 8192, us): 256 x 256 2.04, 128 x 256 1.24, two 128 x 128 1.44.
+// takes for a block of the depth.  Measured, us:
+//   64 x 64     0.36 up to 256 tiles, 0.6 for 512 (two blocks to a compute unit; 64 - 512 rows x 4096 x 4096)
+//   128 x 128   0.72 up to 256 tiles, with three blocks of the depth under way (1024 x 4096 x 4096); 1.29 for 512, with one and two thread
+//               blocks to a compute unit, which start while others work (11532 rows of 64 experts x 1408 x 2048: 62.6 us, 128 x 256 64.7)
+//   128 x 256   1.2 (2048 x 4096 x 4096: 39 us, 128 x 128 45)
+//   256 x 256   2.0 (8192 x 8192 x 4096: 260 us, 128 x 256 315; 65536 rows of 32 experts x 2048 x 4096: 581 us, 128 x 128 696)
 template <int OUT, bool ROWS_W, bool ALONG>
 int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
-    const auto rounds = [&](uint32_t bm, uint32_t bn, uint32_t at_a_time) {
+    const auto tiles = [&](uint32_t bm, uint32_t bn) {
         const uint64_t rows = ALONG ? ceil_div(a.rows, bm) * matrices : ceil_div(a.rows, bm) + (a.groups.offsets ? a.groups.experts / 2 : 0);
-        return (float)ceil_div(rows * ceil_div(a.cols, bn), at_a_time);
+        return rows * ceil_div(a.cols, bn);
     };
-    const float large = 2.04f * rounds(256, 256, 256), wide = 1.24f * rounds(128, 256, 256), small = 1.44f * rounds(128, 128, 512);
-    if constexpr (OUT != DT_F32) {
-        if (large <= wide && large <= small) return go_tiles<OUT, 256, 256, 2, ROWS_W, ALONG>(a, matrices, stream);
-        if (wide <= small) return go_tiles<OUT, 128, 256, 2, ROWS_W, ALONG>(a, matrices, stream);
+    const uint64_t n64 = tiles(64, 64), n128 = tiles(128, 128);
+    const float t64 = n64 <= 256 ? 0.36f : 0.6f * ceil_div(n64, 512), t128 = n128 <= 256 ? 0.72f : 1.29f * ceil_div(n128, 512),
+                wide = 1.2f * ceil_div(tiles(128, 256), 256), large = 2.0f * ceil_div(tiles(256, 256), 256);
+    if (t64 <= t128 && t64 <= wide && t64 <= large) return go_tiles<OUT, 64, 64, 4, 4, ROWS_W, ALONG>(a, matrices, stream);
+    if constexpr (OUT == DT_F32) {       // (operands widened to 16 bits leave no registers for more)
+        return go_tiles<OUT, 128, 128, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
+    } else {
+        if (t128 <= wide && t128 <= large) {
+            if (n128 <= 256) return go_tiles<OUT, 128, 128, 4, 4, ROWS_W, ALONG>(a, matrices, stream);
+            return go_tiles<OUT, 128, 128, 4, 2, ROWS_W, ALONG>(a, matrices, stream);
+        }
+        if (wide <= large) return go_tiles<OUT, 128, 256, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
+        return go_tiles<OUT, 256, 256, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
     }
-    return go_tiles<OUT, 128, 128, 2, ROWS_W, ALONG>(a, matrices, stream);
 }
 
-// Few rows: at most 64 for each weight matrix, on the average.
-bool few_rows(uint64_t rows, uint32_t matrices) { return rows <= 64ull * matrices; }
+// Few rows: at most 32 for each weight matrix, on the average (24 x 4096 x 4096: 7.8 us, with tiles of 64 x 64 11.8; at 64 rows
+// 12.8 and 11.8).
+bool few_rows(uint64_t rows, uint32_t matrices) { return rows <= 32ull * matrices; }
 // ... and so few that the rounding is done on the way
 bool rounded_on_the_way(uint64_t rows, uint32_t matrices) { return rows <= 16ull * matrices; }
 template <int OUT, int X, int MT, int KWAYS>
@@ -710,8 +741,7 @@ int go_rows(const ProductArgs& a, int x_dtype, uint32_t matrices, hipStream_t st
         default: break;
     }
     if (a.rows <= 16ull * matrices) return go_thin<OUT, DT_BYTES, 1>(a, stream);
-    if (a.rows <= 32ull * matrices) return go_thin<OUT, DT_BYTES, 2>(a, stream);
-    if (few_rows(a.rows, matrices)) return go_thin<OUT, DT_BYTES, 4>(a, stream);
+    if (few_rows(a.rows, matrices)) return go_thin<OUT, DT_BYTES, 2>(a, stream);
     return go_product<OUT, false, false>(a, 1, stream);
 }
 
