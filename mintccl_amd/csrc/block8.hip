@@ -26,13 +26,6 @@ __device__ __forceinline__ uint32_t pack8(float a, float b, float c, float d) {
 }
 // Magnitudes are compared as the whole numbers that they are in memory: of a NaN and a number the NaN is larger, and stays.
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-// the largest of the 16 lanes of a row
-__device__ __forceinline__ uint32_t row_max(uint32_t v) {
-    v = max(v, dpp<0xB1, 0xf>(v, 0u));
-    v = max(v, dpp<0x4E, 0xf>(v, 0u));
-    v = max(v, dpp<0x141, 0xf>(v, 0u));
-    return max(v, dpp<0x140, 0xf>(v, 0u));
-}
 // 16 lanes' 8 numbers each, a block of 128, in 8 bits; the scale comes back
 __device__ __forceinline__ float round_block(const float (&v)[8], u32x2& q) {
     uint32_t most = __float_as_uint(kLeastBlock);
@@ -708,7 +701,7 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
             if (n128 <= 256) return go_tiles<OUT, 128, 128, 4, 4, ROWS_W, ALONG>(a, matrices, stream);
             return go_tiles<OUT, 128, 128, 4, 2, ROWS_W, ALONG>(a, matrices, stream);
         }
-        if (wide <= large) return go_tiles<OUT, 128, 256, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
+        if (wide <= large) return go_tiles<OUT, 128, 256, 2, 3, ROWS_W, ALONG>(a, matrices, stream);
         return go_tiles<OUT, 256, 256, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
     }
 }

@@ -90,6 +90,14 @@ __device__ __forceinline__ float wave_max(float v) {
     }));
 }
 
+// the largest of the 16 lanes of a row
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    v = max(v, dpp<0xB1, 0xf>(v, 0u));
+    v = max(v, dpp<0x4E, 0xf>(v, 0u));
+    v = max(v, dpp<0x141, 0xf>(v, 0u));
+    return max(v, dpp<0x140, 0xf>(v, 0u));
+}
+
 inline bool aligned_to(const void* p, uint64_t bytes) { return reinterpret_cast<uint64_t>(p) % bytes == 0; }
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 inline int element_bytes(int dtype) { return dtype == MINT_F32 ? 4 : 2; }

@@ -12,6 +12,8 @@
 // itself always names experts that exist.
 #include "operators.hpp"
 
+#include <algorithm>
+
 namespace mint {
 namespace {
 
@@ -40,13 +42,55 @@ struct RouteArgs {
     uint32_t sigmoid, renormalise;
 };
 
-// A lane has V consecutive experts, so that among equal keys the lowest lane has the lowest expert.
-template <int DT, int V>
+// What LANES lanes have together: 16 (a row, whose lanes the additions' cross-lane operands reach in four steps) or all 64.
+template <int LANES>
+struct Lanes;
+template <>
+struct Lanes<64> {
+    static __device__ __forceinline__ uint32_t max_of(uint32_t v) { return wave_max(v); }
+    static __device__ __forceinline__ float max_of(float v) { return wave_max(v); }
+    static __device__ __forceinline__ float sum_of(float v) { return wave_sum(v); }
+    static __device__ __forceinline__ uint32_t first(bool p) { return __builtin_ctzll(__ballot(p)); }
+};
+template <>
+struct Lanes<16> {
+    template <typename F>
+    static __device__ __forceinline__ float fold(float v, const F& join) {
+        v = join(v, __uint_as_float(dpp<0xB1, 0xf>(__float_as_uint(v), 0u)));
+        v = join(v, __uint_as_float(dpp<0x4E, 0xf>(__float_as_uint(v), 0u)));
+        v = join(v, __uint_as_float(dpp<0x141, 0xf>(__float_as_uint(v), 0u)));
+        return join(v, __uint_as_float(dpp<0x140, 0xf>(__float_as_uint(v), 0u)));
+    }
+    static __device__ __forceinline__ uint32_t max_of(uint32_t v) { return row_max(v); }
+    static __device__ __forceinline__ float max_of(float v) { return fold(v, [](float a, float b) { return fmaxf(a, b); }); }
+    static __device__ __forceinline__ float sum_of(float v) { return fold(v, [](float a, float b) { return a + b; }); }
+    // the first of the row's lanes where p holds (one of them does)
+    static __device__ __forceinline__ uint32_t first(bool p) {
+        const uint32_t row = lane_id() & 48u;
+        return row + (uint32_t)__builtin_ctz((uint32_t)(__ballot(p) >> row) | 0x10000u);
+    }
+};
+// a group's two largest keys joined with those of the lanes that CTRL reaches
+template <int CTRL>
+__device__ __forceinline__ void join_best(uint32_t& best, uint32_t& second) {
+    const uint32_t b = dpp<CTRL, 0xf>(best, 0u), s = dpp<CTRL, 0xf>(second, 0u);
+    second = max(min(best, b), max(second, s));
+    best = max(best, b);
+}
+
+// LANES lanes have a token, a lane V consecutive experts of it, so that among equal keys the lowest lane has the lowest expert.
+// Bound by its vector instructions: a choice is the largest of the lanes' largest keys, taken k times.  With 16 lanes
+// the steps between lanes are for four tokens at once: 65536 tokens, 256 experts in 8 groups, 8 chosen: 104 us with 64 lanes
+// and groups looked at one by one.
+template <int DT, int V, int LANES>
 __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
     using T = typename Elem<DT>::type;
-    const uint32_t token = blockIdx.x * kRouteWaves + wave_in_block(), lane = lane_id(), first = lane * V;
-    if (token >= a.tokens) return;
-    const T* const row = static_cast<const T*>(a.logits) + (int64_t)token * a.row_stride;
+    using L = Lanes<LANES>;
+    constexpr uint32_t TOKENS = 64 * kRouteWaves / LANES;
+    __shared__ int32_t picked[TOKENS][LANES];
+    const uint32_t mine = threadIdx.x / LANES, token = blockIdx.x * TOKENS + mine, lane = threadIdx.x % LANES, first = lane * V;
+    const bool live = token < a.tokens;                      // (all lanes go along: they are reached by others)
+    const T* const row = static_cast<const T*>(a.logits) + (int64_t)(live ? token : a.tokens - 1) * a.row_stride;
     float x[V];
     load_elements<DT, V>(row + first, a.whole && first + V <= a.experts, (int64_t)a.experts - first, x);
     uint32_t key[V];
@@ -57,57 +101,98 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
         key[i] = first + i < a.experts && x[i] != -INFINITY ? order_of(s + b) : 0u;
     }
     if (a.groups > 1) {
-        const uint32_t per = a.experts / a.groups;
-        uint32_t of_group = 0;                               // lane g: the key of group g
-        for (uint32_t g = 0; g < a.groups; ++g) {
+        const uint32_t per = a.experts / a.groups, lanes = per / V;
+        if (per % V == 0 && lanes <= 16 && (lanes & (lanes - 1)) == 0) {
+            // a group is 1, 2, 4, 8 or 16 whole lanes: all groups at once
             uint32_t best = 0, second = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const uint32_t k = first + i - g * per < per ? key[i] : 0u;
-                second = max(second, min(best, k));
-                best = max(best, k);
+                second = max(second, min(best, key[i]));
+                best = max(best, key[i]);
             }
-            uint32_t top = wave_max(best);
-            if (a.group_top == 2 && top != 0u) {
-                const uint32_t holder = __builtin_ctzll(__ballot(best == top));
-                const uint32_t next = wave_max(lane == holder ? second : best);
-                if (next != 0u) top = order_of(number_of(top) + number_of(next));
+            if (lanes > 1) join_best<0xB1>(best, second);
+            if (lanes > 2) join_best<0x4E>(best, second);
+            if (lanes > 4) join_best<0x141>(best, second);
+            if (lanes > 8) join_best<0x140>(best, second);
+            uint32_t of_group = a.group_top == 2 && second != 0u ? order_of(number_of(best) + number_of(second)) : best;
+            bool keep = false;
+            for (uint32_t n = 0; n < a.kept; ++n) {
+                const uint32_t top = L::max_of(of_group), holder = L::first(of_group == top) % LANES;
+                if (top != 0u && lane / lanes == holder / lanes) {
+                    keep = true;
+                    of_group = 0u;
+                }
             }
-            if (lane == g) of_group = top;
-        }
-        uint64_t keep = 0;
-        for (uint32_t n = 0; n < a.kept; ++n) {
-            const uint32_t top = wave_max(of_group);
-            if (top == 0u) break;
-            const uint32_t g = __builtin_ctzll(__ballot(of_group == top));
-            keep |= 1ull << g;
-            if (lane == g) of_group = 0u;
-        }
 #pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = keep >> min((first + i) / per, 63u) & 1u ? key[i] : 0u;
+            for (int i = 0; i < V; ++i) key[i] = keep ? key[i] : 0u;
+        } else {
+            // groups that end inside a lane: one by one, lane g % LANES keeps the key of group g
+            constexpr int PER_LANE = 64 / LANES;
+            uint32_t of_group[PER_LANE];
+#pragma unroll
+            for (int q = 0; q < PER_LANE; ++q) of_group[q] = 0;
+            for (uint32_t g = 0; g < a.groups; ++g) {
+                uint32_t best = 0, second = 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const uint32_t k = first + i - g * per < per ? key[i] : 0u;
+                    second = max(second, min(best, k));
+                    best = max(best, k);
+                }
+                uint32_t top = L::max_of(best);
+                const bool holds = lane == L::first(best == top) % LANES;
+                const uint32_t next = L::max_of(holds ? second : best);
+                if (a.group_top == 2 && next != 0u) top = order_of(number_of(top) + number_of(next));
+#pragma unroll
+                for (int q = 0; q < PER_LANE; ++q) of_group[q] = q * LANES + lane == g ? top : of_group[q];
+            }
+            uint64_t keep = 0;
+            for (uint32_t n = 0; n < a.kept; ++n) {
+                uint32_t best = 0;
+#pragma unroll
+                for (int q = 0; q < PER_LANE; ++q) best = max(best, of_group[q]);
+                const uint32_t top = L::max_of(best);
+                // the lowest group with that key: by q first, then by lane
+                bool done = top == 0u;
+#pragma unroll
+                for (int q = 0; q < PER_LANE; ++q) {
+                    const bool here = !done && L::max_of(of_group[q]) == top;
+                    const uint32_t holder = L::first(of_group[q] == top) % LANES;
+                    if (here) {
+                        keep |= 1ull << (q * LANES + holder);
+                        if (lane == holder) of_group[q] = 0u;
+                        done = true;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = keep >> min((first + i) / per, 63u) & 1u ? key[i] : 0u;
+        }
     }
-    int32_t mine = -1;                                       // lane j: the j-th choice
+    if (lane < a.topk) picked[mine][lane] = -1;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     for (uint32_t j = 0; j < a.topk; ++j) {
         uint32_t best = key[0];
 #pragma unroll
         for (int i = 1; i < V; ++i) best = max(best, key[i]);
-        const uint32_t top = wave_max(best);
-        if (top == 0u) break;
-        const uint32_t holder = __builtin_ctzll(__ballot(best == top));
-        uint32_t at = 0;
+        const uint32_t top = L::max_of(best);
+        const bool wins = top != 0u && lane == L::first(best == top) % LANES;
+        uint32_t at = V;
 #pragma unroll
         for (int i = V - 1; i >= 0; --i) at = key[i] == top ? i : at;
-        const int32_t e = __builtin_amdgcn_readlane((int)(first + at), holder);
+        at = wins ? at : V;
 #pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = first + i == (uint32_t)e ? 0u : key[i];
-        if (lane == j) mine = e;
+        for (int i = 0; i < V; ++i) key[i] = at == (uint32_t)i ? 0u : key[i];
+        if (wins) picked[mine][j] = (int32_t)(first + at);
     }
-    const bool there = mine >= 0;
-    const float l = there ? Elem<DT>::load(row[mine]) : -INFINITY;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int32_t choice = lane < a.topk ? picked[mine][lane] : -1;
+    const bool there = choice >= 0;
+    const float l = there ? Elem<DT>::load(row[choice]) : -INFINITY;
     float s, total = 1.0f;
     if (a.sigmoid) {
         s = there ? sigmoid(l) : 0.0f;
-        if (a.renormalise) total = wave_sum(s);
+        if (a.renormalise) total = L::sum_of(s);
     } else {
         // the largest logit of those in the sum: of the chosen, or of all
         float m = l;
@@ -115,7 +200,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) m = first + i < a.experts ? fmaxf(m, x[i]) : m;
         }
-        m = wave_max(m);
+        m = L::max_of(m);
         m = m == -INFINITY ? 0.0f : m;
         s = there ? expf(l - m) : 0.0f;
         float sum = s;
@@ -124,13 +209,13 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) sum += first + i < a.experts ? expf(x[i] - m) : 0.0f;
         }
-        total = wave_sum(sum);
+        total = L::sum_of(sum);
     }
     // (every chosen score may have vanished: then so have the weights)
     const float w = !there || total == 0.0f ? 0.0f : a.scale * (s / total);
-    if (lane < a.topk) {
+    if (live && lane < a.topk) {
         a.weights[(uint64_t)token * a.topk + lane] = w;
-        a.chosen[(uint64_t)token * a.topk + lane] = mine;
+        a.chosen[(uint64_t)token * a.topk + lane] = choice;
     }
 }
 
@@ -216,14 +301,15 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_grad_kernel(RouteGradA
 // consecutive pairs: it counts them by bucket, and when it knows how many come before them in each bucket it
 // goes through them 64 at a time.  Lanes with the same bucket find each other by ballots over the bucket's
 // bits: the order does not depend on anything's timing.
-constexpr int kSortWaves = 8, kSortChunk = 4096, kSortOne = 16384;     // pairs of a block; of a launch of one block
+constexpr int kSortWaves = 8, kSortOne = 4096;      // a launch of one block sorts so many pairs
 constexpr uint32_t kMostExperts = 1024;
 
 struct AssignArgs {
     const int32_t* chosen;
     int32_t *offsets, *tokens, *slots;
-    uint32_t* counts;        // (blocks, n + 1), then the places where they begin
+    uint32_t* counts;        // (blocks, n + 1)
     uint32_t pairs, topk, first, n, bits;
+    uint32_t share, blocks;  // pairs of a wavefront; thread blocks
 };
 __device__ __forceinline__ uint32_t bucket_of(const AssignArgs& a, uint32_t pair) {
     const uint32_t b = (uint32_t)a.chosen[pair] - a.first;
@@ -288,8 +374,7 @@ __global__ void __launch_bounds__(64 * kSortWaves) assign_one_kernel(AssignArgs 
     const uint32_t w = wave_in_block(), buckets = a.n + 1;
     for (uint32_t i = threadIdx.x; i < kSortWaves * buckets; i += 64 * kSortWaves) next[i / buckets][i % buckets] = 0u;
     __syncthreads();
-    const uint32_t share = ((a.pairs + kSortWaves - 1) / kSortWaves + 63) & ~63u;
-    const uint32_t begin = min(w * share, a.pairs), end = min(begin + share, a.pairs);
+    const uint32_t begin = min(w * a.share, a.pairs), end = min(begin + a.share, a.pairs);
     count_pairs(a, begin, end, next[w]);
     __syncthreads();
     for (uint32_t b = threadIdx.x; b < buckets; b += 64 * kSortWaves) {
@@ -311,84 +396,89 @@ __global__ void __launch_bounds__(64 * kSortWaves) assign_one_kernel(AssignArgs 
     place_pairs(a, begin, end, next[w]);
 }
 
+// Many: a launch counts each block's pairs by bucket, and a second one, in which every block adds up what it needs of
+// those counts (all totals, and its own predecessors': 65536 x 8 pairs, 256 buckets: 17 us; with a launch of one block in
+// between that leaves the sums, 49), places them.
 __global__ void __launch_bounds__(64 * kSortWaves) assign_count_kernel(AssignArgs a) {
     __shared__ uint32_t all[kMostExperts + 1];
     const uint32_t buckets = a.n + 1;
     for (uint32_t i = threadIdx.x; i < buckets; i += 64 * kSortWaves) all[i] = 0u;
     __syncthreads();
-    const uint32_t begin = blockIdx.x * kSortChunk + wave_in_block() * (kSortChunk / kSortWaves);
-    count_pairs(a, min(begin, a.pairs), min(begin + kSortChunk / kSortWaves, a.pairs), all);
+    const uint32_t begin = min((blockIdx.x * kSortWaves + wave_in_block()) * a.share, a.pairs);
+    count_pairs(a, begin, min(begin + a.share, a.pairs), all);
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < buckets; i += 64 * kSortWaves) a.counts[(uint64_t)blockIdx.x * buckets + i] = all[i];
 }
-// counts of all blocks -> where each block's pairs of each bucket begin; one block
-__global__ void __launch_bounds__(1024) assign_scan_kernel(AssignArgs a, uint32_t blocks) {
-    __shared__ uint32_t start[kMostExperts + 1], sums[1024];
-    const uint32_t buckets = a.n + 1;
-    for (uint32_t b = threadIdx.x; b < buckets; b += 1024) {
-        uint32_t total = 0;
-        for (uint32_t i = 0; i < blocks; ++i) {
-            const uint64_t at = (uint64_t)i * buckets + b;
-            const uint32_t c = a.counts[at];
-            a.counts[at] = total;
-            total += c;
-        }
-        start[b] = total;
-    }
-    __syncthreads();
-    block_scan<1024>(start, buckets, sums);
-    for (uint32_t b = threadIdx.x; b < buckets; b += 1024) a.offsets[b] = (int32_t)start[b];
-}
 __global__ void __launch_bounds__(64 * kSortWaves) assign_place_kernel(AssignArgs a) {
-    __shared__ uint32_t next[kSortWaves][kMostExperts + 1];
+    __shared__ uint32_t next[kSortWaves][kMostExperts + 1], start[kMostExperts + 1], sums[64 * kSortWaves];
     const uint32_t w = wave_in_block(), buckets = a.n + 1;
     for (uint32_t i = threadIdx.x; i < kSortWaves * buckets; i += 64 * kSortWaves) next[i / buckets][i % buckets] = 0u;
     __syncthreads();
-    const uint32_t begin = min(blockIdx.x * kSortChunk + w * (kSortChunk / kSortWaves), a.pairs);
-    const uint32_t end = min(begin + kSortChunk / kSortWaves, a.pairs);
+    const uint32_t begin = min((blockIdx.x * kSortWaves + w) * a.share, a.pairs), end = min(begin + a.share, a.pairs);
     count_pairs(a, begin, end, next[w]);
     __syncthreads();
     for (uint32_t b = threadIdx.x; b < buckets; b += 64 * kSortWaves) {
-        uint32_t total = (uint32_t)a.offsets[b] + a.counts[(uint64_t)blockIdx.x * buckets + b];
-        for (int i = 0; i < kSortWaves; ++i) {
-            const uint32_t c = next[i][b];
-            next[i][b] = total;
+        uint32_t before = 0, total = 0;
+#pragma unroll 16
+        for (uint32_t i = 0; i < a.blocks; ++i) {
+            const uint32_t c = a.counts[(uint64_t)i * buckets + b];
+            before += i < blockIdx.x ? c : 0u;
             total += c;
         }
+        start[b] = total;
+        for (int i = 0; i < kSortWaves; ++i) {
+            const uint32_t c = next[i][b];
+            next[i][b] = before;
+            before += c;
+        }
+    }
+    __syncthreads();
+    block_scan<64 * kSortWaves>(start, buckets, sums);
+    for (uint32_t b = threadIdx.x; b < buckets; b += 64 * kSortWaves) {
+        if (blockIdx.x == 0) a.offsets[b] = (int32_t)start[b];
+        for (int i = 0; i < kSortWaves; ++i) next[i][b] += start[b];
     }
     __syncthreads();
     place_pairs(a, begin, end, next[w]);
 }
 
-uint32_t values_per_lane(uint32_t experts) {
+// V of a token's lanes: a power of two.
+uint32_t values_per_lane(uint32_t experts, uint32_t lanes) {
     uint32_t v = 1;
-    while (v * 64 < experts) v *= 2;
+    while (v * lanes < experts) v *= 2;
     return v;
 }
-template <int DT, int V>
+// 16 lanes to a token where they have enough registers, and one for each choice
+uint32_t lanes_of(uint32_t experts, uint32_t topk) { return experts <= 256 && topk <= 16 ? 16 : 64; }
+template <int DT, int V, int LANES>
 int go_route(const RouteArgs& a, hipStream_t stream) {
-    return Launch<&route_kernel<DT, V>>::go((uint32_t)ceil_div(a.tokens, kRouteWaves), 64 * kRouteWaves, 0, stream, a);
+    return Launch<&route_kernel<DT, V, LANES>>::go((uint32_t)ceil_div(a.tokens, 64 * kRouteWaves / LANES), 64 * kRouteWaves, 0, stream, a);
 }
-template <int DT, int V>
+template <int DT, int V, int LANES>
 int go_route_grad(const RouteGradArgs& a, hipStream_t stream) {
     return Launch<&route_grad_kernel<DT, V>>::go((uint32_t)ceil_div(a.tokens, kRouteWaves), 64 * kRouteWaves, 0, stream, a);
 }
-#define MINT_BY_LANE(GO, DT)                            \
-    switch (values_per_lane(a.experts)) {               \
-        case 1: return GO<DT, 1>(a, stream);            \
-        case 2: return GO<DT, 2>(a, stream);            \
-        case 4: return GO<DT, 4>(a, stream);            \
-        case 8: return GO<DT, 8>(a, stream);            \
-        default: return GO<DT, 16>(a, stream);          \
+#define MINT_BY_LANE(GO, DT, LANES)                            \
+    switch (values_per_lane(a.experts, LANES)) {               \
+        case 1: return GO<DT, 1, LANES>(a, stream);            \
+        case 2: return GO<DT, 2, LANES>(a, stream);            \
+        case 4: return GO<DT, 4, LANES>(a, stream);            \
+        case 8: return GO<DT, 8, LANES>(a, stream);            \
+        default: return GO<DT, 16, LANES>(a, stream);          \
     }
-#define MINT_BY_TYPE(GO)                                \
-    switch (dtype) {                                    \
-        case MINT_F16: MINT_BY_LANE(GO, DT_F16)         \
-        case MINT_BF16: MINT_BY_LANE(GO, DT_BF16)       \
-        default: MINT_BY_LANE(GO, DT_F32)               \
+#define MINT_BY_TYPE(GO, LANES)                                \
+    switch (dtype) {                                           \
+        case MINT_F16: MINT_BY_LANE(GO, DT_F16, LANES)         \
+        case MINT_BF16: MINT_BY_LANE(GO, DT_BF16, LANES)       \
+        default: MINT_BY_LANE(GO, DT_F32, LANES)               \
     }
-int launch_route(const RouteArgs& a, int dtype, hipStream_t stream) { MINT_BY_TYPE(go_route) }
-int launch_route_grad(const RouteGradArgs& a, int dtype, hipStream_t stream) { MINT_BY_TYPE(go_route_grad) }
+int launch_route(const RouteArgs& a, int dtype, hipStream_t stream) {
+    if (lanes_of(a.experts, a.topk) == 16) {
+        MINT_BY_TYPE(go_route, 16)
+    }
+    MINT_BY_TYPE(go_route, 64)
+}
+int launch_route_grad(const RouteGradArgs& a, int dtype, hipStream_t stream) { MINT_BY_TYPE(go_route_grad, 64) }
 
 bool routable(uint64_t tokens, uint32_t experts, uint32_t topk, int dtype, int score) {
     return experts >= 1 && experts <= kMostExperts && topk >= 1 && topk <= 64 && topk <= experts && tokens < (1ull << 31) &&
@@ -407,7 +497,7 @@ extern "C" int mint_route(const mint_route_op* op, void* stream) {
         return MINT_ERR_GEOMETRY;
     if (op->tokens == 0) return MINT_OK;
     if (!op->logits || !op->weights || !op->chosen) return MINT_ERR_ARG;
-    const uint32_t vector = values_per_lane(op->experts) * element_bytes(op->dtype);
+    const uint32_t vector = values_per_lane(op->experts, lanes_of(op->experts, op->topk)) * element_bytes(op->dtype);
     const bool whole = aligned_to(reinterpret_cast<void*>(op->logits), vector) && op->row_stride * element_bytes(op->dtype) % vector == 0;
     const RouteArgs a = {reinterpret_cast<const void*>(op->logits), reinterpret_cast<const float*>(op->bias),
                          reinterpret_cast<float*>(op->weights), reinterpret_cast<int32_t*>(op->chosen), op->row_stride,
@@ -420,7 +510,7 @@ extern "C" int mint_route_grad(const mint_route_op* op, uint64_t d_weights, uint
     if (!op || !routable(op->tokens, op->experts, op->topk, op->dtype, op->score)) return MINT_ERR_ARG;
     if (op->tokens == 0) return MINT_OK;
     if (!op->logits || !op->chosen || !d_weights || !d_logits) return MINT_ERR_ARG;
-    const uint32_t size = element_bytes(op->dtype), vector = values_per_lane(op->experts) * size;
+    const uint32_t size = element_bytes(op->dtype), vector = values_per_lane(op->experts, 64) * size;
     const bool whole = aligned_to(reinterpret_cast<void*>(op->logits), vector) && op->row_stride * size % vector == 0;
     const bool d_whole = aligned_to(reinterpret_cast<void*>(d_logits), vector) && d_stride * size % vector == 0;
     const RouteGradArgs a = {reinterpret_cast<const void*>(op->logits), reinterpret_cast<const float*>(d_weights),
@@ -430,8 +520,20 @@ extern "C" int mint_route_grad(const mint_route_op* op, uint64_t d_weights, uint
     return launch_route_grad(a, op->dtype, static_cast<hipStream_t>(stream));
 }
 
+namespace {
+// pairs of a wavefront and thread blocks: 256 blocks at most (each reads the counts of all)
+void shares(uint64_t pairs, uint32_t* share, uint32_t* blocks) {
+    const uint64_t waves = pairs <= kSortOne ? kSortWaves : std::min<uint64_t>(256 * kSortWaves, ceil_div(pairs, 128));
+    *share = (uint32_t)(ceil_div(ceil_div(pairs, waves), 64) * 64);
+    *blocks = pairs ? (uint32_t)ceil_div(pairs, (uint64_t)*share * kSortWaves) : 1;
+}
+}  // namespace
+
 extern "C" size_t mint_assign_workspace(uint64_t pairs, uint32_t experts) {
-    return pairs <= kSortOne ? 0 : ceil_div(pairs, kSortChunk) * ((size_t)experts + 1) * 4;
+    if (pairs <= kSortOne || pairs > 0x7FFFFFFFull) return 0;
+    uint32_t share, blocks;
+    shares(pairs, &share, &blocks);
+    return blocks * ((size_t)experts + 1) * 4;
 }
 
 extern "C" int mint_assign(const void* chosen, uint64_t tokens, uint32_t topk, uint32_t first, uint32_t experts, void* offsets,
@@ -442,15 +544,13 @@ extern "C" int mint_assign(const void* chosen, uint64_t tokens, uint32_t topk, u
     if (pairs && (!chosen || !order || !slots)) return MINT_ERR_ARG;
     const size_t need = mint_assign_workspace(pairs, experts);
     if (need > workspace_bytes || (need && !workspace)) return MINT_ERR_STAGING;
-    uint32_t bits = 0;
+    uint32_t bits = 0, share, blocks;
     while (experts >> bits) ++bits;
+    shares(pairs, &share, &blocks);
     const AssignArgs a = {static_cast<const int32_t*>(chosen), static_cast<int32_t*>(offsets), static_cast<int32_t*>(order),
-                          static_cast<int32_t*>(slots), static_cast<uint32_t*>(workspace), (uint32_t)pairs, topk, first, experts, bits};
+                          static_cast<int32_t*>(slots), static_cast<uint32_t*>(workspace), (uint32_t)pairs, topk, first, experts, bits, share, blocks};
     const auto s = static_cast<hipStream_t>(stream);
     if (!need) return Launch<&assign_one_kernel>::go(1, 64 * kSortWaves, 0, s, a);
-    const uint32_t blocks = (uint32_t)ceil_div(pairs, kSortChunk);
-    int err = Launch<&assign_count_kernel>::go(blocks, 64 * kSortWaves, 0, s, a);
-    if (err == MINT_OK) err = Launch<&assign_scan_kernel>::go(1, 1024, 0, s, a, blocks);
-    if (err == MINT_OK) err = Launch<&assign_place_kernel>::go(blocks, 64 * kSortWaves, 0, s, a);
-    return err;
+    const int err = Launch<&assign_count_kernel>::go(blocks, 64 * kSortWaves, 0, s, a);
+    return err == MINT_OK ? Launch<&assign_place_kernel>::go(blocks, 64 * kSortWaves, 0, s, a) : err;
 }
