@@ -59,15 +59,6 @@ __device__ __forceinline__ uint32_t tiles_of(const Groups& g, uint32_t e, uint32
     }
     return (end - begin + tile_rows - 1) / tile_rows;
 }
-__device__ __forceinline__ uint32_t sum_below(uint32_t v) {       // of the lanes up to this one
-    v += dpp<0x111, 0xf>(v, 0u);        // row_shr:1, 2, 4, 8
-    v += dpp<0x112, 0xf>(v, 0u);
-    v += dpp<0x114, 0xf>(v, 0u);
-    v += dpp<0x118, 0xf>(v, 0u);
-    v += dpp<0x142, 0xa>(v, 0u);        // row_bcast:15 into rows 1 and 3
-    v += dpp<0x143, 0xc>(v, 0u);        // row_bcast:31 into rows 2 and 3
-    return v;
-}
 __device__ __forceinline__ uint32_t count_tiles(const Groups& g, uint32_t tile_rows, bool rest) {
     if (!g.offsets) return (g.rows + tile_rows - 1) / tile_rows;
     uint32_t mine = 0, begin, end;

@@ -90,6 +90,15 @@ __device__ __forceinline__ float wave_max(float v) {
     }));
 }
 
+__device__ __forceinline__ uint32_t sum_below(uint32_t v) {       // of the lanes up to this one
+    v += dpp<0x111, 0xf>(v, 0u);        // row_shr:1, 2, 4, 8
+    v += dpp<0x112, 0xf>(v, 0u);
+    v += dpp<0x114, 0xf>(v, 0u);
+    v += dpp<0x118, 0xf>(v, 0u);
+    v += dpp<0x142, 0xa>(v, 0u);        // row_bcast:15 into rows 1 and 3
+    v += dpp<0x143, 0xc>(v, 0u);        // row_bcast:31 into rows 2 and 3
+    return v;
+}
 // the largest of the 16 lanes of a row
 __device__ __forceinline__ uint32_t row_max(uint32_t v) {
     v = max(v, dpp<0xB1, 0xf>(v, 0u));

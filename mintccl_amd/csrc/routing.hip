@@ -39,7 +39,7 @@ struct RouteArgs {
     uint32_t tokens, experts, topk, groups, kept, group_top;
     float scale;
     uint32_t whole;          // a lane's logits may be loaded as one vector
-    uint32_t sigmoid, renormalise;
+    uint32_t bias_whole, sigmoid, renormalise;
 };
 
 // What LANES lanes have together: 16 (a row, whose lanes the additions' cross-lane operands reach in four steps) or all 64.
@@ -91,14 +91,16 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
     const uint32_t mine = threadIdx.x / LANES, token = blockIdx.x * TOKENS + mine, lane = threadIdx.x % LANES, first = lane * V;
     const bool live = token < a.tokens;                      // (all lanes go along: they are reached by others)
     const T* const row = static_cast<const T*>(a.logits) + (int64_t)(live ? token : a.tokens - 1) * a.row_stride;
-    float x[V];
+    float x[V], bias[V];
     load_elements<DT, V>(row + first, a.whole && first + V <= a.experts, (int64_t)a.experts - first, x);
+#pragma unroll
+    for (int i = 0; i < V; ++i) bias[i] = 0.0f;
+    if (a.bias) load_elements<DT_F32, V>(a.bias + first, a.bias_whole && first + V <= a.experts, (int64_t)a.experts - first, bias);
     uint32_t key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const float s = a.sigmoid ? sigmoid(x[i]) : x[i];
-        const float b = a.bias && first + i < a.experts ? a.bias[first + i] : 0.0f;
-        key[i] = first + i < a.experts && x[i] != -INFINITY ? order_of(s + b) : 0u;
+        key[i] = first + i < a.experts && x[i] != -INFINITY ? order_of(s + bias[i]) : 0u;
     }
     if (a.groups > 1) {
         const uint32_t per = a.experts / a.groups, lanes = per / V;
@@ -177,12 +179,16 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
         for (int i = 1; i < V; ++i) best = max(best, key[i]);
         const uint32_t top = L::max_of(best);
         const bool wins = top != 0u && lane == L::first(best == top) % LANES;
-        uint32_t at = V;
+        const uint32_t taken = wins ? top : 1u;              // (1 is nobody's key)
+        uint32_t at = 0;
+        bool found = false;
 #pragma unroll
-        for (int i = V - 1; i >= 0; --i) at = key[i] == top ? i : at;
-        at = wins ? at : V;
-#pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = at == (uint32_t)i ? 0u : key[i];
+        for (int i = 0; i < V; ++i) {
+            const bool here = key[i] == taken && !found;
+            found |= here;
+            at = here ? i : at;
+            key[i] = here ? 0u : key[i];
+        }
         if (wins) picked[mine][j] = (int32_t)(first + at);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -341,7 +347,7 @@ __device__ __forceinline__ void place_pairs(const AssignArgs& a, uint32_t begin,
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
-// exclusive sums of v[0..n) over the block's threads, left in v; all threads take part
+// exclusive sums of v[0..n), left in v; all threads of the block take part, `sums` is a number for each wavefront
 template <int THREADS>
 __device__ __forceinline__ void block_scan(uint32_t* v, uint32_t n, uint32_t* sums) {
     const uint32_t t = threadIdx.x, per = (n + THREADS - 1) / THREADS;
@@ -354,15 +360,11 @@ __device__ __forceinline__ void block_scan(uint32_t* v, uint32_t n, uint32_t* su
             total += c;
         }
     }
-    sums[t] = total;
+    const uint32_t upto = sum_below(total);
+    if (lane_id() == 63) sums[wave_in_block()] = upto;
     __syncthreads();
-    for (uint32_t d = 1; d < THREADS; d <<= 1) {
-        const uint32_t other = t >= d ? sums[t - d] : 0u;
-        __syncthreads();
-        sums[t] += other;
-        __syncthreads();
-    }
-    const uint32_t base = sums[t] - total;
+    uint32_t base = upto - total;
+    for (int w = 0; w < wave_in_block(); ++w) base += sums[w];
     for (uint32_t i = 0; i < per; ++i)
         if (t * per + i < n) v[t * per + i] += base;
     __syncthreads();
@@ -370,7 +372,7 @@ __device__ __forceinline__ void block_scan(uint32_t* v, uint32_t n, uint32_t* su
 
 // few pairs: all of it in one block
 __global__ void __launch_bounds__(64 * kSortWaves) assign_one_kernel(AssignArgs a) {
-    __shared__ uint32_t next[kSortWaves][kMostExperts + 1], start[kMostExperts + 1], sums[64 * kSortWaves];
+    __shared__ uint32_t next[kSortWaves][kMostExperts + 1], start[kMostExperts + 1], sums[kSortWaves];
     const uint32_t w = wave_in_block(), buckets = a.n + 1;
     for (uint32_t i = threadIdx.x; i < kSortWaves * buckets; i += 64 * kSortWaves) next[i / buckets][i % buckets] = 0u;
     __syncthreads();
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(64 * kSortWaves) assign_count_kernel(AssignArg
     for (uint32_t i = threadIdx.x; i < buckets; i += 64 * kSortWaves) a.counts[(uint64_t)blockIdx.x * buckets + i] = all[i];
 }
 __global__ void __launch_bounds__(64 * kSortWaves) assign_place_kernel(AssignArgs a) {
-    __shared__ uint32_t next[kSortWaves][kMostExperts + 1], start[kMostExperts + 1], sums[64 * kSortWaves];
+    __shared__ uint32_t next[kSortWaves][kMostExperts + 1], start[kMostExperts + 1], sums[kSortWaves];
     const uint32_t w = wave_in_block(), buckets = a.n + 1;
     for (uint32_t i = threadIdx.x; i < kSortWaves * buckets; i += 64 * kSortWaves) next[i / buckets][i % buckets] = 0u;
     __syncthreads();
@@ -499,9 +501,10 @@ extern "C" int mint_route(const mint_route_op* op, void* stream) {
     if (!op->logits || !op->weights || !op->chosen) return MINT_ERR_ARG;
     const uint32_t vector = values_per_lane(op->experts, lanes_of(op->experts, op->topk)) * element_bytes(op->dtype);
     const bool whole = aligned_to(reinterpret_cast<void*>(op->logits), vector) && op->row_stride * element_bytes(op->dtype) % vector == 0;
+    const bool bias_whole = aligned_to(reinterpret_cast<void*>(op->bias), values_per_lane(op->experts, lanes_of(op->experts, op->topk)) * 4);
     const RouteArgs a = {reinterpret_cast<const void*>(op->logits), reinterpret_cast<const float*>(op->bias),
                          reinterpret_cast<float*>(op->weights), reinterpret_cast<int32_t*>(op->chosen), op->row_stride,
-                         (uint32_t)op->tokens, op->experts, op->topk, op->groups, op->kept, op->group_top, op->scale, whole,
+                         (uint32_t)op->tokens, op->experts, op->topk, op->groups, op->kept, op->group_top, op->scale, whole, bias_whole,
                          op->score == MINT_SCORE_SIGMOID, op->renormalise != 0};
     return launch_route(a, op->dtype, static_cast<hipStream_t>(stream));
 }
