@@ -96,7 +96,7 @@ struct RowsArgs {
     uint8_t* q;
     float* scale;
     int64_t x_stride, q_stride, s_row, s_block;
-    uint32_t rows, depth, blocks, whole;     // blocks of a row
+    uint32_t rows, depth, blocks;            // blocks of a row
 };
 // 16 lanes have a block of 128 numbers of a row.  The last block is filled up with zeros.
 template <int DT>
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) rows8_kernel(RowsArgs a) {
     const uint32_t row = (uint32_t)(unit / a.blocks), block = (uint32_t)(unit % a.blocks), at = block * 128 + (threadIdx.x & 15u) * 8;
     if (row >= a.rows) return;
     float v[8];
-    load_elements<DT, 8>(static_cast<const T*>(a.x) + row * a.x_stride + at, a.whole && at + 8 <= a.depth, (int64_t)a.depth - at, v);
+    load_elements<DT, 8>(static_cast<const T*>(a.x) + row * a.x_stride + at, (int64_t)a.depth - at, v);
     u32x2 q;
     const float scale = round_block(v, q);
     *(MINT_GLOBAL u32x2*)as_global(a.q + row * a.q_stride + at) = q;
@@ -120,7 +120,7 @@ struct ColumnsArgs {
     float* scale;                // (blocks, width)
     int64_t x_stride, q_stride;
     Groups groups;
-    uint32_t x_rows, width, whole;
+    uint32_t x_rows, width;
 };
 // A thread block has 64 columns of 128 rows of an expert (fewer where it has no more: zeros follow). They turn in LDS.
 template <int DT>
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(256) columns8_kernel(ColumnsArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
         if (there)
-            load_elements<DT, 8>(static_cast<const T*>(a.x) + row * a.x_stride + col, a.whole && col + 8 <= a.width, (int64_t)a.width - col, v[i]);
+            load_elements<DT, 8>(static_cast<const T*>(a.x) + row * a.x_stride + col, (int64_t)a.width - col, v[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) m[j] = max(m[j], magnitude(v[i][j]));
     }
@@ -182,7 +182,7 @@ struct SquaresArgs {
     uint8_t* q;
     float* scale;
     int64_t w_matrix, w_stride, q_matrix, q_stride;
-    uint32_t rows, depth, blocks, whole;     // blocks of a row
+    uint32_t rows, depth, blocks;            // blocks of a row
 };
 // A thread block has a square of 128 x 128: 16 lanes to a row, eight rows to a thread.
 template <int DT>
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(256) squares8_kernel(SquaresArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
         if (row < a.rows)
-            load_elements<DT, 8>(w + row * a.w_stride + at, a.whole && at + 8 <= a.depth, (int64_t)a.depth - at, v[i]);
+            load_elements<DT, 8>(w + row * a.w_stride + at, (int64_t)a.depth - at, v[i]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) largest = max(largest, magnitude(v[i][j]));
     }
@@ -226,7 +226,7 @@ struct ProductArgs {
     Groups groups;               // experts' rows (or, `along_depth`, experts' blocks of the depth)
     int64_t x_stride, w_stride, w_matrix, out_stride, out_matrix;
     int64_t sx_row, sx_block, sw_matrix, sw_row, sw_block;
-    uint32_t x_rows, rows, cols, depth, col_tiles, row_tiles, out_whole, x_whole;
+    uint32_t x_rows, rows, cols, depth, col_tiles, row_tiles;
 };
 
 // Where a row's 16-byte piece lies in its 128 bytes of LDS: turned by the row's number, so that the lanes that a 16-byte read
@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = acc[i][h * 2 + k / 4][k % 4];
             const uint32_t c = col + h * 32;
-            if (c < a.cols) store_elements<OUT, 8>(to + c, a.out_whole && c + 8 <= a.cols, (int64_t)a.cols - c, v);
+            if (c < a.cols) store_elements<OUT, 8>(to + c, (int64_t)a.cols - c, v);
         }
     }
 }
@@ -609,8 +609,7 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
                     for (uint32_t unit = threadIdx.x / 16; unit < rows * blocks; unit += WAVES * 4) {
                         const uint32_t i = unit / blocks, b = unit % blocks, at = (first + b) * 128 + r16 * 8;
                         float v[8];
-                        load_elements<X, 8>(reinterpret_cast<const TX*>(a.x) + (int64_t)x_row(i) * a.x_stride + at, a.x_whole && at + 8 <= a.depth,
-                                            (int64_t)a.depth - at, v);
+                        load_elements<X, 8>(reinterpret_cast<const TX*>(a.x) + (int64_t)x_row(i) * a.x_stride + at, (int64_t)a.depth - at, v);
                         u32x2 q;
                         const float s = round_block(v, q);
                         *reinterpret_cast<u32x2*>(xs + i * XROW + b * 128 + r16 * 8) = q;
@@ -730,8 +729,6 @@ int go_rows(const ProductArgs& a, int x_dtype, uint32_t matrices, hipStream_t st
 }
 
 bool known(int dtype) { return dtype == MINT_F16 || dtype == MINT_BF16 || dtype == MINT_F32; }
-// eight elements as one vector
-bool vectors(const void* p, int64_t stride, int dtype) { return aligned_to(p, 8 * element_bytes(dtype)) && stride % 8 == 0; }
 constexpr uint64_t kMostRows = 0x7FFFFFFF - 128;
 
 }  // namespace
@@ -751,7 +748,7 @@ extern "C" int mint_rows8(const void* x, int64_t x_stride, uint64_t rows, uint64
     const uint64_t blocks = ceil_div(rows * per_row, 16);
     if (blocks > 0x7FFFFFFFull / 256) return MINT_ERR_TOO_LARGE;
     const RowsArgs a = {x, static_cast<uint8_t*>(q), static_cast<float*>(scale), x_stride, q_stride, s_row, s_block, (uint32_t)rows,
-                        (uint32_t)depth, (uint32_t)per_row, vectors(x, x_stride, dtype)};
+                        (uint32_t)depth, (uint32_t)per_row};
     const auto s = static_cast<hipStream_t>(stream);
     switch (dtype) {
         case MINT_F16: return Launch<&rows8_kernel<DT_F16>>::go((uint32_t)blocks, 256, 0, s, a);
@@ -773,8 +770,7 @@ extern "C" int mint_columns8(const void* x, int64_t x_stride, uint64_t x_rows, u
     if (q_stride < (int64_t)(blocks * 128)) return MINT_ERR_GEOMETRY;
     if (blocks > 0x7FFFFFFFull / 256) return MINT_ERR_TOO_LARGE;
     const ColumnsArgs a = {x, static_cast<const int32_t*>(tokens), static_cast<uint8_t*>(q), static_cast<float*>(scale), x_stride, q_stride,
-                           {static_cast<const int32_t*>(offsets), experts, (uint32_t)rows}, (uint32_t)x_rows, (uint32_t)width,
-                           vectors(x, x_stride, dtype)};
+                           {static_cast<const int32_t*>(offsets), experts, (uint32_t)rows}, (uint32_t)x_rows, (uint32_t)width};
     const auto s = static_cast<hipStream_t>(stream);
     const dim3 grid((uint32_t)blocks, (uint32_t)ceil_div(width, 64));
     switch (dtype) {
@@ -795,7 +791,7 @@ extern "C" int mint_squares8(const void* w, int64_t w_matrix, int64_t w_stride, 
     if (q_stride < (int64_t)(per_row * 128)) return MINT_ERR_GEOMETRY;
     if (blocks > 0x7FFFFFFFull / 256) return MINT_ERR_TOO_LARGE;
     const SquaresArgs a = {w, static_cast<uint8_t*>(q), static_cast<float*>(scale), w_matrix, w_stride, q_matrix, q_stride, (uint32_t)rows,
-                           (uint32_t)depth, (uint32_t)per_row, vectors(w, w_stride, dtype) && w_matrix % 8 == 0};
+                           (uint32_t)depth, (uint32_t)per_row};
     const auto s = static_cast<hipStream_t>(stream);
     const dim3 grid((uint32_t)blocks, matrices);
     switch (dtype) {
@@ -836,14 +832,12 @@ extern "C" int mint_product8(const mint_product_op* op, void* stream) {
     if (need && (op->workspace_bytes < need || !op->workspace)) return MINT_ERR_STAGING;
     if (need && !aligned_to(reinterpret_cast<void*>(op->workspace), 16)) return MINT_ERR_ALIGN;
     const auto s = static_cast<hipStream_t>(stream);
-    const bool whole = vectors(reinterpret_cast<void*>(op->out), op->out_stride, op->dtype) && op->out_matrix % 8 == 0;
     ProductArgs a = {reinterpret_cast<const uint8_t*>(op->x), reinterpret_cast<const uint8_t*>(op->w),
                      reinterpret_cast<const float*>(op->sx), reinterpret_cast<const float*>(op->sw), reinterpret_cast<void*>(op->out),
                      reinterpret_cast<const int32_t*>(op->tokens),
                      {reinterpret_cast<const int32_t*>(op->offsets), op->experts, (uint32_t)(along ? op->group_rows : op->rows)},
                      op->x_stride, op->w_stride, op->w_matrix, op->out_stride, op->out_matrix, op->sx_row, op->sx_block, op->sw_matrix,
-                     op->sw_row, op->sw_block, (uint32_t)op->x_rows, (uint32_t)op->rows, (uint32_t)op->cols, (uint32_t)op->depth, 0, 0, whole,
-                     raw && vectors(reinterpret_cast<void*>(op->x), op->x_stride, op->x_dtype)};
+                     op->sw_row, op->sw_block, (uint32_t)op->x_rows, (uint32_t)op->rows, (uint32_t)op->cols, (uint32_t)op->depth, 0, 0};
     const uint32_t matrices = matrices_of(*op);
     int x_dtype = op->x_dtype;
     if (need && some) {

@@ -16,7 +16,6 @@ struct CombineArgs {
     void* out;
     int64_t row_stride, out_stride;
     uint32_t n_rows, tokens, topk, width, chunks;     // chunks of 64 lanes' elements to a row
-    uint32_t whole;
 };
 constexpr int kCombineV = 8, kCombineWaves = 4;
 
@@ -28,7 +27,6 @@ __global__ void __launch_bounds__(64 * kCombineWaves) combine_kernel(CombineArgs
     const uint64_t unit = (uint64_t)blockIdx.x * kCombineWaves + __builtin_amdgcn_readfirstlane(wave_in_block());
     const uint32_t token = (uint32_t)(unit / a.chunks), at = ((uint32_t)(unit % a.chunks) * 64u + lane_id()) * V;
     if (token >= a.tokens || at >= a.width) return;
-    const bool whole = a.whole && at + V <= a.width;
     const int64_t left = (int64_t)a.width - at;
     const int32_t* const slots = a.slots + (uint64_t)token * a.topk;
     const float* const weights = a.weights ? a.weights + (uint64_t)token * a.topk : nullptr;
@@ -45,14 +43,14 @@ __global__ void __launch_bounds__(64 * kCombineWaves) combine_kernel(CombineArgs
             w[u] = there ? weights ? weights[j] : 1.0f : 0.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i) v[u][i] = 0.0f;
-            if (there) load_elements<DT, V>(static_cast<const T*>(a.rows) + slot * a.row_stride + at, whole, left, v[u]);
+            if (there) load_elements<DT, V>(static_cast<const T*>(a.rows) + slot * a.row_stride + at, left, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int i = 0; i < V; ++i) sum[i] = fmaf(w[u], v[u][i], sum[i]);
     }
-    store_elements<DT, V>(static_cast<T*>(a.out) + token * a.out_stride + at, whole, left, sum);
+    store_elements<DT, V>(static_cast<T*>(a.out) + token * a.out_stride + at, left, sum);
 }
 
 struct CombineGradArgs {
@@ -62,7 +60,7 @@ struct CombineGradArgs {
     void* d_rows;
     float* d_weights;
     int64_t d_stride, row_stride, d_row_stride;
-    uint32_t n_rows, tokens, topk, width, whole;
+    uint32_t n_rows, tokens, topk, width;
 };
 // A thread block has a token; those behind the tokens' clear the rows that are no token's.
 constexpr uint32_t kClearing = 128;
@@ -76,8 +74,7 @@ __global__ void __launch_bounds__(64 * kCombineWaves) combine_grad_kernel(Combin
         const float none[V] = {};
         for (uint64_t row = (uint32_t)max(*a.ends, 0) + (blockIdx.x - a.tokens); row < a.n_rows; row += kClearing)
             for (uint32_t at = threadIdx.x * V; at < a.width; at += step)
-                store_elements<DT, V>(static_cast<T*>(a.d_rows) + row * a.d_row_stride + at, a.whole && at + V <= a.width, (int64_t)a.width - at,
-                                      none);
+                store_elements<DT, V>(static_cast<T*>(a.d_rows) + row * a.d_row_stride + at, (int64_t)a.width - at, none);
         return;
     }
     const uint32_t token = blockIdx.x;
@@ -92,14 +89,13 @@ __global__ void __launch_bounds__(64 * kCombineWaves) combine_grad_kernel(Combin
             w[u] = slot[u] < 0 ? 0.0f : a.weights ? a.weights[(uint64_t)token * a.topk + j0 + u] : 1.0f;
         }
         for (uint32_t at = threadIdx.x * V; at < a.width; at += step) {
-            const bool whole = a.whole && at + V <= a.width;
             const int64_t left = (int64_t)a.width - at;
             float d[V], v[4][V];
-            load_elements<DT, V>(static_cast<const T*>(a.d_out) + token * a.d_stride + at, whole, left, d);
+            load_elements<DT, V>(static_cast<const T*>(a.d_out) + token * a.d_stride + at, left, d);
             if (a.d_weights)
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (slot[u] >= 0) load_elements<DT, V>(static_cast<const T*>(a.rows) + slot[u] * a.row_stride + at, whole, left, v[u]);
+                    if (slot[u] >= 0) load_elements<DT, V>(static_cast<const T*>(a.rows) + slot[u] * a.row_stride + at, left, v[u]);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (slot[u] >= 0) {
@@ -109,7 +105,7 @@ __global__ void __launch_bounds__(64 * kCombineWaves) combine_grad_kernel(Combin
                     float scaled[V];
 #pragma unroll
                     for (int i = 0; i < V; ++i) scaled[i] = w[u] * d[i];
-                    store_elements<DT, V>(static_cast<T*>(a.d_rows) + slot[u] * a.d_row_stride + at, whole, left, scaled);
+                    store_elements<DT, V>(static_cast<T*>(a.d_rows) + slot[u] * a.d_row_stride + at, left, scaled);
                 }
         }
         if (a.d_weights) {
@@ -129,9 +125,6 @@ __global__ void __launch_bounds__(64 * kCombineWaves) combine_grad_kernel(Combin
     }
 }
 
-bool vectors(const void* p, int64_t stride, int dtype) {
-    return !p || (aligned_to(p, kCombineV * element_bytes(dtype)) && stride % kCombineV == 0);
-}
 bool known(int dtype) { return dtype == MINT_F16 || dtype == MINT_BF16 || dtype == MINT_F32; }
 
 }  // namespace
@@ -149,8 +142,7 @@ extern "C" int mint_combine(const void* rows, int64_t row_stride, uint64_t n_row
     const uint64_t blocks = ceil_div(tokens * chunks, kCombineWaves);
     if (blocks > 0x7FFFFFFFull / (64 * kCombineWaves)) return MINT_ERR_TOO_LARGE;
     const CombineArgs a = {rows, static_cast<const int32_t*>(slots), static_cast<const float*>(weights), out, row_stride, out_stride,
-                           (uint32_t)n_rows, (uint32_t)tokens, topk, width, chunks,
-                           vectors(rows, row_stride, dtype) && vectors(out, out_stride, dtype)};
+                           (uint32_t)n_rows, (uint32_t)tokens, topk, width, chunks};
     const auto s = static_cast<hipStream_t>(stream);
     switch (dtype) {
         case MINT_F16: return Launch<&combine_kernel<DT_F16>>::go((uint32_t)blocks, 64 * kCombineWaves, 0, s, a);
@@ -169,8 +161,7 @@ extern "C" int mint_combine_grad(const void* d_out, int64_t d_stride, const void
     if ((tokens && (!slots || !d_out)) || (n_rows && (!d_rows || !rows_used || (d_weights && !rows)))) return MINT_ERR_ARG;
     const CombineGradArgs a = {d_out, rows, static_cast<const int32_t*>(slots), static_cast<const int32_t*>(rows_used),
                                static_cast<const float*>(weights), d_rows, static_cast<float*>(d_weights), d_stride, row_stride, d_row_stride,
-                               (uint32_t)n_rows, (uint32_t)tokens, topk, width,
-                               vectors(d_out, d_stride, dtype) && vectors(rows, row_stride, dtype) && vectors(d_rows, d_row_stride, dtype)};
+                               (uint32_t)n_rows, (uint32_t)tokens, topk, width};
     const auto s = static_cast<hipStream_t>(stream);
     const uint32_t blocks = (uint32_t)(tokens + (n_rows ? kClearing : 0));
     switch (dtype) {

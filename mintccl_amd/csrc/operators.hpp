@@ -27,13 +27,13 @@ template <> struct Elem<DT_BF16> {
     static __device__ __forceinline__ type round(float v) { return (__bf16)v; }
 };
 
-// N consecutive elements as 32-bit numbers.  `whole`: they may be loaded as vectors (the address
-// is aligned to them and all N are there); else the first `left` of them, one by one, zeros behind.
+// N consecutive elements as 32-bit numbers, of which the first `left` are there (zeros for the others): one vector, at any
+// address, where all are.  (Vectors that are not aligned to their size take the same instructions.)
 template <int DT, int N>
-__device__ __forceinline__ void load_elements(const typename Elem<DT>::type* p, bool whole, int64_t left, float (&v)[N]) {
+__device__ __forceinline__ void load_elements(const typename Elem<DT>::type* p, int64_t left, float (&v)[N]) {
     using T = typename Elem<DT>::type;
-    typedef T vec __attribute__((ext_vector_type(N)));
-    if (whole) {
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    if (left >= N) {
         const vec w = *(MINT_GLOBAL const vec*)as_global(p);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = Elem<DT>::load(w[i]);
@@ -43,10 +43,10 @@ __device__ __forceinline__ void load_elements(const typename Elem<DT>::type* p, 
     }
 }
 template <int DT, int N>
-__device__ __forceinline__ void store_elements(typename Elem<DT>::type* p, bool whole, int64_t left, const float (&v)[N]) {
+__device__ __forceinline__ void store_elements(typename Elem<DT>::type* p, int64_t left, const float (&v)[N]) {
     using T = typename Elem<DT>::type;
-    typedef T vec __attribute__((ext_vector_type(N)));
-    if (whole) {
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    if (left >= N) {
         vec w;
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = Elem<DT>::round(v[i]);
@@ -109,6 +109,5 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
 
 inline bool aligned_to(const void* p, uint64_t bytes) { return reinterpret_cast<uint64_t>(p) % bytes == 0; }
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
-inline int element_bytes(int dtype) { return dtype == MINT_F32 ? 4 : 2; }
 
 }  // namespace mint

@@ -38,8 +38,7 @@ struct RouteArgs {
     int64_t row_stride;
     uint32_t tokens, experts, topk, groups, kept, group_top;
     float scale;
-    uint32_t whole;          // a lane's logits may be loaded as one vector
-    uint32_t bias_whole, sigmoid, renormalise;
+    uint32_t sigmoid, renormalise;
 };
 
 // What LANES lanes have together: 16 (a row, whose lanes the additions' cross-lane operands reach in four steps) or all 64.
@@ -92,10 +91,10 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
     const bool live = token < a.tokens;                      // (all lanes go along: they are reached by others)
     const T* const row = static_cast<const T*>(a.logits) + (int64_t)(live ? token : a.tokens - 1) * a.row_stride;
     float x[V], bias[V];
-    load_elements<DT, V>(row + first, a.whole && first + V <= a.experts, (int64_t)a.experts - first, x);
+    load_elements<DT, V>(row + first, (int64_t)a.experts - first, x);
 #pragma unroll
     for (int i = 0; i < V; ++i) bias[i] = 0.0f;
-    if (a.bias) load_elements<DT_F32, V>(a.bias + first, a.bias_whole && first + V <= a.experts, (int64_t)a.experts - first, bias);
+    if (a.bias) load_elements<DT_F32, V>(a.bias + first, (int64_t)a.experts - first, bias);
     uint32_t key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -239,7 +238,7 @@ struct RouteGradArgs {
     int64_t row_stride, d_stride;
     uint32_t tokens, experts, topk;
     float scale;
-    uint32_t whole, d_whole, sigmoid, renormalise;
+    uint32_t sigmoid, renormalise;
 };
 template <int DT, int V>
 __global__ void __launch_bounds__(64 * kRouteWaves) route_grad_kernel(RouteGradArgs a) {
@@ -266,7 +265,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_grad_kernel(RouteGradA
     } else {
         float x[V], m = l;
         if (!a.renormalise) {
-            load_elements<DT, V>(row + first, a.whole && first + V <= a.experts, (int64_t)a.experts - first, x);
+            load_elements<DT, V>(row + first, (int64_t)a.experts - first, x);
 #pragma unroll
             for (int i = 0; i < V; ++i) m = first + i < a.experts ? fmaxf(m, x[i]) : m;
         }
@@ -298,7 +297,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_grad_kernel(RouteGradA
         for (int i = 0; i < V; ++i) out[i] += first + i == e ? more : 0.0f;
     }
     T* const to = static_cast<T*>(a.d_logits) + (int64_t)token * a.d_stride + first;
-    store_elements<DT, V>(to, a.d_whole && first + V <= a.experts, (int64_t)a.experts - first, out);
+    store_elements<DT, V>(to, (int64_t)a.experts - first, out);
 }
 
 // ---- assignment: a counting sort of the pairs by expert, pairs of an expert in their own order -----
@@ -499,12 +498,9 @@ extern "C" int mint_route(const mint_route_op* op, void* stream) {
         return MINT_ERR_GEOMETRY;
     if (op->tokens == 0) return MINT_OK;
     if (!op->logits || !op->weights || !op->chosen) return MINT_ERR_ARG;
-    const uint32_t vector = values_per_lane(op->experts, lanes_of(op->experts, op->topk)) * element_bytes(op->dtype);
-    const bool whole = aligned_to(reinterpret_cast<void*>(op->logits), vector) && op->row_stride * element_bytes(op->dtype) % vector == 0;
-    const bool bias_whole = aligned_to(reinterpret_cast<void*>(op->bias), values_per_lane(op->experts, lanes_of(op->experts, op->topk)) * 4);
     const RouteArgs a = {reinterpret_cast<const void*>(op->logits), reinterpret_cast<const float*>(op->bias),
                          reinterpret_cast<float*>(op->weights), reinterpret_cast<int32_t*>(op->chosen), op->row_stride,
-                         (uint32_t)op->tokens, op->experts, op->topk, op->groups, op->kept, op->group_top, op->scale, whole, bias_whole,
+                         (uint32_t)op->tokens, op->experts, op->topk, op->groups, op->kept, op->group_top, op->scale,
                          op->score == MINT_SCORE_SIGMOID, op->renormalise != 0};
     return launch_route(a, op->dtype, static_cast<hipStream_t>(stream));
 }
@@ -513,12 +509,9 @@ extern "C" int mint_route_grad(const mint_route_op* op, uint64_t d_weights, uint
     if (!op || !routable(op->tokens, op->experts, op->topk, op->dtype, op->score)) return MINT_ERR_ARG;
     if (op->tokens == 0) return MINT_OK;
     if (!op->logits || !op->chosen || !d_weights || !d_logits) return MINT_ERR_ARG;
-    const uint32_t size = element_bytes(op->dtype), vector = values_per_lane(op->experts, 64) * size;
-    const bool whole = aligned_to(reinterpret_cast<void*>(op->logits), vector) && op->row_stride * size % vector == 0;
-    const bool d_whole = aligned_to(reinterpret_cast<void*>(d_logits), vector) && d_stride * size % vector == 0;
     const RouteGradArgs a = {reinterpret_cast<const void*>(op->logits), reinterpret_cast<const float*>(d_weights),
                              reinterpret_cast<const int32_t*>(op->chosen), reinterpret_cast<void*>(d_logits), op->row_stride, d_stride,
-                             (uint32_t)op->tokens, op->experts, op->topk, op->scale, whole, d_whole,
+                             (uint32_t)op->tokens, op->experts, op->topk, op->scale,
                              op->score == MINT_SCORE_SIGMOID, op->renormalise != 0};
     return launch_route_grad(a, op->dtype, static_cast<hipStream_t>(stream));
 }
