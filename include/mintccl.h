@@ -593,6 +593,24 @@ typedef struct {
 size_t mint_product8_workspace(const mint_product_op* op);
 int mint_product8(const mint_product_op* op, void* stream);
 
+/* The gradient of the weights of a product: d^T x of d (rows, cols) and x (rows,
+ * depth; with `tokens` row i is x[tokens[i]]), both rounded as by mint_columns8
+ * and multiplied as MINT_PRODUCT_GRADIENT.  With `offsets` there are `experts`
+ * results, out_matrix elements apart.  workspace: mint_weight_grad8_workspace()
+ * bytes, 16-byte aligned. */
+typedef struct {
+    uint64_t d, x, out;
+    uint64_t tokens;       /* int32 (rows), or 0 */
+    uint64_t offsets;      /* int32 (experts + 1), or 0 */
+    uint64_t workspace, workspace_bytes;
+    uint64_t rows, x_rows, cols, depth;
+    int64_t d_stride, x_stride, out_stride, out_matrix;
+    uint32_t experts;
+    int32_t d_dtype, x_dtype, dtype;   /* of d, x and out: MINT_F16, MINT_BF16, MINT_F32 */
+} mint_weight_grad_op;
+size_t mint_weight_grad8_workspace(const mint_weight_grad_op* op);
+int mint_weight_grad8(const mint_weight_grad_op* op, void* stream);
+
 /* out[t] = sum over j of weights[t, j] * rows[slots[t, j]] (weights 0: all 1), in
  * 32 bits; a slot outside the rows adds nothing.  The gradients: d_rows of every
  * row (those that are no token's, from *rows_used (int32) on, are cleared), and

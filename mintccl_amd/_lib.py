@@ -117,6 +117,15 @@ class ProductOp(ctypes.Structure):
         ("x_dtype", ctypes.c_int32)]
 
 
+class WeightGradOp(ctypes.Structure):
+    """``mint_weight_grad_op``."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("d", "x", "out", "tokens", "offsets", "workspace", "workspace_bytes", "rows",
+                                               "x_rows", "cols", "depth")] + [
+        (n, ctypes.c_int64) for n in ("d_stride", "x_stride", "out_stride", "out_matrix")] + [
+        ("experts", ctypes.c_uint32), ("d_dtype", ctypes.c_int32), ("x_dtype", ctypes.c_int32),
+        ("dtype", ctypes.c_int32)]
+
+
 # name -> (restype, argtypes); every symbol include/mintccl.h declares
 _vp, _sz, _u64, _u32, _i = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint64,
                             ctypes.c_uint32, ctypes.c_int)
@@ -158,6 +167,8 @@ SYMBOLS = {
     "mint_squares8": (_i, [_vp, _i64, _i64, _u32, _u64, _u64, _i, _vp, _i64, _i64, _vp, _vp]),
     "mint_product8_workspace": (_sz, [ctypes.POINTER(ProductOp)]),
     "mint_product8": (_i, [ctypes.POINTER(ProductOp), _vp]),
+    "mint_weight_grad8_workspace": (_sz, [ctypes.POINTER(WeightGradOp)]),
+    "mint_weight_grad8": (_i, [ctypes.POINTER(WeightGradOp), _vp]),
     "mint_combine": (_i, [_vp, _i64, _u64, _vp, _vp, _u64, _u32, _u32, _vp, _i64, _i, _vp]),
     "mint_combine_grad": (_i, [_vp, _i64, _vp, _i64, _u64, _vp, _vp, _vp, _u64, _u32, _u32, _vp, _i64, _vp,
                                _i, _vp]),
@@ -360,10 +371,9 @@ def host():
 
 _experts = None
 #: the entry points that the module of the expert layer's operators calls, in the order of its bind()
-EXPERT_SYMBOLS = ("mint_route", "mint_route_grad", "mint_assign_workspace", "mint_assign", "mint_rows8",
-                  "mint_columns8_blocks", "mint_columns8", "mint_squares8", "mint_product8_workspace",
-                  "mint_product8", "mint_combine",
-                  "mint_combine_grad")
+EXPERT_SYMBOLS = ("mint_route", "mint_route_grad", "mint_assign_workspace", "mint_assign", "mint_rows8", "mint_squares8",
+                  "mint_product8_workspace", "mint_product8", "mint_weight_grad8_workspace", "mint_weight_grad8",
+                  "mint_combine", "mint_combine_grad")
 
 
 def experts():
@@ -376,7 +386,8 @@ def experts():
             raise RuntimeError(f"{EXPERT_HOST_PATH} is missing: run `python -c 'import __graft_entry__ as g; "
                                "g.build()'` in the repository root. There is no Python fallback.")
         from . import _expert_host as module
-        if (module.ROUTE_BYTES, module.PRODUCT_BYTES) != (ctypes.sizeof(RouteOp), ctypes.sizeof(ProductOp)):
+        if (module.ROUTE_BYTES, module.PRODUCT_BYTES, module.WEIGHT_GRAD_BYTES) != tuple(
+                map(ctypes.sizeof, (RouteOp, ProductOp, WeightGradOp))):
             raise RuntimeError(f"{EXPERT_HOST_PATH} was built for other descriptors: rebuild it")
         module.bind(check, *[ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in EXPERT_SYMBOLS])
         _experts = module

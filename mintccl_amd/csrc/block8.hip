@@ -122,13 +122,17 @@ struct ColumnsArgs {
     Groups groups;
     uint32_t x_rows, width;
 };
-// A thread block has 64 columns of 128 rows of an expert (fewer where it has no more: zeros follow). They turn in LDS.
+// A thread block has 64 columns of 128 rows of an expert (fewer where it has no more: zeros follow), which turn in LDS.
+// Two matrices can share a launch: the columns of the second one come behind the first one's.
 template <int DT>
-__global__ void __launch_bounds__(256) columns8_kernel(ColumnsArgs a) {
+__global__ void __launch_bounds__(256) columns8_kernel(ColumnsArgs a0, ColumnsArgs a1) {
     using T = typename Elem<DT>::type;
     __shared__ __attribute__((aligned(16))) uint8_t turned[64][128 + 16];
     __shared__ uint32_t most[4][64];
-    const uint32_t block = blockIdx.x, c0 = blockIdx.y * 64;
+    const uint32_t first_tiles = (a0.width + 63) / 64, block = blockIdx.x;
+    const bool second = blockIdx.y >= first_tiles;
+    const ColumnsArgs& a = second ? a1 : a0;
+    const uint32_t c0 = (blockIdx.y - (second ? first_tiles : 0u)) * 64;
     const Tile t = find_tile(a.groups, block, 128, false);
     if (!t.found) return;
     const uint32_t r0 = t.begin + (block - t.first) * 128;
@@ -699,8 +703,12 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
 // Few rows: at most 32 for each weight matrix, on the average (24 x 4096 x 4096: 7.8 us, with tiles of 64 x 64 11.8; at 64 rows
 // 12.8 and 11.8).
 bool few_rows(uint64_t rows, uint32_t matrices) { return rows <= 32ull * matrices; }
-// ... and so few that the rounding is done on the way
-bool rounded_on_the_way(uint64_t rows, uint32_t matrices) { return rows <= 16ull * matrices; }
+// ... and so few that the rounding is done on the way: 256 blocks of 128 for each weight matrix (all thread blocks
+// do that work again, 0.5 us for 32 blocks, and save a launch: with a depth and 4096 columns of 4096, 1 row 5.7 us for 10.3, 8 rows 9.2
+// for 10.6, 12 rows 11.6 for 10.5)
+bool rounded_on_the_way(uint64_t rows, uint64_t depth, uint32_t matrices) {
+    return rows <= 16ull * matrices && rows * ceil_div(depth, 128) <= 256ull * matrices;
+}
 template <int OUT, int X, int MT, int KWAYS>
 int go_thin_ways(ProductArgs a, hipStream_t stream) {
     a.col_tiles = (uint32_t)ceil_div(a.cols, 16 * (kThinWaves / KWAYS));
@@ -759,25 +767,99 @@ extern "C" int mint_rows8(const void* x, int64_t x_stride, uint64_t rows, uint64
 
 extern "C" size_t mint_columns8_blocks(uint64_t rows, uint32_t experts) { return ceil_div(rows, 128) + experts; }
 
+namespace {
+int go_columns(const ColumnsArgs& a, const ColumnsArgs& b, int dtype, uint32_t blocks, hipStream_t s) {
+    const dim3 grid(blocks, (uint32_t)(ceil_div(a.width, 64) + ceil_div(b.width, 64)));
+    switch (dtype) {
+        case MINT_F16: return Launch<&columns8_kernel<DT_F16>>::go(grid, 256, 0, s, a, b);
+        case MINT_BF16: return Launch<&columns8_kernel<DT_BF16>>::go(grid, 256, 0, s, a, b);
+        default: return Launch<&columns8_kernel<DT_F32>>::go(grid, 256, 0, s, a, b);
+    }
+}
+constexpr uint64_t kMostColumns = 32767ull * 64;
+}  // namespace
+
 extern "C" int mint_columns8(const void* x, int64_t x_stride, uint64_t x_rows, uint64_t width, int dtype, const void* tokens, uint64_t rows,
                              const void* offsets, uint32_t experts, void* q, int64_t q_stride, void* scale, void* stream) {
     if (!known(dtype) || (!offsets && experts)) return MINT_ERR_ARG;
-    if (rows > kMostRows || x_rows > kMostRows || width > 65535ull * 64) return MINT_ERR_TOO_LARGE;
+    if (rows > kMostRows || x_rows > kMostRows || width > kMostColumns) return MINT_ERR_TOO_LARGE;
     if (rows == 0 || width == 0) return MINT_OK;
-    if (!x || !q || !scale || (!tokens && x_rows < rows)) return MINT_ERR_ARG;
+    if (!x || !q || !scale || (!tokens && x_rows < rows) || x_rows == 0) return MINT_ERR_ARG;
     const uint64_t blocks = mint_columns8_blocks(rows, experts);
     if (!aligned_to(q, 16) || q_stride % 16) return MINT_ERR_ALIGN;
     if (q_stride < (int64_t)(blocks * 128)) return MINT_ERR_GEOMETRY;
     if (blocks > 0x7FFFFFFFull / 256) return MINT_ERR_TOO_LARGE;
     const ColumnsArgs a = {x, static_cast<const int32_t*>(tokens), static_cast<uint8_t*>(q), static_cast<float*>(scale), x_stride, q_stride,
                            {static_cast<const int32_t*>(offsets), experts, (uint32_t)rows}, (uint32_t)x_rows, (uint32_t)width};
-    const auto s = static_cast<hipStream_t>(stream);
-    const dim3 grid((uint32_t)blocks, (uint32_t)ceil_div(width, 64));
-    switch (dtype) {
-        case MINT_F16: return Launch<&columns8_kernel<DT_F16>>::go(grid, 256, 0, s, a);
-        case MINT_BF16: return Launch<&columns8_kernel<DT_BF16>>::go(grid, 256, 0, s, a);
-        default: return Launch<&columns8_kernel<DT_F32>>::go(grid, 256, 0, s, a);
+    return go_columns(a, ColumnsArgs{}, dtype, (uint32_t)blocks, static_cast<hipStream_t>(stream));
+}
+
+namespace {
+// 8-bit numbers and scales of both sides, one behind the other: (cols, blocks * 128), (depth, blocks * 128), scales
+struct GradientRoom {
+    uint64_t blocks, x, scales, x_scales, bytes;
+    explicit GradientRoom(const mint_weight_grad_op& op) {
+        blocks = mint_columns8_blocks(op.rows, op.experts);
+        x = op.cols * blocks * 128;
+        scales = x + op.depth * blocks * 128;
+        x_scales = scales + blocks * op.cols * 4;
+        bytes = x_scales + blocks * op.depth * 4;
     }
+};
+}  // namespace
+
+extern "C" size_t mint_weight_grad8_workspace(const mint_weight_grad_op* op) { return op && op->rows ? GradientRoom(*op).bytes : 0; }
+
+extern "C" int mint_weight_grad8(const mint_weight_grad_op* op, void* stream) {
+    if (!op || !known(op->dtype) || !known(op->d_dtype) || !known(op->x_dtype) || (!op->offsets && op->experts)) return MINT_ERR_ARG;
+    if (op->rows > kMostRows || op->x_rows > kMostRows || op->cols > kMostColumns || op->depth > kMostColumns || op->experts > 65535)
+        return MINT_ERR_TOO_LARGE;
+    if (op->cols == 0 || op->depth == 0) return MINT_OK;
+    if (!op->out || (op->rows && (!op->d || !op->x || op->x_rows == 0 || (!op->tokens && op->x_rows < op->rows)))) return MINT_ERR_ARG;
+    const GradientRoom room(*op);
+    if (room.blocks > 0x7FFFFFFFull / 256) return MINT_ERR_TOO_LARGE;
+    auto* const q = reinterpret_cast<uint8_t*>(op->workspace);
+    const int64_t wide = (int64_t)room.blocks * 128;
+    if (op->rows) {
+        if (!q || op->workspace_bytes < room.bytes) return MINT_ERR_STAGING;
+        if (!aligned_to(q, 16)) return MINT_ERR_ALIGN;
+        const Groups groups = {reinterpret_cast<const int32_t*>(op->offsets), op->experts, (uint32_t)op->rows};
+        const ColumnsArgs d = {reinterpret_cast<const void*>(op->d), nullptr, q, reinterpret_cast<float*>(q + room.scales), op->d_stride, wide, groups,
+                               (uint32_t)op->rows, (uint32_t)op->cols};
+        const ColumnsArgs x = {reinterpret_cast<const void*>(op->x), reinterpret_cast<const int32_t*>(op->tokens), q + room.x,
+                               reinterpret_cast<float*>(q + room.x_scales), op->x_stride, wide, groups, (uint32_t)op->x_rows, (uint32_t)op->depth};
+        const auto s = static_cast<hipStream_t>(stream);
+        int err;
+        if (op->d_dtype == op->x_dtype) {
+            err = go_columns(d, x, op->d_dtype, (uint32_t)room.blocks, s);
+        } else {
+            err = go_columns(d, ColumnsArgs{}, op->d_dtype, (uint32_t)room.blocks, s);
+            if (err == MINT_OK) err = go_columns(x, ColumnsArgs{}, op->x_dtype, (uint32_t)room.blocks, s);
+        }
+        if (err != MINT_OK) return err;
+    }
+    mint_product_op p = {};
+    p.kind = MINT_PRODUCT_GRADIENT;
+    p.dtype = op->dtype;
+    p.x_dtype = MINT_BYTES;
+    p.x = reinterpret_cast<uint64_t>(q);
+    p.w = reinterpret_cast<uint64_t>(q + room.x);
+    p.sx = reinterpret_cast<uint64_t>(q + room.scales);
+    p.sw = reinterpret_cast<uint64_t>(q + room.x_scales);
+    p.out = op->out;
+    p.offsets = op->offsets;
+    p.rows = p.x_rows = op->cols;
+    p.cols = op->depth;
+    p.depth = op->rows ? (uint64_t)wide : 0;
+    p.group_rows = op->rows;
+    p.x_stride = p.w_stride = wide;
+    p.out_stride = op->out_stride;
+    p.out_matrix = op->out_matrix;
+    p.sx_row = p.sw_row = 1;
+    p.sx_block = (int64_t)op->cols;
+    p.sw_block = (int64_t)op->depth;
+    p.experts = op->experts;
+    return mint_product8(&p, stream);
 }
 
 extern "C" int mint_squares8(const void* w, int64_t w_matrix, int64_t w_stride, uint32_t matrices, uint64_t rows, uint64_t depth, int dtype,
@@ -805,7 +887,7 @@ namespace {
 uint32_t matrices_of(const mint_product_op& op) { return op.offsets ? op.experts : 1; }
 // 8-bit numbers and scales of activations that come as they are, where that takes a launch of its own
 size_t rounded_bytes(const mint_product_op& op) {
-    if (op.kind != MINT_PRODUCT_ROWS || op.x_dtype == MINT_BYTES || rounded_on_the_way(op.rows, matrices_of(op))) return 0;
+    if (op.kind != MINT_PRODUCT_ROWS || op.x_dtype == MINT_BYTES || rounded_on_the_way(op.rows, op.depth, matrices_of(op))) return 0;
     return (size_t)op.x_rows * ceil_div(op.depth, 128) * 132;
 }
 }  // namespace

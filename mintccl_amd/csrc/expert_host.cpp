@@ -24,11 +24,11 @@ struct Native {
     decltype(&mint_assign_workspace) assign_workspace;
     decltype(&mint_assign) assign;
     decltype(&mint_rows8) rows8;
-    decltype(&mint_columns8_blocks) columns8_blocks;
-    decltype(&mint_columns8) columns8;
     decltype(&mint_squares8) squares8;
     decltype(&mint_product8_workspace) product8_workspace;
     decltype(&mint_product8) product8;
+    decltype(&mint_weight_grad8_workspace) weight_grad8_workspace;
+    decltype(&mint_weight_grad8) weight_grad8;
     decltype(&mint_combine) combine;
     decltype(&mint_combine_grad) combine_grad;
     PyObject* check;             // _lib.check(code, where): raises MintError
@@ -474,54 +474,42 @@ PyObject* host_weight_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
         const int d_code = code_of(d.scalar_type(), "grad"), x_code = code_of(x.scalar_type(), "x");
         const bool by_expert = !a.none(2), gather = a.truth(4);
         if (gather && !by_expert) refuse(PyExc_ValueError, "gather needs an assignment");
-        const int64_t rows = d.size(0), cols = d.size(1), depth = x.size(1), code = a.none(5) ? (int64_t)MINT_F32 : a.integer(5, "dtype", 0, 2);
-        const void *offsets = nullptr, *tokens = nullptr;
+        mint_weight_grad_op op = {};
+        op.d_dtype = d_code;
+        op.x_dtype = x_code;
+        op.dtype = a.none(5) ? (int32_t)MINT_F32 : (int32_t)a.integer(5, "dtype", 0, 2);
+        const int64_t rows = d.size(0), cols = d.size(1), depth = x.size(1);
         int64_t experts = 0;
         if (by_expert) {
-            const Tensor &o = a.tensor(2, "offsets"), &order = a.tensor(3, "tokens");
-            plan_of(x, o, order);
+            const Tensor &offsets = a.tensor(2, "offsets"), &order = a.tensor(3, "tokens");
+            plan_of(x, offsets, order);
             if (order.size(0) != rows) refuse(PyExc_ValueError, "grad must have a row for each place of the assignment");
-            experts = o.size(0) - 1;
+            experts = offsets.size(0) - 1;
             if (experts > 65535) refuse(PyExc_ValueError, "at most 65535 experts");
-            offsets = o.data_ptr();
-            if (gather) tokens = order.data_ptr();
+            op.offsets = address(offsets);
+            if (gather) op.tokens = address(order);
         }
         if (gather ? x.size(0) == 0 && rows != 0 : x.size(0) != rows) refuse(PyExc_ValueError, "x and grad have different numbers of rows");
         OnDevice on(x.get_device());
-        const Tensor out = by_expert ? empty(x, {experts, cols, depth}, type_of(code)) : empty(x, {cols, depth}, type_of(code));
-        const int64_t most = (int64_t)native.columns8_blocks((uint64_t)rows, (uint32_t)experts), wide = most * 128;
-        const Tensor dq = empty(x, {cols, wide}, at::kByte), ds = empty(x, {most, cols}, at::kFloat);
-        const Tensor xq = empty(x, {depth, wide}, at::kByte), xs = empty(x, {most, depth}, at::kFloat);
-        launch("mint_columns8", [&] {
-            return native.columns8(d.data_ptr(), d.stride(0), (uint64_t)rows, (uint64_t)cols, d_code, nullptr, (uint64_t)rows, offsets,
-                                   (uint32_t)experts, dq.data_ptr(), wide, ds.data_ptr(), on.stream);
-        });
-        launch("mint_columns8", [&] {
-            return native.columns8(x.data_ptr(), x.stride(0), (uint64_t)x.size(0), (uint64_t)depth, x_code, tokens, (uint64_t)rows, offsets,
-                                   (uint32_t)experts, xq.data_ptr(), wide, xs.data_ptr(), on.stream);
-        });
-        mint_product_op op = {};
-        op.kind = MINT_PRODUCT_GRADIENT;
-        op.x_dtype = MINT_BYTES;
-        op.dtype = (int32_t)code;
-        op.x = address(dq);
-        op.w = address(xq);
-        op.sx = address(ds);
-        op.sw = address(xs);
+        const Tensor out = by_expert ? empty(x, {experts, cols, depth}, type_of(op.dtype)) : empty(x, {cols, depth}, type_of(op.dtype));
+        op.d = address(d);
+        op.x = address(x);
         op.out = address(out);
-        op.offsets = reinterpret_cast<uint64_t>(offsets);
-        op.rows = op.x_rows = (uint64_t)cols;
-        op.cols = (uint64_t)depth;
-        op.depth = rows ? (uint64_t)wide : 0;
-        op.group_rows = (uint64_t)rows;
-        op.x_stride = op.w_stride = wide;
+        op.rows = (uint64_t)rows;
+        op.x_rows = (uint64_t)x.size(0);
+        op.cols = (uint64_t)cols;
+        op.depth = (uint64_t)depth;
+        op.d_stride = d.stride(0);
+        op.x_stride = x.stride(0);
         op.out_stride = depth;
         op.out_matrix = cols * depth;
-        op.sx_row = op.sw_row = 1;
-        op.sx_block = cols;
-        op.sw_block = depth;
         op.experts = (uint32_t)experts;
-        launch("mint_product8", [&] { return native.product8(&op, on.stream); });
+        Tensor room;
+        if ((op.workspace_bytes = native.weight_grad8_workspace(&op))) {
+            room = empty(x, {(int64_t)op.workspace_bytes}, at::kByte);
+            op.workspace = address(room);
+        }
+        launch("mint_weight_grad8", [&] { return native.weight_grad8(&op, on.stream); });
         return wrap(out);
     });
 }
@@ -631,5 +619,6 @@ PyMODINIT_FUNC PyInit__expert_host(void) {
     if (!m) return nullptr;
     PyModule_AddIntConstant(m, "ROUTE_BYTES", sizeof(mint_route_op));
     PyModule_AddIntConstant(m, "PRODUCT_BYTES", sizeof(mint_product_op));
+    PyModule_AddIntConstant(m, "WEIGHT_GRAD_BYTES", sizeof(mint_weight_grad_op));
     return m;
 }
