@@ -689,7 +689,7 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
                 wide = 1.2f * ceil_div(tiles(128, 256), 256), large = 2.0f * ceil_div(tiles(256, 256), 256);
     if (t64 <= t128 && t64 <= wide && t64 <= large) return go_tiles<OUT, 64, 64, 4, 4, ROWS_W, ALONG>(a, matrices, stream);
     if constexpr (OUT == DT_F32) {       // (operands widened to 16 bits leave no registers for more)
-        return go_tiles<OUT, 128, 128, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
+        return go_tiles<OUT, 128, 256, 2, 3, ROWS_W, ALONG>(a, matrices, stream);
     } else {
         if (t128 <= wide && t128 <= large) {
             if (n128 <= 256) return go_tiles<OUT, 128, 128, 4, 4, ROWS_W, ALONG>(a, matrices, stream);

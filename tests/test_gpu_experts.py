@@ -576,3 +576,56 @@ def test_refusals(dev):
         combine(x, plan, out=torch.zeros(4, 255, device=dev))
     with pytest.raises(TypeError, match="int32"):
         combine(x, Assignment(plan.offsets, plan.tokens, plan.slots.long()))
+
+
+@pytest.mark.parametrize("world,options", [(1, {}), (4, {"score": "sigmoid", "renormalise": True}), (8, {"renormalise": False})])
+def test_a_layer_of_experts_over_ranks(dev, world, options):
+    """Forward and backward over virtual ranks, through the collectives, against the plain layer."""
+    from mintccl_amd import experts
+    for name, off in experts.distances(world, dev, **options).items():
+        assert off < experts.FAR, (name, off)
+
+
+def test_offsets_beyond_32_bits(dev):
+    """Results and inputs of more than 2^31 elements (more than 4 GiB): the last rows are what they are alone."""
+    rows, cols = 600_001, 4096
+    x = randn(rows, 130, seed=1, dtype=torch.bfloat16).to(dev)
+    w = quantise_weight(randn(cols, 130, seed=2).to(dev))
+    y = product(x, w)
+    for at in (slice(0, 64), slice(rows // 2, rows // 2 + 64), slice(rows - 64, rows)):
+        assert torch.equal(y[at], product(x[at], w))
+    q, s = quantise(y)                                   # its input lies beyond 4 GiB
+    want = quantise(y[-3:].clone())
+    assert torch.equal(q[-3:].view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(s[-3:], want.scale)
+    del q, s
+    slots = torch.tensor([[rows - 1, 0], [rows // 2, rows - 2]], dtype=torch.int32, device=dev)
+    plan = Assignment(torch.tensor([rows], dtype=torch.int32, device=dev), slots.view(-1), slots)
+    got = combine(y, plan)
+    assert torch.equal(got, (y[slots[:, 0].long()].float() + y[slots[:, 1].long()].float()).bfloat16())
+    torch.cuda.empty_cache()
+
+
+def test_in_a_graph(dev):
+    """Captured once and replayed with other inputs, eager work between the replays."""
+    logits, tokens = randn(300, 32, seed=1).to(dev), randn(300, 256, seed=2, dtype=torch.bfloat16).to(dev)
+    w = quantise_weight(randn(32, 128, 256, seed=3).to(dev))
+
+    def layer():
+        weights, chosen = route(logits, 4)
+        plan = assign(chosen, 32)
+        y = product(tokens, w, plan, gather=True)
+        out = combine(y, plan, weights)
+        d_rows, d_weights = combine_grad(out, y, plan, weights)
+        return [weights, chosen, *plan, y, out, d_rows, weight_grad(d_rows, tokens, plan, gather=True), route_grad(d_weights, logits, chosen)]
+    layer()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = layer()
+    for i in range(4):
+        logits.copy_(randn(300, 32, seed=10 + i))
+        tokens.copy_(randn(300, 256, seed=20 + i))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, layer()):
+            assert torch.equal(a, b), i
