@@ -123,16 +123,19 @@ struct ColumnsArgs {
     uint32_t x_rows, width;
 };
 // A thread block has 64 columns of 128 rows of an expert (fewer where it has no more: zeros follow), which turn in LDS.
+// Bound by memory: 65536 rows of 2048 numbers 87 us (4.6 TB/s), 4096 gathered from 16384 rows 162 (with a column's blocks side by side in
+// the launch 102 and 184; bank conflicts of the turned stores cost nothing).
 // Two matrices can share a launch: the columns of the second one come behind the first one's.
 template <int DT>
 __global__ void __launch_bounds__(256) columns8_kernel(ColumnsArgs a0, ColumnsArgs a1) {
     using T = typename Elem<DT>::type;
     __shared__ __attribute__((aligned(16))) uint8_t turned[64][128 + 16];
     __shared__ uint32_t most[4][64];
-    const uint32_t first_tiles = (a0.width + 63) / 64, block = blockIdx.x;
-    const bool second = blockIdx.y >= first_tiles;
+    const uint32_t first_tiles = (a0.width + 63) / 64, tiles = first_tiles + (a1.width + 63) / 64;
+    const uint32_t block = blockIdx.x / tiles, tile = blockIdx.x % tiles;      // (rows side by side are read side by side)
+    const bool second = tile >= first_tiles;
     const ColumnsArgs& a = second ? a1 : a0;
-    const uint32_t c0 = (blockIdx.y - (second ? first_tiles : 0u)) * 64;
+    const uint32_t c0 = (tile - (second ? first_tiles : 0u)) * 64;
     const Tile t = find_tile(a.groups, block, 128, false);
     if (!t.found) return;
     const uint32_t r0 = t.begin + (block - t.first) * 128;
@@ -312,6 +315,8 @@ __device__ __forceinline__ void meet() {
     }
 }
 
+constexpr uint32_t DEALT = 32;
+
 // A thread block has BM rows and BN columns of the result, a wavefront 64 columns and BM / WM rows of them.
 // The depth goes by in blocks of 128: while one is multiplied the next STAGES - 1 ones' bytes are on their way into LDS.  One ahead
 // is enough where a block's products take longer than its bytes; many are needed where they do not (few tiles, small ones).
@@ -328,12 +333,14 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
     const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), wm = wave / WN, wn = wave % WN;
 
     // The hardware deals thread blocks to the eight XCDs in turn: each takes an eighth of the tiles that lie together, in
-    // columns of GROUP row tiles, so that those at work at a time share rows and weights in its L2.
+    // columns of GROUP row tiles, so that those at work at a time share rows and weights in its L2.  (Along the depth, where experts
+    // with many rows have the long tiles, DEALT tiles at a time: with eighths 16384 tokens of 32 experts took 800 - 1060 us.)
     constexpr uint32_t GROUP = 4;
     const uint32_t row_tiles = ALONG ? a.row_tiles * (a.groups.offsets ? a.groups.experts : 1u) : count_tiles(a.groups, BM, true);
     const uint32_t total = row_tiles * a.col_tiles, xcd = blockIdx.x & 7u, nth = blockIdx.x >> 3;
-    if (nth >= total / 8 + (xcd < total % 8)) return;
-    const uint32_t id = xcd * (total / 8) + min(xcd, total % 8) + nth;
+    if (!ALONG && nth >= total / 8 + (xcd < total % 8)) return;
+    const uint32_t id = ALONG ? (nth / DEALT * 8 + xcd) * DEALT + nth % DEALT : xcd * (total / 8) + min(xcd, total % 8) + nth;
+    if (id >= total) return;
     const uint32_t group = id / (GROUP * a.col_tiles), in_group = id % (GROUP * a.col_tiles), height = min(GROUP, row_tiles - group * GROUP);
     const uint32_t row_tile = group * GROUP + in_group % height, n0 = in_group / height * BN;
 
@@ -667,9 +674,10 @@ int go_tiles(ProductArgs a, uint32_t matrices, hipStream_t stream) {
     a.col_tiles = (uint32_t)ceil_div(a.cols, BN);
     a.row_tiles = (uint32_t)ceil_div(a.rows, BM);
     const uint64_t blocks = (ALONG ? (uint64_t)a.row_tiles * matrices : most_row_tiles(a, BM)) * a.col_tiles;
-    if (blocks > 0x7FFFFFFFull / (64 * WM * (BN / 64))) return MINT_ERR_TOO_LARGE;
+    if (blocks + 8 * DEALT > 0x7FFFFFFFull / (64 * WM * (BN / 64))) return MINT_ERR_TOO_LARGE;
     if (!blocks) return MINT_OK;
-    return Launch<&product_kernel<OUT, BM, BN, WM, STAGES, ROWS_W, ALONG>>::go((uint32_t)ceil_div(blocks, 8) * 8, 64 * WM * (BN / 64), 0, stream, a);
+    constexpr uint32_t all = ALONG ? 8 * DEALT : 8;
+    return Launch<&product_kernel<OUT, BM, BN, WM, STAGES, ROWS_W, ALONG>>::go((uint32_t)(ceil_div(blocks, all) * all), 64 * WM * (BN / 64), 0, stream, a);
 }
 // The tiles whose rounds over the compute units take least: tiles / (those at work at a time), rounded up, times what a round
 // takes for a block of the depth.  Measured, us:
@@ -769,20 +777,21 @@ extern "C" size_t mint_columns8_blocks(uint64_t rows, uint32_t experts) { return
 
 namespace {
 int go_columns(const ColumnsArgs& a, const ColumnsArgs& b, int dtype, uint32_t blocks, hipStream_t s) {
-    const dim3 grid(blocks, (uint32_t)(ceil_div(a.width, 64) + ceil_div(b.width, 64)));
+    const uint64_t all = (uint64_t)blocks * (ceil_div(a.width, 64) + ceil_div(b.width, 64));
+    if (all > 0x7FFFFFFFull / 256) return MINT_ERR_TOO_LARGE;
+    const uint32_t grid = (uint32_t)all;
     switch (dtype) {
         case MINT_F16: return Launch<&columns8_kernel<DT_F16>>::go(grid, 256, 0, s, a, b);
         case MINT_BF16: return Launch<&columns8_kernel<DT_BF16>>::go(grid, 256, 0, s, a, b);
         default: return Launch<&columns8_kernel<DT_F32>>::go(grid, 256, 0, s, a, b);
     }
 }
-constexpr uint64_t kMostColumns = 32767ull * 64;
 }  // namespace
 
 extern "C" int mint_columns8(const void* x, int64_t x_stride, uint64_t x_rows, uint64_t width, int dtype, const void* tokens, uint64_t rows,
                              const void* offsets, uint32_t experts, void* q, int64_t q_stride, void* scale, void* stream) {
     if (!known(dtype) || (!offsets && experts)) return MINT_ERR_ARG;
-    if (rows > kMostRows || x_rows > kMostRows || width > kMostColumns) return MINT_ERR_TOO_LARGE;
+    if (rows > kMostRows || x_rows > kMostRows || width > kMostRows) return MINT_ERR_TOO_LARGE;
     if (rows == 0 || width == 0) return MINT_OK;
     if (!x || !q || !scale || (!tokens && x_rows < rows) || x_rows == 0) return MINT_ERR_ARG;
     const uint64_t blocks = mint_columns8_blocks(rows, experts);
@@ -812,7 +821,7 @@ extern "C" size_t mint_weight_grad8_workspace(const mint_weight_grad_op* op) { r
 
 extern "C" int mint_weight_grad8(const mint_weight_grad_op* op, void* stream) {
     if (!op || !known(op->dtype) || !known(op->d_dtype) || !known(op->x_dtype) || (!op->offsets && op->experts)) return MINT_ERR_ARG;
-    if (op->rows > kMostRows || op->x_rows > kMostRows || op->cols > kMostColumns || op->depth > kMostColumns || op->experts > 65535)
+    if (op->rows > kMostRows || op->x_rows > kMostRows || op->cols > kMostRows || op->depth > kMostRows || op->experts > 65535)
         return MINT_ERR_TOO_LARGE;
     if (op->cols == 0 || op->depth == 0) return MINT_OK;
     if (!op->out || (op->rows && (!op->d || !op->x || op->x_rows == 0 || (!op->tokens && op->x_rows < op->rows)))) return MINT_ERR_ARG;
