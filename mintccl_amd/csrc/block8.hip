@@ -318,19 +318,21 @@ __device__ __forceinline__ void meet() {
 constexpr uint32_t DEALT = 32;
 
 // A thread block has BM rows and BN columns of the result, a wavefront 64 columns and BM / WM rows of them.
-// The depth goes by in blocks of 128: while one is multiplied the next STAGES - 1 ones' bytes are on their way into LDS.  One ahead
-// is enough where a block's products take longer than its bytes; many are needed where they do not (few tiles, small ones).
+// The depth goes by in blocks of 128: while one is multiplied the next STAGES - 1 ones' bytes are on their way into LDS.
+// SPLIT sets of wavefronts, each with LDS of its own, take the blocks in turn where there are few tiles: a step takes 0.3 us however
+// little there is to multiply.  Their sums are added up in LDS at the end.
 // The weights are the matrix instruction's first operand, so a lane has consecutive columns of one row of the result (column_of).
-template <int OUT, int BM, int BN, int WM, int STAGES, bool ROWS_W, bool ALONG>
-__global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArgs a) {
+template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG>
+__global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(ProductArgs a) {
     using Op = Operand<OUT == DT_F32>;
     using T = typename Elem<OUT>::type;
     constexpr int WN = BN / 64, WAVES = WM * WN, MT = BM / WM / 16, NT = 4;
     constexpr uint32_t kX = BM * 128, kW = BN * 128, kSx = BM * 4, kSw = ROWS_W ? BN * 4 : 256, kStage = kX + kW + kSx + kSw;
     static_assert(BM / 64 <= WAVES && BN / 64 <= WAVES, "a wavefront for each 64 scales");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
-    const uint32_t base = (uint32_t)(uintptr_t)(MINT_LDS uint8_t*)lds;
-    const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), wm = wave / WN, wn = wave % WN;
+    static_assert(SPLIT == 1 || STAGES == 2, "the wavefronts of a split wait for all of their loads");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[SPLIT * STAGES * kStage];
+    const uint32_t lane = lane_id(), all_waves = __builtin_amdgcn_readfirstlane(wave_in_block()), wave = all_waves % WAVES, wm = wave / WN, wn = wave % WN;
+    const uint32_t way = all_waves / WAVES, base = (uint32_t)(uintptr_t)(MINT_LDS uint8_t*)lds + way * STAGES * kStage;
 
     // The hardware deals thread blocks to the eight XCDs in turn: each takes an eighth of the tiles that lie together, in
     // columns of GROUP row tiles, so that those at work at a time share rows and weights in its L2.  (Along the depth, where experts
@@ -367,7 +369,9 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
         m_end = t.end;
         if (a.groups.offsets && expert == a.groups.experts) depth = 0;
     }
-    const uint32_t full = depth / 128, steps = (depth + 127) / 128;
+    // whole blocks of the depth and all of them; of those this way has way, way + SPLIT, ...
+    const uint32_t full_all = depth / 128, all_steps = (depth + 127) / 128;
+    const uint32_t full = (full_all + SPLIT - 1 - way) / SPLIT, steps = (all_steps + SPLIT - 1 - way) / SPLIT;
 
     // A wavefront brings 8 rows of 128 bytes with an instruction: the rows it has of x, then of the weights.
     constexpr int XI = BM / 8 / WAVES, WI = BN / 8 / WAVES;
@@ -380,6 +384,7 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
         return min(row, a.x_rows - 1);
     };
     if (steps) {
+        depth0 += way * 128;
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
             const uint32_t r = (wave * XI + i) * 8 + sub;
@@ -395,18 +400,18 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
         // (of a weight matrix lane i has the scale of the columns of wavefront i)
         const uint32_t col = min(n0 + (ROWS_W ? wave % (BN / 64) * 64 + lane : lane * 64), a.cols - 1);
         from_sw = a.sw + (ROWS_W ? (int64_t)col * a.sw_row + (int64_t)(depth0 / 128) * a.sw_block
-                                 : (int64_t)expert * a.sw_matrix + (int64_t)(col / 128) * a.sw_row);
+                                 : (int64_t)expert * a.sw_matrix + (int64_t)(col / 128) * a.sw_row + (int64_t)way * a.sw_block);
     }
     // Where loads are counted (STAGES > 2) all wavefronts have the same number of them under way: some bring scales that others bring too.
     constexpr int LOADS = XI + WI + 2;
     const auto bring_scales = [&](uint32_t at) MINT_INLINE_LAMBDA {
         if (STAGES > 2 || wave < BM / 64) {
             to_lds4(from_sx, at + kX + kW + wave % (BM / 64) * 256);
-            from_sx += a.sx_block;
+            from_sx += SPLIT * a.sx_block;
         }
         if (STAGES > 2 || (ROWS_W ? wave < BN / 64 : wave == WAVES - 1)) {
             to_lds4(from_sw, at + kX + kW + kSx + (ROWS_W ? wave % (BN / 64) * 256 : 0));
-            from_sw += a.sw_block;
+            from_sw += SPLIT * a.sw_block;
         }
     };
     // piece `n` of XI + WI, the scales with the first
@@ -414,16 +419,16 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
         if (n == 0) bring_scales(at);
         if (n < XI) {
             to_lds16(from_x[n], at + (wave * XI + n) * 1024);
-            from_x[n] += 128;
+            from_x[n] += SPLIT * 128;
         } else {
             to_lds16(from_w[n - XI], at + kX + (wave * WI + (n - XI)) * 1024);
-            from_w[n - XI] += 128;
+            from_w[n - XI] += SPLIT * 128;
         }
     };
     // the last block of a depth that is no multiple of 128 (along the rows there is none)
     const auto bring_tail = [&](uint32_t at) MINT_INLINE_LAMBDA {
         const auto guarded = [&](const uint8_t* from, uint32_t r, uint32_t to) MINT_INLINE_LAMBDA {
-            const int32_t left = (int32_t)(depth - full * 128) - (int32_t)((slot ^ turn(r)) * 16);
+            const int32_t left = (int32_t)(depth % 128) - (int32_t)((slot ^ turn(r)) * 16);
             *(MINT_LDS u32x4*)(uintptr_t)(to + lane * 16) = piece_of(from, left);
         };
 #pragma unroll
@@ -489,29 +494,47 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) product_kernel(ProductArg
         for (int n = MT * NT - LAG; n < MT * NT; ++n) add(n);
     };
 
-    if (steps) {
+    if (all_steps) {
         uint32_t b = 0, at = base, ahead = base + (STAGES - 1) * kStage;
         const auto after = [&](uint32_t stage) MINT_INLINE_LAMBDA { return stage + kStage == base + STAGES * kStage ? base : stage + kStage; };
+        const auto bring_all = [&](uint32_t to) MINT_INLINE_LAMBDA {
+#pragma unroll
+            for (int n = 0; n < XI + WI; ++n) bring(to, n);
+        };
 #pragma unroll
         for (int st = 0; st < STAGES - 1; ++st)
-            if (st < full) {
-#pragma unroll
-                for (int n = 0; n < XI + WI; ++n) bring(base + st * kStage, n);
-            }
-        if (!ALONG && !full) bring_tail(at);
-        for (; b + STAGES - 1 < full; ++b) {
+            if (st < full) bring_all(base + st * kStage);
+        if (!ALONG && steps && !full) bring_tail(at);
+        // (as long as every way has a block to bring)
+        for (; b + STAGES - 1 < full_all / SPLIT; ++b) {
             meet<(STAGES - 2) * LOADS>();
             multiply(at, [&](int n) MINT_INLINE_LAMBDA { bring(ahead, n); });
             at = after(at);
             ahead = after(ahead);
         }
-        for (; b < steps; ++b) {
+        for (; b < (all_steps + SPLIT - 1) / SPLIT; ++b) {
             __syncthreads();             // (waits for the loads into LDS too)
             const uint32_t next = after(at);
+            if (SPLIT > 1 && b + 1 < full) bring_all(next);
             if (!ALONG && b + 1 == full && full < steps) bring_tail(next);
-            multiply(at, [](int) MINT_INLINE_LAMBDA {});
+            if (SPLIT == 1 || b < steps) multiply(at, [](int) MINT_INLINE_LAMBDA {});
             at = next;
         }
+    }
+    if constexpr (SPLIT > 1) {           // the ways' sums, added up in their order
+        static_assert((SPLIT - 1) * BM * BN * 4 <= SPLIT * STAGES * (int)kStage, "they fit LDS");
+        f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+        __syncthreads();
+        if (way) {
+#pragma unroll
+            for (int n = 0; n < MT * NT; ++n) sums[(((way - 1) * WAVES + wave) * MT * NT + n) * 64 + lane] = acc[n / NT][n % NT];
+        }
+        __syncthreads();
+        if (way) return;
+#pragma unroll
+        for (int k = 0; k < SPLIT - 1; ++k)
+#pragma unroll
+            for (int n = 0; n < MT * NT; ++n) acc[n / NT][n % NT] += sums[((k * WAVES + wave) * MT * NT + n) * 64 + lane];
     }
 
     T* const out = static_cast<T*>(a.out) + (ALONG ? (int64_t)expert * a.out_matrix : 0);
@@ -669,23 +692,26 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
 uint64_t most_row_tiles(const ProductArgs& a, uint32_t tile_rows) {
     return ceil_div(a.rows, tile_rows) + (a.groups.offsets ? (uint64_t)a.groups.experts + 1 : 0);
 }
-template <int OUT, int BM, int BN, int WM, int STAGES, bool ROWS_W, bool ALONG>
+template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG>
 int go_tiles(ProductArgs a, uint32_t matrices, hipStream_t stream) {
     a.col_tiles = (uint32_t)ceil_div(a.cols, BN);
     a.row_tiles = (uint32_t)ceil_div(a.rows, BM);
     const uint64_t blocks = (ALONG ? (uint64_t)a.row_tiles * matrices : most_row_tiles(a, BM)) * a.col_tiles;
-    if (blocks + 8 * DEALT > 0x7FFFFFFFull / (64 * WM * (BN / 64))) return MINT_ERR_TOO_LARGE;
+    if (blocks + 8 * DEALT > 0x7FFFFFFFull / (64 * WM * (BN / 64) * SPLIT)) return MINT_ERR_TOO_LARGE;
     if (!blocks) return MINT_OK;
     constexpr uint32_t all = ALONG ? 8 * DEALT : 8;
-    return Launch<&product_kernel<OUT, BM, BN, WM, STAGES, ROWS_W, ALONG>>::go((uint32_t)(ceil_div(blocks, all) * all), 64 * WM * (BN / 64), 0, stream, a);
+    return Launch<&product_kernel<OUT, BM, BN, WM, STAGES, SPLIT, ROWS_W, ALONG>>::go((uint32_t)(ceil_div(blocks, all) * all), 64 * WM * (BN / 64) * SPLIT, 0,
+                                                                                     stream, a);
 }
 // The tiles whose rounds over the compute units take least: tiles / (those at work at a time), rounded up, times what a round
 // takes for a block of the depth.  Measured, us:
-//   64 x 64     0.36 up to 256 tiles, 0.6 for 512 (two blocks to a compute unit; 64 - 512 rows x 4096 x 4096)
-//   128 x 128   0.72 up to 256 tiles, with three blocks of the depth under way (1024 x 4096 x 4096); 1.29 for 512, with one and two thread
-//               blocks to a compute unit, which start while others work (11532 rows of 64 experts x 1408 x 2048: 62.6 us, 128 x 256 64.7)
-//   128 x 256   1.2 (2048 x 4096 x 4096: 39 us, 128 x 128 45)
-//   256 x 256   2.0 (8192 x 8192 x 4096: 260 us, 128 x 256 315; 65536 rows of 32 experts x 2048 x 4096: 581 us, 128 x 128 696)
+//   64 x 64     0.32 up to 256 tiles, the depth dealt to four times four wavefronts (64 x 4096 x 4096: 9.5; undealt 12.0), else 0.5 for 512, dealt
+//               to two and two thread blocks to a compute unit (512 x 4096 x 4096: 17.4; undealt 20.6); up to a depth of 1024 undealt
+//               (64 x 4096 x 1024: 5.3, dealt to four 5.5; 512 x 4096 x 512: 5.0, dealt to two 5.8)
+//   128 x 128   0.72 up to 256 tiles, the depth dealt to two from 2048 on (1024 x 4096 x 4096: 23.7; undealt 25.2; x 1024: 10.1 and 9.2); 1.29
+//               for 512, two thread blocks to a compute unit, which start while others work (11532 rows of 64 experts x 1408 x 2048: 72, 128 x 256 69)
+//   128 x 256   1.2, two blocks of the depth under way (2048 x 4096 x 4096: 39, 128 x 128 45)
+//   256 x 256   2.0 (8192 x 8192 x 4096: 260, 128 x 256 315; 65536 rows of 32 experts x 2048 x 4096: 573, 128 x 256 656)
 template <int OUT, bool ROWS_W, bool ALONG>
 int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
     const auto tiles = [&](uint32_t bm, uint32_t bn) {
@@ -693,23 +719,30 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
         return rows * ceil_div(a.cols, bn);
     };
     const uint64_t n64 = tiles(64, 64), n128 = tiles(128, 128);
-    const float t64 = n64 <= 256 ? 0.36f : 0.6f * ceil_div(n64, 512), t128 = n128 <= 256 ? 0.72f : 1.29f * ceil_div(n128, 512),
+    const float t64 = n64 <= 256 ? 0.32f : 0.5f * ceil_div(n64, 512), t128 = n128 <= 256 ? 0.72f : 1.29f * ceil_div(n128, 512),
                 wide = 1.2f * ceil_div(tiles(128, 256), 256), large = 2.0f * ceil_div(tiles(256, 256), 256);
-    if (t64 <= t128 && t64 <= wide && t64 <= large) return go_tiles<OUT, 64, 64, 4, 4, ROWS_W, ALONG>(a, matrices, stream);
-    if constexpr (OUT == DT_F32) {       // (operands widened to 16 bits leave no registers for more)
-        return go_tiles<OUT, 128, 256, 2, 3, ROWS_W, ALONG>(a, matrices, stream);
+    // (operands widened to 16 bits leave no registers for more wavefronts or larger tiles)
+    constexpr bool WIDE = OUT == DT_F32;
+    const uint64_t blocks = ceil_div(a.depth, 128) / (ALONG && matrices ? matrices : 1);
+    if (t64 <= t128 && t64 <= wide && t64 <= large) {
+        if (blocks <= 8) return go_tiles<OUT, 64, 64, 4, 2, 1, ROWS_W, ALONG>(a, matrices, stream);
+        if (!WIDE && n64 <= 256) return go_tiles<OUT, 64, 64, 4, 2, WIDE ? 2 : 4, ROWS_W, ALONG>(a, matrices, stream);
+        return go_tiles<OUT, 64, 64, 4, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
+    }
+    if constexpr (WIDE) {
+        return go_tiles<OUT, 128, 256, 2, 3, 1, ROWS_W, ALONG>(a, matrices, stream);
     } else {
         if (t128 <= wide && t128 <= large) {
-            if (n128 <= 256) return go_tiles<OUT, 128, 128, 4, 4, ROWS_W, ALONG>(a, matrices, stream);
-            return go_tiles<OUT, 128, 128, 4, 2, ROWS_W, ALONG>(a, matrices, stream);
+            if (!ROWS_W && n128 <= 256 && blocks >= 16) return go_tiles<OUT, 128, 128, 4, 2, ROWS_W ? 1 : 2, ROWS_W, ALONG>(a, matrices, stream);
+            return go_tiles<OUT, 128, 128, 4, 2, 1, ROWS_W, ALONG>(a, matrices, stream);
         }
-        if (wide <= large) return go_tiles<OUT, 128, 256, 2, 3, ROWS_W, ALONG>(a, matrices, stream);
-        return go_tiles<OUT, 256, 256, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
+        if (wide <= large) return go_tiles<OUT, 128, 256, 2, 3, 1, ROWS_W, ALONG>(a, matrices, stream);
+        return go_tiles<OUT, 256, 256, 2, 2, 1, ROWS_W, ALONG>(a, matrices, stream);
     }
 }
 
-// Few rows: at most 32 for each weight matrix, on the average (24 x 4096 x 4096: 7.8 us, with tiles of 64 x 64 11.8; at 64 rows
-// 12.8 and 11.8).
+// Few rows: at most 32 for each weight matrix, on the average (24 x 4096 x 4096: 7.8 us, with tiles of 64 x 64 9.4; at 64 rows
+// 12.8 and 9.5).
 bool few_rows(uint64_t rows, uint32_t matrices) { return rows <= 32ull * matrices; }
 // ... and so few that the rounding is done on the way: 256 blocks of 128 for each weight matrix (all thread blocks
 // do that work again, 0.5 us for 32 blocks, and save a launch: with a depth and 4096 columns of 4096, 1 row 5.7 us for 10.3, 8 rows 9.2
