@@ -359,8 +359,8 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
                 before += n > b ? (n - b + 127) / 128 : 0u;
             }
             const uint32_t b = row_bound(a.groups, expert), n = row_bound(a.groups, expert + 1);
-            depth0 = (uint32_t)__builtin_amdgcn_readlane((int)sum_below(before), 63) * 128;
-            depth = n > b ? (n - b + 127) / 128 * 128 : 0u;
+            depth0 = min((uint32_t)__builtin_amdgcn_readlane((int)sum_below(before), 63) * 128, a.depth);      // (whatever the offsets say)
+            depth = min(n > b ? (n - b + 127) / 128 * 128 : 0u, a.depth - depth0);
         }
     } else {
         const Tile t = find_tile(a.groups, row_tile, BM, true);
