@@ -12,7 +12,14 @@ Operator surface (same names and argument order as the reference scripts):
     allreduce.allreduce(buff)                   8_allreduce.py (planned there, README.md:23)
 
 plus ``common`` (knobs, ``VirtualComm``), ``primitive``, ``protocol`` and
-``topology``.  All compute runs in ``libmintccl.so`` (hand-written HIP); the
+``topology``.  What a layer of experts needs beside the collectives (no counterpart in the reference):
+
+    routing.route(logits, k) / route_grad / assign      tokens to experts, and their places in the experts' order
+    block8.quantise / quantise_weight / product / weight_grad    products in 8 bits with a scale per block of 128
+    combine.combine / combine_grad                      a token's rows added up with their weights
+    experts.ExpertLayer                                 all of it over the ranks of a communicator
+
+All compute runs in ``libmintccl.so`` (hand-written HIP); the
 package raises if that library has not been built.
 """
 from . import _lib  # noqa: F401

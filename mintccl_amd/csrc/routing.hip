@@ -79,8 +79,8 @@ __device__ __forceinline__ void join_best(uint32_t& best, uint32_t& second) {
 
 // LANES lanes have a token, a lane V consecutive experts of it, so that among equal keys the lowest lane has the lowest expert.
 // Bound by its vector instructions: a choice is the largest of the lanes' largest keys, taken k times.  With 16 lanes
-// the steps between lanes are for four tokens at once: 65536 tokens, 256 experts in 8 groups, 8 chosen: 104 us with 64 lanes
-// and groups looked at one by one.
+// the steps between lanes are for four tokens at once: 65536 tokens, 256 experts in 8 groups, 8 chosen: 44 us (with 64 lanes
+// and groups looked at one by one 104), of which the 71 MB that it reads and writes are 15.
 template <int DT, int V, int LANES>
 __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
     using T = typename Elem<DT>::type;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
 //   softmax                 scale p_i (d_i [chosen] - sum w' d)
 //   sigmoid, renormalised   scale (d_j - sum w' d) s_j (1 - s_j) / sum s
 //   sigmoid                 scale d_j s_j (1 - s_j)
-// The scores are computed again from the logits: they cost less than they would to keep.
+// The scores are computed again from the logits: they cost less than they would to keep.  4099 tokens of 64 experts: 3 us, a launch's time.
 struct RouteGradArgs {
     const void* logits;
     const float* d_weights;
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(64 * kSortWaves) assign_one_kernel(AssignArgs 
 }
 
 // Many: a launch counts each block's pairs by bucket, and a second one, in which every block adds up what it needs of
-// those counts (all totals, and its own predecessors': 65536 x 8 pairs, 256 buckets: 17 us; with a launch of one block in
+// those counts (all totals, and its own predecessors': 65536 x 8 pairs, 256 buckets: 20 us; with a launch of one block in
 // between that leaves the sums, 49), places them.
 __global__ void __launch_bounds__(64 * kSortWaves) assign_count_kernel(AssignArgs a) {
     __shared__ uint32_t all[kMostExperts + 1];
