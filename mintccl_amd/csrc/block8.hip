@@ -253,17 +253,21 @@ __device__ __forceinline__ void to_lds16(const uint8_t* from, uint32_t lds) {
 __device__ __forceinline__ void to_lds4(const float* from, uint32_t lds) {
     __builtin_amdgcn_global_load_lds((MINT_GLOBAL const void*)as_global(from), (MINT_LDS void*)(uintptr_t)lds, 4, 0, 0);
 }
-// 16 bytes of a row of which the first `left` are there, zeros behind.  (A piece that begins in the row may be read
-// to its end: it is aligned, so it lies in the same page.)
-__device__ __forceinline__ u32x4 piece_of(const uint8_t* from, int32_t left) {
-    u32x4 v = {0, 0, 0, 0};
-    if (left > 0) v = *(MINT_GLOBAL const u32x4*)as_global(from);
+// the first `left` bytes, zeros behind
+__device__ __forceinline__ u32x4 first_of(u32x4 v, int32_t left) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int32_t bytes = left - 4 * i;
         v[i] &= bytes >= 4 ? 0xFFFFFFFFu : bytes <= 0 ? 0u : (1u << 8 * bytes) - 1u;
     }
     return v;
+}
+// 16 bytes of a row of which the first `left` are there.  (A piece that begins in the row may be read to its end: it is
+// aligned, so it lies in the same page.)
+__device__ __forceinline__ u32x4 piece_of(const uint8_t* from, int32_t left) {
+    u32x4 v = {0, 0, 0, 0};
+    if (left > 0) v = *(MINT_GLOBAL const u32x4*)as_global(from);
+    return first_of(v, left);
 }
 __device__ __forceinline__ u32x4 lds16(uint32_t at) { return *(MINT_LDS const u32x4*)(uintptr_t)at; }
 __device__ __forceinline__ float lds_float(uint32_t at) { return *(MINT_LDS const float*)(uintptr_t)at; }
@@ -332,7 +336,6 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
     constexpr int WN = BN / 64, WAVES = WM * WN, MT = BM / WM / 16, NT = 4;
     constexpr uint32_t kX = BM * 128, kW = BN * 128, kSx = BM * 4, kSw = ROWS_W ? BN * 4 : 256, kStage = kX + kW + kSx + kSw;
     static_assert(BM / 64 <= WAVES && BN / 64 <= WAVES, "a wavefront for each 64 scales");
-    static_assert(SPLIT == 1 || STAGES == 2, "the wavefronts of a split wait for all of their loads");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[SPLIT * STAGES * kStage];
     const uint32_t lane = lane_id(), all_waves = __builtin_amdgcn_readfirstlane(wave_in_block()), wave = all_waves % WAVES, wm = wave / WN, wn = wave % WN;
     const uint32_t way = all_waves / WAVES, base = (uint32_t)(uintptr_t)(MINT_LDS uint8_t*)lds + way * STAGES * kStage;
@@ -429,16 +432,23 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
         }
     };
     // the last block of a depth that is no multiple of 128 (along the rows there is none)
+    // It comes like the others, a piece that lies behind the depth from the block's first one; what is not the row's becomes zeros in LDS.
+    const auto left_of = [&](uint32_t r) MINT_INLINE_LAMBDA { return (int32_t)(depth % 128) - (int32_t)((slot ^ turn(r)) * 16); };
     const auto bring_tail = [&](uint32_t at) MINT_INLINE_LAMBDA {
-        const auto guarded = [&](const uint8_t* from, uint32_t r, uint32_t to) MINT_INLINE_LAMBDA {
-            const int32_t left = (int32_t)(depth % 128) - (int32_t)((slot ^ turn(r)) * 16);
-            *(MINT_LDS u32x4*)(uintptr_t)(to + lane * 16) = piece_of(from, left);
-        };
+        const auto piece_from = [&](const uint8_t* from, uint32_t r) MINT_INLINE_LAMBDA { return left_of(r) > 0 ? from : from - (slot ^ turn(r)) * 16; };
 #pragma unroll
-        for (int i = 0; i < XI; ++i) guarded(from_x[i], (wave * XI + i) * 8 + sub, at + (wave * XI + i) * 1024);
+        for (int i = 0; i < XI; ++i) to_lds16(piece_from(from_x[i], (wave * XI + i) * 8 + sub), at + (wave * XI + i) * 1024);
 #pragma unroll
-        for (int i = 0; i < WI; ++i) guarded(from_w[i], (wave * WI + i) * 8 + sub, at + kX + (wave * WI + i) * 1024);
+        for (int i = 0; i < WI; ++i) to_lds16(piece_from(from_w[i], (wave * WI + i) * 8 + sub), at + kX + (wave * WI + i) * 1024);
         bring_scales(at);
+    };
+    const auto clear_tail = [&](uint32_t at) MINT_INLINE_LAMBDA {
+        const auto clear = [&](uint32_t r, uint32_t to) MINT_INLINE_LAMBDA {
+            const auto v = (MINT_LDS u32x4*)(uintptr_t)(to + lane * 16);
+            *v = first_of(*v, left_of(r));
+        };
+        for (int i = 0; i < XI; ++i) clear((wave * XI + i) * 8 + sub, at + (wave * XI + i) * 1024);
+        for (int i = 0; i < WI; ++i) clear((wave * WI + i) * 8 + sub, at + kX + (wave * WI + i) * 1024);
     };
 
     f32x4 acc[MT][NT];
@@ -505,9 +515,10 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
             for (int n = 0; n < XI + WI; ++n) bring(to, n);
         };
 #pragma unroll
-        for (int st = 0; st < STAGES - 1; ++st)
+        for (int st = 0; st < STAGES - 1; ++st) {
             if (st < full) bring_all(base + st * kStage);
-        if (!ALONG && steps && !full) bring_tail(at);
+            if (!ALONG && st == full && full < steps) bring_tail(base + st * kStage);
+        }
         // (as long as every way has a block to bring)
         for (; b + STAGES - 1 < full_all / SPLIT; ++b) {
             meet<(STAGES - 2) * LOADS>();
@@ -517,11 +528,15 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
         }
         for (; b < (all_steps + SPLIT - 1) / SPLIT; ++b) {
             __syncthreads();             // (waits for the loads into LDS too)
-            const uint32_t next = after(at);
-            if (SPLIT > 1 && b + 1 < full) bring_all(next);
-            if (!ALONG && b + 1 == full && full < steps) bring_tail(next);
+            if (SPLIT > 1 && b + STAGES - 1 < full) bring_all(ahead);
+            if (!ALONG && b + STAGES - 1 == full && full < steps) bring_tail(ahead);
+            if (!ALONG && depth % 128 && b == full_all / SPLIT) {
+                if (way == full_all % SPLIT) clear_tail(at);
+                __syncthreads();
+            }
             if (SPLIT == 1 || b < steps) multiply(at, [](int) MINT_INLINE_LAMBDA {});
-            at = next;
+            at = after(at);
+            ahead = after(ahead);
         }
     }
     if constexpr (SPLIT > 1) {           // the ways' sums, added up in their order
@@ -709,10 +724,11 @@ int go_tiles(ProductArgs a, uint32_t matrices, hipStream_t stream) {
 }
 // The tiles whose rounds over the compute units take least: tiles / (those at work at a time), rounded up, times what a round
 // takes for a block of the depth.  Measured, us:
-//   64 x 64     0.32 up to 256 tiles, the depth dealt to four times four wavefronts (64 x 4096 x 4096: 9.5; undealt 12.0), else 0.5 for 512, dealt
-//               to two and two thread blocks to a compute unit (512 x 4096 x 4096: 17.4; undealt 20.6); up to a depth of 1024 undealt
-//               (64 x 4096 x 1024: 5.3, dealt to four 5.5; 512 x 4096 x 512: 5.0, dealt to two 5.8)
-//   128 x 128   0.72 up to 256 tiles, the depth dealt to two from 2048 on (1024 x 4096 x 4096: 23.7; undealt 25.2; x 1024: 10.1 and 9.2); 1.29
+//   64 x 64     0.32 up to 256 tiles, the depth dealt to two times four wavefronts, three blocks under way for each (weights used in turn, 64 x 4096
+//               x 4096: 11.3; one block under way and dealt to four 11.9, to two 14.0, undealt 18.8; eight in one row 12.9), else 0.5 for 512, dealt to two with
+//               one block under way and two thread blocks to a compute unit (512 x 4096 x 4096: 17.3; undealt 20.2, three under way 19.3); up to a depth of 1024
+//               undealt (64 x 4096 x 1024: 5.2, dealt 5.3; 512 x 4096 x 512: 4.9, dealt 5.7)
+//   128 x 128   0.72 up to 256 tiles, two blocks under way (1024 x 4096 x 4096: 23.0, one 26.5, three 23.2; dealt to two 23.7); 1.29
 //               for 512, two thread blocks to a compute unit, which start while others work (11532 rows of 64 experts x 1408 x 2048: 72, 128 x 256 69)
 //   128 x 256   1.2, two blocks of the depth under way (2048 x 4096 x 4096: 39, 128 x 128 45)
 //   256 x 256   2.0 (8192 x 8192 x 4096: 260, 128 x 256 315; 65536 rows of 32 experts x 2048 x 4096: 573, 128 x 256 656)
@@ -730,14 +746,14 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
     const uint64_t blocks = ceil_div(a.depth, 128) / (ALONG && matrices ? matrices : 1);
     if (t64 <= t128 && t64 <= wide && t64 <= large) {
         if (blocks <= 8) return go_tiles<OUT, 64, 64, 4, 2, 1, ROWS_W, ALONG>(a, matrices, stream);
-        if (!WIDE && n64 <= 256) return go_tiles<OUT, 64, 64, 4, 2, WIDE ? 2 : 4, ROWS_W, ALONG>(a, matrices, stream);
+        if (!WIDE && n64 <= 256) return go_tiles<OUT, 64, 64, 4, WIDE ? 2 : 4, 2, ROWS_W, ALONG>(a, matrices, stream);
         return go_tiles<OUT, 64, 64, 4, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
     }
     if constexpr (WIDE) {
         return go_tiles<OUT, 128, 256, 2, 3, 1, ROWS_W, ALONG>(a, matrices, stream);
     } else {
         if (t128 <= wide && t128 <= large) {
-            if (!ROWS_W && n128 <= 256 && blocks >= 16) return go_tiles<OUT, 128, 128, 4, 2, ROWS_W ? 1 : 2, ROWS_W, ALONG>(a, matrices, stream);
+            if (n128 <= 256) return go_tiles<OUT, 128, 128, 4, 3, 1, ROWS_W, ALONG>(a, matrices, stream);
             return go_tiles<OUT, 128, 128, 4, 2, 1, ROWS_W, ALONG>(a, matrices, stream);
         }
         if (wide <= large) return go_tiles<OUT, 128, 256, 2, 3, 1, ROWS_W, ALONG>(a, matrices, stream);
