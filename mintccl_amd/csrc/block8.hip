@@ -97,6 +97,8 @@ struct RowsArgs {
     float* scale;
     int64_t x_stride, q_stride, s_row, s_block;
     uint32_t rows, depth, blocks;            // blocks of a row
+    uint32_t clears;
+    uint32_t* clear;                         // so many words that the product behind it counts in, or none
 };
 // 16 lanes have a block of 128 numbers of a row, 16 bytes each.  The last block is filled up with zeros.
 // Bound by memory: 8192 x 8192 numbers of 16 bits 40 us (5.1 TB/s), 8192 x 4096 22 (4.7).
@@ -104,6 +106,7 @@ template <int DT>
 __global__ void __launch_bounds__(256) rows8_kernel(RowsArgs a) {
     using T = typename Elem<DT>::type;
     const uint64_t unit = (uint64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < a.clears; i += gridDim.x * 256) a.clear[i] = 0;
     const uint32_t row = (uint32_t)(unit / a.blocks), block = (uint32_t)(unit % a.blocks), at = block * 128 + (threadIdx.x & 15u) * 8;
     if (row >= a.rows) return;
     float v[8];
@@ -235,6 +238,9 @@ struct ProductArgs {
     int64_t x_stride, w_stride, w_matrix, out_stride, out_matrix;
     int64_t sx_row, sx_block, sw_matrix, sw_row, sw_block;
     uint32_t x_rows, rows, cols, depth, col_tiles, row_tiles;
+    uint32_t parts;              // JOINED: thread blocks that have a part of a tile's depth, a tile's wavefronts' counts of those that are
+    uint32_t* arrived;           // done, and their sums
+    uint64_t* sums;
 };
 
 // Where a row's 16-byte piece lies in its 128 bytes of LDS: turned by the row's number, so that the lanes that a 16-byte read
@@ -326,10 +332,12 @@ constexpr uint32_t DEALT = 32;
 // The depth goes by in blocks of 128: while one is multiplied the next STAGES - 1 ones' bytes are on their way into LDS.
 // SPLIT sets of wavefronts, each with LDS of its own, take the blocks in turn where there are few tiles: a step takes 0.3 us however
 // little there is to multiply.  Their sums are added up in LDS at the end.
+// JOINED: the same over `parts` thread blocks, where there are fewer tiles than compute units.  A wavefront leaves its sums in memory and
+// counts itself; the last one of those that have the same place adds them all up, in the parts' order.  (No one waits for another.)
 // Bound by how steadily the matrix instructions are fed: at 8192 x 8192 x 4096 (260 us, 2.1 PFLOP/s) they are at work for 57 % of the cycles, no read
 // of LDS conflicts, and the rest is what a round of tiles takes to begin and to store (6 - 8 us of 65) and the scaling between them.
 // The weights are the matrix instruction's first operand, so a lane has consecutive columns of one row of the result (column_of).
-template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG>
+template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG, bool JOINED>
 __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(ProductArgs a) {
     using Op = Operand<OUT == DT_F32>;
     using T = typename Elem<OUT>::type;
@@ -345,10 +353,12 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
     // with many rows have the long tiles, DEALT tiles at a time: with eighths 16384 tokens of 32 experts took 800 - 1060 us.)
     constexpr uint32_t GROUP = 4;
     const uint32_t row_tiles = ALONG ? a.row_tiles * (a.groups.offsets ? a.groups.experts : 1u) : count_tiles(a.groups, BM, true);
-    const uint32_t total = row_tiles * a.col_tiles, xcd = blockIdx.x & 7u, nth = blockIdx.x >> 3;
+    const uint32_t parts = JOINED ? a.parts : 1u, ways = SPLIT * parts;
+    const uint32_t total = row_tiles * a.col_tiles * parts, xcd = blockIdx.x & 7u, nth = blockIdx.x >> 3;
     if (!ALONG && nth >= total / 8 + (xcd < total % 8)) return;
-    const uint32_t id = ALONG ? (nth / DEALT * 8 + xcd) * DEALT + nth % DEALT : xcd * (total / 8) + min(xcd, total % 8) + nth;
-    if (id >= total) return;
+    const uint32_t all_id = ALONG ? (nth / DEALT * 8 + xcd) * DEALT + nth % DEALT : xcd * (total / 8) + min(xcd, total % 8) + nth;
+    if (all_id >= total) return;
+    const uint32_t id = all_id / parts, part_of_depth = all_id % parts, turn_of_way = part_of_depth * SPLIT + way;
     const uint32_t group = id / (GROUP * a.col_tiles), in_group = id % (GROUP * a.col_tiles), height = min(GROUP, row_tiles - group * GROUP);
     const uint32_t row_tile = group * GROUP + in_group % height, n0 = in_group / height * BN;
 
@@ -375,9 +385,9 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
         m_end = t.end;
         if (a.groups.offsets && expert == a.groups.experts) depth = 0;
     }
-    // whole blocks of the depth and all of them; of those this way has way, way + SPLIT, ...
+    // whole blocks of the depth and all of them; of those this way has one of `ways`
     const uint32_t full_all = depth / 128, all_steps = (depth + 127) / 128;
-    const uint32_t full = (full_all + SPLIT - 1 - way) / SPLIT, steps = (all_steps + SPLIT - 1 - way) / SPLIT;
+    const uint32_t full = (full_all + ways - 1 - turn_of_way) / ways, steps = (all_steps + ways - 1 - turn_of_way) / ways;
 
     // A wavefront brings 8 rows of 128 bytes with an instruction: the rows it has of x, then of the weights.
     constexpr int XI = BM / 8 / WAVES, WI = BN / 8 / WAVES;
@@ -390,7 +400,7 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
         return min(row, a.x_rows - 1);
     };
     if (steps) {
-        depth0 += way * 128;
+        depth0 += turn_of_way * 128;
 #pragma unroll
         for (int i = 0; i < XI; ++i) {
             const uint32_t r = (wave * XI + i) * 8 + sub;
@@ -406,18 +416,18 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
         // (of a weight matrix lane i has the scale of the columns of wavefront i)
         const uint32_t col = min(n0 + (ROWS_W ? wave % (BN / 64) * 64 + lane : lane * 64), a.cols - 1);
         from_sw = a.sw + (ROWS_W ? (int64_t)col * a.sw_row + (int64_t)(depth0 / 128) * a.sw_block
-                                 : (int64_t)expert * a.sw_matrix + (int64_t)(col / 128) * a.sw_row + (int64_t)way * a.sw_block);
+                                 : (int64_t)expert * a.sw_matrix + (int64_t)(col / 128) * a.sw_row + (int64_t)turn_of_way * a.sw_block);
     }
     // Where loads are counted (STAGES > 2) all wavefronts have the same number of them under way: some bring scales that others bring too.
     constexpr int LOADS = XI + WI + 2;
     const auto bring_scales = [&](uint32_t at) MINT_INLINE_LAMBDA {
         if (STAGES > 2 || wave < BM / 64) {
             to_lds4(from_sx, at + kX + kW + wave % (BM / 64) * 256);
-            from_sx += SPLIT * a.sx_block;
+            from_sx += ways * a.sx_block;
         }
         if (STAGES > 2 || (ROWS_W ? wave < BN / 64 : wave == WAVES - 1)) {
             to_lds4(from_sw, at + kX + kW + kSx + (ROWS_W ? wave % (BN / 64) * 256 : 0));
-            from_sw += SPLIT * a.sw_block;
+            from_sw += ways * a.sw_block;
         }
     };
     // piece `n` of XI + WI, the scales with the first
@@ -425,10 +435,10 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
         if (n == 0) bring_scales(at);
         if (n < XI) {
             to_lds16(from_x[n], at + (wave * XI + n) * 1024);
-            from_x[n] += SPLIT * 128;
+            from_x[n] += ways * 128;
         } else {
             to_lds16(from_w[n - XI], at + kX + (wave * WI + (n - XI)) * 1024);
-            from_w[n - XI] += SPLIT * 128;
+            from_w[n - XI] += ways * 128;
         }
     };
     // the last block of a depth that is no multiple of 128 (along the rows there is none)
@@ -520,18 +530,18 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
             if (!ALONG && st == full && full < steps) bring_tail(base + st * kStage);
         }
         // (as long as every way has a block to bring)
-        for (; b + STAGES - 1 < full_all / SPLIT; ++b) {
+        for (; b + STAGES - 1 < full_all / ways; ++b) {
             meet<(STAGES - 2) * LOADS>();
             multiply(at, [&](int n) MINT_INLINE_LAMBDA { bring(ahead, n); });
             at = after(at);
             ahead = after(ahead);
         }
-        for (; b < (all_steps + SPLIT - 1) / SPLIT; ++b) {
+        for (; b < (all_steps + ways - 1) / ways; ++b) {
             __syncthreads();             // (waits for the loads into LDS too)
             if (SPLIT > 1 && b + STAGES - 1 < full) bring_all(ahead);
             if (!ALONG && b + STAGES - 1 == full && full < steps) bring_tail(ahead);
-            if (!ALONG && depth % 128 && b == full_all / SPLIT) {
-                if (way == full_all % SPLIT) clear_tail(at);
+            if (!ALONG && depth % 128 && b == full_all / ways) {
+                if (turn_of_way == full_all % ways) clear_tail(at);
                 __syncthreads();
             }
             if (SPLIT == 1 || b < steps) multiply(at, [](int) MINT_INLINE_LAMBDA {});
@@ -553,6 +563,42 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
         for (int k = 0; k < SPLIT - 1; ++k)
 #pragma unroll
             for (int n = 0; n < MT * NT; ++n) acc[n / NT][n % NT] += sums[((k * WAVES + wave) * MT * NT + n) * 64 + lane];
+    }
+
+    if constexpr (JOINED) {
+        constexpr uint32_t N = MT * NT * 2;                      // words of 64 bits that a lane has
+        const uint64_t place = (uint64_t)id * WAVES + wave;
+        uint64_t* const sums = a.sums + place * parts * (N * 64) + lane;
+#pragma unroll
+        for (uint32_t n = 0; n < N; ++n) {
+            const f32x4 v = acc[n / 2 / NT][n / 2 % NT];
+            const uint32_t lo = __float_as_uint(v[n % 2 * 2]), hi = __float_as_uint(v[n % 2 * 2 + 1]);
+            st64_agent(sums + (part_of_depth * N + n) * 64, (uint64_t)hi << 32 | lo);
+        }
+        wait_stores_visible();
+        uint32_t before = 0;
+        if (lane == 0) before = __hip_atomic_fetch_add(a.arrived + place, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if ((uint32_t)__builtin_amdgcn_readfirstlane((int)before) != parts - 1) return;
+        compiler_fence();
+#pragma unroll
+        for (uint32_t n = 0; n < N / 2; ++n) acc[n / NT][n % NT] = f32x4{0, 0, 0, 0};
+        for (uint32_t p0 = 0; p0 < parts; p0 += 4) {
+            uint64_t v[4][N];
+#pragma unroll
+            for (uint32_t p = 0; p < 4; ++p)
+#pragma unroll
+                for (uint32_t n = 0; n < N; ++n) v[p][n] = ld64_agent(sums + (min(p0 + p, parts - 1) * N + n) * 64);
+#pragma unroll
+            for (uint32_t p = 0; p < 4; ++p)
+                if (p0 + p < parts) {
+#pragma unroll
+                    for (uint32_t n = 0; n < N; ++n) {
+                        f32x4& sum = acc[n / 2 / NT][n / 2 % NT];
+                        sum[n % 2 * 2] += __uint_as_float((uint32_t)v[p][n]);
+                        sum[n % 2 * 2 + 1] += __uint_as_float((uint32_t)(v[p][n] >> 32));
+                    }
+                }
+        }
     }
 
     T* const out = static_cast<T*>(a.out) + (ALONG ? (int64_t)expert * a.out_matrix : 0);
@@ -711,15 +757,15 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
 uint64_t most_row_tiles(const ProductArgs& a, uint32_t tile_rows) {
     return ceil_div(a.rows, tile_rows) + (a.groups.offsets ? (uint64_t)a.groups.experts + 1 : 0);
 }
-template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG>
+template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG, bool JOINED = false>
 int go_tiles(ProductArgs a, uint32_t matrices, hipStream_t stream) {
     a.col_tiles = (uint32_t)ceil_div(a.cols, BN);
     a.row_tiles = (uint32_t)ceil_div(a.rows, BM);
-    const uint64_t blocks = (ALONG ? (uint64_t)a.row_tiles * matrices : most_row_tiles(a, BM)) * a.col_tiles;
+    const uint64_t blocks = (ALONG ? (uint64_t)a.row_tiles * matrices : most_row_tiles(a, BM)) * a.col_tiles * (JOINED ? a.parts : 1);
     if (blocks + 8 * DEALT > 0x7FFFFFFFull / (64 * WM * (BN / 64) * SPLIT)) return MINT_ERR_TOO_LARGE;
     if (!blocks) return MINT_OK;
     constexpr uint32_t all = ALONG ? 8 * DEALT : 8;
-    return Launch<&product_kernel<OUT, BM, BN, WM, STAGES, SPLIT, ROWS_W, ALONG>>::go((uint32_t)(ceil_div(blocks, all) * all), 64 * WM * (BN / 64) * SPLIT, 0,
+    return Launch<&product_kernel<OUT, BM, BN, WM, STAGES, SPLIT, ROWS_W, ALONG, JOINED>>::go((uint32_t)(ceil_div(blocks, all) * all), 64 * WM * (BN / 64) * SPLIT, 0,
                                                                                      stream, a);
 }
 // The tiles whose rounds over the compute units take least: tiles / (those at work at a time), rounded up, times what a round
@@ -745,6 +791,8 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
     constexpr bool WIDE = OUT == DT_F32;
     const uint64_t blocks = ceil_div(a.depth, 128) / (ALONG && matrices ? matrices : 1);
     if (t64 <= t128 && t64 <= wide && t64 <= large) {
+        if constexpr (!ALONG)
+            if (a.parts > 1) return go_tiles<OUT, 64, 64, 4, WIDE ? 2 : 4, 2, ROWS_W, ALONG, true>(a, matrices, stream);
         if (blocks <= 8) return go_tiles<OUT, 64, 64, 4, 2, 1, ROWS_W, ALONG>(a, matrices, stream);
         if (!WIDE && n64 <= 256) return go_tiles<OUT, 64, 64, 4, WIDE ? 2 : 4, 2, ROWS_W, ALONG>(a, matrices, stream);
         return go_tiles<OUT, 64, 64, 4, 2, 2, ROWS_W, ALONG>(a, matrices, stream);
@@ -761,6 +809,14 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
     }
 }
 
+// Where a product of one matrix has tiles of 64 x 64 for at most half of the compute units and a long depth: thread blocks to a tile. Rounded
+// before, us, with one and with these (and with results in 32 bits): 64 x 4096 x 4096 14.1 and 12.4 (18.1 and 13.1), 40 x 2048 x 8192 19.0 and 13.7,
+// 100 x 1000 x 8000 19.4 and 13.6, 128 x 4096 x 4096 14.4 and 13.2, 50 x 5000 x 2500 11.5 and 11.6 (14.1 and 12.2), 48 x 7168 x 2048 10.0 and 11.2.
+uint32_t parts_of(uint64_t rows, uint64_t cols, uint64_t depth, int dtype) {
+    const uint64_t tiles = ceil_div(rows, 64) * ceil_div(cols, 64), blocks = ceil_div(depth, 128);
+    if (tiles == 0 || tiles > 128 || blocks < (dtype == MINT_F32 ? 20 : 32)) return 1;
+    return (uint32_t)std::min<uint64_t>(256 / tiles, blocks / 6);
+}
 // Few rows: at most 32 for each weight matrix, on the average (24 x 4096 x 4096: 7.8 us, with tiles of 64 x 64 9.4; at 64 rows
 // 12.8 and 9.5).
 bool few_rows(uint64_t rows, uint32_t matrices) { return rows <= 32ull * matrices; }
@@ -805,8 +861,9 @@ constexpr uint64_t kMostRows = 0x7FFFFFFF - 128;
 
 using namespace mint;
 
-extern "C" int mint_rows8(const void* x, int64_t x_stride, uint64_t rows, uint64_t depth, int dtype, void* q, int64_t q_stride,
-                          void* scale, int64_t s_row, int64_t s_block, void* stream) {
+namespace {
+int go_rows8(const void* x, int64_t x_stride, uint64_t rows, uint64_t depth, int dtype, void* q, int64_t q_stride, void* scale, int64_t s_row,
+             int64_t s_block, uint32_t* clear, uint32_t clears, void* stream) {
     if (!known(dtype)) return MINT_ERR_ARG;
     if (rows > kMostRows || depth > kMostRows) return MINT_ERR_TOO_LARGE;
     if (rows == 0 || depth == 0) return MINT_OK;
@@ -817,13 +874,19 @@ extern "C" int mint_rows8(const void* x, int64_t x_stride, uint64_t rows, uint64
     const uint64_t blocks = ceil_div(rows * per_row, 16);
     if (blocks > 0x7FFFFFFFull / 256) return MINT_ERR_TOO_LARGE;
     const RowsArgs a = {x, static_cast<uint8_t*>(q), static_cast<float*>(scale), x_stride, q_stride, s_row, s_block, (uint32_t)rows,
-                        (uint32_t)depth, (uint32_t)per_row};
+                        (uint32_t)depth, (uint32_t)per_row, clears, clear};
     const auto s = static_cast<hipStream_t>(stream);
     switch (dtype) {
         case MINT_F16: return Launch<&rows8_kernel<DT_F16>>::go((uint32_t)blocks, 256, 0, s, a);
         case MINT_BF16: return Launch<&rows8_kernel<DT_BF16>>::go((uint32_t)blocks, 256, 0, s, a);
         default: return Launch<&rows8_kernel<DT_F32>>::go((uint32_t)blocks, 256, 0, s, a);
     }
+}
+}  // namespace
+
+extern "C" int mint_rows8(const void* x, int64_t x_stride, uint64_t rows, uint64_t depth, int dtype, void* q, int64_t q_stride,
+                          void* scale, int64_t s_row, int64_t s_block, void* stream) {
+    return go_rows8(x, x_stride, rows, depth, dtype, q, q_stride, scale, s_row, s_block, nullptr, 0, stream);
 }
 
 extern "C" size_t mint_columns8_blocks(uint64_t rows, uint32_t experts) { return ceil_div(rows, 128) + experts; }
@@ -947,14 +1010,29 @@ extern "C" int mint_squares8(const void* w, int64_t w_matrix, int64_t w_stride, 
 
 namespace {
 uint32_t matrices_of(const mint_product_op& op) { return op.offsets ? op.experts : 1; }
-// 8-bit numbers and scales of activations that come as they are, where that takes a launch of its own
-size_t rounded_bytes(const mint_product_op& op) {
-    if (op.kind != MINT_PRODUCT_ROWS || op.x_dtype == MINT_BYTES || rounded_on_the_way(op.rows, op.depth, matrices_of(op))) return 0;
-    return (size_t)op.x_rows * ceil_div(op.depth, 128) * 132;
-}
+// What a product needs: 8-bit numbers and scales of activations that come as they are, where rounding them takes a launch of its
+// own, and behind them the sums of a tile's parts and their counts (which that launch clears, or one that does nothing else: a product
+// has the same bits whoever rounded its rows)
+struct ProductRoom {
+    uint64_t rounded = 0, sums_at = 0, sums = 0, clears = 0, bytes = 0;
+    uint32_t parts = 1;
+    explicit ProductRoom(const mint_product_op& op) {
+        if (op.kind != MINT_PRODUCT_ROWS) return;
+        if (op.x_dtype != MINT_BYTES && !rounded_on_the_way(op.rows, op.depth, matrices_of(op)))
+            bytes = rounded = op.x_rows * ceil_div(op.depth, 128) * 132;
+        if (op.offsets || few_rows(op.rows, 1)) return;
+        parts = parts_of(op.rows, op.cols, op.depth, op.dtype);
+        if (parts == 1) return;
+        const uint64_t tiles = ceil_div(op.rows, 64) * ceil_div(op.cols, 64);
+        sums_at = ceil_div(rounded, 16) * 16;
+        sums = tiles * parts * (64 * 64 * 4);
+        clears = tiles * 4;
+        bytes = sums_at + sums + clears * 4;
+    }
+};
 }  // namespace
 
-extern "C" size_t mint_product8_workspace(const mint_product_op* op) { return op ? rounded_bytes(*op) : 0; }
+extern "C" size_t mint_product8_workspace(const mint_product_op* op) { return op ? ProductRoom(*op).bytes : 0; }
 
 extern "C" int mint_product8(const mint_product_op* op, void* stream) {
     if (!op || !known(op->dtype) || (op->kind != MINT_PRODUCT_ROWS && op->kind != MINT_PRODUCT_GRADIENT)) return MINT_ERR_ARG;
@@ -972,7 +1050,8 @@ extern "C" int mint_product8(const mint_product_op* op, void* stream) {
                  op->w_stride % 16 || op->w_matrix % 16))
         return MINT_ERR_ALIGN;
     if (along && op->depth % 128) return MINT_ERR_GEOMETRY;
-    const size_t need = rounded_bytes(*op);
+    const ProductRoom room(*op);
+    const size_t need = room.bytes;
     if (need && (op->workspace_bytes < need || !op->workspace)) return MINT_ERR_STAGING;
     if (need && !aligned_to(reinterpret_cast<void*>(op->workspace), 16)) return MINT_ERR_ALIGN;
     const auto s = static_cast<hipStream_t>(stream);
@@ -981,14 +1060,25 @@ extern "C" int mint_product8(const mint_product_op* op, void* stream) {
                      reinterpret_cast<const int32_t*>(op->tokens),
                      {reinterpret_cast<const int32_t*>(op->offsets), op->experts, (uint32_t)(along ? op->group_rows : op->rows)},
                      op->x_stride, op->w_stride, op->w_matrix, op->out_stride, op->out_matrix, op->sx_row, op->sx_block, op->sw_matrix,
-                     op->sw_row, op->sw_block, (uint32_t)op->x_rows, (uint32_t)op->rows, (uint32_t)op->cols, (uint32_t)op->depth, 0, 0};
+                     op->sw_row, op->sw_block, (uint32_t)op->x_rows, (uint32_t)op->rows, (uint32_t)op->cols, (uint32_t)op->depth, 0, 0, 1, nullptr, nullptr};
     const uint32_t matrices = matrices_of(*op);
     int x_dtype = op->x_dtype;
     if (need && some) {
+        a.parts = room.parts;
+        a.sums = reinterpret_cast<uint64_t*>(op->workspace + room.sums_at);
+        a.arrived = reinterpret_cast<uint32_t*>(op->workspace + room.sums_at + room.sums);
+    }
+    if (room.clears && !room.rounded && some) {
+        const RowsArgs none = {nullptr, nullptr, nullptr, 0, 0, 0, 0, 0, 0, 1, (uint32_t)room.clears, a.arrived};
+        const int err = Launch<&rows8_kernel<DT_F32>>::go((uint32_t)ceil_div(room.clears, 256), 256, 0, s, none);
+        if (err != MINT_OK) return err;
+    }
+    if (room.rounded && some) {
         const uint64_t per_row = ceil_div(op->depth, 128);
         auto* const q = reinterpret_cast<uint8_t*>(op->workspace);
         auto* const scale = reinterpret_cast<float*>(q + op->x_rows * per_row * 128);
-        const int err = mint_rows8(a.x, op->x_stride, op->x_rows, op->depth, x_dtype, q, (int64_t)per_row * 128, scale, 1, (int64_t)op->x_rows, stream);
+        const int err = go_rows8(a.x, op->x_stride, op->x_rows, op->depth, x_dtype, q, (int64_t)per_row * 128, scale, 1, (int64_t)op->x_rows, a.arrived,
+                                 (uint32_t)room.clears, stream);
         if (err != MINT_OK) return err;
         a.x = q;
         a.x_stride = (int64_t)per_row * 128;
@@ -996,7 +1086,7 @@ extern "C" int mint_product8(const mint_product_op* op, void* stream) {
         a.sx_row = 1;
         a.sx_block = (int64_t)op->x_rows;
     }
-    if (need) x_dtype = MINT_BYTES;
+    if (room.rounded) x_dtype = MINT_BYTES;
     if (along) {
         switch (op->dtype) {
             case MINT_F16: return go_product<DT_F16, true, true>(a, matrices, s);

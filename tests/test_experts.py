@@ -96,6 +96,19 @@ def test_workspaces():
     assert L.mint_columns8_blocks(300, 5) == 8
 
 
+def test_workspace_of_a_shared_tile():
+    """Few tiles of 64 x 64 and a long depth: sums of four wavefronts, 16 KiB a tile and part, and their counts, behind what is rounded."""
+    L = _lib.lib()
+    op = product_op(rows=64, x_rows=64, cols=4096, depth=4096)
+    sums = 64 * 4 * 16384 + 64 * 4 * 4
+    assert L.mint_product8_workspace(op) == sums
+    op.x_dtype = _lib.F32
+    assert L.mint_product8_workspace(op) == 64 * 32 * 132 + sums
+    op.depth = 31 * 128                                      # (results in 16 bits: not worth it)
+    assert L.mint_product8_workspace(op) == 64 * 31 * 132
+
+
+
 def test_weight_grad_rounding_and_combination_refuse():
     L = _lib.lib()
     base = dict(d=4096, x=4096, out=4096, rows=300, x_rows=300, cols=10, depth=20, d_dtype=2, x_dtype=2, dtype=2)

@@ -311,6 +311,42 @@ def test_product(dev, rows, cols, depth, dt):
     assert torch.equal(out, got) and (room[:, :3] == 7).all() and (room[:, 3 + cols:] == 7).all()
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols,depth", [(33, 70, 4100), (64, 130, 9001), (130, 1000, 5000), (65, 4096, 2600), (40, 20, 33000)])
+def test_product_of_few_tiles_and_a_long_depth(dev, rows, cols, depth, dt):
+    """Thread blocks that share a tile: every call adds the same parts in the same order, whatever the workspace held."""
+    x = randn(rows, depth, seed=depth, dtype=DT[dt]).to(dev)
+    w = quantise_weight(randn(cols, depth, seed=cols).to(dev))
+    got = product(x, w, dtype=DT[dt])
+    assert near_product(got, values(x.cpu(), 1), weight64(w), DT[dt])
+    rounded = quantise(x)
+    for fill in (0, 1, 255):
+        room = torch.full((64 << 20,), fill, dtype=torch.uint8, device=dev)
+        del room                                                     # (what the next workspace is made of)
+        assert torch.equal(product(x, w, dtype=DT[dt]), got)
+        assert torch.equal(product(rounded, w, dtype=DT[dt]), got)
+
+
+def test_product_of_few_tiles_in_a_graph(dev):
+    x = randn(50, 6000, seed=1, dtype=torch.bfloat16).to(dev)
+    w = quantise_weight(randn(300, 6000, seed=2).to(dev))
+    out = torch.empty(50, 300, dtype=torch.bfloat16, device=dev)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        product(x, w, out=out)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            product(x, w, out=out)
+    for seed in range(4):
+        x.copy_(randn(50, 6000, seed=10 + seed, dtype=torch.bfloat16))
+        want = product(x, w)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+
 def test_product_reads_nothing_behind_a_row(dev):
     """8-bit rows in a wider buffer whose rest is NaN."""
     for rows, cols, depth in ((5, 70, 200), (130, 140, 1000), (40, 33, 17)):
