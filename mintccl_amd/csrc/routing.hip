@@ -322,13 +322,21 @@ __device__ __forceinline__ uint32_t bucket_of(const AssignArgs& a, uint32_t pair
 }
 // counts of each wavefront's pairs [begin, end) in `mine`
 __device__ __forceinline__ void count_pairs(const AssignArgs& a, uint32_t begin, uint32_t end, uint32_t* mine) {
-    for (uint32_t p = begin + lane_id(); p < end; p += 64) atomicAdd(mine + bucket_of(a, p), 1u);
+    for (uint32_t p = begin + lane_id(); p < end; p += 256) {
+        uint32_t b[4];                   // (asked for together)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) b[i] = bucket_of(a, min(p + i * 64, end - 1));
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (p + i * 64 < end) atomicAdd(mine + b[i], 1u);
+    }
 }
 __device__ __forceinline__ void place_pairs(const AssignArgs& a, uint32_t begin, uint32_t end, uint32_t* next) {
+    uint32_t ahead = begin < end ? bucket_of(a, min(begin + lane_id(), end - 1)) : 0u;
     for (uint32_t p0 = begin; p0 < end; p0 += 64) {
-        const uint32_t p = p0 + lane_id();
+        const uint32_t p = p0 + lane_id(), b = ahead;
         const bool in = p < end;
-        const uint32_t b = in ? bucket_of(a, p) : 0u;
+        if (p0 + 64 < end) ahead = bucket_of(a, min(p + 64, end - 1));
         uint64_t same = __ballot(in);
         for (uint32_t i = 0; i < a.bits; ++i) {
             const uint64_t set = __ballot(b >> i & 1u);
@@ -397,8 +405,28 @@ __global__ void __launch_bounds__(64 * kSortWaves) assign_one_kernel(AssignArgs 
     place_pairs(a, begin, end, next[w]);
 }
 
+// The sum of blocks [i, end)'s counts: a chain of round trips to the cache, with 32 asked for together (65536 x 8 pairs, 256 buckets: 16.2 us for
+// the whole assignment; with 16 18.3, with 64 16.3) and what is left over in 16s, too many of them rather than one by one.
+__device__ __forceinline__ uint32_t sum_of_counts(const uint32_t* counts, uint32_t buckets, uint32_t i, uint32_t end) {
+    uint32_t sum = 0;
+    for (; i + 32 <= end; i += 32) {
+        uint32_t c[32];
+#pragma unroll
+        for (uint32_t u = 0; u < 32; ++u) c[u] = counts[(i + u) * buckets];
+#pragma unroll
+        for (uint32_t u = 0; u < 32; ++u) sum += c[u];
+    }
+    for (; i < end; i += 16) {
+        uint32_t c[16];
+#pragma unroll
+        for (uint32_t u = 0; u < 16; ++u) c[u] = counts[min(i + u, end - 1) * buckets];
+#pragma unroll
+        for (uint32_t u = 0; u < 16; ++u) sum += i + u < end ? c[u] : 0u;
+    }
+    return sum;
+}
 // Many: a launch counts each block's pairs by bucket, and a second one, in which every block adds up what it needs of
-// those counts (all totals, and its own predecessors': 65536 x 8 pairs, 256 buckets: 20 us; with a launch of one block in
+// those counts (all totals, and its own predecessors': 65536 x 8 pairs, 256 buckets: 16 us; with a launch of one block in
 // between that leaves the sums, 49), places them.
 __global__ void __launch_bounds__(64 * kSortWaves) assign_count_kernel(AssignArgs a) {
     __shared__ uint32_t all[kMostExperts + 1];
@@ -419,13 +447,8 @@ __global__ void __launch_bounds__(64 * kSortWaves) assign_place_kernel(AssignArg
     count_pairs(a, begin, end, next[w]);
     __syncthreads();
     for (uint32_t b = threadIdx.x; b < buckets; b += 64 * kSortWaves) {
-        uint32_t before = 0, total = 0;
-#pragma unroll 16
-        for (uint32_t i = 0; i < a.blocks; ++i) {
-            const uint32_t c = a.counts[(uint64_t)i * buckets + b];
-            before += i < blockIdx.x ? c : 0u;
-            total += c;
-        }
+        uint32_t before = sum_of_counts(a.counts + b, buckets, 0, blockIdx.x);
+        const uint32_t total = before + sum_of_counts(a.counts + b, buckets, blockIdx.x, a.blocks);
         start[b] = total;
         for (int i = 0; i < kSortWaves; ++i) {
             const uint32_t c = next[i][b];
