@@ -9,10 +9,13 @@
 // scaled and added in 32 bits.
 //
 // The 8-bit matrix instructions do not keep all of a sum: of eight products at a time, each is cut off at 2^-13 of the largest
-// one's power of two before they are added in 32 bits (all their forms; measured: 1.4e-5 of a sum of 128
-// normal numbers' products, 1.5e-5 of the magnitudes' sum at most).  That is far below what a result loses that is rounded to 16 bits, so those results
-// take them; a 32-bit result has its 8-bit numbers widened to 16-bit floats, exactly, and takes the 16-bit
-// instructions, which keep every bit (9e-9) at half the rate.
+// one's power of two before they are added in 32 bits (all their forms).  The largest has 8 bits and stays whole, so eight
+// products lose less than 7 * 2^-13 of it, and a sum less than 8.5e-4 of its magnitudes' sum.  What that is in practice hangs on how
+// unlike the products are: 1.5e-5 at most in sums of 128 normal numbers' products, 1e-4 and more where some channels are much larger
+// than the others, the bound itself where one of eight is 2^13 times the rest (all relative to the magnitudes' sum).  Half an ulp of bf16
+// is 2.0e-3 - 3.9e-3: results in bf16 take these instructions.  Half an ulp of f16 is 2.4e-4 - 4.9e-4, less than the bound: results in
+// f16, like those in 32 bits, have their 8-bit numbers widened to 16-bit floats, exactly, and take the 16-bit
+// instructions, which keep every bit of a product and add in 32 bits (9e-9 of a sum of 128 normal numbers' products), at half the rate.
 #include "operators.hpp"
 
 namespace mint {
@@ -289,6 +292,9 @@ __device__ __forceinline__ f16x8 widened(int a, int b) {
     const f16x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false), v3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
     return f16x8{v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
 }
+// Whether results of type OUT are made from widened numbers (above).
+template <int OUT>
+constexpr bool kWidened = OUT != DT_BF16;
 // A 16 x 128 piece of an operand as the matrix instructions take it, and their sum over its depth.
 template <bool WIDE>
 struct Operand {
@@ -339,7 +345,7 @@ constexpr uint32_t DEALT = 32;
 // The weights are the matrix instruction's first operand, so a lane has consecutive columns of one row of the result (column_of).
 template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG, bool JOINED>
 __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(ProductArgs a) {
-    using Op = Operand<OUT == DT_F32>;
+    using Op = Operand<kWidened<OUT>>;
     using T = typename Elem<OUT>::type;
     constexpr int WN = BN / 64, WAVES = WM * WN, MT = BM / WM / 16, NT = 4;
     constexpr uint32_t kX = BM * 128, kW = BN * 128, kSx = BM * 4, kSw = ROWS_W ? BN * 4 : 256, kStage = kX + kW + kSx + kSw;
@@ -648,7 +654,7 @@ struct Strip {
 // X: the activations' type, DT_BYTES if they are in 8 bits
 template <int OUT, int X, int MT, int KWAYS>
 __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a) {
-    using Op = Operand<OUT == DT_F32>;
+    using Op = Operand<kWidened<OUT>>;
     using T = typename Elem<OUT>::type;
     constexpr bool ROUND = X != DT_BYTES;
     constexpr int WAVES = kThinWaves, BM = 16 * MT, BN = 16 * (WAVES / KWAYS), AHEAD = 4 / MT;
@@ -788,7 +794,7 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
     const float t64 = n64 <= 256 ? 0.32f : 0.5f * ceil_div(n64, 512), t128 = n128 <= 256 ? 0.72f : 1.29f * ceil_div(n128, 512),
                 wide = 1.2f * ceil_div(tiles(128, 256), 256), large = 2.0f * ceil_div(tiles(256, 256), 256);
     // (operands widened to 16 bits leave no registers for more wavefronts or larger tiles)
-    constexpr bool WIDE = OUT == DT_F32;
+    constexpr bool WIDE = kWidened<OUT>;
     const uint64_t blocks = ceil_div(a.depth, 128) / (ALONG && matrices ? matrices : 1);
     if (t64 <= t128 && t64 <= wide && t64 <= large) {
         if constexpr (!ALONG)
@@ -810,11 +816,11 @@ int go_product(const ProductArgs& a, uint32_t matrices, hipStream_t stream) {
 }
 
 // Where a product of one matrix has tiles of 64 x 64 for at most half of the compute units and a long depth: thread blocks to a tile. Rounded
-// before, us, with one and with these (and with results in 32 bits): 64 x 4096 x 4096 14.1 and 12.4 (18.1 and 13.1), 40 x 2048 x 8192 19.0 and 13.7,
+// before, us, with one and with these (and with widened operands): 64 x 4096 x 4096 14.1 and 12.4 (18.1 and 13.1), 40 x 2048 x 8192 19.0 and 13.7,
 // 100 x 1000 x 8000 19.4 and 13.6, 128 x 4096 x 4096 14.4 and 13.2, 50 x 5000 x 2500 11.5 and 11.6 (14.1 and 12.2), 48 x 7168 x 2048 10.0 and 11.2.
 uint32_t parts_of(uint64_t rows, uint64_t cols, uint64_t depth, int dtype) {
     const uint64_t tiles = ceil_div(rows, 64) * ceil_div(cols, 64), blocks = ceil_div(depth, 128);
-    if (tiles == 0 || tiles > 128 || blocks < (dtype == MINT_F32 ? 20 : 32)) return 1;
+    if (tiles == 0 || tiles > 128 || blocks < (dtype == MINT_BF16 ? 32 : 20)) return 1;
     return (uint32_t)std::min<uint64_t>(256 / tiles, blocks / 6);
 }
 // Few rows: at most 32 for each weight matrix, on the average (24 x 4096 x 4096: 7.8 us, with tiles of 64 x 64 9.4; at 64 rows

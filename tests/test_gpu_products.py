@@ -1,0 +1,71 @@
+"""Products in 8 bits against their definition in 64 bits where sums, rows and kernels can go wrong."""
+import pytest
+import torch
+
+from mintccl_amd.block8 import product, quantise, quantise_weight, weight_grad
+from mintccl_amd.routing import Assignment, assign
+from tests.expert_oracle import off_by, randn, rounded8, unlike, weight64
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+# ---- sums ------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("rows,cols,depth", [(1, 70, 384), (5, 300, 256), (20, 130, 384), (50, 200, 384), (100, 1000, 128), (64, 96, 256), (700, 1999, 384)])
+def test_sums_of_products_that_are_unlike(dev, rows, cols, depth, dt):
+    """Large products that cancel among small ones: the sums are whole numbers that results in 16-bit floats and in 32 bits have exactly."""
+    x, weights = unlike(rows, depth)
+    x, wf = x.to(dev), weights(cols).to(dev)
+    w = quantise_weight(wf)
+    assert torch.equal(w.q.float(), wf) and (w.scale == 1).all()
+    want = x.double() @ wf.double().t()
+    assert torch.equal(want.half().double(), want)
+    for given in (x, x.to(DT[dt]), quantise(x)):
+        got = product(given, w, dtype=DT[dt])
+        if dt == "bf16":
+            assert off_by(got, x.double(), wf.double()) <= 0
+        else:
+            assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+def test_sums_of_weights_gradients_that_are_unlike(dev, dt):
+    for rows, cols, depth in ((128, 40, 70), (384, 130, 300), (256, 700, 1100)):
+        x, weights = unlike(depth, rows)
+        x, d = x.t().contiguous().to(dev), weights(cols).t().contiguous().to(dev)
+        want = d.double().t() @ x.double()
+        got = weight_grad(d, x, dtype=DT[dt])
+        if dt == "bf16":
+            assert off_by(got, d.double().t(), x.double().t()) <= 0
+        else:
+            assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("rows,cols,depth", [(3, 200, 1000), (40, 130, 1000), (200, 300, 2048), (1000, 2000, 512)])
+def test_sums_with_large_channels(dev, rows, cols, depth, dt):
+    """One channel in eight 60 times larger than the others, as layers' outputs have them."""
+    x = randn(rows, depth, seed=rows, dev=dev)
+    x[:, ::8] *= 60
+    x = x.to(DT[dt])
+    w = quantise_weight(randn(cols, depth, seed=cols, dev=dev))
+    assert off_by(product(x, w, dtype=DT[dt]), rounded8(x, 1), weight64(w)) <= 0
+    assert off_by(product(x, w, dtype=torch.float32), rounded8(x, 1), weight64(w)) <= 0
+    d = randn(rows, 90, seed=3, dev=dev)
+    d[::8] *= 60
+    got = weight_grad(d, x, dtype=DT[dt])
+    assert off_by(got, rounded8(d, 0).t(), rounded8(x, 0).t()) <= 0
+
+
+def test_sums_by_expert_that_are_unlike(dev):
+    x, weights = unlike(300, 256)
+    wf = torch.stack([weights(130), -weights(130), weights(130).flip(0)]).to(dev)
+    counts = torch.tensor([0] * 200 + [1] * 3 + [2] * 90 + [-1] * 7, dtype=torch.int32)
+    plan = assign(counts[torch.randperm(300, generator=torch.Generator().manual_seed(1))][:, None].contiguous().to(dev), 3)
+    x = x.to(dev)
+    got = product(x, quantise_weight(wf), plan, gather=True, dtype=torch.float16)
+    at = plan.offsets.tolist()
+    for e in range(3):
+        rows = x[plan.tokens[at[e]:at[e + 1]].long()]
+        assert torch.equal(got[at[e]:at[e + 1]].double(), rows.double() @ wf[e].double().t())
