@@ -543,7 +543,7 @@ int mint_assign(const void* chosen, uint64_t tokens, uint32_t topk, uint32_t fir
  *   columns8  blocks along a column, q turned: (width, q_stride), scale
  *             (blocks, width).  With `offsets` (int32, experts + 1) the rows of an
  *             expert begin a new block; with `tokens` (int32, rows) row i is
- *             x[tokens[i]].  mint_columns8_blocks(rows, experts) blocks at most
+ *             x[tokens[i]], zeros if x has no such row.  mint_columns8_blocks(rows, experts) blocks at most
  *   squares8  squares of 128 x 128 of `matrices` matrices; scale
  *             (matrices, blocks of rows, blocks of depth) */
 int mint_rows8(const void* x, int64_t x_stride, uint64_t rows, uint64_t depth, int dtype, void* q,
@@ -566,8 +566,9 @@ int mint_squares8(const void* w, int64_t w_matrix, int64_t w_stride, uint32_t ma
  *                          `offsets` there are `experts` matrices w_matrix bytes apart,
  *                          rows offsets[e] .. offsets[e + 1] - 1 of out are made with
  *                          matrix e, and rows behind the last are zeros; with `tokens`
- *                          row i of out is made from row tokens[i] of x
- *   MINT_PRODUCT_GRADIENT  both operands as mint_columns8 leaves them: x (rows,
+ *                          row i of out is made from row tokens[i] of x, and is
+ *                          zeros if x has no such row
+ *   MINT_PRODUCT_GRADIENT  both operands as mint_columns8 leaves them: x (rows = x_rows,
  *                          depth), w (cols, depth), each with scales by rows and
  *                          blocks.  With `offsets` (experts' rows among group_rows, as for
  *                          mint_columns8) there are `experts` results out_matrix
@@ -598,7 +599,7 @@ size_t mint_product8_workspace(const mint_product_op* op);
 int mint_product8(const mint_product_op* op, void* stream);
 
 /* The gradient of the weights of a product: d^T x of d (rows, cols) and x (rows,
- * depth; with `tokens` row i is x[tokens[i]]), both rounded as by mint_columns8
+ * depth; with `tokens` row i is x[tokens[i]], zeros if x has no such row), both rounded as by mint_columns8
  * and multiplied as MINT_PRODUCT_GRADIENT.  With `offsets` there are `experts`
  * results, out_matrix elements apart.  workspace: mint_weight_grad8_workspace()
  * bytes, 16-byte aligned. */

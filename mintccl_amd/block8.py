@@ -64,8 +64,8 @@ def product(x: torch.Tensor | Blocks, weight: Blocks, plan: Assignment | None = 
     :class:`Blocks` yet; ``weight`` (cols, depth).  With ``plan`` the weight is
     (experts, cols, depth) and the result has a row for each place of the
     assignment, made with its expert's matrix from that row of ``x`` or, with
-    ``gather``, from the row of ``x`` that belongs to its token; rows that are no
-    expert's are zeros."""
+    ``gather``, from the row of ``x`` that belongs to its token (a token that ``x`` does
+    not have counts as zeros); rows that are no expert's are zeros."""
     q, scale = x if isinstance(x, Blocks) else (x, None)
     return _lib.experts().product(q, scale, weight.q, weight.scale, None if plan is None else plan.offsets,
                                   None if plan is None else plan.tokens, gather, _code(dtype), out)

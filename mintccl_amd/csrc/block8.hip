@@ -236,7 +236,7 @@ struct ProductArgs {
     const uint8_t *x, *w;
     const float *sx, *sw;
     void* out;
-    const int32_t* tokens;       // 0, or the row of x that row i of the result is made from
+    const int32_t* tokens;       // 0, or the row of x that row i of the result is made from (zeros if x has no such row)
     Groups groups;               // experts' rows (or, `along_depth`, experts' blocks of the depth)
     int64_t x_stride, w_stride, w_matrix, out_stride, out_matrix;
     int64_t sx_row, sx_block, sw_matrix, sw_row, sw_block;
@@ -476,6 +476,13 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
     const uint32_t r16 = lane & 15u, part = lane >> 4;
     const uint32_t xr = wm * (BM / WM) + r16, wr = wn * 64 + r16;
     const uint32_t x_at = xr * 128 + ((part ^ turn(xr)) * 16), w_at = kX + wr * 128 + ((part ^ turn(wr)) * 16);
+    // Which of a lane's rows of the result (bit i: the i-th) are made from rows that x does not have: those are zeros, whatever was brought in
+    // their place.
+    uint32_t absent = 0;
+    if (!ALONG && a.tokens && all_steps) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) absent |= ((uint32_t)a.tokens[min(m0 + xr + i * 16, m_end - 1)] >= a.x_rows ? 1u : 0u) << i;
+    }
     const uint32_t sx_at = kX + kW + xr * 4, sw_at = kX + kW + kSx + (ROWS_W ? wn * 64 + part * 8 : wn) * 4;
     // The matrix instructions' sums are scaled and added LAG instructions later: the two units work side by side.
     constexpr int LAG = 3;
@@ -618,7 +625,7 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
         for (int h = 0; h < 2; ++h) {
             float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = acc[i][h * 2 + k / 4][k % 4];
+            for (int k = 0; k < 8; ++k) v[k] = absent >> i & 1u ? 0.0f : acc[i][h * 2 + k / 4][k % 4];
             const uint32_t c = col + h * 32;
             if (c < a.cols) store_elements<OUT, 8>(to + c, (int64_t)a.cols - c, v);
         }
@@ -663,6 +670,7 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
     __shared__ float sums[WAVES][BM][17];
     __shared__ __attribute__((aligned(16))) uint8_t xs[ROUND ? 16 * XROW : 16];
     __shared__ float xscale[ROUND ? CHUNK : 1][16];
+    __shared__ bool gone[16];                                       // ROUND: rows that x does not have
     const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), r16 = lane & 15u, part = lane >> 4;
     const uint32_t way = wave % KWAYS, row_tile = blockIdx.x / a.col_tiles, n0 = blockIdx.x % a.col_tiles * BN, n = n0 + wave / KWAYS * 16;
     const Tile t = find_tile(a.groups, row_tile, BM, true);
@@ -674,15 +682,20 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
     const auto x_row = [&](uint32_t i) MINT_INLINE_LAMBDA {
-        uint32_t row = m0 + min(i, rows - 1);       // (lanes beyond the last row have that one too: what they make is not stored)
-        if (a.tokens) row = (uint32_t)a.tokens[row];
-        return min(row, a.x_rows - 1);
+        const uint32_t row = m0 + min(i, rows - 1);       // (lanes beyond the last row have that one too: what they make is not stored)
+        return a.tokens ? (uint32_t)a.tokens[row] : row;
     };
     const uint8_t* const w = a.w + (int64_t)t.expert * a.w_matrix + (int64_t)min(n + r16, a.cols - 1) * a.w_stride + part * 16;
     const float* const sw = a.sw + (int64_t)t.expert * a.sw_matrix + (int64_t)(min(n, a.cols - 1) / 128) * a.sw_row;
+    // (a row that x does not have is read as its last one, and makes zeros)
     uint32_t row[MT];
+    bool absent[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) row[i] = ROUND || !steps ? 0u : x_row(i * 16 + r16);
+    for (int i = 0; i < MT; ++i) {
+        row[i] = ROUND || !steps ? 0u : x_row(i * 16 + r16);
+        absent[i] = !ROUND && row[i] >= a.x_rows;
+        row[i] = min(row[i], a.x_rows - 1);
+    }
 
     // blocks of the depth from `first` on, CHUNK of them at most where they are rounded here
     for (uint32_t first = 0; first < steps; first += CHUNK) {
@@ -713,12 +726,14 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
                     const uint32_t blocks = end - first;
                     for (uint32_t unit = threadIdx.x / 16; unit < rows * blocks; unit += WAVES * 4) {
                         const uint32_t i = unit / blocks, b = unit % blocks, at = (first + b) * 128 + r16 * 8;
+                        const uint32_t from = x_row(i);
                         float v[8];
-                        load_elements<X, 8>(reinterpret_cast<const TX*>(a.x) + (int64_t)x_row(i) * a.x_stride + at, (int64_t)a.depth - at, v);
+                        load_elements<X, 8>(reinterpret_cast<const TX*>(a.x) + (int64_t)(a.tokens ? min(from, a.x_rows - 1) : from) * a.x_stride + at, (int64_t)a.depth - at, v);
                         u32x2 q;
                         const float s = round_block(v, q);
                         *reinterpret_cast<u32x2*>(xs + i * XROW + b * 128 + r16 * 8) = q;
                         if (r16 == 0) xscale[b][i] = s;
+                        if (a.tokens && r16 == 0 && b == 0) gone[i] = from >= a.x_rows;
                     }
                     __syncthreads();
                 }
@@ -746,9 +761,11 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
         if (!ROUND) break;
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) {
+        const bool zero = ROUND ? a.tokens && steps && gone[r16] : absent[i];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sums[wave][i * 16 + r16][part * 4 + k] = acc[i][k];
+        for (int k = 0; k < 4; ++k) sums[wave][i * 16 + r16][part * 4 + k] = zero ? 0.0f : acc[i][k];
+    }
     __syncthreads();
     for (uint32_t at = threadIdx.x; at < BM * BN; at += 64 * WAVES) {
         const uint32_t m = at / BN, c = at % BN;
@@ -1051,7 +1068,7 @@ extern "C" int mint_product8(const mint_product_op* op, void* stream) {
     // (nothing to multiply: the result is zeros, and neither operand is read)
     const bool some = op->depth != 0;
     if (some && (!op->x || !op->w || (!raw && !op->sx) || !op->sw || op->x_rows == 0)) return MINT_ERR_ARG;
-    if (some && !along && !op->tokens && op->x_rows < op->rows) return MINT_ERR_ARG;
+    if (some && (along || !op->tokens) && op->x_rows < op->rows) return MINT_ERR_ARG;
     if (some && ((!raw && (!aligned_to(reinterpret_cast<void*>(op->x), 16) || op->x_stride % 16)) || !aligned_to(reinterpret_cast<void*>(op->w), 16) ||
                  op->w_stride % 16 || op->w_matrix % 16))
         return MINT_ERR_ALIGN;

@@ -145,3 +145,7 @@ def test_the_operators_take_device_tensors():
         route(x, 2, score="tanh")
     with pytest.raises(TypeError, match="float16, bfloat16"):
         product(x, w, dtype=torch.int8)
+
+
+def test_the_gradients_product_refuses_fewer_rows_than_its_result():
+    assert _lib.lib().mint_product8(product_op(kind=1, rows=5, x_rows=4, sw_row=1), None) == _lib.ERR_ARG

@@ -69,3 +69,42 @@ def test_sums_by_expert_that_are_unlike(dev):
     for e in range(3):
         rows = x[plan.tokens[at[e]:at[e + 1]].long()]
         assert torch.equal(got[at[e]:at[e + 1]].double(), rows.double() @ wf[e].double().t())
+
+
+# ---- rows -------------------------------------------------------------------------
+def planned(dev, counts, tokens, k, seed):
+    """An assignment with `counts` places for its experts, the rest of tokens * k pairs without."""
+    flat = torch.full((tokens * k,), -1, dtype=torch.int32)
+    flat[:sum(counts)] = torch.repeat_interleave(torch.arange(len(counts), dtype=torch.int32), torch.tensor(counts))
+    return assign(flat[torch.randperm(tokens * k, generator=torch.Generator().manual_seed(seed))].view(tokens, k).to(dev), len(counts))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("counts,tokens,k,cols,depth", [
+    ([3, 0, 5], 8, 1, 70, 300), ([20, 30, 22], 40, 2, 130, 256), ([200, 1, 99, 300], 300, 2, 200, 384), ([1500, 0, 600], 1100, 2, 2000, 200),
+    ([2100, 1900], 2000, 2, 3700, 130)])
+def test_gathered_rows_that_are_not_there_are_zeros(dev, counts, tokens, k, cols, depth, dt):
+    """Token numbers outside x among an expert's rows: forward, and as the weights' gradient has them."""
+    plan, e = planned(dev, counts, tokens, k, seed=tokens), len(counts)
+    x = randn(tokens, depth, seed=1, dtype=DT[dt], dev=dev)
+    x[-1] = float("nan")                                     # (nothing of a row that stands in for another)
+    w = quantise_weight(randn(e, cols, depth, seed=2, dev=dev))
+    lost = torch.randperm(sum(counts), generator=torch.Generator().manual_seed(3))[:1 + sum(counts) // 7].to(dev)
+    named = plan.tokens.clone()
+    named[lost] = torch.tensor([-1, tokens, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device=dev)[torch.arange(len(lost), device=dev) % 4]
+    missing = torch.zeros(tokens * k, dtype=torch.bool, device=dev)
+    missing[lost] = True
+    broken = Assignment(plan.offsets, named, plan.slots)
+    for given in (x, quantise(x)):
+        want = torch.where(missing[:, None], 0, product(given, w, plan, gather=True, dtype=DT[dt]))
+        got = product(given, w, broken, gather=True, dtype=DT[dt])
+        assert torch.equal(got[missing], want[missing])
+        there = ~missing & (plan.tokens != tokens - 1)
+        assert torch.equal(got[there], want[there]) and torch.isfinite(got[there]).all()
+    x[-1] = 1.0
+    d = randn(tokens * k, 90, seed=4, dtype=DT[dt], dev=dev)
+    at = plan.offsets.tolist()
+    got = weight_grad(d, x, broken, gather=True, dtype=DT[dt])
+    for i in range(e):
+        own = torch.where(missing[at[i]:at[i + 1], None], 0, x[plan.tokens[at[i]:at[i + 1]].long()])
+        assert off_by(got[i], rounded8(d[at[i]:at[i + 1]], 0).t(), rounded8(own, 0).t()) <= 0
