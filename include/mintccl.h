@@ -565,7 +565,7 @@ int mint_squares8(const void* w, int64_t w_matrix, int64_t w_stride, uint32_t ma
  *                          depth) with a scale for each square of 128 x 128.  With
  *                          `offsets` there are `experts` matrices w_matrix bytes apart,
  *                          rows offsets[e] .. offsets[e + 1] - 1 of out are made with
- *                          matrix e, and rows behind the last are zeros; with `tokens`
+ *                          matrix e, and rows that are no matrix's are zeros; with `tokens`
  *                          row i of out is made from row tokens[i] of x, and is
  *                          zeros if x has no such row
  *   MINT_PRODUCT_GRADIENT  both operands as mint_columns8 leaves them: x (rows = x_rows,

@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t row_bound(const Groups& g, uint32_t i) {
     return min((uint32_t)max(g.offsets[i], 0), g.rows);
 }
 // The tiles of expert e, how many there are in all, and the expert of tile `t`.  `rest`: the rows that are no
-// expert's follow as those of an expert with number g.experts.  Every wavefront looks for itself, 64 experts at a time.
+// expert's follow as those of an expert with number g.experts, the ones before the first expert's and then those behind the last one's.  Every wavefront looks for itself, 64 experts at a time.
 __device__ __forceinline__ uint32_t tiles_of(const Groups& g, uint32_t e, uint32_t tile_rows, bool rest, uint32_t& begin, uint32_t& end) {
     begin = end = 0;
     if (e < g.experts + rest) {
@@ -66,7 +66,8 @@ __device__ __forceinline__ uint32_t count_tiles(const Groups& g, uint32_t tile_r
     if (!g.offsets) return (g.rows + tile_rows - 1) / tile_rows;
     uint32_t mine = 0, begin, end;
     for (uint32_t e = lane_id(); e < g.experts + rest; e += 64) mine += tiles_of(g, e, tile_rows, rest, begin, end);
-    return (uint32_t)__builtin_amdgcn_readlane((int)sum_below(mine), 63);
+    const uint32_t before = rest ? (row_bound(g, 0) + tile_rows - 1) / tile_rows : 0u;
+    return (uint32_t)__builtin_amdgcn_readlane((int)sum_below(mine), 63) + before;
 }
 __device__ __forceinline__ Tile find_tile(const Groups& g, uint32_t t, uint32_t tile_rows, bool rest) {
     Tile r = {0, 0, 0, g.rows, true};
@@ -88,8 +89,14 @@ __device__ __forceinline__ Tile find_tile(const Groups& g, uint32_t t, uint32_t 
     }
     r.expert = g.experts;
     r.first = base;
-    r.begin = row_bound(g, g.experts);
-    r.found = rest && t - base < (r.end - r.begin + tile_rows - 1) / tile_rows;
+    r.end = row_bound(g, 0);
+    const uint32_t before = (r.end + tile_rows - 1) / tile_rows;
+    if (t - base >= before) {
+        r.first = base + before;
+        r.begin = row_bound(g, g.experts);
+        r.end = g.rows;
+    }
+    r.found = rest && t - r.first < (r.end - r.begin + tile_rows - 1) / tile_rows;
     return r;
 }
 
@@ -776,9 +783,11 @@ __global__ void __launch_bounds__(64 * kThinWaves, 4) thin_kernel(ProductArgs a)
     }
 }
 
-// How many tiles of `tile_rows` rows there are at most, and about how many there will be (an expert's last is half full).
+// How many tiles of `tile_rows` rows there are at most: an expert's last one, and those of the rows before and behind the experts', may have a
+// single row.
 uint64_t most_row_tiles(const ProductArgs& a, uint32_t tile_rows) {
-    return ceil_div(a.rows, tile_rows) + (a.groups.offsets ? (uint64_t)a.groups.experts + 1 : 0);
+    if (!a.groups.offsets) return ceil_div(a.rows, tile_rows);
+    return std::min<uint64_t>(a.rows, (a.rows + ((uint64_t)a.groups.experts + 2) * (tile_rows - 1)) / tile_rows);
 }
 template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG, bool JOINED = false>
 int go_tiles(ProductArgs a, uint32_t matrices, hipStream_t stream) {

@@ -108,3 +108,21 @@ def test_gathered_rows_that_are_not_there_are_zeros(dev, counts, tokens, k, cols
     for i in range(e):
         own = torch.where(missing[at[i]:at[i + 1], None], 0, x[plan.tokens[at[i]:at[i + 1]].long()])
         assert off_by(got[i], rounded8(d[at[i]:at[i + 1]], 0).t(), rounded8(own, 0).t()) <= 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("offsets,rows,cols,depth", [
+    ([2, 2, 5], 6, 70, 300), ([1, 9, 9, 17], 40, 130, 256), ([17, 17, 30, 60], 64, 40, 200), ([70, 100, 300], 300, 200, 384),
+    ([300, 900, 900, 1500], 2100, 2000, 200), ([600, 600], 600, 100, 128), ([5] * 71, 80, 64, 100), ([513, 2500, 3600], 4000, 3700, 130)])
+def test_rows_that_are_no_experts_are_zeros(dev, offsets, rows, cols, depth, dt):
+    """Rows before the first expert's too, whatever the result's memory held."""
+    at, e = torch.tensor(offsets, dtype=torch.int32, device=dev), len(offsets) - 1
+    x, w = randn(rows, depth, seed=1, dtype=DT[dt], dev=dev), quantise_weight(randn(e, cols, depth, seed=2, dev=dev))
+    tokens = torch.arange(rows, dtype=torch.int32, device=dev)
+    plan = Assignment(at, tokens, tokens[:, None])
+    for given in (x, quantise(x)):
+        got = product(given, w, plan, out=torch.full((rows, cols), float("nan"), dtype=DT[dt], device=dev))
+        assert (got[:offsets[0]] == 0).all() and (got[offsets[-1]:] == 0).all()
+        for i in range(e):
+            own = slice(offsets[i], offsets[i + 1])
+            assert off_by(got[own], rounded8(x[own], 1), weight64(type(w)(w.q[i], w.scale[i]))) <= 0
