@@ -28,6 +28,9 @@ class Blocks(NamedTuple):
     scale: torch.Tensor      #: float32: (rows, blocks), of weights (blocks of rows, blocks), with as many dimensions as q
 
 
+_NO_PLAN = (None, None, None)
+
+
 def _code(dtype: torch.dtype | None) -> int | None:
     if dtype is not None and dtype not in DTYPE_CODE:
         raise TypeError("products come in float16, bfloat16 or float32")
@@ -64,11 +67,10 @@ def product(x: torch.Tensor | Blocks, weight: Blocks, plan: Assignment | None = 
     :class:`Blocks` yet; ``weight`` (cols, depth).  With ``plan`` the weight is
     (experts, cols, depth) and the result has a row for each place of the
     assignment, made with its expert's matrix from that row of ``x`` or, with
-    ``gather``, from the row of ``x`` that belongs to its token (a token that ``x`` does
-    not have counts as zeros); rows that are no expert's are zeros."""
+    ``gather``, from the row of ``x`` that belongs to its token (``x`` has one for each
+    token of the assignment; a token number that is none of them counts as zeros); rows that are no expert's are zeros."""
     q, scale = x if isinstance(x, Blocks) else (x, None)
-    return _lib.experts().product(q, scale, weight.q, weight.scale, None if plan is None else plan.offsets,
-                                  None if plan is None else plan.tokens, gather, _code(dtype), out)
+    return _lib.experts().product(q, scale, weight.q, weight.scale, *(plan or _NO_PLAN), gather, _code(dtype), out)
 
 
 def weight_grad(grad: torch.Tensor, x: torch.Tensor, plan: Assignment | None = None, *, gather: bool = False,
@@ -77,5 +79,4 @@ def weight_grad(grad: torch.Tensor, x: torch.Tensor, plan: Assignment | None = N
     from its result's ``grad``: ``grad.T @ x``, of ``dtype`` (float32 if none is
     named), for each expert where there is a ``plan``.  Both sides are rounded to
     8 bits in blocks of 128 rows (of an expert's 128 rows)."""
-    return _lib.experts().weight_grad(grad, x, None if plan is None else plan.offsets, None if plan is None else plan.tokens,
-                                      gather, _code(dtype))
+    return _lib.experts().weight_grad(grad, x, *(plan or _NO_PLAN), gather, _code(dtype))

@@ -373,15 +373,22 @@ void plan_of(const Tensor& like, const Tensor& offsets, const Tensor& order) {
     dense(order, "tokens");
     if (offsets.size(0) < 1) refuse(PyExc_ValueError, "offsets must have a number at least");
 }
+// rows that are gathered by an assignment's tokens, of which its slots, where they are known, have a row each
+void gathered(const Args& a, int slots, const Tensor& x) {
+    if (a.none(slots)) return;
+    const Tensor& t = a.tensor(slots, "slots");
+    dims(t, 2, "slots");
+    if (x.size(0) < t.size(0)) refuse(PyExc_ValueError, "x has %lld rows, the assignment %lld tokens", (long long)x.size(0), (long long)t.size(0));
+}
 
-// product(x, x_scale or None, wq, w_scale, offsets or None, tokens or None, gather, dtype, out or None)
+// product(x, x_scale or None, wq, w_scale, offsets or None, tokens or None, slots or None, gather, dtype, out or None)
 PyObject* host_product(PyObject*, PyObject* const* list, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        const Args a(list, n, 9);
+        const Args a(list, n, 10);
         const Tensor &x = a.tensor(0, "x"), &w = a.tensor(2, "weight"), &sw = a.tensor(3, "the weight's scale");
         rows_of(x, "x");
         same_device(x, w, "weight");
-        const bool by_expert = !a.none(4), gather = a.truth(6);
+        const bool by_expert = !a.none(4), gather = a.truth(7);
         if (gather && !by_expert) refuse(PyExc_ValueError, "gather needs an assignment");
         dims(w, by_expert ? 3 : 2, "weight");
         eight_rows(w, "weight");
@@ -404,20 +411,21 @@ PyObject* host_product(PyObject*, PyObject* const* list, Py_ssize_t n) {
             op.w_matrix = apart(w, 0);
             op.sw_matrix = apart(sw, 0);
             if (gather) {
+                gathered(a, 6, x);
                 op.tokens = address(order);
                 if (x.size(0) == 0 && rows) refuse(PyExc_ValueError, "x has no rows to gather");
             }
         }
         int64_t code;
-        const bool given = !a.none(8);
+        const bool given = !a.none(9);
         if (given) {
-            const Tensor& out = a.tensor(8, "out");
+            const Tensor& out = a.tensor(9, "out");
             same_device(x, out, "out");
             result(out, rows, cols, "out");
             code = code_of(out.scalar_type(), "out");
-            if (!a.none(7) && a.integer(7, "dtype", 0, 2) != code) refuse(PyExc_TypeError, "out is of another type than dtype");
+            if (!a.none(8) && a.integer(8, "dtype", 0, 2) != code) refuse(PyExc_TypeError, "out is of another type than dtype");
         } else {
-            code = a.none(7) ? (int64_t)MINT_BF16 : a.integer(7, "dtype", 0, 2);
+            code = a.none(8) ? (int64_t)MINT_BF16 : a.integer(8, "dtype", 0, 2);
         }
         const bool already = !a.none(1);
         if (already) {
@@ -427,7 +435,7 @@ PyObject* host_product(PyObject*, PyObject* const* list, Py_ssize_t n) {
             code_of(x.scalar_type(), "x");
         }
         OnDevice on(x.get_device());
-        const Tensor out = given ? a.tensor(8, "out") : empty(x, {rows, cols}, type_of(code));
+        const Tensor out = given ? a.tensor(9, "out") : empty(x, {rows, cols}, type_of(code));
         op.x = address(x);
         if (already) {
             const Tensor& sx = a.tensor(1, "x's scale");
@@ -458,26 +466,26 @@ PyObject* host_product(PyObject*, PyObject* const* list, Py_ssize_t n) {
             op.workspace = address(room);
         }
         launch("mint_product8", [&] { return native.product8(&op, on.stream); });
-        if (given) return Py_NewRef(list[8]);
+        if (given) return Py_NewRef(list[9]);
         return wrap(out);
     });
 }
 
-// weight_grad(d, x, offsets or None, tokens or None, gather, dtype)
+// weight_grad(d, x, offsets or None, tokens or None, slots or None, gather, dtype)
 PyObject* host_weight_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
-        const Args a(list, n, 6);
+        const Args a(list, n, 7);
         const Tensor &d = a.tensor(0, "grad"), &x = a.tensor(1, "x");
         rows_of(d, "grad");
         rows_of(x, "x");
         same_device(x, d, "grad");
         const int d_code = code_of(d.scalar_type(), "grad"), x_code = code_of(x.scalar_type(), "x");
-        const bool by_expert = !a.none(2), gather = a.truth(4);
+        const bool by_expert = !a.none(2), gather = a.truth(5);
         if (gather && !by_expert) refuse(PyExc_ValueError, "gather needs an assignment");
         mint_weight_grad_op op = {};
         op.d_dtype = d_code;
         op.x_dtype = x_code;
-        op.dtype = a.none(5) ? (int32_t)MINT_F32 : (int32_t)a.integer(5, "dtype", 0, 2);
+        op.dtype = a.none(6) ? (int32_t)MINT_F32 : (int32_t)a.integer(6, "dtype", 0, 2);
         const int64_t rows = d.size(0), cols = d.size(1), depth = x.size(1);
         int64_t experts = 0;
         if (by_expert) {
@@ -487,7 +495,10 @@ PyObject* host_weight_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
             experts = offsets.size(0) - 1;
             if (experts > 65535) refuse(PyExc_ValueError, "at most 65535 experts");
             op.offsets = address(offsets);
-            if (gather) op.tokens = address(order);
+            if (gather) {
+                gathered(a, 4, x);
+                op.tokens = address(order);
+            }
         }
         if (gather ? x.size(0) == 0 && rows != 0 : x.size(0) != rows) refuse(PyExc_ValueError, "x and grad have different numbers of rows");
         OnDevice on(x.get_device());

@@ -126,3 +126,17 @@ def test_rows_that_are_no_experts_are_zeros(dev, offsets, rows, cols, depth, dt)
         for i in range(e):
             own = slice(offsets[i], offsets[i + 1])
             assert off_by(got[own], rounded8(x[own], 1), weight64(type(w)(w.q[i], w.scale[i]))) <= 0
+
+
+def test_an_assignment_of_more_tokens_than_rows_is_refused(dev):
+    plan = planned(dev, [4, 3], 6, 2, seed=1)
+    x, w, d = randn(5, 128, seed=1, dev=dev), quantise_weight(randn(2, 64, 128, seed=2, dev=dev)), randn(12, 64, seed=3, dev=dev)
+    for call in (lambda: product(x, w, plan, gather=True), lambda: product(quantise(x), w, plan, gather=True),
+                 lambda: weight_grad(d, x, plan, gather=True)):
+        with pytest.raises(ValueError, match="x has 5 rows, the assignment 6 tokens"):
+            call()
+    more = randn(9, 128, seed=1, dev=dev)                       # (rows behind the tokens' are nobody's)
+    assert torch.equal(product(more, w, plan, gather=True), product(more[:6], w, plan, gather=True))
+    for call in (lambda: product(x, w, gather=True), lambda: weight_grad(d, d, gather=True)):
+        with pytest.raises(ValueError, match="gather needs"):
+            call()
