@@ -65,9 +65,12 @@ class ExpertLayer:
         self.comm.run(lambda r: reducescatter(rows[r].view(world, -1), self.comm))
         return [rows[r].view(world, -1, width)[r] for r in range(world)]
 
-    def forward(self, tokens: list[torch.Tensor]) -> list[torch.Tensor]:
-        """``tokens``: (n, width) of each rank, the same number on all, bfloat16 or float16."""
-        sums, self.kept = [], []
+    def forward(self, tokens: list[torch.Tensor], kept: list | None = None) -> list[torch.Tensor]:
+        """``tokens``: (n, width) of each rank, the same number on all, bfloat16 or float16.  ``kept``, an empty
+        list, takes what :meth:`backward` needs of this pass; without it nothing stays behind."""
+        if kept:
+            raise ValueError("kept holds what another pass needs")
+        sums = []
         for r, x in enumerate(self._gathered(tokens)):
             rank = self.ranks[r]
             logits = x.float() @ self.router.t()
@@ -77,15 +80,18 @@ class ExpertLayer:
             h = F.silu(u)
             y = product(h, rank["down"], plan, dtype=x.dtype)
             sums.append(combine(y, plan, weights))
-            self.kept.append((x, logits, weights, experts, plan, u, h, y))
+            if kept is not None:
+                kept.append((x, logits, weights, experts, plan, u, h, y))
         return self._summed(sums)
 
-    def backward(self, grads: list[torch.Tensor]) -> tuple[list[torch.Tensor], list[dict[str, torch.Tensor]]]:
-        """From the outputs' gradients: each rank's tokens' and its weights' (``up``, ``down``
-        of its own experts; ``router``, the same on all ranks)."""
+    def backward(self, grads: list[torch.Tensor], kept: list) -> tuple[list[torch.Tensor], list[dict[str, torch.Tensor]]]:
+        """From the outputs' gradients and what the forward pass that they belong to has ``kept``: each rank's tokens' and its weights'
+        gradients (``up``, ``down`` of its own experts; ``router``, the same on all ranks)."""
+        if len(kept) != self.comm.world_size:
+            raise ValueError("kept must be what a forward pass of this layer has left")
         sums, found = [], []
         for r, d in enumerate(self._gathered(grads)):
-            rank, (x, logits, weights, experts, plan, u, h, y) = self.ranks[r], self.kept[r]
+            rank, (x, logits, weights, experts, plan, u, h, y) = self.ranks[r], kept[r]
             d_y, d_weights = combine_grad(d, y, plan, weights)
             d_h = product(d_y, rank["down_t"], plan, dtype=x.dtype)
             d_down = weight_grad(d_y, h, plan)
@@ -129,8 +135,9 @@ def distances(world: int, device, **options) -> dict[str, float]:
     """How far a small layer's outputs and gradients are from the plain one's in 64 bits (2-norms)."""
     s = small_layer(world, device)
     layer = ExpertLayer(VirtualComm(world_size=world, device=device), s["router"], s["up"], s["down"], 4, **options)
-    out = layer.forward(s["tokens"])
-    d_tokens, found = layer.backward(s["grads"])
+    kept: list = []
+    out = layer.forward(s["tokens"], kept)
+    d_tokens, found = layer.backward(s["grads"], kept)
     layer.comm.check()
     leaf = {n: s[n].double().requires_grad_() for n in ("router", "up", "down")}
     x = torch.cat(s["tokens"]).double().requires_grad_()
