@@ -59,11 +59,12 @@ class ExpertLayer:
         self.comm.run(lambda r: allgather(buffers[r], self.comm))
         return [b.view(-1, width) for b in buffers]
 
-    def _summed(self, rows: list[torch.Tensor]) -> list[torch.Tensor]:
-        """Each rank's own rows of the ranks' sum; ``rows`` are used up."""
-        world, width = self.comm.world_size, rows[0].shape[1]
-        self.comm.run(lambda r: reducescatter(rows[r].view(world, -1), self.comm))
-        return [rows[r].view(world, -1, width)[r] for r in range(world)]
+    def _summed(self, rows: list[torch.Tensor], dtype: torch.dtype) -> list[torch.Tensor]:
+        """Each rank's own rows of the ranks' sum; ``rows`` are used up.  They travel in float32, so that the sum is rounded once, at its
+        end (in 16 bits, half the bytes, every rank on the way would round it)."""
+        world, (total, width) = self.comm.world_size, rows[0].shape
+        self.comm.run(lambda r: reducescatter(rows[r].view(world, total // world * width), self.comm))
+        return [rows[r].view(world, total // world, width)[r].to(dtype) for r in range(world)]
 
     def forward(self, tokens: list[torch.Tensor], kept: list | None = None) -> list[torch.Tensor]:
         """``tokens``: (n, width) of each rank, the same number on all, bfloat16 or float16.  ``kept``, an empty
@@ -79,10 +80,11 @@ class ExpertLayer:
             u = product(x, rank["up"], plan, gather=True, dtype=x.dtype)
             h = F.silu(u)
             y = product(h, rank["down"], plan, dtype=x.dtype)
-            sums.append(combine(y, plan, weights))
+            # (a rank's part is rounded once more, to the type of the rows that it is made from)
+            sums.append(combine(y, plan, weights).float())
             if kept is not None:
                 kept.append((x, logits, weights, experts, plan, u, h, y))
-        return self._summed(sums)
+        return self._summed(sums, tokens[0].dtype)
 
     def backward(self, grads: list[torch.Tensor], kept: list) -> tuple[list[torch.Tensor], list[dict[str, torch.Tensor]]]:
         """From the outputs' gradients and what the forward pass that they belong to has ``kept``: each rank's tokens' and its weights'
@@ -101,10 +103,10 @@ class ExpertLayer:
             # (pairs of other ranks' experts have no gradient here: the ranks' sums are the whole ones)
             d_logits = route_grad(d_weights, logits, experts, **self.grad_options)
             d_x = combine(product(d_u, rank["up_t"], plan, dtype=x.dtype), plan)
-            sums.append((d_x.float() + d_logits @ self.router).to(x.dtype))
+            sums.append(d_x.float() + d_logits @ self.router)
             found.append({"up": d_up, "down": d_down, "router": d_logits.t() @ x.float()})
         self.comm.run(lambda r: allreduce(found[r]["router"], self.comm))
-        return self._summed(sums), found
+        return self._summed(sums, grads[0].dtype), found
 
 
 def plain_layer(x, router, up, down, k, bias=None, score="softmax", renormalise=True):
