@@ -580,8 +580,9 @@ PyObject* host_combine_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
         if (d.size(0) != slots.size(0) || d.size(1) != rows.size(1)) refuse(PyExc_ValueError, "grad must be what the combination's result is like");
         if (rows.size(0) != slots.numel()) refuse(PyExc_ValueError, "rows must have one for each place of the assignment");
         if (rows.size(1) > 0x7FFFFFFF - 8192) refuse(PyExc_ValueError, "the rows are too long");
-        const void* weights = nullptr;
-        if (!a.none(4)) {
+        const void* weights = nullptr;                 // (of no tokens there are none either way)
+        const bool weighted = !a.none(4);
+        if (weighted) {
             const Tensor& w = a.tensor(4, "weights");
             weights_of(w, slots, "weights");
             weights = w.data_ptr();
@@ -589,14 +590,14 @@ PyObject* host_combine_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
         OnDevice on(rows.get_device());
         const Tensor d_rows = empty(rows, rows.sizes(), rows.scalar_type());
         Tensor d_weights;
-        if (weights) d_weights = empty(rows, slots.sizes(), at::kFloat);
+        if (weighted) d_weights = empty(rows, slots.sizes(), at::kFloat);
         const int32_t* const used = static_cast<const int32_t*>(offsets.data_ptr()) + (offsets.size(0) - 1);
         launch("mint_combine_grad", [&] {
             return native.combine_grad(d.data_ptr(), d.stride(0), rows.data_ptr(), rows.stride(0), (uint64_t)rows.size(0), slots.data_ptr(), weights,
                                        used, (uint64_t)slots.size(0), (uint32_t)slots.size(1), (uint32_t)rows.size(1), d_rows.data_ptr(),
-                                       d_rows.stride(0), weights ? d_weights.data_ptr() : nullptr, dtype, on.stream);
+                                       d_rows.stride(0), weighted ? d_weights.data_ptr() : nullptr, dtype, on.stream);
         });
-        return pack({wrap(d_rows), weights ? wrap(d_weights) : Py_NewRef(Py_None)});
+        return pack({wrap(d_rows), weighted ? wrap(d_weights) : Py_NewRef(Py_None)});
     });
 }
 

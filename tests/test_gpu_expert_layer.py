@@ -146,3 +146,13 @@ def test_a_layers_steps_one_by_one(dev, world, options):
     assert near(torch.cat(d_tokens), d_x + d_logits @ s["router"].double())
     for f in found:
         assert near(f["router"], d_logits.t() @ x.double())
+
+
+def test_a_layer_of_no_tokens(dev):
+    layer, s = small(4, dev)
+    none = [t[:0] for t in s["tokens"]]
+    kept = []
+    assert [tuple(t.shape) for t in layer.forward(none, kept)] == [(0, 320)] * 4
+    d_tokens, found = layer.backward(none, kept)
+    assert [tuple(t.shape) for t in d_tokens] == [(0, 320)] * 4
+    assert all((f[n] == 0).all() for f in found for n in ("up", "down", "router"))
