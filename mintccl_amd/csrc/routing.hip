@@ -13,6 +13,7 @@
 #include "operators.hpp"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace mint {
 namespace {
@@ -27,6 +28,13 @@ __device__ __forceinline__ uint32_t order_of(float v) {
 }
 __device__ __forceinline__ float number_of(uint32_t key) {
     return key == 0u ? -INFINITY : __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+// The key of a group whose two largest keys are these (the second may be missing): of two that are there the sum is too, also where it is
+// beyond 32 bits' range, as that of two masks of the type's lowest number.
+__device__ __forceinline__ uint32_t sum_of_two(uint32_t best, uint32_t second) {
+    if (second == 0u) return best;
+    const float sum = number_of(best) + number_of(second);
+    return order_of(sum == -INFINITY ? -FLT_MAX : sum);
 }
 __device__ __forceinline__ float sigmoid(float x) { return 1.0f / (1.0f + expf(-x)); }
 
@@ -115,7 +123,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
             if (lanes > 2) join_best<0x4E>(best, second);
             if (lanes > 4) join_best<0x141>(best, second);
             if (lanes > 8) join_best<0x140>(best, second);
-            uint32_t of_group = a.group_top == 2 && second != 0u ? order_of(number_of(best) + number_of(second)) : best;
+            uint32_t of_group = a.group_top == 2 ? sum_of_two(best, second) : best;
             bool keep = false;
             for (uint32_t n = 0; n < a.kept; ++n) {
                 const uint32_t top = L::max_of(of_group), holder = L::first(of_group == top) % LANES;
@@ -143,7 +151,7 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_kernel(RouteArgs a) {
                 uint32_t top = L::max_of(best);
                 const bool holds = lane == L::first(best == top) % LANES;
                 const uint32_t next = L::max_of(holds ? second : best);
-                if (a.group_top == 2 && next != 0u) top = order_of(number_of(top) + number_of(next));
+                if (a.group_top == 2) top = sum_of_two(top, next);
 #pragma unroll
                 for (int q = 0; q < PER_LANE; ++q) of_group[q] = q * LANES + lane == g ? top : of_group[q];
             }

@@ -21,3 +21,25 @@ def test_gradients_of_no_tokens(dev):
     assert combine_grad(rows, rows, plan)[1] is None
     logits = torch.zeros(0, 8, device=dev)
     assert route_grad(d_weights, logits, plan.slots).shape == (0, 8)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("experts,groups", [(16, 4), (12, 4), (256, 8), (320, 8), (18, 3)])
+def test_groups_masked_by_the_lowest_number(dev, experts, groups, dt):
+    """Groups whose two best keys are the type's lowest number: their sum is beyond 32 bits' range, and their experts are there all the same, behind all
+    others and in order."""
+    per, low = experts // groups, torch.finfo(dt).min
+    x = torch.full((4, experts), low)
+    x[1, per * (groups - 1):] = torch.arange(per).flip(0).float()       # the last group counts
+    x[2, per:2 * per] = -math.inf                                       # the second one is masked altogether
+    x[3] = -math.inf
+    x[3, 2 * per + 1:2 * per + 3] = low                                 # (two experts of the third group)
+    x = x.to(dt).to(dev)
+    w, chosen = (v.cpu() for v in route(x, 4, groups=groups, kept=2, group_top=2))
+    first = list(range(min(4, per))) + list(range(per, per + 4))
+    assert chosen[0].tolist() == first[:4]
+    last = [per * (groups - 1) + i for i in range(per)]
+    assert chosen[1].tolist() == (last + first)[:4]
+    assert chosen[2].tolist() == (list(range(min(4, per))) + [2 * per + i for i in range(4)])[:4]
+    assert chosen[3].tolist() == [2 * per + 1, 2 * per + 2, -1, -1]
+    assert torch.allclose(w[0], torch.full((4,), 0.25)) and w[3].tolist() == [0.5, 0.5, 0.0, 0.0]
