@@ -264,7 +264,8 @@ __global__ void __launch_bounds__(64 * kRouteWaves) route_grad_kernel(RouteGradA
         const float s = there ? sigmoid(l) : 0.0f, slope = there ? e / ((1.0f + e) * (1.0f + e)) : 0.0f;
         if (a.renormalise) {
             const float total = wave_sum(s), mean = wave_sum(there ? s * d : 0.0f);
-            g = total == 0.0f ? 0.0f : a.scale * ((d - mean / total) / total) * slope;
+            // (a slope is at most its score: the quotients stay in range however small the scores are)
+            g = total == 0.0f ? 0.0f : a.scale * (d - mean / total) * (slope / total);
         } else {
             g = a.scale * d * slope;
         }

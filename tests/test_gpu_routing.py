@@ -43,3 +43,20 @@ def test_groups_masked_by_the_lowest_number(dev, experts, groups, dt):
     assert chosen[2].tolist() == (list(range(min(4, per))) + [2 * per + i for i in range(4)])[:4]
     assert chosen[3].tolist() == [2 * per + 1, 2 * per + 2, -1, -1]
     assert torch.allclose(w[0], torch.full((4,), 0.25)) and w[3].tolist() == [0.5, 0.5, 0.0, 0.0]
+
+
+def test_gradient_of_scores_that_almost_vanish(dev):
+    """Sigmoids near the end of 32 bits' range, divided by their sum: the quotients are ordinary numbers, and so are the gradients."""
+    x = torch.tensor([[-88.0, -88.5, -87.5, -95.0], [-80.0, -85.0, -88.0, -70.0], [-86.0, -86.0, -86.0, -86.0], [-20.0, 3.0, -60.0, 0.0]], device=dev)
+    d = torch.tensor([[4.0, -7.0, 100.0], [1.0, 2.0, -3.0], [1.0, 0.0, 0.0], [1.0, -1.0, 2.0]], device=dev)
+    w, chosen = route(x, 3, score="sigmoid")
+    assert chosen.tolist() == [[2, 0, 1], [3, 0, 1], [0, 1, 2], [1, 3, 0]]
+    x64 = x.double().requires_grad_()
+    s = torch.sigmoid(x64).gather(1, chosen.long())
+    want = s / s.sum(-1, keepdim=True)
+    # a score of 2^-126 and less has 22 bits here at -88.5: 2^-21 of it, three scores, a sum and quotients
+    assert torch.allclose(w.double(), want, rtol=2.0 ** -17, atol=0)
+    (want * d.double()).sum().backward()
+    got = route_grad(d, x, chosen, score="sigmoid")
+    assert torch.isfinite(got).all()
+    assert ((got.double() - x64.grad).abs() <= 2.0 ** -15 * d.abs().max(1, keepdim=True).values.double()).all()
