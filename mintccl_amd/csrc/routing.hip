@@ -513,6 +513,17 @@ int launch_route(const RouteArgs& a, int dtype, hipStream_t stream) {
 }
 int launch_route_grad(const RouteGradArgs& a, int dtype, hipStream_t stream) { MINT_BY_TYPE(go_route_grad, 64) }
 
+// A launch has fewer than 2^32 threads, and a token up to 64 of them: more tokens take several launches.
+constexpr uint64_t kTokensOfLaunch = 1ull << 25;
+template <typename F>
+int in_launches(uint64_t tokens, const F& go) {
+    int err = MINT_OK;
+    for (uint64_t t = 0; t < tokens && err == MINT_OK; t += kTokensOfLaunch) err = go(t, (uint32_t)std::min(tokens - t, kTokensOfLaunch));
+    return err;
+}
+// element i of numbers of a type
+const void* element(uint64_t base, int64_t i, int dtype) { return reinterpret_cast<const void*>(base + i * (dtype == MINT_F32 ? 4 : 2)); }
+
 bool routable(uint64_t tokens, uint32_t experts, uint32_t topk, int dtype, int score) {
     return experts >= 1 && experts <= kMostExperts && topk >= 1 && topk <= 64 && topk <= experts && tokens < (1ull << 31) &&
            (dtype == MINT_F16 || dtype == MINT_BF16 || dtype == MINT_F32) && (score == MINT_SCORE_SOFTMAX || score == MINT_SCORE_SIGMOID);
@@ -530,22 +541,27 @@ extern "C" int mint_route(const mint_route_op* op, void* stream) {
         return MINT_ERR_GEOMETRY;
     if (op->tokens == 0) return MINT_OK;
     if (!op->logits || !op->weights || !op->chosen) return MINT_ERR_ARG;
-    const RouteArgs a = {reinterpret_cast<const void*>(op->logits), reinterpret_cast<const float*>(op->bias),
-                         reinterpret_cast<float*>(op->weights), reinterpret_cast<int32_t*>(op->chosen), op->row_stride,
-                         (uint32_t)op->tokens, op->experts, op->topk, op->groups, op->kept, op->group_top, op->scale,
-                         op->score == MINT_SCORE_SIGMOID, op->renormalise != 0};
-    return launch_route(a, op->dtype, static_cast<hipStream_t>(stream));
+    return in_launches(op->tokens, [&](uint64_t t, uint32_t n) {
+        const RouteArgs a = {element(op->logits, (int64_t)t * op->row_stride, op->dtype), reinterpret_cast<const float*>(op->bias),
+                             reinterpret_cast<float*>(op->weights) + t * op->topk, reinterpret_cast<int32_t*>(op->chosen) + t * op->topk, op->row_stride,
+                             n, op->experts, op->topk, op->groups, op->kept, op->group_top, op->scale,
+                             op->score == MINT_SCORE_SIGMOID, op->renormalise != 0};
+        return launch_route(a, op->dtype, static_cast<hipStream_t>(stream));
+    });
 }
 
 extern "C" int mint_route_grad(const mint_route_op* op, uint64_t d_weights, uint64_t d_logits, int64_t d_stride, void* stream) {
     if (!op || !routable(op->tokens, op->experts, op->topk, op->dtype, op->score)) return MINT_ERR_ARG;
     if (op->tokens == 0) return MINT_OK;
     if (!op->logits || !op->chosen || !d_weights || !d_logits) return MINT_ERR_ARG;
-    const RouteGradArgs a = {reinterpret_cast<const void*>(op->logits), reinterpret_cast<const float*>(d_weights),
-                             reinterpret_cast<const int32_t*>(op->chosen), reinterpret_cast<void*>(d_logits), op->row_stride, d_stride,
-                             (uint32_t)op->tokens, op->experts, op->topk, op->scale,
-                             op->score == MINT_SCORE_SIGMOID, op->renormalise != 0};
-    return launch_route_grad(a, op->dtype, static_cast<hipStream_t>(stream));
+    return in_launches(op->tokens, [&](uint64_t t, uint32_t n) {
+        const RouteGradArgs a = {element(op->logits, (int64_t)t * op->row_stride, op->dtype), reinterpret_cast<const float*>(d_weights) + t * op->topk,
+                                 reinterpret_cast<const int32_t*>(op->chosen) + t * op->topk,
+                                 const_cast<void*>(element(d_logits, (int64_t)t * d_stride, op->dtype)), op->row_stride, d_stride,
+                                 n, op->experts, op->topk, op->scale,
+                                 op->score == MINT_SCORE_SIGMOID, op->renormalise != 0};
+        return launch_route_grad(a, op->dtype, static_cast<hipStream_t>(stream));
+    });
 }
 
 namespace {

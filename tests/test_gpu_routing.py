@@ -60,3 +60,24 @@ def test_gradient_of_scores_that_almost_vanish(dev):
     got = route_grad(d, x, chosen, score="sigmoid")
     assert torch.isfinite(got).all()
     assert ((got.double() - x64.grad).abs() <= 2.0 ** -15 * d.abs().max(1, keepdim=True).values.double()).all()
+
+
+def test_more_tokens_than_a_launch_has_threads_for(dev):
+    """2^26 tokens and some, 64 threads each in the gradient: the same as alone at the ends and where launches meet."""
+    n, k = (1 << 26) + 77, 2
+    some = randn(1 << 16, 8, seed=1, dtype=torch.bfloat16, dev=dev)
+    x = torch.empty(n, 8, dtype=torch.bfloat16, device=dev)
+    for at in range(0, n, 1 << 16):                  # (no two parts alike)
+        x[at:at + (1 << 16)] = some[:n - at].roll(at >> 16, 0)
+    d = torch.ones(n, k, device=dev)
+    d[1::3, 1] = -2.0
+    w, chosen = route(x, k)
+    got = route_grad(d, x, chosen)
+    for at in (0, (1 << 25) - 50, (1 << 26) - 50, n - 100):
+        own = slice(at, at + 100)
+        alone = route(x[own], k)
+        assert torch.equal(w[own], alone[0]) and torch.equal(chosen[own], alone[1])
+        assert torch.equal(got[own], route_grad(d[own], x[own], alone[1]))
+    assert (chosen >= 0).all() and torch.isfinite(w.view(-1)).all()
+    del x, w, chosen, got, d
+    torch.cuda.empty_cache()
