@@ -1,5 +1,5 @@
 """The combination of the experts' rows: a token's rows, added up with its weights,
-and the gradients of both.  No counterpart in the reference."""
+and the gradients of both (calls of their own, as in :mod:`~mintccl_amd.routing`).  No counterpart in the reference."""
 from __future__ import annotations
 
 import torch

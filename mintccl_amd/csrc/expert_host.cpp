@@ -7,6 +7,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -110,10 +111,14 @@ struct Args {
         if (n != wanted) refuse(PyExc_TypeError, "%zd arguments are wanted", wanted);
     }
     bool none(int i) const { return list[i] == Py_None; }
-    const Tensor& tensor(int i, const char* name) const {
+    // `history`: whether the results have a gradient by it
+    const Tensor& tensor(int i, const char* name, bool history = true) const {
         if (!THPVariable_Check(list[i])) refuse(PyExc_TypeError, "%s must be a device tensor", name);
         const Tensor& t = THPVariable_Unpack(list[i]);
         if (!t.is_cuda() || t.layout() != at::kStrided) refuse(PyExc_TypeError, "%s must be a device tensor", name);
+        // (a result without a history would end the gradient here without a word)
+        if (history && t.requires_grad() && c10::GradMode::is_enabled())
+            refuse(PyExc_RuntimeError, "%s requires a gradient, and these operators record none: detach it, or call under torch.no_grad()", name);
         return t;
     }
     int64_t integer(int i, const char* name, int64_t least, int64_t most) const {
@@ -216,7 +221,7 @@ PyObject* host_route(PyObject*, PyObject* const* list, Py_ssize_t n) {
         op.logits = address(x);
         op.row_stride = x.stride(0);
         if (!a.none(3)) {
-            const Tensor& bias = a.tensor(3, "bias");
+            const Tensor& bias = a.tensor(3, "bias", false);
             same_device(x, bias, "bias");
             typed(bias, at::kFloat, "bias", "float32");
             dims(bias, 1, "bias");

@@ -40,6 +40,7 @@ class ExpertLayer:
                  bias: torch.Tensor | None = None, **options) -> None:
         if router.shape[0] % comm.world_size:
             raise ValueError("the experts do not divide over the ranks")
+        router, up, down = router.detach(), up.detach(), down.detach()           # (their gradients are backward()'s)
         self.comm, self.router, self.k, self.bias, self.options = comm, router, k, bias, options
         self.own = router.shape[0] // comm.world_size
         self.grad_options = {o: options[o] for o in ("score", "renormalise", "scale") if o in options}

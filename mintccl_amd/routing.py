@@ -5,7 +5,9 @@ What stands in front of the experts of a layer that is spread over ranks: from
 a token's logits, the experts it goes to and their weights (``route``), and
 where each pair of a token and an expert stands when the pairs are sorted by
 expert (``assign``), which is what :mod:`~mintccl_amd.block8`'s products by
-expert and :mod:`~mintccl_amd.combine` go by.  No counterpart in the reference.
+expert and :mod:`~mintccl_amd.combine` go by.  Nothing is recorded for automatic
+differentiation: gradients are calls of their own, and a tensor that requires one is
+refused unless it is detached or gradients are off.  No counterpart in the reference.
 """
 from __future__ import annotations
 

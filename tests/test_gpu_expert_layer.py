@@ -156,3 +156,39 @@ def test_a_layer_of_no_tokens(dev):
     d_tokens, found = layer.backward(none, kept)
     assert [tuple(t.shape) for t in d_tokens] == [(0, 320)] * 4
     assert all((f[n] == 0).all() for f in found for n in ("up", "down", "router"))
+
+
+def test_tensors_that_require_a_gradient_are_refused(dev):
+    """Their results would have no history, and the gradient would end there without a word."""
+    from mintccl_amd.block8 import product, quantise, quantise_weight, weight_grad
+    from mintccl_amd.combine import combine_grad
+    from mintccl_amd.routing import assign, route, route_grad
+    x, w = randn(6, 128, seed=1, dev=dev), quantise_weight(randn(64, 128, seed=2, dev=dev))
+    weights, chosen = route(x, 2)
+    plan = assign(chosen, 128)
+    rows = randn(12, 128, seed=3, dev=dev)
+    leaf = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda f: route(f(x), 2), lambda f: route_grad(f(weights), x, chosen), lambda f: quantise(f(x)), lambda f: quantise_weight(f(x)),
+             lambda f: product(f(x), w), lambda f: weight_grad(x, f(x)), lambda f: combine(rows, plan, f(weights)),
+             lambda f: combine_grad(f(x), rows, plan, weights)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            call(leaf)
+        with torch.no_grad():
+            got = call(leaf)
+        want = call(lambda t: t)
+        detached = call(lambda t: leaf(t).detach())
+        for a, b, c in zip(*(v if isinstance(v, tuple) else (v,) for v in (got, want, detached))):
+            a, b, c = (v.view(torch.uint8) if v.element_size() == 1 else v for v in (a, b, c))
+            assert torch.equal(a, b) and torch.equal(a, c) and not a.requires_grad
+    # (the choice has no gradient, and so the bias has none)
+    assert torch.equal(route(x, 2, bias=leaf(x[0]))[1], route(x, 2, bias=x[0])[1])
+    # a layer of parameters has its own backward pass; tokens that want a gradient of torch's get none here
+    s = small_layer(2, dev)
+    layer = ExpertLayer(VirtualComm(world_size=2, device=dev), *(torch.nn.Parameter(s[n]) for n in ("router", "up", "down")), 4)
+    kept = []
+    out = layer.forward(s["tokens"], kept)
+    assert all(torch.equal(a, b) for a, b in zip(out, small(2, dev)[0].forward(s["tokens"])))
+    assert not any(f["up"].requires_grad for f in layer.backward(s["grads"], kept)[1])
+    with pytest.raises(RuntimeError, match="requires a gradient"):
+        layer.forward([leaf(t) for t in s["tokens"]])
