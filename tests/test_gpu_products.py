@@ -140,3 +140,166 @@ def test_an_assignment_of_more_tokens_than_rows_is_refused(dev):
     for call in (lambda: product(x, w, gather=True), lambda: weight_grad(d, d, gather=True)):
         with pytest.raises(ValueError, match="gather needs"):
             call()
+
+
+# ---- kernels ------------------------------------------------------------------------
+def ran(call):
+    """What `call` returns, and the names of the kernels that it launched, without blanks."""
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        got = call()
+        torch.cuda.synchronize()
+    return got, [e.name.replace(" ", "").replace("mint::(anonymousnamespace)::", "").removeprefix("void") for e in prof.events() if "_kernel<" in e.name]
+
+
+CODE = {"f16": 0, "bf16": 1, "f32": 2, "bytes": 3}
+#: Tiles by their template arguments: rows, columns, wavefronts down, blocks of the depth in LDS, sets of wavefronts.  For each the
+#: results that take it, and (rows, columns) and depths with which it is chosen: fewer blocks of the depth than are under way, as
+#: many, more, and a last one that is not whole.
+DENSE = [
+    ("64,64,4,2,1", ("bf16", "f16", "f32"), (100, 300), (1, 100, 128, 130, 256, 300, 1000)),
+    ("64,64,4,4,2", ("bf16",), (130, 900), (1100, 1152, 1280, 2500)),
+    ("64,64,4,2,2", ("f16", "f32"), (130, 900), (1100, 1152, 2400)),
+    ("64,64,4,2,2", ("bf16",), (1000, 2000), (1100, 1152)),
+    ("128,128,4,3,1", ("bf16",), (1500, 2000), (1, 100, 128, 130, 256, 384, 400, 512, 1000)),
+    ("128,128,4,2,1", ("bf16",), (38401, 128), (100, 128, 130, 256, 300, 640)),
+    ("128,256,2,3,1", ("bf16", "f16", "f32"), (2000, 4000), (1, 100, 128, 130, 256, 384, 400, 512, 1000)),
+    ("256,256,2,2,1", ("bf16",), (4000, 4000), (1, 100, 128, 130, 256, 300, 384, 1000)),
+]
+
+
+def for_each_type(cases):
+    return [(tile, dt, *rest) for tile, types, *rest in cases for dt in types]
+
+
+def kernel(tile, dt, along=False, joined=False):
+    return f"product_kernel<{CODE[dt]},{tile},{str(along).lower()},{str(along).lower()},{str(joined).lower()}>"
+
+
+@pytest.mark.parametrize("tile,dt,shape,depths", for_each_type(DENSE))
+def test_every_tile(dev, tile, dt, shape, depths):
+    rows, cols = shape
+    for depth in depths:
+        x, w = randn(rows, depth, seed=depth, dtype=DT[dt], dev=dev), quantise_weight(randn(cols, depth, seed=1, dev=dev))
+        got, names = ran(lambda: product(x, w, dtype=DT[dt]))
+        assert any(n.startswith(kernel(tile, dt)) for n in names), names
+        assert off_by(got, rounded8(x, 1), weight64(w)) <= 0, depth
+
+
+@pytest.mark.parametrize("dt,tile,depths", [("bf16", "64,64,4,4,2", (4096, 4100, 9001)), ("f16", "64,64,4,2,2", (2560, 2600, 9001)),
+                                            ("f32", "64,64,4,2,2", (2560, 2600, 9001))])
+def test_every_shared_tile(dev, dt, tile, depths):
+    for (rows, cols), depth in zip(((50, 300), (33, 64), (128, 4000)), depths):
+        x, w = randn(rows, depth, seed=depth, dtype=DT[dt], dev=dev), quantise_weight(randn(cols, depth, seed=1, dev=dev))
+        got, names = ran(lambda: product(quantise(x), w, dtype=DT[dt]))
+        assert any(n.startswith(kernel(tile, dt, joined=True)) for n in names), names
+        assert off_by(got, rounded8(x, 1), weight64(w)) <= 0, depth
+
+
+THIN = [((5, 300), "given", "1,8"), ((16, 50), "given", "1,8"), ((3, 12400), "given", "1,2"), ((5, 300), "bytes", "1,8"), ((3, 12400), "bytes", "1,2"),
+        ((20, 300), "bytes", "2,8"), ((32, 12400), "bytes", "2,2")]
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("shape,given,variant", THIN)
+def test_every_kernel_of_few_rows(dev, shape, given, variant, dt):
+    rows, cols = shape
+    for depth in (1, 100, 128, 130, 1000, 1024) + ((4100, 6500) if cols < 1000 and rows < 6 else ()):
+        x, w = randn(rows, depth, seed=depth, dtype=DT[dt], dev=dev), quantise_weight(randn(cols, depth, seed=1, dev=dev))
+        operand = quantise(x) if given == "bytes" else x
+        got, names = ran(lambda: product(operand, w, dtype=DT[dt]))
+        assert any(n.startswith(f"thin_kernel<{CODE[dt]},{CODE[dt if given == 'given' else 'bytes']},{variant}>") for n in names), names
+        assert off_by(got, rounded8(x, 1), weight64(w)) <= 0, depth
+
+
+BY_EXPERT = [
+    ("64,64,4,2,1", ("bf16", "f32"), [60, 0, 71], 900, (1, 128, 300, 1000)),
+    ("64,64,4,4,2", ("bf16",), [60, 70], 900, (1100, 1152)),
+    ("64,64,4,2,2", ("f16", "f32"), [60, 70], 900, (1100, 1152)),
+    ("64,64,4,2,2", ("bf16",), [900, 100], 1850, (1100,)),
+    ("128,128,4,3,1", ("bf16",), [1400, 100], 2000, (1, 100, 256, 384, 400, 1000)),
+    ("128,128,4,2,1", ("bf16",), [10000, 9000], 384, (100, 130, 384)),
+    ("128,256,2,3,1", ("bf16", "f16", "f32"), [1200, 800], 3700, (1, 100, 256, 384, 400, 1000)),
+    ("256,256,2,2,1", ("bf16",), [3000, 0, 1000], 3700, (1, 100, 256, 300, 1000)),
+]
+
+
+@pytest.mark.parametrize("tile,dt,counts,cols,depths", for_each_type(BY_EXPERT))
+def test_every_tile_by_expert(dev, tile, dt, counts, cols, depths):
+    tokens, e = (sum(counts) + 1) // 2, len(counts)
+    plan = planned(dev, counts, tokens, 2, seed=tokens)
+    at = plan.offsets.tolist()
+    for depth in depths:
+        x, w = randn(tokens, depth, seed=depth, dtype=DT[dt], dev=dev), quantise_weight(randn(e, cols, depth, seed=1, dev=dev))
+        got, names = ran(lambda: product(x, w, plan, gather=True, dtype=DT[dt]))
+        assert any(n.startswith(kernel(tile, dt)) for n in names), names
+        for i in range(e):
+            rows = slice(at[i], at[i + 1])
+            assert off_by(got[rows], rounded8(x[plan.tokens[rows].long()], 1), weight64(type(w)(w.q[i], w.scale[i]))) <= 0, (depth, i)
+        assert (got[at[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("counts,given,variant", [([3, 0, 20, 1], "given", "1,8"), ([3, 0, 70, 1], "bytes", "2,8"), ([1] * 40 + [30, 0], "given", "1,2"),
+                                                  ([20] * 40, "bytes", "2,2")])
+def test_every_kernel_of_few_rows_by_expert(dev, counts, given, variant, dt):
+    e, cols = len(counts), 70 if len(counts) < 10 else 500
+    tokens = sum(counts)
+    plan = planned(dev, counts, tokens, 1, seed=tokens)
+    at = plan.offsets.tolist()
+    for depth in (1, 128, 300, 1000):
+        x, w = randn(tokens, depth, seed=depth, dtype=DT[dt], dev=dev), quantise_weight(randn(e, cols, depth, seed=1, dev=dev))
+        operand = quantise(x) if given == "bytes" else x
+        got, names = ran(lambda: product(operand, w, plan, gather=True, dtype=DT[dt]))
+        assert any(n.startswith(f"thin_kernel<{CODE[dt]},{CODE[dt if given == 'given' else 'bytes']},{variant}>") for n in names), names
+        for i in range(e):
+            rows = slice(at[i], at[i + 1])
+            assert off_by(got[rows], rounded8(x[plan.tokens[rows].long()], 1), weight64(type(w)(w.q[i], w.scale[i]))) <= 0, (depth, i)
+
+
+GRADIENTS = [
+    ("64,64,4,2,1", ("bf16", "f16", "f32"), (100, 300), (1, 128, 130, 300, 1000)),
+    ("64,64,4,4,2", ("bf16",), (130, 900), (1100, 2500)),
+    ("64,64,4,2,2", ("f16", "f32"), (130, 900), (1100, 2500)),
+    ("64,64,4,2,2", ("bf16",), (1000, 2000), (1100,)),
+    ("128,128,4,3,1", ("bf16",), (1500, 2000), (1, 130, 300, 512, 1000)),
+    ("128,128,4,2,1", ("bf16",), (38401, 128), (100, 300, 512)),
+    ("128,256,2,3,1", ("bf16", "f16", "f32"), (2000, 4000), (1, 130, 300, 512, 1000)),
+    ("256,256,2,2,1", ("bf16",), (4000, 4000), (1, 130, 300, 512, 1000)),
+]
+
+
+@pytest.mark.parametrize("tile,dt,shape,rows", for_each_type(GRADIENTS))
+def test_every_tile_of_a_gradient(dev, tile, dt, shape, rows):
+    cols, depth = shape
+    for n in rows:
+        d, x = randn(n, cols, seed=n, dtype=DT[dt], dev=dev), randn(n, depth, seed=1, dtype=DT[dt], dev=dev)
+        got, names = ran(lambda: weight_grad(d, x, dtype=DT[dt]))
+        assert any(n_.startswith(kernel(tile, dt, along=True)) for n_ in names), names
+        assert off_by(got, rounded8(d, 0).t(), rounded8(x, 0).t()) <= 0, n
+
+
+GRADIENTS_BY_EXPERT = [
+    ("64,64,4,2,1", ("bf16", "f32"), [300, 0, 129], (100, 200)),
+    ("64,64,4,4,2", ("bf16",), [2000, 700], (100, 200)),
+    ("64,64,4,2,2", ("f16", "f32"), [2000, 700], (100, 200)),
+    ("128,128,4,3,1", ("bf16",), [300, 129], (700, 2000)),
+    ("128,128,4,2,1", ("bf16",), [300, 129], (19200, 128)),
+    ("128,256,2,3,1", ("bf16", "f16", "f32"), [300, 129], (1300, 2000)),
+    ("256,256,2,2,1", ("bf16",), [700, 0, 129], (2000, 2500)),
+]
+
+
+@pytest.mark.parametrize("tile,dt,counts,shape", for_each_type(GRADIENTS_BY_EXPERT))
+def test_every_tile_of_a_gradient_by_expert(dev, tile, dt, counts, shape):
+    (cols, depth), e, tokens = shape, len(counts), sum(counts) // 2 + 5
+    plan = planned(dev, counts, tokens, 2, seed=tokens)
+    at = plan.offsets.tolist()
+    d, x = randn(tokens * 2, cols, seed=2, dtype=DT[dt], dev=dev), randn(tokens, depth, seed=1, dtype=DT[dt], dev=dev)
+    got, names = ran(lambda: weight_grad(d, x, plan, gather=True, dtype=DT[dt]))
+    assert any(n.startswith(kernel(tile, dt, along=True)) for n in names), names
+    for i in range(e):
+        rows = slice(at[i], at[i + 1])
+        if at[i] == at[i + 1]:
+            assert (got[i] == 0).all()
+        else:
+            assert off_by(got[i], rounded8(d[rows], 0).t(), rounded8(x[plan.tokens[rows].long()], 0).t()) <= 0, i
