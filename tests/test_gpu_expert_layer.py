@@ -192,3 +192,24 @@ def test_tensors_that_require_a_gradient_are_refused(dev):
     assert not any(f["up"].requires_grad for f in layer.backward(s["grads"], kept)[1])
     with pytest.raises(RuntimeError, match="requires a gradient"):
         layer.forward([leaf(t) for t in s["tokens"]])
+
+
+def test_the_operators_one_behind_the_other(dev):
+    """As a program calls them that has all experts: from logits to the tokens' sums."""
+    from mintccl_amd.block8 import product, quantise_weight
+    from mintccl_amd.routing import assign, route
+    experts, width, inner, tokens = 16, 256, 192, 50
+    x, logits, b = randn(tokens, width, seed=1, dtype=torch.bfloat16, dev=dev), randn(tokens, experts, seed=2, dev=dev), randn(experts, seed=3, scale=0.1, dev=dev)
+    up, down = randn(experts, inner, width, seed=4, scale=width ** -0.5, dev=dev), randn(experts, width, inner, seed=5, scale=inner ** -0.5, dev=dev)
+    up8, down8 = quantise_weight(up), quantise_weight(down)
+    weights, chosen = route(logits, 6, score="sigmoid", bias=b, groups=8, kept=4, renormalise=True)
+    plan = assign(chosen, experts)
+    act = torch.nn.functional.silu
+    y = combine(product(act(product(x, up8, plan, gather=True)), down8, plan), plan, weights)
+    want = torch.zeros(tokens, width, dtype=torch.float64, device=dev)
+    for e in range(experts):
+        token, choice = (chosen == e).nonzero(as_tuple=True)
+        u, d = (weight64(Blocks(w.q[e], w.scale[e])) for w in (up8, down8))
+        h = act((rounded8(x[token], 1) @ u.t()).bfloat16())
+        want.index_add_(0, token, weights[token, choice].double()[:, None] * (rounded8(h, 1) @ d.t()).bfloat16().double())
+    assert float((y.double() - want).norm() / want.norm()) < 0.01            # (as the layer's steps above)
