@@ -137,7 +137,7 @@ struct ColumnsArgs {
     uint32_t x_rows, width;
 };
 // A thread block has 64 columns of 128 rows of an expert (fewer where it has no more: zeros follow), which turn in LDS.
-// Bound by memory: 65536 rows of 2048 numbers 87 us (4.6 TB/s), 4096 gathered from 16384 rows 162 (with a column's blocks side by side in
+// Bound by memory: 65536 rows of 2048 numbers 87 us (4.6 TB/s), 4096 gathered from 16384 rows 162, both in a launch 269 (with a column's blocks side by side in
 // the launch 102 and 184; bank conflicts of the turned stores cost nothing).
 // Two matrices can share a launch: the columns of the second one come behind the first one's.
 template <int DT>
@@ -205,7 +205,8 @@ struct SquaresArgs {
     int64_t w_matrix, w_stride, q_matrix, q_stride;
     uint32_t rows, depth, blocks;            // blocks of a row
 };
-// A thread block has a square of 128 x 128: 16 lanes to a row, eight rows to a thread.
+// A thread block has a square of 128 x 128: 16 lanes to a row, eight rows to a thread, read once and held until the square's largest is known.
+// Bound by memory: 8192 x 4096 numbers of 16 bits 18 us (5.6 TB/s), 32 matrices of 2048 x 4096 147 (5.5; of 32 bits 230, 5.8).
 template <int DT>
 __global__ void __launch_bounds__(256) squares8_kernel(SquaresArgs a) {
     using T = typename Elem<DT>::type;
@@ -347,7 +348,7 @@ constexpr uint32_t DEALT = 32;
 // little there is to multiply.  Their sums are added up in LDS at the end.
 // JOINED: the same over `parts` thread blocks, where there are fewer tiles than compute units.  A wavefront leaves its sums in memory and
 // counts itself; the last one of those that have the same place adds them all up, in the parts' order.  (No one waits for another.)
-// Bound by how steadily the matrix instructions are fed: at 8192 x 8192 x 4096 (260 us, 2.1 PFLOP/s) they are at work for 57 % of the cycles, no read
+// Bound by how steadily the matrix instructions are fed: at 8192 x 8192 x 4096 (253 - 266 us, 2.1 - 2.2 PFLOP/s) they are at work for 56 % of the cycles, no read
 // of LDS conflicts, and the rest is what a round of tiles takes to begin and to store (6 - 8 us of 65) and the scaling between them.
 // The weights are the matrix instruction's first operand, so a lane has consecutive columns of one row of the result (column_of).
 template <int OUT, int BM, int BN, int WM, int STAGES, int SPLIT, bool ROWS_W, bool ALONG, bool JOINED>
@@ -640,8 +641,9 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) product_kernel(Pr
 }
 
 // ---- products of few rows ------------------------------------------------------------
-// Bound by reading the weights: 16 MT rows need them once (1 x 4096 x 4096: 5.3 us, 3.2 TB/s, most of it the launch and one round trip to
-// memory; 8 rows over 64 experts of 1024 x 2048, of which 34 have any: 71 MB in 12.8 us, 5.6 TB/s).  A wavefront has 16 columns and every KWAYS-th block of the
+// Bound by reading the weights: 16 MT rows need them once (1 x 4096 x 4096: 5.4 us, most of it the launch and one round trip to
+// memory; 8 rows over 64 experts of 1024 x 2048, of which 34 have any: 71 MB in 16.1, 4.4 TB/s).  Those weights come from the last-level cache in part: with
+// as many others in between that all of them come from memory, 6.6 us and 19.5 (3.8 TB/s).  A wavefront has 16 columns and every KWAYS-th block of the
 // depth, straight from memory into registers: it asks for AHEAD blocks before it multiplies the first, which is what
 // keeps enough bytes on their way.  The KWAYS wavefronts' sums of a column are added up in LDS, in their order.
 // Activations that are not in 8 bits yet (X) are rounded by the thread block, CHUNK numbers of each row at a time, while the first weights
