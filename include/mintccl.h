@@ -618,8 +618,8 @@ int mint_weight_grad8(const mint_weight_grad_op* op, void* stream);
 
 /* out[t] = sum over j of weights[t, j] * rows[slots[t, j]] (weights 0: all 1), in
  * 32 bits; a slot outside the rows adds nothing.  The gradients: d_rows of every
- * row (those that are no token's, from *rows_used (int32) on, are cleared), and
- * d_weights unless it is 0. */
+ * row that a slot names (those that are no token's, from *rows_used (int32) on, are cleared, and
+ * a slot that names one of them counts as none), and d_weights unless it is 0. */
 int mint_combine(const void* rows, int64_t row_stride, uint64_t n_rows, const void* slots,
                  const void* weights, uint64_t tokens, uint32_t topk, uint32_t width, void* out,
                  int64_t out_stride, int dtype, void* stream);

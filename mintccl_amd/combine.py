@@ -20,6 +20,6 @@ def combine(rows: torch.Tensor, plan: Assignment, weights: torch.Tensor | None =
 
 def combine_grad(grad: torch.Tensor, rows: torch.Tensor, plan: Assignment,
                  weights: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """The gradients of the rows, in their type (zeros where a row is no token's),
-    and of the weights in float32 (``None`` without weights) from the result's."""
+    """The gradients of the rows, in their type (zeros behind the last expert's places,
+    where no row is a token's), and of the weights in float32 (``None`` without weights) from the result's."""
     return _lib.experts().combine_grad(grad, rows, plan.offsets, plan.slots, weights)

@@ -56,24 +56,25 @@ __global__ void __launch_bounds__(64 * kCombineWaves) combine_kernel(CombineArgs
 
 struct CombineGradArgs {
     const void *d_out, *rows;
-    const int32_t *slots, *ends;      // ends: the number of rows that some token has, or 0
+    const int32_t *slots, *ends;      // ends: the number of rows that some token has
     const float* weights;
     void* d_rows;
     float* d_weights;
     int64_t d_stride, row_stride, d_row_stride;
     uint32_t n_rows, tokens, topk, width;
 };
-// A thread block has a token; those behind the tokens' clear the rows that are no token's.
+// A thread block has a token; those behind the tokens' clear the rows that are no token's.  (A slot that is one of those counts as none:
+// no row is written by two.)
 constexpr uint32_t kClearing = 128;
 template <int DT>
 __global__ void __launch_bounds__(64 * kCombineWaves) combine_grad_kernel(CombineGradArgs a) {
     using T = typename Elem<DT>::type;
     constexpr int V = kCombineV;
     __shared__ float part[kCombineWaves][4];
-    const uint32_t step = 64 * kCombineWaves * V;
+    const uint32_t step = 64 * kCombineWaves * V, used = a.n_rows ? min((uint32_t)max(*a.ends, 0), a.n_rows) : 0u;
     if (blockIdx.x >= a.tokens) {
         const float none[V] = {};
-        for (uint64_t row = (uint32_t)max(*a.ends, 0) + (blockIdx.x - a.tokens); row < a.n_rows; row += kClearing)
+        for (uint64_t row = (uint64_t)used + (blockIdx.x - a.tokens); row < a.n_rows; row += kClearing)
             for (uint32_t at = threadIdx.x * V; at < a.width; at += step)
                 store_elements<DT, V>(static_cast<T*>(a.d_rows) + row * a.d_row_stride + at, (int64_t)a.width - at, none);
         return;
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(64 * kCombineWaves) combine_grad_kernel(Combin
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             slot[u] = j0 + u < a.topk ? slots[j0 + u] : -1;
-            if ((uint32_t)slot[u] >= a.n_rows) slot[u] = -1;
+            if ((uint32_t)slot[u] >= used) slot[u] = -1;
             w[u] = slot[u] < 0 ? 0.0f : a.weights ? a.weights[(uint64_t)token * a.topk + j0 + u] : 1.0f;
         }
         for (uint32_t at = threadIdx.x * V; at < a.width; at += step) {

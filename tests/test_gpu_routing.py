@@ -81,3 +81,16 @@ def test_more_tokens_than_a_launch_has_threads_for(dev):
     assert (chosen >= 0).all() and torch.isfinite(w.view(-1)).all()
     del x, w, chosen, got, d
     torch.cuda.empty_cache()
+
+
+def test_slots_behind_the_experts_places_have_no_gradient(dev):
+    """Places that the offsets do not count: their rows are cleared, by the same blocks every time, whatever the slots say."""
+    plan = assign(torch.arange(4096, dtype=torch.int32, device=dev).view(1024, 4) % 8, 8)
+    some = plan._replace(offsets=plan.offsets[:5])                # four of the eight experts
+    used = int(some.offsets[-1])
+    rows, d, w = randn(4096, 520, seed=1, dev=dev), randn(1024, 520, seed=2, dev=dev), randn(1024, 4, seed=3, dev=dev)
+    whole, there = combine_grad(d, rows, plan, w), plan.slots < used
+    for _ in range(5):
+        d_rows, d_weights = combine_grad(d, rows, some, w)
+        assert torch.equal(d_rows[:used], whole[0][:used]) and (d_rows[used:] == 0).all()
+        assert torch.equal(d_weights[there], whole[1][there]) and (d_weights[~there] == 0).all()
