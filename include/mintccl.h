@@ -628,6 +628,134 @@ int mint_combine_grad(const void* d_out, int64_t d_stride, const void* rows, int
                       uint64_t tokens, uint32_t topk, uint32_t width, void* d_rows, int64_t d_row_stride,
                       void* d_weights, int dtype, void* stream);
 
+/* ---- operators around an expert layer -------------------------------------------
+ * What stands before and after the layer in a block of a model: norms with the
+ * residual stream, dense products in 16 and 32 bits, the loss that balances the
+ * experts.  The same conventions.  No counterpart in the reference. */
+
+/* Activations of gates (none, sigmoid, tanh, silu ...) and of products; GELU with
+ * the normal distribution, GELU_TANH its approximation by a hyperbolic tangent. */
+typedef enum {
+    MINT_ACT_NONE = 0, MINT_ACT_RELU = 1, MINT_ACT_SILU = 2, MINT_ACT_SIGMOID = 3, MINT_ACT_TANH = 4,
+    MINT_ACT_GELU = 5, MINT_ACT_GELU_TANH = 6
+} mint_activation;
+
+/* (x - m) q w + b of a row x: RMS m = 0, q = 1 / sqrt(mean x^2 + eps); LAYER m =
+ * mean x, q = 1 / sqrt(mean (x - m)^2 + eps).  Statistics are in 32 bits. */
+typedef enum { MINT_NORM_NONE = 0, MINT_NORM_RMS = 1, MINT_NORM_LAYER = 2 } mint_norm_kind;
+typedef struct {
+    uint64_t weight, bias; /* (width) of `dtype`, side by side; 0: ones, zeros */
+    int32_t kind, dtype;
+    float eps;
+    uint32_t reserved;     /* 0 */
+} mint_norm;
+
+/* Of rows of a residual stream s and of a block's output y (rows, width):
+ *   u = after(y), or y         r = carry * s + scale * a(g) * u      -> new_stream
+ *   h = before(r as it is stored)                                    -> next, unless that is 0
+ * g: gate by channel (width), by row (gate_row apart) or of every number (rows
+ * gate_row apart), a its activation; 0: none.  With y = 0 only h = before(s) is
+ * made.  new_stream may be the stream itself.  The stream is of `dtype`
+ * (that of y and h) or MINT_F32. */
+typedef enum { MINT_GATE_CHANNEL = 1, MINT_GATE_ROW = 2, MINT_GATE_ALL = 3 } mint_gate_form;
+typedef struct {
+    uint64_t stream, y, gate, new_stream, next;
+    int64_t stream_stride, y_stride, gate_row, new_stride, next_stride;
+    uint64_t rows, width;
+    mint_norm after, before;
+    int32_t stream_dtype, dtype, gate_dtype;
+    int32_t gate_by;       /* mint_activation */
+    int32_t gate_form;     /* mint_gate_form, where there is a gate */
+    float scale, carry;
+    uint32_t reserved;     /* 0 */
+} mint_join_op;
+int mint_join(const mint_join_op* op, void* stream);
+
+/* The gradients, from those of r (d_stream, of the stream's type) and of h (d_next,
+ * of y's); either may be 0.  join: as for mint_join, with the NEW stream (r) in
+ * `stream` (it is read only where there is d_next); new_stream and next are not looked
+ * at.  Written where not 0: to_stream, to_y, to_gate and the norms' weights' and biases'
+ * gradients, each of its own type; none may overlap what is read.  Gradients of weights
+ * are sums over rows in 32 bits with a fixed order.  workspace:
+ * mint_join_grad_workspace() bytes, 4-byte aligned. */
+typedef struct {
+    mint_join_op join;
+    uint64_t d_stream, d_next, to_stream, to_y, to_gate;
+    uint64_t to_before_weight, to_before_bias, to_after_weight, to_after_bias;
+    int64_t d_stream_stride, d_next_stride, to_stream_stride, to_y_stride, to_gate_stride;
+    uint64_t workspace, workspace_bytes;
+} mint_join_grad_op;
+size_t mint_join_grad_workspace(const mint_join_grad_op* op);
+int mint_join_grad(const mint_join_grad_op* op, void* stream);
+
+/* Dense products of matrices of `dtype` with sums in 32 bits:
+ *   PRODUCT      out = residual + a(z), z = x w^T + bias; x (rows, depth), w (cols, depth)
+ *   INPUT_GRAD   out = x w; x (rows, depth), w (depth, cols)
+ *   WEIGHT_GRAD  out = x^T w; x (depth, rows), w (depth, cols)
+ * out (and residual) are of out_dtype: `dtype`, or MINT_F32; bias and z of `dtype`.
+ * PRODUCT alone takes bias, residual, activation and z (0: not wanted).  Rows
+ * may be any distance apart and start at any element; where they start at
+ * multiples of 16 bytes a row is read up to the 16 bytes that it ends in.
+ * residual may be out itself.  workspace: mint_dense_workspace() bytes, 16-byte aligned. */
+typedef enum { MINT_DENSE_PRODUCT = 0, MINT_DENSE_INPUT_GRAD = 1, MINT_DENSE_WEIGHT_GRAD = 2 } mint_dense_form;
+typedef struct {
+    int32_t form;          /* mint_dense_form */
+    int32_t dtype, out_dtype;
+    int32_t activation;    /* mint_activation */
+    uint64_t x, w, bias, residual, out, z;
+    uint64_t rows, cols, depth;
+    int64_t x_stride, w_stride, residual_stride, out_stride, z_stride;
+    uint64_t workspace, workspace_bytes;
+} mint_dense_op;
+size_t mint_dense_workspace(const mint_dense_op* op);
+int mint_dense(const mint_dense_op* op, void* stream);
+
+/* d_z = d * a'(z), of `dtype`, and d_bias = the sum over rows of it before it is
+ * rounded; either may be 0.  d (rows, cols) is of d_dtype: `dtype` or MINT_F32; z of `dtype`
+ * (not looked at without activation).  workspace, where d_bias is wanted:
+ * mint_activation_grad_workspace() bytes, 4-byte aligned. */
+typedef struct {
+    uint64_t d, z, d_z, d_bias;
+    uint64_t rows, cols;
+    int64_t d_stride, z_stride, d_z_stride;
+    int32_t d_dtype, dtype, activation;
+    uint32_t reserved;     /* 0 */
+    uint64_t workspace, workspace_bytes;
+} mint_activation_grad_op;
+size_t mint_activation_grad_workspace(uint64_t rows, uint64_t cols);
+int mint_activation_grad(const mint_activation_grad_op* op, void* stream);
+
+/* The loss that balances experts, with p a token's softmax, or its sigmoids divided by
+ * their sum, k = topk, and the tokens of sequence s (offsets[s] .. offsets[s + 1] - 1;
+ * without offsets all tokens are one sequence) that have an expert left, n_s of them:
+ *   counts (sequences, experts) int32: choices of the sequence that name the expert
+ *   shares (sequences, experts) f32:   the mean of p over the n_s tokens
+ *   there  (sequences) int32:          n_s
+ *   loss   f32: mean over sequences with n_s > 0 of sum_e experts * counts / (k n_s) * shares,
+ *               + z * mean over all tokens counted of lse(logits)^2
+ * A logit of -inf masks its expert.  The gradient: every row of d_logits is written
+ * (zeros for tokens that count nowhere), plus `add` (of the logits' type, may be 0, and
+ * may be d_logits itself).  Everything but counts, shares and there has to be what the loss was made
+ * with; counts and there are read on the device, so that a caller may put sums over ranks there.
+ * workspace: mint_balance_workspace() bytes, 8-byte aligned. */
+typedef struct {
+    uint64_t logits;       /* (tokens, experts) of `dtype`, rows row_stride apart */
+    uint64_t chosen;       /* int32 (tokens, topk); -1: none */
+    uint64_t offsets;      /* int32 (sequences + 1), or 0 */
+    int64_t row_stride;
+    uint64_t tokens, sequences;
+    uint32_t experts, topk;
+    int32_t dtype;
+    int32_t score;         /* mint_score */
+    float z;
+    uint32_t reserved;     /* 0 */
+} mint_balance_op;
+size_t mint_balance_workspace(const mint_balance_op* op);
+int mint_balance(const mint_balance_op* op, uint64_t loss, uint64_t counts, uint64_t shares, uint64_t there,
+                 void* workspace, size_t workspace_bytes, void* stream);
+int mint_balance_grad(const mint_balance_op* op, uint64_t d_loss, uint64_t counts, uint64_t there, uint64_t add,
+                      int64_t add_stride, uint64_t d_logits, int64_t d_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,8 +23,9 @@ CODEC_SRC = os.path.join(_CSRC, "codec.hip")
 FAMILY_SRC = os.path.join(_CSRC, "ring_family.hip")     # compiled once per element type
 HOST_SRC = os.path.join(_CSRC, "host.cpp")              # the extension module _host
 HOST_PATH = os.path.join(_PKG, "_host.so")
-# the expert layer's operators, and the extension module _expert_host that calls them
-EXPERT_SRCS = [os.path.join(_CSRC, f) for f in ("routing.hip", "block8.hip", "combine.hip")]
+# the operators of an expert layer and around it, and the extension module _expert_host that calls them
+EXPERT_SRCS = [os.path.join(_CSRC, f) for f in ("routing.hip", "block8.hip", "combine.hip", "balance.hip", "norms.hip", "dense.hip")]
+NORMS_SRC = os.path.join(_CSRC, "norms_family.hip")     # compiled once per pair of types
 EXPERT_HOST_SRC = os.path.join(_CSRC, "expert_host.cpp")
 EXPERT_HOST_PATH = os.path.join(_PKG, "_expert_host.so")
 BUILD_DIR = os.path.join(_PKG, "_build")
@@ -126,6 +127,55 @@ class WeightGradOp(ctypes.Structure):
         ("dtype", ctypes.c_int32)]
 
 
+class NormSpec(ctypes.Structure):
+    """``mint_norm``."""
+    _fields_ = [("weight", ctypes.c_uint64), ("bias", ctypes.c_uint64), ("kind", ctypes.c_int32),
+                ("dtype", ctypes.c_int32), ("eps", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
+class JoinOp(ctypes.Structure):
+    """``mint_join_op``."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("stream", "y", "gate", "new_stream", "next")] + [
+        (n, ctypes.c_int64) for n in ("stream_stride", "y_stride", "gate_row", "new_stride", "next_stride")] + [
+        ("rows", ctypes.c_uint64), ("width", ctypes.c_uint64), ("after", NormSpec), ("before", NormSpec)] + [
+        (n, ctypes.c_int32) for n in ("stream_dtype", "dtype", "gate_dtype", "gate_by", "gate_form")] + [
+        ("scale", ctypes.c_float), ("carry", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
+class JoinGradOp(ctypes.Structure):
+    """``mint_join_grad_op``."""
+    _fields_ = [("join", JoinOp)] + [
+        (n, ctypes.c_uint64) for n in ("d_stream", "d_next", "to_stream", "to_y", "to_gate", "to_before_weight",
+                                       "to_before_bias", "to_after_weight", "to_after_bias")] + [
+        (n, ctypes.c_int64) for n in ("d_stream_stride", "d_next_stride", "to_stream_stride", "to_y_stride",
+                                      "to_gate_stride")] + [
+        ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class DenseOp(ctypes.Structure):
+    """``mint_dense_op``."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("form", "dtype", "out_dtype", "activation")] + [
+        (n, ctypes.c_uint64) for n in ("x", "w", "bias", "residual", "out", "z", "rows", "cols", "depth")] + [
+        (n, ctypes.c_int64) for n in ("x_stride", "w_stride", "residual_stride", "out_stride", "z_stride")] + [
+        ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class ActivationGradOp(ctypes.Structure):
+    """``mint_activation_grad_op``."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("d", "z", "d_z", "d_bias", "rows", "cols")] + [
+        (n, ctypes.c_int64) for n in ("d_stride", "z_stride", "d_z_stride")] + [
+        (n, ctypes.c_int32) for n in ("d_dtype", "dtype", "activation")] + [("reserved", ctypes.c_uint32)] + [
+        ("workspace", ctypes.c_uint64), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class BalanceOp(ctypes.Structure):
+    """``mint_balance_op``."""
+    _fields_ = [(n, ctypes.c_uint64) for n in ("logits", "chosen", "offsets")] + [("row_stride", ctypes.c_int64)] + [
+        (n, ctypes.c_uint64) for n in ("tokens", "sequences")] + [
+        (n, ctypes.c_uint32) for n in ("experts", "topk")] + [("dtype", ctypes.c_int32), ("score", ctypes.c_int32),
+                                                              ("z", ctypes.c_float), ("reserved", ctypes.c_uint32)]
+
+
 # name -> (restype, argtypes); every symbol include/mintccl.h declares
 _vp, _sz, _u64, _u32, _i = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint64,
                             ctypes.c_uint32, ctypes.c_int)
@@ -172,6 +222,16 @@ SYMBOLS = {
     "mint_combine": (_i, [_vp, _i64, _u64, _vp, _vp, _u64, _u32, _u32, _vp, _i64, _i, _vp]),
     "mint_combine_grad": (_i, [_vp, _i64, _vp, _i64, _u64, _vp, _vp, _vp, _u64, _u32, _u32, _vp, _i64, _vp,
                                _i, _vp]),
+    "mint_join": (_i, [ctypes.POINTER(JoinOp), _vp]),
+    "mint_join_grad_workspace": (_sz, [ctypes.POINTER(JoinGradOp)]),
+    "mint_join_grad": (_i, [ctypes.POINTER(JoinGradOp), _vp]),
+    "mint_dense_workspace": (_sz, [ctypes.POINTER(DenseOp)]),
+    "mint_dense": (_i, [ctypes.POINTER(DenseOp), _vp]),
+    "mint_activation_grad_workspace": (_sz, [_u64, _u64]),
+    "mint_activation_grad": (_i, [ctypes.POINTER(ActivationGradOp), _vp]),
+    "mint_balance_workspace": (_sz, [ctypes.POINTER(BalanceOp)]),
+    "mint_balance": (_i, [ctypes.POINTER(BalanceOp), _u64, _u64, _u64, _u64, _vp, _sz, _vp]),
+    "mint_balance_grad": (_i, [ctypes.POINTER(BalanceOp), _u64, _u64, _u64, _u64, _i64, _u64, _i64, _vp]),
     "mint_torn_line_probe": (_i, [_vp, _sz, _i, _i, _i, _i, _i, _u32, _u32, _vp, _vp]),
 }
 
@@ -240,6 +300,9 @@ def build(verbose: bool = False, defines: tuple[str, ...] = (), so_path: str | N
              (CODEC_SRC, [*PRELOAD_FLAGS, *defines], os.path.join(build_dir, "codec.o"))]
     for src in EXPERT_SRCS:
         units.append((src, list(defines), os.path.join(build_dir, os.path.basename(src)[:-4] + ".o")))
+    for pair in range(5):
+        units.append((NORMS_SRC, [f"-DMINT_NORM_PAIR={pair}", *defines],
+                      os.path.join(build_dir, f"norms_family_{pair}.o")))
     for dt in range(4):
         units.append((FAMILY_SRC, [f"-DMINT_FAMILY_DT={dt}", *defines],
                       os.path.join(build_dir, f"ring_family_{dt}.o")))
@@ -370,10 +433,12 @@ def host():
 
 
 _experts = None
-#: the entry points that the module of the expert layer's operators calls, in the order of its bind()
+#: the entry points that the module of the operators of an expert layer and around it calls, in the order of its bind()
 EXPERT_SYMBOLS = ("mint_route", "mint_route_grad", "mint_assign_workspace", "mint_assign", "mint_rows8", "mint_squares8",
                   "mint_product8_workspace", "mint_product8", "mint_weight_grad8_workspace", "mint_weight_grad8",
-                  "mint_combine", "mint_combine_grad")
+                  "mint_combine", "mint_combine_grad", "mint_join", "mint_join_grad_workspace", "mint_join_grad",
+                  "mint_dense_workspace", "mint_dense", "mint_activation_grad_workspace", "mint_activation_grad",
+                  "mint_balance_workspace", "mint_balance", "mint_balance_grad")
 
 
 def experts():
@@ -386,8 +451,8 @@ def experts():
             raise RuntimeError(f"{EXPERT_HOST_PATH} is missing: run `python -c 'import __graft_entry__ as g; "
                                "g.build()'` in the repository root. There is no Python fallback.")
         from . import _expert_host as module
-        if (module.ROUTE_BYTES, module.PRODUCT_BYTES, module.WEIGHT_GRAD_BYTES) != tuple(
-                map(ctypes.sizeof, (RouteOp, ProductOp, WeightGradOp))):
+        if getattr(module, "DESCRIPTOR_BYTES", None) != tuple(map(ctypes.sizeof, (
+                RouteOp, ProductOp, WeightGradOp, JoinOp, JoinGradOp, DenseOp, ActivationGradOp, BalanceOp))):
             raise RuntimeError(f"{EXPERT_HOST_PATH} was built for other descriptors: rebuild it")
         module.bind(check, *[ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in EXPERT_SYMBOLS])
         _experts = module

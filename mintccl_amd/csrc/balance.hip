@@ -1,0 +1,464 @@
+// The loss that keeps experts in balance, with their counts, and its gradient.
+//
+//   p_te = softmax(x_t)_e, or sigmoid(x_te) / sum_i sigmoid(x_ti)          shares of a token's scores
+//   c_se: how many choices of sequence s name expert e     n_s: its tokens that have an expert left     S: sequences that have such a token
+//   f_se = E c_se / (k n_s)     P_se = sum over tokens of p_te / n_s
+//   loss = 1 / S sum_s sum_e f_se P_se + z / N sum_t lse(x_t)^2            N = sum n_s
+//
+// The choice has no gradient, so with a_se = f_se / (S n_s) and <p, a> over a token's experts:
+//
+//   softmax   d x_te = p_te (a_se - <p, a>)         sigmoid   d x_te = p_te (1 - sigmoid(x_te)) (a_se - <p, a>)
+//   z         d x_te += 2 z / N lse_t softmax(x_t)_e
+//
+// A logit of -inf masks its expert (p 0, gradient 0); a token with no expert left, or in no sequence, counts nowhere and has a gradient of
+// zeros.  Tokens go by in tiles that do not reach over sequences; a tile's sums are left in memory and added up in the tiles' order, so
+// the bits repeat.
+#include "operators.hpp"
+
+#include <algorithm>
+
+namespace mint {
+namespace {
+
+constexpr uint32_t kMostExperts = 1024;
+constexpr int kWaves = 4;                       // wavefronts of a thread block
+
+struct BalanceArgs {
+    const void* logits;
+    const int32_t *chosen, *offsets;            // offsets 0: one sequence of all tokens
+    int64_t row_stride;
+    uint32_t tokens, experts, topk, sequences, tile, tiles;      // tokens of a tile; tiles at most
+    uint32_t sigmoid;
+    float z;
+    // what a tile leaves: shares' sums (tiles, experts), counts (tiles, experts), {squares' sum, tokens} (tiles, 2)
+    float *shares, *square;
+    uint32_t *counts;
+    // ... a sequence: its term of the loss and its squares' sum by block of experts (sequences, blocks, 2)
+    float* terms;
+    uint32_t* arrived;
+    int32_t *out_counts, *out_tokens;
+    float *out_shares, *out_loss;
+};
+
+// Where tile `t` of `tile` tokens is.  Offsets are device data: whatever they say, tokens stay inside.
+struct Span {
+    uint32_t sequence, begin, end, first;       // tokens [begin, end); the first tile of its sequence
+    bool found;
+};
+__device__ __forceinline__ uint32_t token_bound(const int32_t* offsets, uint32_t i, uint32_t tokens) { return min((uint32_t)max(offsets[i], 0), tokens); }
+__device__ __forceinline__ uint32_t tiles_in(const int32_t* offsets, uint32_t s, uint32_t sequences, uint32_t tokens, uint32_t tile, uint32_t& begin, uint32_t& end) {
+    begin = end = 0;
+    if (s < sequences) {
+        begin = token_bound(offsets, s, tokens);
+        end = max(begin, token_bound(offsets, s + 1, tokens));
+    }
+    return (end - begin + tile - 1) / tile;
+}
+__device__ __forceinline__ Span find_span(const BalanceArgs& a, uint32_t t) {
+    if (!a.offsets) return {0, min(t * a.tile, a.tokens), min(t * a.tile + a.tile, a.tokens), 0, t * a.tile < a.tokens};
+    uint32_t base = 0;
+    for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
+        uint32_t begin, end;
+        const uint32_t n = tiles_in(a.offsets, s0 + lane_id(), a.sequences, a.tokens, a.tile, begin, end), sum = sum_below(n);
+        const uint64_t behind = __ballot(base + sum > t);
+        if (behind) {
+            const int at = __builtin_ctzll(behind);
+            const uint32_t first = base + (uint32_t)__builtin_amdgcn_readlane((int)(sum - n), at);
+            const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)begin, at), e = (uint32_t)__builtin_amdgcn_readlane((int)end, at);
+            const uint32_t from = b + (t - first) * a.tile;
+            return {s0 + at, from, min(from + a.tile, e), first, true};
+        }
+        base += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    }
+    return {a.sequences, 0, 0, base, false};
+}
+// the tiles of sequence s
+__device__ __forceinline__ void tiles_of_sequence(const BalanceArgs& a, uint32_t s, uint32_t& first, uint32_t& end) {
+    if (!a.offsets) {
+        first = 0;
+        end = a.tiles;
+        return;
+    }
+    uint32_t before = 0, b, e;
+    for (uint32_t i = lane_id(); i < s; i += 64) before += tiles_in(a.offsets, i, a.sequences, a.tokens, a.tile, b, e);
+    first = min((uint32_t)__builtin_amdgcn_readlane((int)sum_below(before), 63), a.tiles);
+    end = min(first + tiles_in(a.offsets, s, a.sequences, a.tokens, a.tile, b, e), a.tiles);
+}
+
+// Of a token's logits (V consecutive ones of a lane): the largest, the exponentials' sum, the scores and their sum.
+template <int V>
+struct Token {
+    float p[V];                                 // scores divided by their sum; zeros where the token counts nowhere
+    float lse, power;                           // log of the exponentials' sum; 1 / that sum at the largest logit, 0 where there is none
+    float top;
+    bool there;
+    __device__ __forceinline__ Token(const float (&x)[V], uint32_t first, uint32_t experts, bool use_sigmoid, bool wants_lse) {
+        float m = -INFINITY;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const bool in = first + i < experts;
+            m = in ? fmaxf(m, x[i]) : m;
+            nan |= in && x[i] != x[i];
+        }
+        top = wave_max(m);
+        // (a NaN is a number that is there, and makes the token's shares NaN)
+        there = top != -INFINITY || __ballot(nan) != 0;
+        top = there && top != -INFINITY ? top : 0.0f;
+        float sum = 0.0f, s_sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const bool in = first + i < experts && x[i] != -INFINITY;
+            const float e = in && (!use_sigmoid || wants_lse) ? expf(x[i] - top) : 0.0f;
+            sum += e;
+            p[i] = use_sigmoid ? in ? 1.0f / (1.0f + expf(-x[i])) : 0.0f : e;
+            s_sum += p[i];
+        }
+        sum = !use_sigmoid || wants_lse ? wave_sum(sum) : 1.0f;
+        s_sum = use_sigmoid ? wave_sum(s_sum) : sum;
+        lse = there && wants_lse ? top + logf(sum) : 0.0f;
+        power = there ? 1.0f / sum : 0.0f;
+        // (sigmoids that have all vanished have no shares)
+        const float r = there && s_sum != 0.0f ? 1.0f / s_sum : 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) p[i] *= r;
+    }
+};
+
+// A wavefront has every kWaves-th token of the tile, a lane V consecutive experts.
+template <int DT, int V>
+__global__ void __launch_bounds__(64 * kWaves) balance_tiles_kernel(BalanceArgs a) {
+    using T = typename Elem<DT>::type;
+    __shared__ float shares[kWaves][64 * V];
+    __shared__ uint32_t counts[kMostExperts], there[kWaves];
+    __shared__ float square[kWaves];
+    const Span span = find_span(a, blockIdx.x);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.arrived = 0u;
+    if (!span.found) return;
+    for (uint32_t e = threadIdx.x; e < a.experts; e += 64 * kWaves) counts[e] = 0u;
+    __syncthreads();
+    const uint32_t lane = lane_id(), wave = wave_in_block(), first = lane * V;
+    // choices: whole numbers, whose sum has no order
+    for (uint64_t i = (uint64_t)span.begin * a.topk + threadIdx.x; i < (uint64_t)span.end * a.topk; i += 64 * kWaves) {
+        const uint32_t e = (uint32_t)a.chosen[i];
+        if (e < a.experts) atomicAdd(counts + e, 1u);
+    }
+    float sum[V], squares = 0.0f;
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum[i] = 0.0f;
+    for (uint32_t t = span.begin + wave; t < span.end; t += kWaves) {
+        float x[V];
+        load_elements<DT, V>(static_cast<const T*>(a.logits) + (int64_t)t * a.row_stride + first, (int64_t)a.experts - first, x);
+        const Token<V> token(x, first, a.experts, a.sigmoid, a.z != 0.0f);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += token.p[i];
+        squares = fmaf(token.lse, token.lse, squares);
+        n += token.there;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) shares[wave][first + i] = sum[i];
+    if (lane == 0) {
+        square[wave] = squares;
+        there[wave] = n;
+    }
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < a.experts; e += 64 * kWaves) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) s += shares[w][e];
+        a.shares[(uint64_t)blockIdx.x * a.experts + e] = s;
+        a.counts[(uint64_t)blockIdx.x * a.experts + e] = counts[e];
+    }
+    if (threadIdx.x == 0) {
+        float s = 0.0f;
+        uint32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            s += square[w];
+            all += there[w];
+        }
+        a.square[blockIdx.x * 2] = s;
+        a.square[blockIdx.x * 2 + 1] = __uint_as_float(all);
+    }
+}
+
+// A thread block has 64 experts of a sequence, a wavefront every kJoinWaves-th tile's sums of them.  The last block that is done adds the
+// sequences' terms up, in their order.
+constexpr int kJoinWaves = 8;
+__global__ void __launch_bounds__(64 * kJoinWaves) balance_join_kernel(BalanceArgs a) {
+    __shared__ float shares[kJoinWaves][64], square[kJoinWaves];
+    __shared__ uint32_t counts[kJoinWaves][64], there[kJoinWaves];
+    __shared__ bool last;
+    const uint32_t blocks = (a.experts + 63) / 64, s = blockIdx.x / blocks, block = blockIdx.x % blocks;
+    const uint32_t e = block * 64 + lane_id(), from = min(e, a.experts - 1), wave = wave_in_block();
+    uint32_t first, end;
+    tiles_of_sequence(a, s, first, end);
+    float sum = 0.0f, squares = 0.0f;
+    uint32_t count = 0, n = 0;
+    for (uint32_t t0 = first + wave; t0 < end; t0 += kJoinWaves * 4) {
+        float v[4], q[4];
+        uint32_t c[4], k[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+            const uint64_t t = min(t0 + u * kJoinWaves, end - 1);
+            v[u] = a.shares[t * a.experts + from];
+            c[u] = a.counts[t * a.experts + from];
+            q[u] = a.square[t * 2];
+            k[u] = __float_as_uint(a.square[t * 2 + 1]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+            if (t0 + u * kJoinWaves < end) {
+                sum += v[u];
+                count += c[u];
+                squares += q[u];
+                n += k[u];
+            }
+    }
+    shares[wave][lane_id()] = sum;
+    counts[wave][lane_id()] = count;
+    if (lane_id() == 0) {
+        square[wave] = squares;
+        there[wave] = n;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        sum = squares = 0.0f;
+        count = n = 0;
+#pragma unroll
+        for (int w = 0; w < kJoinWaves; ++w) {
+            sum += shares[w][lane_id()];
+            count += counts[w][lane_id()];
+            squares += square[w];
+            n += there[w];
+        }
+        const float some = (float)max(n, 1u), share = sum / some;
+        const float often = (float)count * (float)a.experts / ((float)a.topk * some);
+        if (e < a.experts) {
+            a.out_counts[(uint64_t)s * a.experts + e] = (int32_t)count;
+            a.out_shares[(uint64_t)s * a.experts + e] = share;
+        }
+        const float term = wave_sum(e < a.experts ? often * share : 0.0f);
+        if (lane_id() == 0) {
+            if (block == 0) a.out_tokens[s] = (int32_t)n;
+            // (read by another block of this launch: past the caches that are not shared)
+            st64_agent(reinterpret_cast<uint64_t*>(a.terms) + blockIdx.x, (uint64_t)__float_as_uint(squares) << 32 | __float_as_uint(term));
+            if (block == 0) st64_agent(reinterpret_cast<uint64_t*>(a.terms) + gridDim.x + s, n);
+            wait_stores_visible();
+            last = __hip_atomic_fetch_add(a.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        }
+    }
+    __syncthreads();
+    if (!last || wave != 0) return;
+    compiler_fence();
+    const uint64_t* const terms = reinterpret_cast<const uint64_t*>(a.terms);
+    float total = 0.0f, all_squares = 0.0f;
+    uint32_t sequences = 0;
+    uint64_t tokens = 0;
+    // (lanes have sequences in turn, and then add each other's up: a fixed order too)
+    for (uint32_t i = lane_id(); i < a.sequences; i += 64) {
+        const uint64_t k = ld64_agent(terms + gridDim.x + i);
+        sequences += k != 0;
+        tokens += k;
+        float of_one = 0.0f;
+        for (uint32_t b = 0; b < blocks; ++b) of_one += __uint_as_float((uint32_t)ld64_agent(terms + i * blocks + b));
+        total += of_one;
+        all_squares += __uint_as_float((uint32_t)(ld64_agent(terms + i * blocks) >> 32));
+    }
+    total = wave_sum(total);
+    all_squares = wave_sum(all_squares);
+    const uint32_t some = (uint32_t)__builtin_amdgcn_readlane((int)sum_below(sequences), 63);
+    const uint32_t every = (uint32_t)__builtin_amdgcn_readlane((int)sum_below((uint32_t)tokens), 63);
+    if (lane_id() == 0) *a.out_loss = total / (float)max(some, 1u) + (a.z != 0.0f ? a.z * (all_squares / (float)max(every, 1u)) : 0.0f);
+}
+
+struct BalanceGradArgs {
+    BalanceArgs f;
+    const float* d_loss;
+    const int32_t *counts, *there;              // (sequences, experts), (sequences)
+    const void* add;                            // a gradient that is added, or 0
+    void* d_logits;
+    int64_t add_stride, d_stride;
+};
+template <int DT, int V>
+__global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradArgs a) {
+    using T = typename Elem<DT>::type;
+    const BalanceArgs& f = a.f;
+    const uint32_t lane = lane_id(), first = lane * V;
+    const int64_t left = (int64_t)f.experts - first;
+    Span span = find_span(f, blockIdx.x);
+    if (!span.found) {
+        // the tokens before the first sequence and behind the last one
+        const uint32_t begin = token_bound(f.offsets, 0, f.tokens), end = max(begin, token_bound(f.offsets, f.sequences, f.tokens));
+        const uint32_t nth = blockIdx.x - span.first, outside = begin + (f.tokens - end);
+        for (uint32_t i = nth * f.tile + wave_in_block(); i < min(outside, (nth + 1) * f.tile); i += kWaves) {
+            const uint32_t t = i < begin ? i : end + (i - begin);
+            float none[V] = {};
+            if (a.add) load_elements<DT, V>(static_cast<const T*>(a.add) + (int64_t)t * a.add_stride + first, left, none);
+            if (left > 0) store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, none);
+        }
+        return;
+    }
+    // sequences that have a token, and all tokens
+    uint32_t some = 0, every = 0;
+    for (uint32_t s = lane; s < f.sequences; s += 64) {
+        const uint32_t n = (uint32_t)max(a.there[s], 0);
+        some += n != 0;
+        every += n;
+    }
+    some = max((uint32_t)__builtin_amdgcn_readlane((int)sum_below(some), 63), 1u);
+    every = max((uint32_t)__builtin_amdgcn_readlane((int)sum_below(every), 63), 1u);
+    const float d = *a.d_loss, n = (float)max(a.there[span.sequence], 1);
+    const float by = d * (float)f.experts / ((float)f.topk * n) / ((float)some * n), by_z = f.z != 0.0f ? 2.0f * f.z * d / (float)every : 0.0f;
+    float often[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) often[i] = first + i < f.experts ? by * (float)a.counts[(uint64_t)span.sequence * f.experts + first + i] : 0.0f;
+    for (uint32_t t = span.begin + wave_in_block(); t < span.end; t += kWaves) {
+        float x[V], more[V];
+        load_elements<DT, V>(static_cast<const T*>(f.logits) + (int64_t)t * f.row_stride + first, left, x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) more[i] = 0.0f;
+        if (a.add) load_elements<DT, V>(static_cast<const T*>(a.add) + (int64_t)t * a.add_stride + first, left, more);
+        const Token<V> token(x, first, f.experts, f.sigmoid, f.z != 0.0f);
+        float mean = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) mean = fmaf(token.p[i], often[i], mean);
+        mean = wave_sum(mean);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const bool masked = x[i] == -INFINITY;
+            float slope = token.p[i];
+            if (f.sigmoid) slope *= masked ? 0.0f : 1.0f / (1.0f + expf(x[i]));
+            float dx = slope * (often[i] - mean);
+            if (f.z != 0.0f && !masked) dx = fmaf(by_z * token.lse, expf(x[i] - token.top) * token.power, dx);
+            more[i] += masked || !token.there ? 0.0f : dx;
+        }
+        if (left > 0) store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, more);
+    }
+}
+
+uint32_t values_per_lane(uint32_t experts) {
+    uint32_t v = 1;
+    while (v * 64 < experts) v *= 2;
+    return v;
+}
+template <int DT, int V>
+int go_tiles(const BalanceArgs& a, hipStream_t s) { return Launch<&balance_tiles_kernel<DT, V>>::go(a.tiles, 64 * kWaves, 0, s, a); }
+template <int DT, int V>
+int go_grad(const BalanceGradArgs& a, hipStream_t s) {
+    // (tokens of no sequence are dealt to the tiles that are left over)
+    return Launch<&balance_grad_kernel<DT, V>>::go(a.f.tiles + (a.f.offsets ? 1u : 0u), 64 * kWaves, 0, s, a);
+}
+#define MINT_BY_VALUES(GO, DT)                     \
+    switch (values_per_lane(op->experts)) {        \
+        case 1: return GO<DT, 1>(a, s);            \
+        case 2: return GO<DT, 2>(a, s);            \
+        case 4: return GO<DT, 4>(a, s);            \
+        case 8: return GO<DT, 8>(a, s);            \
+        default: return GO<DT, 16>(a, s);          \
+    }
+#define MINT_BY_TYPES(GO)                                  \
+    switch (op->dtype) {                                   \
+        case MINT_F16: MINT_BY_VALUES(GO, DT_F16)          \
+        case MINT_BF16: MINT_BY_VALUES(GO, DT_BF16)        \
+        default: MINT_BY_VALUES(GO, DT_F32)                \
+    }
+
+bool known(int dtype) { return dtype == MINT_F16 || dtype == MINT_BF16 || dtype == MINT_F32; }
+uint32_t sequences_of(const mint_balance_op& op) { return op.offsets ? (uint32_t)op.sequences : 1u; }
+// Tokens of a tile: so that there are about as many tiles as fill the device.
+uint32_t tile_of(uint64_t tokens) { return (uint32_t)std::min<uint64_t>(256, std::max<uint64_t>(16, ceil_div(tokens, 1024))); }
+// tiles at most: the last one of each sequence may have a single token, and in the gradient so may those of the tokens of none
+uint64_t tiles_of(const mint_balance_op& op) {
+    const uint64_t tile = tile_of(op.tokens);
+    return std::min<uint64_t>(op.tokens, ceil_div(op.tokens, tile) + (op.offsets ? op.sequences : 0));
+}
+int balance_checks(const mint_balance_op* op) {
+    if (!op || !known(op->dtype) || (op->score != MINT_SCORE_SOFTMAX && op->score != MINT_SCORE_SIGMOID)) return MINT_ERR_ARG;
+    if (op->experts < 1 || op->experts > kMostExperts || op->topk < 1 || op->topk > kMostExperts) return MINT_ERR_ARG;
+    if (op->tokens > 0x7FFFFFFFull / op->topk || (op->offsets && op->sequences > (1u << 20))) return MINT_ERR_TOO_LARGE;
+    if (op->offsets && op->sequences == 0) return MINT_ERR_ARG;
+    if (op->tokens && (!op->logits || !op->chosen)) return MINT_ERR_ARG;
+    return MINT_OK;
+}
+BalanceArgs balance_args(const mint_balance_op& op) {
+    BalanceArgs a = {};
+    a.logits = reinterpret_cast<const void*>(op.logits);
+    a.chosen = reinterpret_cast<const int32_t*>(op.chosen);
+    a.offsets = reinterpret_cast<const int32_t*>(op.offsets);
+    a.row_stride = op.row_stride;
+    a.tokens = (uint32_t)op.tokens;
+    a.experts = op.experts;
+    a.topk = op.topk;
+    a.sequences = sequences_of(op);
+    a.tile = tile_of(op.tokens);
+    a.tiles = (uint32_t)tiles_of(op);
+    a.sigmoid = op.score == MINT_SCORE_SIGMOID;
+    a.z = op.z;
+    return a;
+}
+// shares, counts, squares of the tiles; terms and tokens of the sequences; the count of blocks that are done
+struct BalanceRoom {
+    uint64_t terms, shares, counts, square, arrived, bytes;
+    explicit BalanceRoom(const mint_balance_op& op) {
+        const uint64_t tiles = tiles_of(op), s = sequences_of(op), blocks = ceil_div(op.experts, 64);
+        terms = 0;
+        shares = terms + s * (blocks + 1) * 8;
+        counts = shares + tiles * op.experts * 4;
+        square = counts + tiles * op.experts * 4;
+        arrived = square + tiles * 8;
+        bytes = arrived + 4;
+    }
+};
+
+}  // namespace
+}  // namespace mint
+
+using namespace mint;
+
+extern "C" size_t mint_balance_workspace(const mint_balance_op* op) { return balance_checks(op) == MINT_OK ? BalanceRoom(*op).bytes : 0; }
+
+extern "C" int mint_balance(const mint_balance_op* op, uint64_t loss, uint64_t counts, uint64_t shares, uint64_t there, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+    if (const int err = balance_checks(op)) return err;
+    if (!loss || !counts || !shares || !there) return MINT_ERR_ARG;
+    const BalanceRoom room(*op);
+    if (!workspace || workspace_bytes < room.bytes) return MINT_ERR_STAGING;
+    if (!aligned_to(workspace, 8)) return MINT_ERR_ALIGN;
+    BalanceArgs a = balance_args(*op);
+    auto* const at = static_cast<uint8_t*>(workspace);
+    a.terms = reinterpret_cast<float*>(at + room.terms);
+    a.shares = reinterpret_cast<float*>(at + room.shares);
+    a.counts = reinterpret_cast<uint32_t*>(at + room.counts);
+    a.square = reinterpret_cast<float*>(at + room.square);
+    a.arrived = reinterpret_cast<uint32_t*>(at + room.arrived);
+    a.out_counts = reinterpret_cast<int32_t*>(counts);
+    a.out_tokens = reinterpret_cast<int32_t*>(there);
+    a.out_shares = reinterpret_cast<float*>(shares);
+    a.out_loss = reinterpret_cast<float*>(loss);
+    const auto s = static_cast<hipStream_t>(stream);
+    const uint64_t blocks = a.sequences * ceil_div(a.experts, 64);
+    if (blocks * 64 * kJoinWaves > 0xFFFFFFFFull) return MINT_ERR_TOO_LARGE;
+    // (of no tokens a block that finds none still clears the count)
+    const uint32_t real = a.tiles;
+    const auto tiles = [&]() -> int {
+        a.tiles = std::max(real, 1u);
+        MINT_BY_TYPES(go_tiles)
+    };
+    const int err = tiles();
+    if (err != MINT_OK) return err;
+    a.tiles = real;
+    return Launch<&balance_join_kernel>::go((uint32_t)blocks, 64 * kJoinWaves, 0, s, a);
+}
+
+extern "C" int mint_balance_grad(const mint_balance_op* op, uint64_t d_loss, uint64_t counts, uint64_t there, uint64_t add, int64_t add_stride,
+                                 uint64_t d_logits, int64_t d_stride, void* stream) {
+    if (const int err = balance_checks(op)) return err;
+    if (op->tokens == 0) return MINT_OK;
+    if (!d_loss || !counts || !there || !d_logits) return MINT_ERR_ARG;
+    const BalanceGradArgs a = {balance_args(*op), reinterpret_cast<const float*>(d_loss), reinterpret_cast<const int32_t*>(counts),
+                               reinterpret_cast<const int32_t*>(there), reinterpret_cast<const void*>(add), reinterpret_cast<void*>(d_logits), add_stride, d_stride};
+    const auto s = static_cast<hipStream_t>(stream);
+    MINT_BY_TYPES(go_grad)
+}

@@ -1,5 +1,5 @@
-// mintccl_amd._expert_host: the host side of the expert layer's operators (routing.py, block8.py,
-// combine.py), native: a call for one token takes the GPU a few us, and so must the checks of
+// mintccl_amd._expert_host: the host side of the operators of an expert layer (routing.py, block8.py,
+// combine.py) and around it (norms.py, dense.py), native: a call for one token takes the GPU a few us, and so must the checks of
 // its arguments, its outputs' allocation and the launch.  What a call allocates for itself
 // comes from torch's allocator on the calling thread's current stream, on which it launches too.
 #define PY_SSIZE_T_CLEAN
@@ -32,6 +32,16 @@ struct Native {
     decltype(&mint_weight_grad8) weight_grad8;
     decltype(&mint_combine) combine;
     decltype(&mint_combine_grad) combine_grad;
+    decltype(&mint_join) join;
+    decltype(&mint_join_grad_workspace) join_grad_workspace;
+    decltype(&mint_join_grad) join_grad;
+    decltype(&mint_dense_workspace) dense_workspace;
+    decltype(&mint_dense) dense;
+    decltype(&mint_activation_grad_workspace) activation_grad_workspace;
+    decltype(&mint_activation_grad) activation_grad;
+    decltype(&mint_balance_workspace) balance_workspace;
+    decltype(&mint_balance) balance;
+    decltype(&mint_balance_grad) balance_grad;
     PyObject* check;             // _lib.check(code, where): raises MintError
 } native = {};
 
@@ -606,6 +616,441 @@ PyObject* host_combine_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
     });
 }
 
+// ---- norms and the residual stream ------------------------------------------------
+// four arguments from `i` on: kind, weight or None, bias or None, eps
+void norm_of(const Args& a, int i, const Tensor& like, int64_t width, mint_norm& n, const char* name) {
+    n.kind = (int32_t)a.integer(i, "kind", MINT_NORM_NONE, MINT_NORM_LAYER);
+    if (n.kind == MINT_NORM_NONE) return;
+    n.eps = a.number(i + 3);
+    n.dtype = MINT_F32;
+    for (int k = 1; k <= 2; ++k) {
+        if (a.none(i + k)) continue;
+        const Tensor& t = a.tensor(i + k, name);
+        same_device(like, t, name);
+        dims(t, 1, name);
+        dense(t, name);
+        if (t.size(0) != width) refuse(PyExc_ValueError, "%s must have a number for each of %lld channels", name, (long long)width);
+        const int code = code_of(t.scalar_type(), name);
+        if (k == 2 && n.weight && code != n.dtype) refuse(PyExc_TypeError, "%s: weight and bias must be of one type", name);
+        n.dtype = code;
+        (k == 1 ? n.weight : n.bias) = address(t);
+    }
+}
+// What join and its gradient have in common: stream, y or None, gate or None, gate_by, scale, carry, then after's and before's norm (arguments i .. i + 13)
+void join_of(const Args& a, int i, mint_join_op& op) {
+    const Tensor& s = a.tensor(i, "stream");
+    rows_of(s, "stream");
+    op.stream_dtype = code_of(s.scalar_type(), "stream");
+    op.dtype = op.stream_dtype;
+    op.rows = (uint64_t)s.size(0);
+    op.width = (uint64_t)s.size(1);
+    if (s.size(0) > 0x7FFFFFFF / 4 || s.size(1) > 0x7FFFFFFF - 8192) refuse(PyExc_ValueError, "stream is too large");
+    op.stream = address(s);
+    op.stream_stride = s.stride(0);
+    op.gate_by = (int32_t)a.integer(i + 3, "gate_by", MINT_ACT_NONE, MINT_ACT_GELU_TANH);
+    op.scale = a.number(i + 4);
+    op.carry = a.number(i + 5);
+    norm_of(a, i + 6, s, s.size(1), op.after, "after");
+    norm_of(a, i + 10, s, s.size(1), op.before, "before");
+    if (!a.none(i + 1)) {
+        const Tensor& y = a.tensor(i + 1, "y");
+        same_device(s, y, "y");
+        rows_of(y, "y");
+        op.dtype = code_of(y.scalar_type(), "y");
+        if (op.stream_dtype != op.dtype && op.stream_dtype != MINT_F32) refuse(PyExc_TypeError, "stream must be of y's type or float32");
+        if (y.sizes() != s.sizes()) refuse(PyExc_ValueError, "y must be like stream");
+        op.y = address(y);
+        op.y_stride = y.stride(0);
+    }
+    if (!a.none(i + 2)) {
+        const Tensor& g = a.tensor(i + 2, "gate");
+        same_device(s, g, "gate");
+        op.gate_dtype = code_of(g.scalar_type(), "gate");
+        op.gate = address(g);
+        if (g.dim() == 1 && g.size(0) == s.size(1)) {
+            dense(g, "gate");
+            op.gate_form = MINT_GATE_CHANNEL;
+        } else if (g.sizes() == s.sizes()) {
+            rows_of(g, "gate");
+            op.gate_form = MINT_GATE_ALL;
+            op.gate_row = g.stride(0);
+        } else if (g.dim() == 2 && g.size(0) == s.size(0) && g.size(1) == 1) {
+            op.gate_form = MINT_GATE_ROW;
+            op.gate_row = g.stride(0);
+        } else {
+            refuse(PyExc_ValueError, "gate must be (width,), (rows, 1) or (rows, width)");
+        }
+    }
+}
+constexpr int kJoinArguments = 14;
+
+// join(stream, y, gate, gate_by, scale, carry, after x 4, before x 4, dtype or None, out or None): (stream or None, next or None)
+PyObject* host_join(PyObject*, PyObject* const* list, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Args a(list, n, kJoinArguments + 2);
+        mint_join_op op = {};
+        join_of(a, 0, op);
+        const Tensor& s = a.tensor(0, "stream");
+        if (!a.none(kJoinArguments)) {
+            const int64_t code = a.integer(kJoinArguments, "dtype", 0, 2);
+            if (op.y ? code != op.dtype : code != op.stream_dtype && op.stream_dtype != MINT_F32)
+                refuse(PyExc_TypeError, "dtype must be that of y, or of x, or anything if that is float32");
+            op.dtype = (int32_t)code;
+        }
+        const bool block = !a.none(1), next = op.before.kind != MINT_NORM_NONE, given = !a.none(kJoinArguments + 1);
+        if (!block && !next) refuse(PyExc_ValueError, "there is neither a block's output nor a norm");
+        if (given) {
+            const Tensor& out = a.tensor(kJoinArguments + 1, "out");
+            same_device(s, out, "out");
+            result(out, s.size(0), s.size(1), "out");
+            if (code_of(out.scalar_type(), "out") != (block ? op.stream_dtype : op.dtype)) refuse(PyExc_TypeError, "out is of another type than the result");
+        }
+        OnDevice on(s.get_device());
+        Tensor stream, h;
+        if (block) {
+            stream = given ? a.tensor(kJoinArguments + 1, "out") : empty(s, s.sizes(), s.scalar_type());
+            op.new_stream = address(stream);
+            op.new_stride = s.size(0) > 1 ? stream.stride(0) : s.size(1);
+        }
+        if (next) {
+            h = given && !block ? a.tensor(kJoinArguments + 1, "out") : empty(s, s.sizes(), type_of(op.dtype));
+            op.next = address(h);
+            op.next_stride = s.size(0) > 1 ? h.stride(0) : s.size(1);
+        }
+        launch("mint_join", [&] { return native.join(&op, on.stream); });
+        return pack({block ? given ? Py_NewRef(list[kJoinArguments + 1]) : wrap(stream) : Py_NewRef(Py_None),
+                     next ? given && !block ? Py_NewRef(list[kJoinArguments + 1]) : wrap(h) : Py_NewRef(Py_None)});
+    });
+}
+
+// join_grad(d_stream or None, d_next or None, stream, ... as above): (d_stream, d_y, d_gate, d_after_weight, d_after_bias, d_before_weight,
+// d_before_bias), None in the place of those that there are none of
+PyObject* host_join_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Args a(list, n, kJoinArguments + 2);
+        mint_join_grad_op op = {};
+        join_of(a, 2, op.join);
+        const Tensor& s = a.tensor(2, "stream");
+        const bool block = !a.none(3);
+        if (a.none(0) && a.none(1)) refuse(PyExc_ValueError, "there is no gradient to go on with");
+        if (!a.none(1)) {
+            const Tensor& d = a.tensor(1, "the norm's grad");
+            same_device(s, d, "the norm's grad");
+            rows_of(d, "the norm's grad");
+            if (d.sizes() != s.sizes()) refuse(PyExc_ValueError, "the norm's grad must be like its result");
+            const int code = code_of(d.scalar_type(), "the norm's grad");
+            if (block ? code != op.join.dtype : code != op.join.stream_dtype && op.join.stream_dtype != MINT_F32)
+                refuse(PyExc_TypeError, "the norm's grad must be of its result's type");
+            op.join.dtype = code;
+            if (op.join.before.kind == MINT_NORM_NONE) refuse(PyExc_ValueError, "there is no norm that this is the gradient of");
+            op.d_next = address(d);
+            op.d_next_stride = d.stride(0);
+        }
+        if (!a.none(0)) {
+            const Tensor& d = a.tensor(0, "the stream's grad");
+            same_device(s, d, "the stream's grad");
+            rows_of(d, "the stream's grad");
+            if (d.sizes() != s.sizes()) refuse(PyExc_ValueError, "the stream's grad must be like the stream");
+            if (d.scalar_type() != s.scalar_type()) refuse(PyExc_TypeError, "the stream's grad must be of the stream's type");
+            op.d_stream = address(d);
+            op.d_stream_stride = d.stride(0);
+        }
+        OnDevice on(s.get_device());
+        const auto make = [&](int i, uint64_t& at) {
+            if (a.none(i)) return Tensor();
+            const Tensor& like = a.tensor(i, "a weight");
+            Tensor t = empty(like, like.sizes(), like.scalar_type());
+            at = address(t);
+            return t;
+        };
+        const Tensor to_stream = empty(s, s.sizes(), s.scalar_type());
+        op.to_stream = address(to_stream);
+        op.to_stream_stride = s.size(1);
+        Tensor to_y, to_gate, aw, ab, bw, bb;
+        if (block) {
+            to_y = empty(s, s.sizes(), type_of(op.join.dtype));
+            op.to_y = address(to_y);
+            op.to_y_stride = s.size(1);
+            to_gate = make(4, op.to_gate);
+            op.to_gate_stride = op.join.gate_form == MINT_GATE_ALL ? s.size(1) : 1;
+            if (op.join.after.kind) {
+                aw = make(9, op.to_after_weight);
+                ab = make(10, op.to_after_bias);
+            }
+        }
+        if (op.join.before.kind) {
+            bw = make(13, op.to_before_weight);
+            bb = make(14, op.to_before_bias);
+        }
+        Tensor room;
+        if ((op.workspace_bytes = native.join_grad_workspace(&op))) {
+            room = empty(s, {(int64_t)op.workspace_bytes}, at::kByte);
+            op.workspace = address(room);
+        }
+        launch("mint_join_grad", [&] { return native.join_grad(&op, on.stream); });
+        const auto give = [](const Tensor& t) { return t.defined() ? wrap(t) : Py_NewRef(Py_None); };
+        return pack({wrap(to_stream), give(to_y), give(to_gate), give(aw), give(ab), give(bw), give(bb)});
+    });
+}
+
+// ---- dense products ------------------------------------------------------------------
+void dense_launch(mint_dense_op& op, const Tensor& like, OnDevice& on) {
+    Tensor room;
+    if ((op.workspace_bytes = native.dense_workspace(&op))) {
+        room = empty(like, {(int64_t)op.workspace_bytes}, at::kByte);
+        op.workspace = address(room);
+    }
+    launch("mint_dense", [&] { return native.dense(&op, on.stream); });
+}
+// both operands of a dense product
+void operands(const Tensor& x, const Tensor& w, const char* x_name, const char* w_name, mint_dense_op& op) {
+    rows_of(x, x_name);
+    rows_of(w, w_name);
+    same_device(x, w, w_name);
+    op.dtype = code_of(x.scalar_type(), x_name);
+    if (w.scalar_type() != x.scalar_type()) refuse(PyExc_TypeError, "%s must be of the type of %s", w_name, x_name);
+    op.x = address(x);
+    op.w = address(w);
+    op.x_stride = x.stride(0);
+    op.w_stride = w.stride(0);
+}
+// the result's type, where one is named or `out` is given, and the result
+Tensor dense_out(const Args& a, int dtype_at, int out_at, const Tensor& x, int64_t rows, int64_t cols, mint_dense_op& op) {
+    int64_t code = a.none(dtype_at) ? op.dtype : a.integer(dtype_at, "dtype", 0, 2);
+    const bool given = out_at >= 0 && !a.none(out_at);
+    if (given) {
+        const Tensor& out = a.tensor(out_at, "out");
+        same_device(x, out, "out");
+        result(out, rows, cols, "out");
+        const int of_out = code_of(out.scalar_type(), "out");
+        if (!a.none(dtype_at) && code != of_out) refuse(PyExc_TypeError, "out is of another type than dtype");
+        code = of_out;
+    }
+    if (code != op.dtype && code != MINT_F32) refuse(PyExc_TypeError, "the result must be of the operands' type or float32");
+    op.out_dtype = (int32_t)code;
+    const Tensor out = given ? a.tensor(out_at, "out") : empty(x, {rows, cols}, type_of(code));
+    op.out = address(out);
+    op.out_stride = rows > 1 ? out.stride(0) : cols;
+    op.rows = (uint64_t)rows;
+    op.cols = (uint64_t)cols;
+    return out;
+}
+
+// dense_product(x, weight, bias or None, activation, residual or None, keep, dtype or None, out or None): out, or (out, z)
+PyObject* host_dense_product(PyObject*, PyObject* const* list, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Args a(list, n, 8);
+        const Tensor &x = a.tensor(0, "x"), &w = a.tensor(1, "weight");
+        mint_dense_op op = {};
+        op.form = MINT_DENSE_PRODUCT;
+        operands(x, w, "x", "weight", op);
+        if (x.size(1) != w.size(1)) refuse(PyExc_ValueError, "x has rows of %lld, the weight of %lld", (long long)x.size(1), (long long)w.size(1));
+        const int64_t rows = x.size(0), cols = w.size(0);
+        op.depth = (uint64_t)x.size(1);
+        if (!a.none(2)) {
+            const Tensor& b = a.tensor(2, "bias");
+            same_device(x, b, "bias");
+            dims(b, 1, "bias");
+            dense(b, "bias");
+            if (b.scalar_type() != x.scalar_type()) refuse(PyExc_TypeError, "bias must be of x's type");
+            if (b.size(0) != cols) refuse(PyExc_ValueError, "bias must have a number for each of %lld columns", (long long)cols);
+            op.bias = address(b);
+        }
+        op.activation = (int32_t)a.integer(3, "activation", MINT_ACT_NONE, MINT_ACT_GELU_TANH);
+        const bool keep = a.truth(5), given = !a.none(7);
+        OnDevice on(x.get_device());
+        const Tensor out = dense_out(a, 6, 7, x, rows, cols, op);
+        if (!a.none(4)) {
+            const Tensor& r = a.tensor(4, "residual");
+            same_device(x, r, "residual");
+            rows_of(r, "residual");
+            if (r.size(0) != rows || r.size(1) != cols) refuse(PyExc_ValueError, "residual must be (%lld, %lld)", (long long)rows, (long long)cols);
+            if (code_of(r.scalar_type(), "residual") != op.out_dtype) refuse(PyExc_TypeError, "residual must be of the result's type");
+            op.residual = address(r);
+            op.residual_stride = r.stride(0);
+        }
+        Tensor z;
+        if (keep) {
+            z = empty(x, {rows, cols}, x.scalar_type());
+            op.z = address(z);
+            op.z_stride = cols;
+        }
+        dense_launch(op, x, on);
+        PyObject* const result = given ? Py_NewRef(list[7]) : wrap(out);
+        return keep ? pack({result, wrap(z)}) : result;
+    });
+}
+// dense_input_grad(grad, weight, dtype or None)
+PyObject* host_dense_input_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Args a(list, n, 3);
+        const Tensor &d = a.tensor(0, "grad"), &w = a.tensor(1, "weight");
+        mint_dense_op op = {};
+        op.form = MINT_DENSE_INPUT_GRAD;
+        operands(d, w, "grad", "weight", op);
+        if (d.size(1) != w.size(0)) refuse(PyExc_ValueError, "grad has rows of %lld, the weight %lld rows", (long long)d.size(1), (long long)w.size(0));
+        op.depth = (uint64_t)w.size(0);
+        OnDevice on(d.get_device());
+        const Tensor out = dense_out(a, 2, -1, d, d.size(0), w.size(1), op);
+        dense_launch(op, d, on);
+        return wrap(out);
+    });
+}
+// dense_weight_grad(grad, x, dtype or None)
+PyObject* host_dense_weight_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Args a(list, n, 3);
+        const Tensor &d = a.tensor(0, "grad"), &x = a.tensor(1, "x");
+        mint_dense_op op = {};
+        op.form = MINT_DENSE_WEIGHT_GRAD;
+        operands(d, x, "grad", "x", op);
+        if (d.size(0) != x.size(0)) refuse(PyExc_ValueError, "x and grad have different numbers of rows");
+        op.depth = (uint64_t)x.size(0);
+        OnDevice on(d.get_device());
+        const Tensor out = dense_out(a, 2, -1, d, d.size(1), x.size(1), op);
+        dense_launch(op, d, on);
+        return wrap(out);
+    });
+}
+// activation_grad(grad, z or None, activation, bias, dtype): (d_z, d_bias or None)
+PyObject* host_activation_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Args a(list, n, 5);
+        const Tensor& d = a.tensor(0, "grad");
+        rows_of(d, "grad");
+        mint_activation_grad_op op = {};
+        op.d_dtype = code_of(d.scalar_type(), "grad");
+        op.activation = (int32_t)a.integer(2, "activation", MINT_ACT_NONE, MINT_ACT_GELU_TANH);
+        const bool bias = a.truth(3);
+        if (!a.none(1)) {
+            const Tensor& z = a.tensor(1, "z");
+            same_device(d, z, "z");
+            rows_of(z, "z");
+            if (z.sizes() != d.sizes()) refuse(PyExc_ValueError, "z must be like grad");
+            op.dtype = code_of(z.scalar_type(), "z");
+            if (!a.none(4) && a.integer(4, "dtype", 0, 2) != op.dtype) refuse(PyExc_TypeError, "z is of another type than dtype");
+            op.z = address(z);
+            op.z_stride = z.stride(0);
+        } else {
+            if (op.activation != MINT_ACT_NONE) refuse(PyExc_ValueError, "z is wanted: what the activation was applied to");
+            op.dtype = a.none(4) ? op.d_dtype : (int32_t)a.integer(4, "dtype", 0, 2);
+        }
+        if (op.d_dtype != op.dtype && op.d_dtype != MINT_F32) refuse(PyExc_TypeError, "grad must be of the operands' type or float32");
+        op.rows = (uint64_t)d.size(0);
+        op.cols = (uint64_t)d.size(1);
+        op.d = address(d);
+        op.d_stride = d.stride(0);
+        // (without an activation there may be nothing to change)
+        const bool same = op.activation == MINT_ACT_NONE && op.dtype == op.d_dtype;
+        OnDevice on(d.get_device());
+        Tensor d_z, d_bias, room;
+        if (!same) {
+            d_z = empty(d, d.sizes(), type_of(op.dtype));
+            op.d_z = address(d_z);
+            op.d_z_stride = d.size(1);
+        }
+        if (bias) {
+            d_bias = empty(d, {d.size(1)}, type_of(op.dtype));
+            op.d_bias = address(d_bias);
+            if ((op.workspace_bytes = native.activation_grad_workspace(op.rows, op.cols))) {
+                room = empty(d, {(int64_t)op.workspace_bytes}, at::kByte);
+                op.workspace = address(room);
+            }
+        }
+        launch("mint_activation_grad", [&] { return native.activation_grad(&op, on.stream); });
+        return pack({same ? Py_NewRef(list[0]) : wrap(d_z), bias ? wrap(d_bias) : Py_NewRef(Py_None)});
+    });
+}
+
+// ---- the loss that balances experts ----------------------------------------------------
+// logits, experts, score, offsets or None, z: arguments i .. i + 4
+void balance_of(const Args& a, int i, mint_balance_op& op) {
+    const Tensor &x = a.tensor(i, "logits"), &chosen = a.tensor(i + 1, "experts");
+    rows_of(x, "logits");
+    same_device(x, chosen, "experts");
+    choices(chosen, "experts");
+    if (x.size(1) < 1 || x.size(1) > 1024) refuse(PyExc_ValueError, "logits must be of 1..1024 experts");
+    if (chosen.size(0) != x.size(0) || chosen.size(1) > 1024) refuse(PyExc_ValueError, "experts must be what was chosen by these logits");
+    op.dtype = code_of(x.scalar_type(), "logits");
+    op.logits = address(x);
+    op.chosen = address(chosen);
+    op.row_stride = x.stride(0);
+    op.tokens = (uint64_t)x.size(0);
+    op.experts = (uint32_t)x.size(1);
+    op.topk = (uint32_t)chosen.size(1);
+    op.score = (int32_t)a.integer(i + 2, "score", 0, 1);
+    op.sequences = 1;
+    if (!a.none(i + 3)) {
+        const Tensor& offsets = a.tensor(i + 3, "offsets");
+        same_device(x, offsets, "offsets");
+        typed(offsets, at::kInt, "offsets", "int32");
+        dims(offsets, 1, "offsets");
+        dense(offsets, "offsets");
+        if (offsets.size(0) < 2) refuse(PyExc_ValueError, "offsets must have two numbers at least");
+        if (offsets.size(0) - 1 > 1 << 20) refuse(PyExc_ValueError, "at most %d sequences", 1 << 20);
+        op.offsets = address(offsets);
+        op.sequences = (uint64_t)offsets.size(0) - 1;
+    }
+    op.z = a.number(i + 4);
+}
+// balance(logits, experts, score, offsets or None, z): (loss, counts, shares, there)
+PyObject* host_balance(PyObject*, PyObject* const* list, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Args a(list, n, 5);
+        mint_balance_op op = {};
+        balance_of(a, 0, op);
+        const Tensor& x = a.tensor(0, "logits");
+        const int64_t s = (int64_t)op.sequences, e = op.experts;
+        OnDevice on(x.get_device());
+        const Tensor loss = empty(x, {}, at::kFloat), counts = empty(x, {s, e}, at::kInt), shares = empty(x, {s, e}, at::kFloat),
+                     there = empty(x, {s}, at::kInt);
+        const size_t need = native.balance_workspace(&op);
+        const Tensor room = empty(x, {(int64_t)need}, at::kByte);
+        launch("mint_balance", [&] {
+            return native.balance(&op, address(loss), address(counts), address(shares), address(there), room.data_ptr(), need, on.stream);
+        });
+        return pack({wrap(loss), wrap(counts), wrap(shares), wrap(there)});
+    });
+}
+// balance_grad(grad, logits, experts, score, offsets or None, z, counts, there, add or None)
+PyObject* host_balance_grad(PyObject*, PyObject* const* list, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        const Args a(list, n, 9);
+        mint_balance_op op = {};
+        balance_of(a, 1, op);
+        const Tensor &d = a.tensor(0, "grad"), &x = a.tensor(1, "logits"), &counts = a.tensor(6, "counts"), &there = a.tensor(7, "there");
+        same_device(x, d, "grad");
+        same_device(x, counts, "counts");
+        same_device(x, there, "there");
+        typed(d, at::kFloat, "grad", "float32");
+        typed(counts, at::kInt, "counts", "int32");
+        typed(there, at::kInt, "there", "int32");
+        dense(counts, "counts");
+        dense(there, "there");
+        if (d.numel() != 1) refuse(PyExc_ValueError, "grad must be one number");
+        if (counts.dim() != 2 || counts.size(0) != (int64_t)op.sequences || counts.size(1) != (int64_t)op.experts || there.dim() != 1 ||
+            there.size(0) != (int64_t)op.sequences)
+            refuse(PyExc_ValueError, "counts and there must be of these sequences and experts");
+        uint64_t add = 0;
+        int64_t add_stride = 0;
+        if (!a.none(8)) {
+            const Tensor& more = a.tensor(8, "add");
+            same_device(x, more, "add");
+            rows_of(more, "add");
+            if (more.sizes() != x.sizes()) refuse(PyExc_ValueError, "add must be like logits");
+            if (more.scalar_type() != x.scalar_type()) refuse(PyExc_TypeError, "add must be of the logits' type");
+            add = address(more);
+            add_stride = more.stride(0);
+        }
+        OnDevice on(x.get_device());
+        const Tensor out = empty(x, x.sizes(), x.scalar_type());
+        launch("mint_balance_grad", [&] {
+            return native.balance_grad(&op, address(d), address(counts), address(there), add, add_stride, address(out), x.size(1), on.stream);
+        });
+        return wrap(out);
+    });
+}
+
 // bind(check, addresses in the order of Native's)
 PyObject* host_bind(PyObject*, PyObject* const* list, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
@@ -626,7 +1071,9 @@ PyObject* host_bind(PyObject*, PyObject* const* list, Py_ssize_t n) {
 #define MINT_METHOD(name) {#name, (PyCFunction)(void (*)(void))host_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MINT_METHOD(bind), MINT_METHOD(route), MINT_METHOD(route_grad), MINT_METHOD(assign), MINT_METHOD(quantise),
                          MINT_METHOD(quantise_weight), MINT_METHOD(product), MINT_METHOD(weight_grad), MINT_METHOD(combine),
-                         MINT_METHOD(combine_grad), {nullptr, nullptr, 0, nullptr}};
+                         MINT_METHOD(combine_grad), MINT_METHOD(join), MINT_METHOD(join_grad), MINT_METHOD(dense_product),
+                         MINT_METHOD(dense_input_grad), MINT_METHOD(dense_weight_grad), MINT_METHOD(activation_grad), MINT_METHOD(balance),
+                         MINT_METHOD(balance_grad), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_expert_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
@@ -634,8 +1081,15 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_expert_host", nullptr, -1, method
 PyMODINIT_FUNC PyInit__expert_host(void) {
     PyObject* m = PyModule_Create(&module);
     if (!m) return nullptr;
-    PyModule_AddIntConstant(m, "ROUTE_BYTES", sizeof(mint_route_op));
-    PyModule_AddIntConstant(m, "PRODUCT_BYTES", sizeof(mint_product_op));
-    PyModule_AddIntConstant(m, "WEIGHT_GRAD_BYTES", sizeof(mint_weight_grad_op));
+    const size_t bytes[] = {sizeof(mint_route_op), sizeof(mint_product_op), sizeof(mint_weight_grad_op), sizeof(mint_join_op),
+                            sizeof(mint_join_grad_op), sizeof(mint_dense_op), sizeof(mint_activation_grad_op), sizeof(mint_balance_op)};
+    constexpr Py_ssize_t kinds = sizeof(bytes) / sizeof(bytes[0]);
+    PyObject* const list = PyTuple_New(kinds);
+    for (Py_ssize_t i = 0; list && i < kinds; ++i) PyTuple_SET_ITEM(list, i, PyLong_FromSize_t(bytes[i]));
+    if (!list || PyModule_AddObject(m, "DESCRIPTOR_BYTES", list) < 0) {
+        Py_XDECREF(list);
+        Py_DECREF(m);
+        return nullptr;
+    }
     return m;
 }

@@ -1,5 +1,5 @@
-"""Routing of tokens to experts, its gradient, and the assignment of the chosen
-pairs to places in the experts' order.
+"""Routing of tokens to experts, its gradient, the assignment of the chosen
+pairs to places in the experts' order, and the loss that keeps the experts in balance.
 
 What stands in front of the experts of a layer that is spread over ranks: from
 a token's logits, the experts it goes to and their weights (``route``), and
@@ -25,6 +25,14 @@ class Assignment(NamedTuple):
     offsets: torch.Tensor    #: (experts + 1) int32: where each expert's places begin, and their end
     tokens: torch.Tensor     #: (tokens * k) int32: the token at each place; -1 behind the end
     slots: torch.Tensor      #: (tokens, k) int32: the place of each pair; -1 where it is no expert's
+
+
+class Balance(NamedTuple):
+    """How a batch's tokens are spread over the experts."""
+    loss: torch.Tensor       #: () float32
+    counts: torch.Tensor     #: (sequences, experts) int32: the choices of each expert
+    shares: torch.Tensor     #: (sequences, experts) float32: each expert's share of a token's scores, on the average
+    there: torch.Tensor      #: (sequences,) int32: tokens that have an expert left
 
 
 def _score(name: str) -> int:
@@ -67,3 +75,28 @@ def assign(experts: torch.Tensor, count: int, first: int = 0) -> Assignment:
     their own order.  Only the experts ``first .. first + count - 1`` take part:
     the ones that a rank has; the other pairs have no place."""
     return Assignment(*_lib.experts().assign(experts, count, first))
+
+
+def balance(logits: torch.Tensor, experts: torch.Tensor, *, score: str = "softmax", offsets: torch.Tensor | None = None,
+            z: float = 0.0) -> Balance:
+    """The loss that keeps experts in balance, and the counts and shares that it is made of.
+
+    ``logits`` (tokens, experts) as for :func:`route`, ``experts`` (tokens, k) int32 what was chosen by them (-1: none).  A
+    token's shares p are the softmax of its logits, or their sigmoids divided by the sum of these.  For a sequence of n tokens that
+    have an expert left (a logit above -inf), an expert counted c times has the load f = experts * c / (k * n) and the mean
+    share P; the loss is the sum of f * P over the experts, its mean over the sequences that have such a token, plus ``z`` times the
+    mean over all these tokens of the squared log of their logits' exponentials' sum.  It is 1 where all is even.
+    ``offsets`` (sequences + 1) int32 says where each sequence begins, and the end; tokens outside count nowhere, and
+    without it all tokens are one sequence.
+
+    The counts are whole numbers, and their sum over ranks is that of all ranks' tokens: put into the place of a rank's own
+    (with ``there``'s), :func:`balance_grad` takes the load of all of them."""
+    return Balance(*_lib.experts().balance(logits, experts, _score(score), offsets, z))
+
+
+def balance_grad(grad: torch.Tensor, logits: torch.Tensor, experts: torch.Tensor, found: Balance, *, score: str = "softmax",
+                 offsets: torch.Tensor | None = None, z: float = 0.0, add: torch.Tensor | None = None) -> torch.Tensor:
+    """The logits' gradient, in their type, from the loss's ``grad`` (one float32 on the device), for what
+    :func:`balance` ``found`` with these options; the choice, and so the counts, have none.  ``add``, the logits'
+    gradient from elsewhere (:func:`route_grad`), is added before the sum is rounded."""
+    return _lib.experts().balance_grad(grad, logits, experts, _score(score), offsets, z, found.counts, found.there, add)
