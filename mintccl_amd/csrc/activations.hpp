@@ -1,47 +1,112 @@
-// Activations and their slopes, of gates (norms.hip) and of products (dense.hip), in 32 bits.  Which one is uniform over a
+// Activations and their slopes, of gates (norms.hpp) and of products (dense.hip), in 32 bits.  Which one is uniform over a
 // launch.  No counterpart in the reference.
 #pragma once
 #include "operators.hpp"
 
 namespace mint {
 
-__device__ __forceinline__ float logistic(float x) { return 1.0f / (1.0f + expf(-x)); }
+// e^x: 2^p of the rounded product p = x log2(e), and what the rounding left over to the first order; a few units of 2^-24 off, in
+// eight instructions.  Beyond the range it is infinite, or 0.
+__device__ __forceinline__ float exponential(float x) {
+    constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;
+    const float p = x * kLog2e, left = fmaf(x, kRest, fmaf(x, kLog2e, -p)), power = __builtin_amdgcn_exp2f(p);
+    return fabsf(p) < 126.0f ? fmaf(power, left * kLn2, power) : power;
+}
+__device__ __forceinline__ float reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ float logistic(float x) { return reciprocal(1.0f + exponential(-x)); }
+// P(N > x) of a normal N for x >= 0: Abramowitz and Stegun, 7.1.26 (1.5e-7 off at most, for twice of it), with e^(-x^2 / 2) as `power`.
+__device__ __forceinline__ float normal_above(float x, float power) {
+    const float t = reciprocal(fmaf(0.3275911f * 0.70710678f, x, 1.0f));
+    const float poly = fmaf(fmaf(fmaf(fmaf(1.061405429f, t, -1.453152027f), t, 1.421413741f), t, -0.284496736f), t, 0.254829592f) * t;
+    return 0.5f * poly * power;
+}
 
-// MINT_ACT_GELU is x * P(N <= x) of a normal N, MINT_ACT_GELU_TANH the approximation of it by a hyperbolic tangent.
-__device__ __forceinline__ float activated(int kind, float x) {
+// MINT_ACT_GELU is x * P(N <= x) of a normal N, MINT_ACT_GELU_TANH the approximation of it by a hyperbolic tangent: 1 + tanh(u) = 2 logistic(2 u).
+template <int N>
+__device__ __forceinline__ void activate(int kind, float (&v)[N]) {
     switch (kind) {
-        case MINT_ACT_RELU: return x > 0.0f || x != x ? x : 0.0f;
-        case MINT_ACT_SILU: return x * logistic(x);
-        case MINT_ACT_SIGMOID: return logistic(x);
-        case MINT_ACT_TANH: return tanhf(x);
-        case MINT_ACT_GELU: return 0.5f * x * erfcf(-0.70710678f * x);
-        case MINT_ACT_GELU_TANH: return 0.5f * x * (1.0f + tanhf(0.79788456f * (x + 0.044715f * x * x * x)));
-        default: return x;
+        case MINT_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = v[i] > 0.0f || v[i] != v[i] ? v[i] : 0.0f;
+            break;
+        case MINT_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] *= logistic(v[i]);
+            break;
+        case MINT_ACT_SIGMOID:
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = logistic(v[i]);
+            break;
+        case MINT_ACT_TANH:
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = tanhf(v[i]);
+            break;
+        case MINT_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float above = normal_above(fabsf(v[i]), exponential(-0.5f * v[i] * v[i]));
+                v[i] *= v[i] < 0.0f ? above : 1.0f - above;
+            }
+            break;
+        case MINT_ACT_GELU_TANH:
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] *= logistic(1.5957691f * fmaf(0.044715f * v[i], v[i] * v[i], v[i]));
+            break;
+        default: break;
     }
 }
-__device__ __forceinline__ float slope_of(int kind, float x) {
+// ... v becomes the activation's slope there
+template <int N>
+__device__ __forceinline__ void slopes(int kind, float (&v)[N]) {
     switch (kind) {
-        case MINT_ACT_RELU: return x > 0.0f ? 1.0f : x != x ? x : 0.0f;
-        case MINT_ACT_SILU: {
-            const float s = logistic(x);
-            return s * (1.0f + x * (1.0f - s));
-        }
-        case MINT_ACT_SIGMOID: {
-            const float e = expf(-fabsf(x));             // (of either sign without a difference that cancels)
-            return e / ((1.0f + e) * (1.0f + e));
-        }
-        case MINT_ACT_TANH: {
-            const float t = tanhf(x);
-            return 1.0f - t * t;
-        }
-        case MINT_ACT_GELU: return 0.5f * erfcf(-0.70710678f * x) + x * (0.39894228f * expf(-0.5f * x * x));
-        case MINT_ACT_GELU_TANH: {
-            const float t = tanhf(0.79788456f * (x + 0.044715f * x * x * x));
-            return 0.5f * (1.0f + t) + 0.5f * x * (1.0f - t * t) * (0.79788456f * (1.0f + 3.0f * 0.044715f * x * x));
-        }
-        default: return 1.0f;
+        case MINT_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = v[i] > 0.0f ? 1.0f : v[i] != v[i] ? v[i] : 0.0f;
+            break;
+        case MINT_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float s = logistic(v[i]);
+                v[i] = s * fmaf(v[i], 1.0f - s, 1.0f);
+            }
+            break;
+        case MINT_ACT_SIGMOID:
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float e = exponential(-fabsf(v[i])), r = reciprocal(1.0f + e);      // (of either sign without a difference that cancels)
+                v[i] = e * r * r;
+            }
+            break;
+        case MINT_ACT_TANH:
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float t = tanhf(v[i]);
+                v[i] = 1.0f - t * t;
+            }
+            break;
+        case MINT_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float power = exponential(-0.5f * v[i] * v[i]), above = normal_above(fabsf(v[i]), power);
+                v[i] = fmaf(v[i], 0.39894228f * power, v[i] < 0.0f ? above : 1.0f - above);
+            }
+            break;
+        case MINT_ACT_GELU_TANH:
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float x = v[i], s = logistic(1.5957691f * fmaf(0.044715f * x, x * x, x));
+                const float inner = s * (1.0f - s);              // (0 where x is far out: then so is what it is multiplied with)
+                v[i] = inner == 0.0f ? s : fmaf(x * inner, 1.5957691f * fmaf(3.0f * 0.044715f * x, x, 1.0f), s);
+            }
+            break;
+        default:
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = 1.0f;
+            break;
     }
 }
+inline bool activation_known(int kind) { return kind >= MINT_ACT_NONE && kind <= MINT_ACT_GELU_TANH; }
+
 // Of a gate: none, sigmoid, tanh or silu, in as little code as that takes (it stands in many kernels).
 __device__ __forceinline__ float gate_value(int kind, float g) {
     if (kind == MINT_ACT_NONE) return g;
@@ -54,10 +119,9 @@ __device__ __forceinline__ float gate_slope(int kind, float g) {
         const float t = tanhf(g);
         return 1.0f - t * t;
     }
-    const float e = expf(-fabsf(g)), s = (g < 0.0f ? e : 1.0f) / (1.0f + e), slope = e / ((1.0f + e) * (1.0f + e));
+    const float e = exponential(-fabsf(g)), r = reciprocal(1.0f + e), s = (g < 0.0f ? e : 1.0f) * r, slope = e * r * r;
     return kind == MINT_ACT_SILU ? fmaf(g, slope, s) : slope;
 }
 inline bool gate_known(int kind) { return kind == MINT_ACT_NONE || kind == MINT_ACT_SIGMOID || kind == MINT_ACT_TANH || kind == MINT_ACT_SILU; }
-inline bool activation_known(int kind) { return kind >= MINT_ACT_NONE && kind <= MINT_ACT_GELU_TANH; }
 
 }  // namespace mint

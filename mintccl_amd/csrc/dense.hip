@@ -17,36 +17,34 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-// 32 bytes of an operand's row or column as the matrix instructions take them: a lane has 16 bytes of the first half of the
-// depth's block and 16 of the second.
+// 16 bytes of an operand's row or column, of which four lanes have a block of the depth: as the matrix instructions take them.
 template <int DT>
-struct Pair {
-    u32x4 v[2];
-    static __device__ __forceinline__ f32x4 multiply(const Pair& a, const Pair& b, f32x4 c) {
+__device__ __forceinline__ f32x4 multiply_add(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (DT == DT_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    } else if constexpr (DT == DT_F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if constexpr (DT == DT_BF16) {
-                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v[h]), __builtin_bit_cast(bf16x8, b.v[h]), c, 0, 0, 0);
-            } else if constexpr (DT == DT_F16) {
-                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v[h]), __builtin_bit_cast(f16x8, b.v[h]), c, 0, 0, 0);
-            } else {
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a.v[h][t]), __uint_as_float(b.v[h][t]), c, 0, 0, 0);
-            }
-        }
+        for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[t]), __uint_as_float(b[t]), c, 0, 0, 0);
         return c;
     }
-};
+}
 template <int DT>
 constexpr uint32_t kSize = sizeof(typename Elem<DT>::type);
 template <int DT>
-constexpr uint32_t kBlock = 128 / kSize<DT>;            // numbers of the depth that go by together
+constexpr uint32_t kHalf = 64 / kSize<DT>;              // numbers of the depth that go by in a step
+template <int DT>
+constexpr uint32_t kBlock = 2 * kHalf<DT>;              // ... and in a block, two steps
 
-__device__ __forceinline__ void to_lds16(const uint8_t* from, uint32_t lds) {
-    __builtin_amdgcn_global_load_lds((MINT_GLOBAL const void*)as_global(from), (MINT_LDS void*)(uintptr_t)lds, 16, 0, 0);
+using LdsBytes = MINT_LDS uint8_t*;
+// 16 bytes of a lane's own, at a 32-bit offset from where the wavefront's are, into LDS, the lanes' side by side.  (By the buffer's form: for
+// the global one the compiler holds every read of LDS back until all such loads, and all reads, are done.)
+__device__ __forceinline__ void to_lds16(const uint8_t* from, uint32_t offset, LdsBytes to) {
+    const auto whole = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, 0xFFFFFFFFu, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(whole, (MINT_LDS void*)to, 16, offset, 0, 0, 0);
 }
-__device__ __forceinline__ u32x4 lds16(uint32_t at) { return *(MINT_LDS const u32x4*)(uintptr_t)at; }
+__device__ __forceinline__ u32x4 lds16(LdsBytes at) { return *(MINT_LDS const u32x4*)at; }
 // the first `left` bytes, zeros behind
 __device__ __forceinline__ u32x4 first_of(u32x4 v, int64_t left) {
 #pragma unroll
@@ -72,17 +70,19 @@ __device__ __forceinline__ u32x4 piece_of(const uint8_t* from, int64_t left) {
     }
     return v;
 }
-// All but the N latest of a wavefront's loads are done; then all wavefronts meet.
+// All but the N latest of a wavefront's loads are done.
 template <int N>
+__device__ __forceinline__ void wait_loads() {
+    compiler_fence();
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);
+    compiler_fence();
+}
+// All wavefronts meet, what they read from LDS and wrote there behind them.
 __device__ __forceinline__ void meet() {
-    if constexpr (N == 0) {
-        __syncthreads();
-    } else {
-        __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4 | 15 << 8);
-        compiler_fence();
-        __builtin_amdgcn_s_barrier();
-        compiler_fence();
-    }
+    compiler_fence();
+    __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);          // (LDS only)
+    __builtin_amdgcn_s_barrier();
+    compiler_fence();
 }
 
 // An operand: `n` rows or columns of the result.  ALONG: row i of it at p + i * stride, the depth along it; else depth d at p + d * stride.
@@ -91,27 +91,28 @@ struct Side {
     int64_t stride;              // bytes
     uint32_t n;
 };
-// B of them in LDS, a block of the depth: B * 128 bytes either way, in pieces of 16.
-//   along    a row of 128 bytes for each of them, pieces turned by the row's number: the lanes that a 16-byte read serves
-//            together are of different rows
-//   across   a row of B numbers for each number of the depth; a lane's numbers of one column are gathered by the
-//            transposing reads (16 bits: 16 lanes have four rows of 16 numbers), or one by one (32 bits).  The groups of 16 numbers are
-//            turned by the row's number likewise
+// B of them in LDS, a part of the depth, in pieces of 16 bytes.
+//   along    a block: a row of 128 bytes for each of them, its pieces turned so that the 16 lanes that a 16-byte read serves together (0 - 3,
+//            12 - 15 and 20 - 27 of 32, then the others; 16 lanes side by side are 16 rows) are on different banks.  (Half a block at a time would
+//            be 64 bytes of a row with each request: 8192 x 8192 x 4096 485 us for 440)
+//   across   a step's half: a row of B numbers for each number of the depth; a lane's numbers of one column are gathered by the
+//            transposing reads (16 bits: 16 lanes have four rows of 16 numbers), or one by one (32 bits).  Which 16 numbers lie
+//            where in a row is turned by the row's number, so that those reads have different banks too
 template <int DT, int B, bool ALONG>
 struct Staged {
-    static constexpr uint32_t SIZE = kSize<DT>, PIECES = ALONG ? 8 : B * SIZE / 16;      // of an LDS row
+    static constexpr uint32_t SIZE = kSize<DT>, PIECES = ALONG ? 8 : B * SIZE / 16, BYTES = B * (ALONG ? 128 : 64);
     static __device__ __forceinline__ uint32_t turn(uint32_t row) {
         if constexpr (ALONG) return (row >> 1) & 7u;
         else if constexpr (SIZE == 4) return (row >> 2 & 3u) * 4;
         else if constexpr (PIECES == 8) return ((row >> 1 & 1u) | (row >> 2 & 2u)) * 2;
         else return ((row & 3u) | (row >> 1 & 4u)) * 2;
     }
-    // where unit u (16 bytes in LDS, in order) comes from: its LDS row and its piece of the row in memory
+    // where 16 bytes in LDS, the u-th, come from: their row and their piece of that row
     static __device__ __forceinline__ uint32_t row_of(uint32_t u) { return u / PIECES; }
     static __device__ __forceinline__ uint32_t piece_of(uint32_t u) { return (u % PIECES) ^ turn(u / PIECES); }
 
-    // A lane's part of the g-th 16 of them.
-    uint32_t base;               // along: the lane's first piece of the first 16; across: the lane's numbers of its LDS row's first 16
+    // A lane's part of the g-th 16 of them, of a half of the depth's block.
+    uint32_t base;               // along: the lane's piece of the first 16; across: the lane's numbers of its row's first 16
     uint32_t turned;             // across: what the number of the 16 is turned by in that row
     __device__ __forceinline__ explicit Staged(uint32_t lane) {
         const uint32_t r16 = lane & 15u, part = lane >> 4;
@@ -122,35 +123,26 @@ struct Staged {
             base = part * 4 * (B * 4) + r16 * 4;
             turned = part;
         } else {
-            const uint32_t row = part * 8 + (r16 >> 2);          // (4 and 32 rows on the turning is the same)
+            const uint32_t row = part * 8 + (r16 >> 2);          // (4 rows on the turning is the same)
             base = row * (B * 2) + (r16 & 3u) * 8;
             turned = turn(row) / 2;
         }
     }
-    __device__ __forceinline__ Pair<DT> load(uint32_t at, uint32_t g) const {
-        Pair<DT> p;
+    __device__ __forceinline__ u32x4 load(LdsBytes at, uint32_t g, uint32_t half) const {
         if constexpr (ALONG) {
-            p.v[0] = lds16(at + g * 2048 + base);
-            p.v[1] = lds16(at + g * 2048 + (base ^ 64u));
+            return lds16(at + (g * 2048 + (base ^ half * 64)));
         } else if constexpr (SIZE == 4) {
-            const uint32_t from = at + base + (g ^ turned) * 64;
+            const LdsBytes from = at + (base + (g ^ turned) * 64);
+            u32x4 v;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int t = 0; t < 4; ++t) p.v[h][t] = *(MINT_LDS const uint32_t*)(uintptr_t)(from + (h * 16 + t) * (B * 4));
+            for (int t = 0; t < 4; ++t) v[t] = *(MINT_LDS const uint32_t*)(from + t * (B * 4));
+            return v;
         } else {
-            const uint32_t from = at + base + (g ^ turned) * 32;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                i16x4 q[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    q[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((MINT_LDS i16x4*)(uintptr_t)(from + (h * 32 + j * 4) * (B * 2)));
-                const u32x2 lo = __builtin_bit_cast(u32x2, q[0]), hi = __builtin_bit_cast(u32x2, q[1]);
-                p.v[h] = u32x4{lo.x, lo.y, hi.x, hi.y};
-            }
+            const LdsBytes from = at + (base + (g ^ turned) * 32);
+            const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MINT_LDS i16x4*)from));
+            const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MINT_LDS i16x4*)(from + 4 * (B * 2))));
+            return u32x4{lo.x, lo.y, hi.x, hi.y};
         }
-        return p;
     }
 };
 
@@ -168,29 +160,31 @@ template <int DT>
 __device__ __forceinline__ void store8(void* p, int64_t at, int64_t left, const float (&v)[8]) {
     store_elements<DT, 8>(static_cast<typename Elem<DT>::type*>(p) + at, left, v);
 }
+template <int DT>
+__device__ __forceinline__ void bias8(const Finish& f, uint32_t col, uint32_t cols, float (&bias)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
+    if (f.bias && col < cols) load8<DT>(f.bias, col, (int64_t)cols - col, bias);
+}
+template <int DT>
+__device__ __forceinline__ void residual8(const Finish& f, uint32_t row, uint32_t col, uint32_t cols, float (&more)[8]) {
+    const int64_t left = (int64_t)cols - col;
+    if (f.out_dtype == MINT_F32) load8<DT_F32>(f.residual, (int64_t)row * f.residual_stride + col, left, more);
+    else load8<DT>(f.residual, (int64_t)row * f.residual_stride + col, left, more);
+}
 // Eight sums of a row of the result become what is stored.  Results are of the operands' type or in 32 bits.
 template <int DT>
-__device__ __forceinline__ void finish8(const Finish& f, uint32_t row, uint32_t col, uint32_t cols, float (&v)[8]) {
+__device__ __forceinline__ void finish8(const Finish& f, uint32_t row, uint32_t col, uint32_t cols, const float (&bias)[8], const float (&more)[8], float (&v)[8]) {
     const int64_t left = (int64_t)cols - col;
-    float more[8];
-    if (f.bias) {
-        load8<DT>(f.bias, col, left, more);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += more[i];
-    }
+    for (int i = 0; i < 8; ++i) v[i] += bias[i];
     if (f.z) store8<DT>(f.z, (int64_t)row * f.z_stride + col, left, v);
-    if (f.activation != MINT_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = activated(f.activation, v[i]);
-    }
-    const bool wide = f.out_dtype == MINT_F32;
+    if (f.activation != MINT_ACT_NONE) activate(f.activation, v);
     if (f.residual) {
-        if (wide) load8<DT_F32>(f.residual, (int64_t)row * f.residual_stride + col, left, more);
-        else load8<DT>(f.residual, (int64_t)row * f.residual_stride + col, left, more);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += more[i];
     }
-    if (wide) store8<DT_F32>(f.out, (int64_t)row * f.out_stride + col, left, v);
+    if (f.out_dtype == MINT_F32) store8<DT_F32>(f.out, (int64_t)row * f.out_stride + col, left, v);
     else store8<DT>(f.out, (int64_t)row * f.out_stride + col, left, v);
 }
 
@@ -202,23 +196,305 @@ struct DenseArgs {
     float* sums;                         // (parts, rows, cols)
 };
 
-// A thread block has BM rows and BN columns of the result, a wavefront BM / WM rows and 64 columns of them.  The depth goes by in blocks of
-// 128 bytes; while one is multiplied the next STAGES - 1 ones are on their way into LDS.  DIRECT: rows in memory begin at
-// multiples of 16 bytes, and their pieces go straight into LDS; else they pass through registers.
-template <int DT, int BM, int BN, int WM, int STAGES, bool X_ALONG, bool W_ALONG, bool DIRECT>
-__global__ void __launch_bounds__(64 * WM * (BN / 64)) dense_kernel(DenseArgs a) {
-    constexpr int WN = BN / 64, WAVES = WM * WN, MT = BM / WM / 16, NT = 4, XI = BM / 8 / WAVES, WI = BN / 8 / WAVES, ALL = XI + WI;
-    constexpr uint32_t SIZE = kSize<DT>, K = kBlock<DT>, kX = BM * 128, kStage = (BM + BN) * 128;
-    constexpr uint32_t SLABS = MT < 4 ? MT : 4, PITCH = 68;               // of the sums' way out: slabs of 16 rows of 64 columns
-    constexpr uint32_t kOut = WAVES * SLABS * 16 * PITCH * 4, kLds = STAGES * kStage > kOut ? STAGES * kStage : kOut;
-    static_assert(XI * 8 * WAVES == BM && WI * 8 * WAVES == BN, "every wavefront brings as much");
-    static_assert(kLds <= 160 * 1024, "it fits LDS");
-    using SX = Staged<DT, BM, X_ALONG>;
-    using SW = Staged<DT, BN, W_ALONG>;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
-    const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), wm = wave / WN, wn = wave % WN;
-    const uint32_t base = (uint32_t)(uintptr_t)(MINT_LDS uint8_t*)lds;
+// One operand of a tile, on its way from memory into a ring of N places in LDS.  A unit is a block of the depth (along) or half of one.
+template <int DT, int B, int WAVES, int N, bool ALONG>
+struct Ring {
+    using S = Staged<DT, B, ALONG>;
+    static constexpr int EACH = S::BYTES / 1024 / WAVES;         // instructions of a wavefront for a unit
+    static constexpr uint32_t SIZE = kSize<DT>, UNIT = ALONG ? kBlock<DT> : kHalf<DT>, BYTES = S::BYTES;
+    static_assert(EACH * 1024 * WAVES == BYTES, "every wavefront brings as much");
+    const uint8_t* from;         // the unit to ask for, the same for the wavefront ...
+    uint32_t at[EACH];           // ... and what the lane brings of it
+    int64_t stride;
+    uint32_t left;               // of the depth, from that unit on
+    uint32_t wave, lane;
+    LdsBytes base, ask;
 
+    __device__ __forceinline__ uint32_t unit(int n) const { return (wave * EACH + n) * 64 + lane; }
+    __device__ __forceinline__ Ring(const Side& s, uint32_t first, uint32_t depth0, uint32_t depth, LdsBytes to, uint32_t w, uint32_t l)
+        : stride(s.stride), left(depth), wave(w), lane(l), base(to), ask(to) {
+        from = ALONG ? s.p + (int64_t)first * stride + (int64_t)depth0 * SIZE : s.p + (int64_t)depth0 * stride + (int64_t)first * SIZE;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const uint32_t row = S::row_of(unit(n)), piece = S::piece_of(unit(n)) * 16;
+            // (rows behind the operand's last one: that one instead; in the place of a piece behind a row's last one, that one)
+            at[n] = ALONG ? min(row, s.n - 1 - first) * (uint32_t)stride + piece : row * (uint32_t)stride + min(piece, (min(s.n - first, 4096u) * SIZE - 1) / 16 * 16);
+        }
+    }
+    __device__ __forceinline__ LdsBytes on(LdsBytes p) const { return p + BYTES == base + N * BYTES ? base : p + BYTES; }
+    __device__ __forceinline__ void advance() {
+        from += ALONG ? 128 : (int64_t)UNIT * stride;
+        left -= min(left, UNIT);
+        ask = on(ask);
+    }
+    // piece n of a whole unit, into `to`; the last one goes on
+    __device__ __forceinline__ void bring(LdsBytes to, int n) {
+        to_lds16(from, at[n], to + (wave * EACH + n) * 1024);
+        if (n == EACH - 1) advance();
+    }
+    // All of a unit that may not be whole: what lies behind the depth comes from the unit's beginning.  The depth's units behind its last number are
+    // cleared only.  Its own pieces are cleared, when they are there, by whoever brought them; `there` is what it has.
+    __device__ __forceinline__ void bring_any(LdsBytes to, uint32_t& there) {
+        there = left;
+        if (left) {
+#pragma unroll
+            for (int n = 0; n < EACH; ++n) {
+                const uint32_t row = S::row_of(unit(n)), piece = S::piece_of(unit(n)) * 16;
+                const uint32_t back = ALONG ? piece < left * SIZE ? 0u : piece : row < left ? 0u : row * (uint32_t)stride;
+                to_lds16(from, at[n] - back, to + (wave * EACH + n) * 1024);
+            }
+        }
+        advance();
+    }
+    __device__ __forceinline__ void clear(LdsBytes to, uint32_t there) const {
+        if (there >= UNIT) return;
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const auto v = (MINT_LDS u32x4*)(to + unit(n) * 16);
+            const int64_t bytes = ALONG ? (int64_t)(there * SIZE) - S::piece_of(unit(n)) * 16 : S::row_of(unit(n)) < there ? 16 : 0;
+            *v = first_of(*v, bytes);
+        }
+    }
+};
+
+// A thread block has BM rows and BN columns of the result, a wavefront BM / WM rows and 64 columns of them.  The depth goes by in blocks of
+// 128 bytes, two steps each, in rings of NX and NW places.  In a step
+//   - what the last step read of x last is multiplied, while the first of this one is read: no one waits behind the meeting
+//   - the rest follows, each operand read some products ahead, and w's for the next step
+//   - units of x NX - 1 on and of w NW on are asked for, into places that are no longer read: w's of a step has been read before it
+// and at its end the wavefronts meet when what the next step reads has come: asked for two steps before and more.  DIRECT: rows in memory
+// begin at multiples of 16 bytes, and their pieces go straight into LDS; else they pass through registers, a block at a time.
+template <int DT, int BM, int BN, int WM, int NX, int NW, bool X_ALONG, bool W_ALONG>
+struct Tile {
+    static constexpr int WN = BN / 64, WAVES = WM * WN, MT = BM / WM / 16, NT = 4;
+    static constexpr int LAG = MT > 2 ? 2 : 1;                            // rows of products that are left to the next step
+    static constexpr uint32_t K = kBlock<DT>;
+    using X = Ring<DT, BM, WAVES, NX, X_ALONG>;
+    using W = Ring<DT, BN, WAVES, NW, W_ALONG>;
+    static constexpr uint32_t kStages = NX * X::BYTES + NW * W::BYTES;
+    static constexpr uint32_t SLABS = MT < 4 ? MT : 4, PITCH = 68;        // of the sums' way out: slabs of 16 rows of 64 columns
+    static constexpr uint32_t kOut = WAVES * SLABS * 16 * PITCH * 4, kLds = kStages > kOut ? kStages : kOut;
+    static_assert(kLds <= 160 * 1024, "it fits LDS");
+
+    // What is asked for in a step (0: a block's first), x's before w's, and how much of it may be on its way when the step ends.
+    static constexpr int asks_x(int step) { return X_ALONG ? (step & 1 ? 0 : X::EACH) : X::EACH; }
+    static constexpr int asks_w(int step) { return W_ALONG ? (step & 1 ? W::EACH : 0) : W::EACH; }
+    static constexpr int later(int first, int end) {                      // asked in steps [first, end]
+        int n = 0;
+        for (int s = first; s <= end; ++s) n += asks_x(s & 1) + asks_w(s & 1);
+        return n;
+    }
+    static constexpr int under_way(int step) {
+        const int s = 64 + step;                                          // (any block)
+        int most = 63;
+        // w of step s + 2 is read in the next step, x of step s + 1 too
+        const int w_asked = W_ALONG ? (step ? -1 : s + 3 - 2 * NW) : s + 2 - NW, x_asked = X_ALONG ? (step ? s + 3 - 2 * NX : -1) : s + 2 - NX;
+        if (w_asked >= 0 && later(w_asked + 1, s) < most) most = later(w_asked + 1, s);
+        if (x_asked >= 0 && later(x_asked + 1, s) + asks_w(x_asked & 1) < most) most = later(x_asked + 1, s) + asks_w(x_asked & 1);
+        return most;
+    }
+    // blocks that are asked for ahead of the one at work
+    static constexpr int x_ahead = X_ALONG ? NX - 1 : NX / 2, w_ahead = W_ALONG ? NW : (NW + 1) / 2, LEAD = x_ahead > w_ahead ? x_ahead : w_ahead;
+
+    const DenseArgs& a;
+    uint32_t lane, wave, m0, n0, depth0, depth;
+    typename X::S sx;
+    typename W::S sw;
+    f32x4 acc[MT][NT];
+
+    __device__ __forceinline__ uint32_t wm() const { return wave / WN; }
+    __device__ __forceinline__ uint32_t wn() const { return wave % WN; }
+    __device__ __forceinline__ Tile(const DenseArgs& args, uint32_t m, uint32_t n, uint32_t part)
+        : a(args), lane(lane_id()), wave(__builtin_amdgcn_readfirstlane(wave_in_block())), m0(m), n0(n), sx(lane), sw(lane) {
+        // this part's blocks of the depth; the last of all may not be whole
+        const uint32_t blocks = (a.depth + K - 1) / K, share = (blocks + a.parts - 1) / a.parts;
+        depth0 = min(part * share * K, a.depth);
+        depth = min(share * K, a.depth - depth0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    }
+    __device__ __forceinline__ u32x4 load_x(LdsBytes at, int i, uint32_t half) const { return sx.load(at, wm() * MT + i, half); }
+    __device__ __forceinline__ u32x4 load_w(LdsBytes at, int j, uint32_t half) const { return sw.load(at, wn() * 4 + j, half); }
+    __device__ __forceinline__ void products(int i, const u32x4 (&w)[NT], u32x4 x) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = multiply_add<DT>(w[j], x, acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    // A step: of the block at x_at with `w`, which has been read.  `before` has w of the step before, which is still wanted for what it left (in `lag`), and
+    // takes that of the next one, at w_at.
+    template <typename F>
+    __device__ __forceinline__ void step(LdsBytes x_at, uint32_t x_half, LdsBytes w_at, uint32_t w_half, u32x4 (&w)[NT], u32x4 (&before)[NT], u32x4 (&lag)[LAG],
+                                         int asks, const F& meanwhile) {
+        constexpr int FIRST = MT > LAG ? LAG + 1 : MT, SLOTS = MT > LAG ? MT - LAG : 1, READS = SLOTS > 2 ? (NT + SLOTS - 2) / (SLOTS - 1) : NT;
+        u32x4 x[MT];
+#pragma unroll
+        for (int i = 0; i < FIRST; ++i) x[i] = load_x(x_at, i, x_half);
+        const int pieces = (asks + SLOTS - 1) / SLOTS;
+#pragma unroll
+        for (int i = 0; i < LAG; ++i) products(MT - LAG + i, before, lag[i]);
+        // (nothing is read during the last products: the meeting waits for the reads, so that what is asked for behind it may lie where they read)
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+            if (i + FIRST < MT) x[i + FIRST] = load_x(x_at, i + FIRST, x_half);
+            // (the loads go out between the products: all at once they would stand in each other's way)
+#pragma unroll
+            for (int n = 0; n < pieces; ++n)
+                if (i * pieces + n < asks) meanwhile(i * pieces + n);
+#pragma unroll
+            for (int n = 0; n < READS; ++n)
+                if (i * READS + n < NT) before[i * READS + n] = load_w(w_at, i * READS + n, w_half);
+            if (i < MT - LAG) products(i, w, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < LAG; ++i) lag[i] = x[MT - LAG + i];
+    }
+    // The two steps of a block, where all that they ask for is whole.  Reads are from four places (a block along the depth has two of them alike), what is
+    // asked for goes to four; w's of the second step may be where the first one read, behind a meeting.  That no read is of what is on
+    // its way is what the compiler has to know, or it waits for all of that.
+    __device__ __forceinline__ void block(X& rx, W& rw, LdsBytes __restrict x0, LdsBytes __restrict x1, LdsBytes __restrict w0, LdsBytes __restrict w1,
+                                          LdsBytes __restrict to_x0, LdsBytes __restrict to_x1, LdsBytes __restrict to_w0, LdsBytes __restrict to_w1,
+                                          u32x4 (&w)[NT], u32x4 (&other)[NT], u32x4 (&lag)[LAG]) {
+        step(x0, 0, w0, 1, w, other, lag, asks_x(0) + asks_w(0), [&](int n) MINT_INLINE_LAMBDA {
+            if (n < asks_x(0)) rx.bring(to_x0, n);
+            else rw.bring(to_w0, n - asks_x(0));
+        });
+        wait_loads<under_way(0)>();
+        meet();
+        step(x1, 1, w1, 0, other, w, lag, asks_x(1) + asks_w(1), [&](int n) MINT_INLINE_LAMBDA {
+            if (n < asks_x(1)) rx.bring(to_x1, n);
+            else rw.bring(to_w1, n - asks_x(1));
+        });
+        wait_loads<under_way(1)>();
+        meet();
+    }
+    __device__ __forceinline__ void run_direct(LdsBytes lds) {
+        const uint32_t blocks = (depth + K - 1) / K, full = depth / K;
+        if (!blocks) return;
+        X rx(a.x, m0, depth0, depth, lds, wave, lane);
+        W rw(a.w, n0, depth0, depth, lds + NX * X::BYTES, wave, lane);
+        const auto bring_x = [&]() MINT_INLINE_LAMBDA {
+            const LdsBytes to = rx.ask;
+            uint32_t there;
+            rx.bring_any(to, there);
+            return there;
+        };
+        {
+            uint32_t x_there[NX - 1], w_there[NW];
+#pragma unroll
+            for (int u = 0; u < NX - 1; ++u) x_there[u] = bring_x();
+#pragma unroll
+            for (int u = 0; u < NW; ++u) {
+                const LdsBytes to = rw.ask;
+                rw.bring_any(to, w_there[u]);
+            }
+            wait_loads<0>();
+#pragma unroll
+            for (int u = 0; u < NX - 1; ++u) rx.clear(rx.base + u * X::BYTES, x_there[u]);
+#pragma unroll
+            for (int u = 0; u < NW; ++u) rw.clear(rw.base + u * W::BYTES, w_there[u]);
+        }
+        meet();
+        u32x4 w[NT], other[NT], lag[LAG];
+        LdsBytes x_at = rx.base, w_at = rw.base;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            w[j] = load_w(w_at, j, 0);
+            other[j] = u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < LAG; ++i) lag[i] = u32x4{0, 0, 0, 0};
+        meet();
+        uint32_t b = 0;
+#pragma unroll 1
+        for (; b + LEAD < full; ++b) {
+            const LdsBytes x1 = X_ALONG ? x_at : rx.on(x_at), w0 = W_ALONG ? w_at : rw.on(w_at), w1 = rw.on(w0);
+            // (where a unit is a block one of the two steps asks for it)
+            const LdsBytes to_x0 = rx.ask, to_x1 = rx.on(to_x0), to_w0 = rw.ask, to_w1 = W_ALONG ? to_w0 : rw.on(to_w0);
+            block(rx, rw, x_at, x1, w0, w1, to_x0, to_x1, to_w0, to_w1, w, other, lag);
+            x_at = rx.on(x1);
+            w_at = w1;
+        }
+        // the last blocks: what they ask for, if anything, may not be whole, and everything is waited for
+#pragma unroll 1
+        for (; b < blocks; ++b) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const LdsBytes to_x = rx.ask, to_w = rw.ask;
+                uint32_t x_there = X::UNIT, w_there = W::UNIT;
+                if (asks_x(h)) rx.bring_any(to_x, x_there);
+                if (asks_w(h)) rw.bring_any(to_w, w_there);
+                const LdsBytes next_w = W_ALONG && h == 0 ? w_at : rw.on(w_at);
+                step(x_at, h, next_w, 1 - h, h ? other : w, h ? w : other, lag, 0, [](int) MINT_INLINE_LAMBDA {});
+                wait_loads<0>();
+                rx.clear(to_x, x_there);
+                rw.clear(to_w, w_there);
+                meet();
+                if (!X_ALONG || h) x_at = rx.on(x_at);
+                w_at = next_w;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < LAG; ++i) products(MT - LAG + i, other, lag[i]);
+    }
+    // (the places: two blocks in turn, so that there is one meeting to a block)
+    static constexpr uint32_t kHeldX = BM * 128, kHeld = (BM + BN) * 128;
+    __device__ __forceinline__ void run_held(LdsBytes lds) {
+        constexpr uint32_t SIZE = kSize<DT>;
+        constexpr int XI = BM / 8 / WAVES, WI = BN / 8 / WAVES;          // pieces of a lane
+        u32x4 held[XI + WI];
+        // of the u-th 16 bytes of an operand's block: its row and piece (across: the second half's behind the first one's)
+        const auto fetch = [&](uint32_t b) MINT_INLINE_LAMBDA {
+            const uint32_t d0 = depth0 + b * K;                          // (the depth from here on)
+            const auto one = [&](const Side& s, bool along, uint32_t first, uint32_t row, uint32_t piece) MINT_INLINE_LAMBDA {
+                if (along)
+                    return ::mint::piece_of<SIZE>(s.p + (int64_t)min(first + row, s.n - 1) * s.stride + ((int64_t)d0 * SIZE + piece * 16),
+                                                  ((int64_t)a.depth - d0) * SIZE - piece * 16);
+                const int64_t left = ((int64_t)s.n - first) * SIZE - piece * 16;
+                return ::mint::piece_of<SIZE>(s.p + (int64_t)min(d0 + row, a.depth - 1) * s.stride + ((int64_t)first * SIZE + piece * 16),
+                                              d0 + row < a.depth ? left : 0);
+            };
+#pragma unroll
+            for (int n = 0; n < XI; ++n) {
+                const uint32_t u = (wave * XI + n) * 64 + lane;
+                held[n] = one(a.x, X_ALONG, m0, X::S::row_of(u), X::S::piece_of(u));
+            }
+#pragma unroll
+            for (int n = 0; n < WI; ++n) {
+                const uint32_t u = (wave * WI + n) * 64 + lane;
+                held[XI + n] = one(a.w, W_ALONG, n0, W::S::row_of(u), W::S::piece_of(u));
+            }
+        };
+        const uint32_t blocks = (depth + K - 1) / K;
+        if (blocks) fetch(0);
+#pragma unroll 1
+        for (uint32_t b = 0; b < blocks; ++b) {
+            const LdsBytes at = lds + (b & 1u) * kHeld;
+#pragma unroll
+            for (int n = 0; n < XI; ++n) *(MINT_LDS u32x4*)(at + ((wave * XI + n) * 64 + lane) * 16) = held[n];
+#pragma unroll
+            for (int n = 0; n < WI; ++n) *(MINT_LDS u32x4*)(at + (kHeldX + ((wave * WI + n) * 64 + lane) * 16)) = held[XI + n];
+            __syncthreads();
+            if (b + 1 < blocks) fetch(b + 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u32x4 w[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) w[j] = load_w(at + (kHeldX + (W_ALONG ? 0 : h * BN * 64)), j, h);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) products(i, w, load_x(at + (X_ALONG ? 0 : h * BM * 64), i, h));
+            }
+        }
+    }
+};
+
+template <int DT, int BM, int BN, int WM, int NX, int NW, bool X_ALONG, bool W_ALONG, bool DIRECT>
+__global__ void __launch_bounds__(64 * WM * (BN / 64)) dense_kernel(DenseArgs a) {
+    using T = Tile<DT, BM, BN, WM, NX, NW, X_ALONG, W_ALONG>;
+    constexpr uint32_t SLABS = T::SLABS, PITCH = T::PITCH;
+    static_assert(DIRECT || 2 * T::kHeld <= T::kLds, "they have room");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::kLds];
     // The hardware deals thread blocks to the eight XCDs in turn: each takes an eighth of the tiles that lie together, in
     // columns of GROUP row tiles, so that those at work at a time share operands in its L2.
     constexpr uint32_t GROUP = 4;
@@ -227,161 +503,43 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) dense_kernel(DenseArgs a)
     const uint32_t all_id = xcd * (total / 8) + min(xcd, total % 8) + nth, id = all_id / a.parts, part = all_id % a.parts;
     const uint32_t group = id / (GROUP * a.col_tiles), in_group = id % (GROUP * a.col_tiles), height = min(GROUP, a.row_tiles - group * GROUP);
     const uint32_t m0 = (group * GROUP + in_group % height) * BM, n0 = in_group / height * BN;
-
-    // this part's blocks of the depth; the last of all may not be whole
-    const uint32_t blocks = (a.depth + K - 1) / K, share = (blocks + a.parts - 1) / a.parts, b0 = min(part * share, blocks);
-    const uint32_t steps = min(share, blocks - b0), tail = a.depth % K, full = steps && tail && b0 + steps == blocks ? steps - 1 : steps;
-
-    // The 16 bytes that this lane brings with instruction n of the operand: from there, and how much of them is there
-    const auto unit = [&](int n, int each) MINT_INLINE_LAMBDA { return (wave * each + n) * 64 + lane; };
-    const auto start = [&](const Side& s, uint32_t first, bool along, uint32_t row, uint32_t piece) MINT_INLINE_LAMBDA {
-        if (along) return s.p + (int64_t)min(first + row, s.n - 1) * s.stride + ((int64_t)b0 * 128 + piece * 16);
-        // (a piece behind the last one: that one instead)
-        return s.p + ((int64_t)b0 * K + row) * s.stride + min((int64_t)first * SIZE + piece * 16, ((int64_t)s.n * SIZE - 1) / 16 * 16);
-    };
-    const uint8_t *from_x[XI], *from_w[WI];
-    const int64_t step_x = X_ALONG ? 128 : (int64_t)K * a.x.stride, step_w = W_ALONG ? 128 : (int64_t)K * a.w.stride;
-    if (steps) {
-#pragma unroll
-        for (int n = 0; n < XI; ++n) from_x[n] = start(a.x, m0, X_ALONG, SX::row_of(unit(n, XI)), SX::piece_of(unit(n, XI)));
-#pragma unroll
-        for (int n = 0; n < WI; ++n) from_w[n] = start(a.w, n0, W_ALONG, SW::row_of(unit(n, WI)), SW::piece_of(unit(n, WI)));
-    }
-
-    f32x4 acc[MT][NT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    const SX sx(lane);
-    const SW sw(lane);
-    const auto multiply = [&](uint32_t at, const auto& meanwhile) MINT_INLINE_LAMBDA {
-        const Pair<DT> w[NT] = {sw.load(at + kX, wn * 4), sw.load(at + kX, wn * 4 + 1), sw.load(at + kX, wn * 4 + 2), sw.load(at + kX, wn * 4 + 3)};
-        Pair<DT> x = sx.load(at, wm * MT);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            // (the next block's loads go out between the products: all at once they would stand in each other's way)
-            constexpr int PIECES = MT > 1 ? (ALL * 2 + MT - 1) / MT : ALL;
-#pragma unroll
-            for (int n = 0; n < PIECES; ++n)
-                if (i * PIECES + n < ALL) meanwhile(i * PIECES + n);
-            Pair<DT> next = x;
-            if (i + 1 < MT) next = sx.load(at, wm * MT + i + 1);
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = Pair<DT>::multiply(w[j], x, acc[i][j]);
-            x = next;
-        }
-    };
-
-    if constexpr (DIRECT) {
-        const auto bring = [&](uint32_t at, int n) MINT_INLINE_LAMBDA {
-            if (n < XI) {
-                to_lds16(from_x[n], at + (wave * XI + n) * 1024);
-                from_x[n] += step_x;
-            } else {
-                to_lds16(from_w[n - XI], at + kX + (wave * WI + (n - XI)) * 1024);
-                from_w[n - XI] += step_w;
-            }
-        };
-        // The depth's last block where it is not whole comes like the others, what lies behind the depth from the block's beginning; then
-        // it is cleared in LDS.
-        const auto bring_tail = [&](uint32_t at) MINT_INLINE_LAMBDA {
-            const auto inside = [&](const uint8_t* from, bool along, uint32_t row, uint32_t piece, int64_t stride) MINT_INLINE_LAMBDA {
-                if (along) return piece * 16 < tail * SIZE ? from : from - piece * 16;
-                return row < tail ? from : from - (int64_t)row * stride;
-            };
-#pragma unroll
-            for (int n = 0; n < XI; ++n)
-                to_lds16(inside(from_x[n], X_ALONG, SX::row_of(unit(n, XI)), SX::piece_of(unit(n, XI)), a.x.stride), at + (wave * XI + n) * 1024);
-#pragma unroll
-            for (int n = 0; n < WI; ++n)
-                to_lds16(inside(from_w[n], W_ALONG, SW::row_of(unit(n, WI)), SW::piece_of(unit(n, WI)), a.w.stride), at + kX + (wave * WI + n) * 1024);
-        };
-        const auto clear_tail = [&](uint32_t at) MINT_INLINE_LAMBDA {
-            const auto clear = [&](bool along, uint32_t row, uint32_t piece, uint32_t to) MINT_INLINE_LAMBDA {
-                const auto v = (MINT_LDS u32x4*)(uintptr_t)to;
-                *v = first_of(*v, along ? (int64_t)(tail * SIZE) - piece * 16 : row < tail ? 16 : 0);
-            };
-#pragma unroll
-            for (int n = 0; n < XI; ++n) clear(X_ALONG, SX::row_of(unit(n, XI)), SX::piece_of(unit(n, XI)), at + unit(n, XI) * 16);
-#pragma unroll
-            for (int n = 0; n < WI; ++n) clear(W_ALONG, SW::row_of(unit(n, WI)), SW::piece_of(unit(n, WI)), at + kX + unit(n, WI) * 16);
-        };
-        uint32_t b = 0, at = base, ahead = base + (STAGES - 1) * kStage;
-        const auto after = [&](uint32_t stage) MINT_INLINE_LAMBDA { return stage + kStage == base + STAGES * kStage ? base : stage + kStage; };
-        const auto bring_all = [&](uint32_t to) MINT_INLINE_LAMBDA {
-#pragma unroll
-            for (int n = 0; n < ALL; ++n) bring(to, n);
-        };
-#pragma unroll
-        for (int st = 0; st < STAGES - 1; ++st) {
-            if ((uint32_t)st < full) bring_all(base + st * kStage);
-            else if ((uint32_t)st == full && full < steps) bring_tail(base + st * kStage);
-        }
-        for (; b + STAGES - 1 < full; ++b) {
-            meet<(STAGES - 2) * ALL>();
-            multiply(at, [&](int n) MINT_INLINE_LAMBDA { bring(ahead, n); });
-            at = after(at);
-            ahead = after(ahead);
-        }
-        for (; b < steps; ++b) {
-            __syncthreads();             // (waits for the loads into LDS too)
-            if (b + STAGES - 1 == full && full < steps) bring_tail(ahead);
-            if (b == full) {
-                clear_tail(at);
-                __syncthreads();
-            }
-            multiply(at, [](int) MINT_INLINE_LAMBDA {});
-            at = after(at);
-            ahead = after(ahead);
-        }
-    } else {
-        u32x4 held[ALL];
-        const auto fetch = [&](uint32_t b) MINT_INLINE_LAMBDA {
-            const uint32_t d0 = (b0 + b) * K;            // (depth that is there from here on)
-            const auto one = [&](const Side& s, bool along, uint32_t first, uint32_t row, uint32_t piece) MINT_INLINE_LAMBDA {
-                if (along)
-                    return piece_of<SIZE>(s.p + (int64_t)min(first + row, s.n - 1) * s.stride + ((int64_t)d0 * SIZE + piece * 16), ((int64_t)a.depth - d0) * SIZE - piece * 16);
-                const int64_t left = ((int64_t)s.n - first) * SIZE - piece * 16;
-                return piece_of<SIZE>(s.p + (int64_t)min(d0 + row, a.depth - 1) * s.stride + ((int64_t)first * SIZE + piece * 16), d0 + row < a.depth ? left : 0);
-            };
-#pragma unroll
-            for (int n = 0; n < XI; ++n) held[n] = one(a.x, X_ALONG, m0, SX::row_of(unit(n, XI)), SX::piece_of(unit(n, XI)));
-#pragma unroll
-            for (int n = 0; n < WI; ++n) held[XI + n] = one(a.w, W_ALONG, n0, SW::row_of(unit(n, WI)), SW::piece_of(unit(n, WI)));
-        };
-        if (steps) fetch(0);
-        for (uint32_t b = 0; b < steps; ++b) {
-            __syncthreads();
-#pragma unroll
-            for (int n = 0; n < XI; ++n) *(MINT_LDS u32x4*)(uintptr_t)(base + unit(n, XI) * 16) = held[n];
-#pragma unroll
-            for (int n = 0; n < WI; ++n) *(MINT_LDS u32x4*)(uintptr_t)(base + kX + unit(n, WI) * 16) = held[XI + n];
-            __syncthreads();
-            if (b + 1 < steps) fetch(b + 1);
-            multiply(base, [](int) MINT_INLINE_LAMBDA {});
-        }
-    }
+    T t(a, m0, n0, part);
+    if constexpr (DIRECT) t.run_direct((LdsBytes)lds);
+    else t.run_held((LdsBytes)lds);
 
     // The sums' way out: a lane has four columns of 16 rows each; through LDS it gets eight of a row, and eight lanes side by side 64.
     __syncthreads();
-    float* const room = reinterpret_cast<float*>(lds) + wave * (SLABS * 16 * PITCH);
-    const uint32_t r16 = lane & 15u, quarter = lane >> 4, col = n0 + wn * 64 + (lane & 7u) * 8;
+    const uint32_t lane = t.lane;
+    float* const room = reinterpret_cast<float*>(lds) + t.wave * (SLABS * 16 * PITCH);
+    const uint32_t r16 = lane & 15u, quarter = lane >> 4, col = n0 + t.wn() * 64 + (lane & 7u) * 8, row0 = m0 + t.wm() * (BM / WM) + (lane >> 3);
+    float bias[8];
+    bias8<DT>(a.f, col, a.w.n, bias);
 #pragma unroll
-    for (int s0 = 0; s0 < MT; s0 += SLABS) {
+    for (int s0 = 0; s0 < T::MT; s0 += SLABS) {
 #pragma unroll
         for (int s = 0; s < (int)SLABS; ++s)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) *reinterpret_cast<f32x4*>(room + (s * 16 + r16) * PITCH + j * 16 + quarter * 4) = acc[s0 + s][j];
+            for (int j = 0; j < T::NT; ++j) *reinterpret_cast<f32x4*>(room + (s * 16 + r16) * PITCH + j * 16 + quarter * 4) = t.acc[s0 + s][j];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        // two rows at a time, so that what they read is asked for together
 #pragma unroll 1
-        for (uint32_t p = 0; p < SLABS * 2; ++p) {
-            const uint32_t in = p * 8 + (lane >> 3), row = m0 + wm * (BM / WM) + s0 * 16 + in;
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(room + in * PITCH + (lane & 7u) * 8), hi = *reinterpret_cast<const f32x4*>(room + in * PITCH + (lane & 7u) * 8 + 4);
-            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            if (row < a.x.n && col < a.w.n) {
-                if (a.parts > 1) store_elements<DT_F32, 8>(a.sums + ((uint64_t)part * a.x.n + row) * a.w.n + col, (int64_t)a.w.n - col, v);
-                else finish8<DT>(a.f, row, col, a.w.n, v);
+        for (uint32_t p = 0; p < SLABS * 2; p += 2) {
+            float more[2][8], v[2][8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t in = (p + u) * 8, row = row0 + s0 * 16 + in;
+                const float* const from = room + (in + (lane >> 3)) * PITCH + (lane & 7u) * 8;
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(from), hi = *reinterpret_cast<const f32x4*>(from + 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][i] = i < 4 ? lo[i & 3] : hi[i & 3];
+                if (a.f.residual && a.parts == 1 && row < a.x.n && col < a.w.n) residual8<DT>(a.f, row, col, a.w.n, more[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t row = row0 + s0 * 16 + (p + u) * 8;
+                if (row >= a.x.n || col >= a.w.n) continue;
+                if (a.parts > 1) store_elements<DT_F32, 8>(a.sums + ((uint64_t)part * a.x.n + row) * a.w.n + col, (int64_t)a.w.n - col, v[u]);
+                else finish8<DT>(a.f, row, col, a.w.n, bias, more[u], v[u]);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -395,7 +553,9 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
     const uint64_t unit = (uint64_t)blockIdx.x * 256 + threadIdx.x;
     const uint32_t row = (uint32_t)(unit / per_row), col = (uint32_t)(unit % per_row) * 8;
     if (row >= a.x.n) return;
-    float sum[8] = {};
+    float sum[8] = {}, bias[8], more[8];
+    bias8<DT>(a.f, col, a.w.n, bias);
+    if (a.f.residual) residual8<DT>(a.f, row, col, a.w.n, more);
     for (uint32_t p0 = 0; p0 < a.parts; p0 += 4) {
         float v[4][8];
 #pragma unroll
@@ -406,7 +566,7 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum[i] += p0 + p < a.parts ? v[p][i] : 0.0f;
     }
-    finish8<DT>(a.f, row, col, a.w.n, sum);
+    finish8<DT>(a.f, row, col, a.w.n, bias, more, sum);
 }
 
 // ---- products of few rows ------------------------------------------------------------
@@ -415,8 +575,8 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
 constexpr int kThinWaves = 8;
 template <int DT, int MT, int KWAYS>
 __global__ void __launch_bounds__(64 * kThinWaves) dense_thin_kernel(DenseArgs a) {
-    constexpr int WAVES = kThinWaves, BM = 16 * MT, BN = 16 * (WAVES / KWAYS), AHEAD = 4;
-    constexpr uint32_t SIZE = kSize<DT>, K = kBlock<DT>;
+    constexpr int WAVES = kThinWaves, BM = 16 * MT, BN = 16 * (WAVES / KWAYS), AHEAD = 8;
+    constexpr uint32_t SIZE = kSize<DT>, K = kHalf<DT>;
     __shared__ __attribute__((aligned(16))) float sums[WAVES][BM][20];
     const uint32_t lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_in_block()), r16 = lane & 15u, part = lane >> 4, way = wave % KWAYS;
     const uint32_t m0 = blockIdx.x / a.col_tiles * BM, n0 = blockIdx.x % a.col_tiles * BN, n = n0 + wave / KWAYS * 16;
@@ -429,33 +589,27 @@ __global__ void __launch_bounds__(64 * kThinWaves) dense_thin_kernel(DenseArgs a
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i] = f32x4{0, 0, 0, 0};
     const auto load = [&](const uint8_t* row, uint32_t b) MINT_INLINE_LAMBDA {
-        Pair<DT> p;
-        const int64_t left = ((int64_t)a.depth - (int64_t)b * K) * SIZE - part * 16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) p.v[h] = piece_of<SIZE>(row + (int64_t)b * 128 + h * 64, left - h * 64);
-        return p;
+        return piece_of<SIZE>(row + (int64_t)b * 64, ((int64_t)a.depth - (int64_t)b * K) * SIZE - part * 16);
     };
     const uint32_t full = a.depth / K;
     uint32_t b = way;
     for (; b + (AHEAD - 1) * KWAYS < full; b += AHEAD * KWAYS) {
-        Pair<DT> wv[AHEAD], xv[AHEAD][MT];
+        u32x4 wv[AHEAD], xv[AHEAD][MT];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            wv[u] = *(MINT_GLOBAL const u32x4_any*)as_global(w + (int64_t)(b + u * KWAYS) * 64);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[u][i] = *(MINT_GLOBAL const u32x4_any*)as_global(x[i] + (int64_t)(b + u * KWAYS) * 64);
+        }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                wv[u].v[h] = *(MINT_GLOBAL const u32x4_any*)as_global(w + (int64_t)(b + u * KWAYS) * 128 + h * 64);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) xv[u][i].v[h] = *(MINT_GLOBAL const u32x4_any*)as_global(x[i] + (int64_t)(b + u * KWAYS) * 128 + h * 64);
-            }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i] = Pair<DT>::multiply(wv[u], xv[u][i], acc[i]);
+            for (int i = 0; i < MT; ++i) acc[i] = multiply_add<DT>(wv[u], xv[u][i], acc[i]);
     }
     for (; b < steps; b += KWAYS) {
-        const Pair<DT> wv = load(w, b);
+        const u32x4 wv = load(w, b);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = Pair<DT>::multiply(wv, load(x[i], b), acc[i]);
+        for (int i = 0; i < MT; ++i) acc[i] = multiply_add<DT>(wv, load(x[i], b), acc[i]);
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(&sums[wave][i * 16 + r16][part * 4]) = acc[i];
@@ -463,12 +617,14 @@ __global__ void __launch_bounds__(64 * kThinWaves) dense_thin_kernel(DenseArgs a
     for (uint32_t at = threadIdx.x; at < BM * BN / 8; at += 64 * WAVES) {
         const uint32_t m = at / (BN / 8), c = at % (BN / 8) * 8;
         if (m0 + m >= a.x.n || n0 + c >= a.w.n) continue;
-        float v[8] = {};
+        float v[8] = {}, bias[8], more[8];
+        bias8<DT>(a.f, n0 + c, a.w.n, bias);
+        if (a.f.residual) residual8<DT>(a.f, m0 + m, n0 + c, a.w.n, more);
 #pragma unroll
         for (int k = 0; k < KWAYS; ++k)
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] += sums[c / 16 * KWAYS + k][m][c % 16 + i];
-        finish8<DT>(a.f, m0 + m, n0 + c, a.w.n, v);
+        finish8<DT>(a.f, m0 + m, n0 + c, a.w.n, bias, more, v);
     }
 }
 
@@ -495,8 +651,9 @@ __global__ void __launch_bounds__(64 * kGradWaves) activation_grad_kernel(Activa
         load8<D>(a.d, (int64_t)row * a.d_stride + col, left, d);
         if (a.z) {
             load8<DT>(a.z, (int64_t)row * a.z_stride + col, left, z);
+            slopes(a.activation, z);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) d[i] *= slope_of(a.activation, z[i]);
+            for (int i = 0; i < 8; ++i) d[i] *= z[i];
         }
         if (a.d_z) store8<DT>(a.d_z, (int64_t)row * a.d_z_stride + col, left, d);
 #pragma unroll
@@ -550,30 +707,33 @@ Choice choose(const mint_dense_op& op) {
 }
 bool direct(const mint_dense_op& op) {
     const int64_t size = size_of(op.dtype);
-    // (a stride is looked at only where there is more than one row)
+    // (a stride is looked at only where there is more than one row; a tile's rows have to be in reach of 32 bits)
+    const int64_t far = 1ll << 23;
     const uint64_t x_rows = op.form == MINT_DENSE_WEIGHT_GRAD ? op.depth : op.rows, w_rows = op.form == MINT_DENSE_PRODUCT ? op.cols : op.depth;
-    return op.x % 16 == 0 && op.w % 16 == 0 && (x_rows <= 1 || op.x_stride * size % 16 == 0) && (w_rows <= 1 || op.w_stride * size % 16 == 0);
+    return op.x % 16 == 0 && op.w % 16 == 0 && (x_rows <= 1 || (op.x_stride * size % 16 == 0 && op.x_stride >= 0 && op.x_stride * size < far)) &&
+           (w_rows <= 1 || (op.w_stride * size % 16 == 0 && op.w_stride >= 0 && op.w_stride * size < far));
 }
-template <int DT, int BM, int BN, int WM, int STAGES, bool X_ALONG, bool W_ALONG, bool DIRECT>
+template <int DT, int BM, int BN, int WM, int NX, int NW, bool X_ALONG, bool W_ALONG, bool DIRECT>
 int go_tiles(DenseArgs a, hipStream_t s) {
     a.row_tiles = (uint32_t)ceil_div(a.x.n, BM);
     a.col_tiles = (uint32_t)ceil_div(a.w.n, BN);
     const uint64_t blocks = ceil_div((uint64_t)a.row_tiles * a.col_tiles * a.parts, 8) * 8;
     if (blocks > 0x7FFFFFFFull / (64 * WM * (BN / 64))) return MINT_ERR_TOO_LARGE;
-    return Launch<&dense_kernel<DT, BM, BN, WM, STAGES, X_ALONG, W_ALONG, DIRECT>>::go((uint32_t)blocks, 64 * WM * (BN / 64), 0, s, a);
+    return Launch<&dense_kernel<DT, BM, BN, WM, NX, NW, X_ALONG, W_ALONG, DIRECT>>::go((uint32_t)blocks, 64 * WM * (BN / 64), 0, s, a);
 }
 template <int DT, bool X_ALONG, bool W_ALONG>
 int go_form(const DenseArgs& a, const Choice& c, bool is_direct, hipStream_t s) {
+    constexpr bool XA = X_ALONG, WA = W_ALONG;
     if (!is_direct) {
-        if (c.tile >= 128) return go_tiles<DT, 128, 128, 4, 1, X_ALONG, W_ALONG, false>(a, s);
-        return go_tiles<DT, 64, 64, 4, 1, X_ALONG, W_ALONG, false>(a, s);
+        if (c.tile >= 128) return go_tiles<DT, 128, 128, 4, XA ? 2 : 4, WA ? 2 : 4, XA, WA, false>(a, s);
+        return go_tiles<DT, 64, 64, 4, XA ? 2 : 4, WA ? 2 : 4, XA, WA, false>(a, s);
     }
     if constexpr (DT != DT_F32) {
-        if (c.tile == 256) return go_tiles<DT, 256, 256, 2, 2, X_ALONG, W_ALONG, true>(a, s);
-        if (c.cols == 256) return go_tiles<DT, 128, 256, 2, 3, X_ALONG, W_ALONG, true>(a, s);
+        if (c.tile == 256) return go_tiles<DT, 256, 256, 2, XA ? 3 : 5, WA ? 2 : XA ? 4 : 5, XA, WA, true>(a, s);
+        if (c.cols == 256) return go_tiles<DT, 128, 256, 2, XA ? 4 : 8, WA ? 3 : 6, XA, WA, true>(a, s);
     }
-    if (c.tile == 128) return go_tiles<DT, 128, 128, 4, 3, X_ALONG, W_ALONG, true>(a, s);
-    return go_tiles<DT, 64, 64, 4, 4, X_ALONG, W_ALONG, true>(a, s);
+    if (c.tile == 128) return go_tiles<DT, 128, 128, 4, XA ? 3 : 5, WA ? 2 : 4, XA, WA, true>(a, s);
+    return go_tiles<DT, 64, 64, 4, XA ? 4 : 8, WA ? 3 : 6, XA, WA, true>(a, s);
 }
 template <int DT, int MT, int KWAYS>
 int go_thin(DenseArgs a, hipStream_t s) {
