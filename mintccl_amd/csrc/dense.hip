@@ -17,17 +17,28 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-// 16 bytes of an operand's row or column, of which four lanes have a block of the depth: as the matrix instructions take them.
+// 16 bytes of an operand's row or column, of which four lanes have a step's part of the depth, as the matrix instructions take them: in 32 bits
+// number T of them, else all.
 template <int DT>
+constexpr int kTurns = DT == DT_F32 ? 4 : 1;
+template <int DT, int T>
 __device__ __forceinline__ f32x4 multiply_add(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (DT == DT_BF16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    } else if constexpr (DT == DT_F16) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    } else {
+    if constexpr (DT == DT_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else if constexpr (DT == DT_F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[T]), __uint_as_float(b[T]), c, 0, 0, 0);
+}
+// c[n] += a[n] b for N sums, one behind the other (those of one sum would wait for each other)
+template <int DT, int N>
+__device__ __forceinline__ void multiply_add(const u32x4 (&a)[N], u32x4 b, f32x4 (&c)[N]) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[t]), __uint_as_float(b[t]), c, 0, 0, 0);
-        return c;
+    for (int n = 0; n < N; ++n) c[n] = multiply_add<DT, 0>(a[n], b, c[n]);
+    if constexpr (kTurns<DT> > 1) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) c[n] = multiply_add<DT, 1>(a[n], b, c[n]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) c[n] = multiply_add<DT, 2>(a[n], b, c[n]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) c[n] = multiply_add<DT, 3>(a[n], b, c[n]);
     }
 }
 template <int DT>
@@ -273,8 +284,7 @@ struct Tile {
     using W = Ring<DT, BN, WAVES, NW, W_ALONG>;
     static constexpr uint32_t kStages = NX * X::BYTES + NW * W::BYTES;
     static constexpr uint32_t SLABS = MT < 4 ? MT : 4, PITCH = 68;        // of the sums' way out: slabs of 16 rows of 64 columns
-    static constexpr uint32_t kOut = WAVES * SLABS * 16 * PITCH * 4, kLds = kStages > kOut ? kStages : kOut;
-    static_assert(kLds <= 160 * 1024, "it fits LDS");
+    static constexpr uint32_t kOut = WAVES * SLABS * 16 * PITCH * 4;
 
     // What is asked for in a step (0: a block's first), x's before w's, and how much of it may be on its way when the step ends.
     static constexpr int asks_x(int step) { return X_ALONG ? (step & 1 ? 0 : X::EACH) : X::EACH; }
@@ -297,19 +307,19 @@ struct Tile {
     static constexpr int x_ahead = X_ALONG ? NX - 1 : NX / 2, w_ahead = W_ALONG ? NW : (NW + 1) / 2, LEAD = x_ahead > w_ahead ? x_ahead : w_ahead;
 
     const DenseArgs& a;
-    uint32_t lane, wave, m0, n0, depth0, depth;
+    uint32_t lane, wave, m0, n0, depth0, depth, blocks;
     typename X::S sx;
     typename W::S sw;
     f32x4 acc[MT][NT];
 
     __device__ __forceinline__ uint32_t wm() const { return wave / WN; }
     __device__ __forceinline__ uint32_t wn() const { return wave % WN; }
-    __device__ __forceinline__ Tile(const DenseArgs& args, uint32_t m, uint32_t n, uint32_t part)
-        : a(args), lane(lane_id()), wave(__builtin_amdgcn_readfirstlane(wave_in_block())), m0(m), n0(n), sx(lane), sw(lane) {
-        // this part's blocks of the depth; the last of all may not be whole
-        const uint32_t blocks = (a.depth + K - 1) / K, share = (blocks + a.parts - 1) / a.parts;
-        depth0 = min(part * share * K, a.depth);
-        depth = min(share * K, a.depth - depth0);
+    // part `part` of `parts`: whole blocks of the depth, as many for each (some may be behind its end); the last of all may not be whole
+    __device__ __forceinline__ Tile(const DenseArgs& args, uint32_t m, uint32_t n, uint32_t part, uint32_t parts)
+        : a(args), lane(lane_id()), wave(__builtin_amdgcn_readfirstlane(wave_in_block()) % WAVES), m0(m), n0(n), sx(lane), sw(lane) {
+        blocks = ((a.depth + K - 1) / K + parts - 1) / parts;
+        depth0 = min(part * blocks * K, a.depth);
+        depth = min(blocks * K, a.depth - depth0);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -318,8 +328,7 @@ struct Tile {
     __device__ __forceinline__ u32x4 load_x(LdsBytes at, int i, uint32_t half) const { return sx.load(at, wm() * MT + i, half); }
     __device__ __forceinline__ u32x4 load_w(LdsBytes at, int j, uint32_t half) const { return sw.load(at, wn() * 4 + j, half); }
     __device__ __forceinline__ void products(int i, const u32x4 (&w)[NT], u32x4 x) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = multiply_add<DT>(w[j], x, acc[i][j]);
+        multiply_add<DT, NT>(w, x, acc[i]);
         __builtin_amdgcn_sched_barrier(0);
     }
     // A step: of the block at x_at with `w`, which has been read.  `before` has w of the step before, which is still wanted for what it left (in `lag`), and
@@ -370,7 +379,7 @@ struct Tile {
         meet();
     }
     __device__ __forceinline__ void run_direct(LdsBytes lds) {
-        const uint32_t blocks = (depth + K - 1) / K, full = depth / K;
+        const uint32_t full = depth / K;
         if (!blocks) return;
         X rx(a.x, m0, depth0, depth, lds, wave, lane);
         W rw(a.w, n0, depth0, depth, lds + NX * X::BYTES, wave, lane);
@@ -450,10 +459,10 @@ struct Tile {
             const auto one = [&](const Side& s, bool along, uint32_t first, uint32_t row, uint32_t piece) MINT_INLINE_LAMBDA {
                 if (along)
                     return ::mint::piece_of<SIZE>(s.p + (int64_t)min(first + row, s.n - 1) * s.stride + ((int64_t)d0 * SIZE + piece * 16),
-                                                  ((int64_t)a.depth - d0) * SIZE - piece * 16);
+                                                  ((int64_t)(depth0 + depth) - d0) * SIZE - piece * 16);
                 const int64_t left = ((int64_t)s.n - first) * SIZE - piece * 16;
                 return ::mint::piece_of<SIZE>(s.p + (int64_t)min(d0 + row, a.depth - 1) * s.stride + ((int64_t)first * SIZE + piece * 16),
-                                              d0 + row < a.depth ? left : 0);
+                                              d0 + row < depth0 + depth ? left : 0);
             };
 #pragma unroll
             for (int n = 0; n < XI; ++n) {
@@ -466,7 +475,6 @@ struct Tile {
                 held[XI + n] = one(a.w, W_ALONG, n0, W::S::row_of(u), W::S::piece_of(u));
             }
         };
-        const uint32_t blocks = (depth + K - 1) / K;
         if (blocks) fetch(0);
 #pragma unroll 1
         for (uint32_t b = 0; b < blocks; ++b) {
@@ -489,12 +497,15 @@ struct Tile {
     }
 };
 
-template <int DT, int BM, int BN, int WM, int NX, int NW, bool X_ALONG, bool W_ALONG, bool DIRECT>
-__global__ void __launch_bounds__(64 * WM * (BN / 64)) dense_kernel(DenseArgs a) {
+// SPLIT sets of wavefronts, each with a part of the depth and LDS of its own, where tiles leave few wavefronts on a compute unit; their sums are
+// added up in LDS, in the parts' order.
+template <int DT, int BM, int BN, int WM, int NX, int NW, int SPLIT, bool X_ALONG, bool W_ALONG, bool DIRECT>
+__global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) dense_kernel(DenseArgs a) {
     using T = Tile<DT, BM, BN, WM, NX, NW, X_ALONG, W_ALONG>;
-    constexpr uint32_t SLABS = T::SLABS, PITCH = T::PITCH;
-    static_assert(DIRECT || 2 * T::kHeld <= T::kLds, "they have room");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[T::kLds];
+    constexpr uint32_t SLABS = T::SLABS, PITCH = T::PITCH, kRoom = DIRECT ? T::kStages : 2 * T::kHeld;
+    constexpr uint32_t kLds = SPLIT * kRoom > T::kOut ? SPLIT * kRoom : T::kOut;
+    static_assert(kLds <= 160 * 1024, "it fits LDS");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
     // The hardware deals thread blocks to the eight XCDs in turn: each takes an eighth of the tiles that lie together, in
     // columns of GROUP row tiles, so that those at work at a time share operands in its L2.
     constexpr uint32_t GROUP = 4;
@@ -503,12 +514,30 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64)) dense_kernel(DenseArgs a)
     const uint32_t all_id = xcd * (total / 8) + min(xcd, total % 8) + nth, id = all_id / a.parts, part = all_id % a.parts;
     const uint32_t group = id / (GROUP * a.col_tiles), in_group = id % (GROUP * a.col_tiles), height = min(GROUP, a.row_tiles - group * GROUP);
     const uint32_t m0 = (group * GROUP + in_group % height) * BM, n0 = in_group / height * BN;
-    T t(a, m0, n0, part);
-    if constexpr (DIRECT) t.run_direct((LdsBytes)lds);
-    else t.run_held((LdsBytes)lds);
+    const uint32_t way = SPLIT > 1 ? (uint32_t)__builtin_amdgcn_readfirstlane(wave_in_block()) / T::WAVES : 0u;
+    T t(a, m0, n0, part * SPLIT + way, a.parts * SPLIT);
+    if constexpr (DIRECT) t.run_direct((LdsBytes)lds + way * kRoom);
+    else t.run_held((LdsBytes)lds + way * kRoom);
+    if constexpr (SPLIT > 1) {
+        static_assert((SPLIT - 1) * BM * BN * 4 <= kLds, "they have room");
+        f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+        __syncthreads();
+        if (way) {
+#pragma unroll
+            for (int n = 0; n < T::MT * T::NT; ++n) sums[(((way - 1) * T::WAVES + t.wave) * T::MT * T::NT + n) * 64 + t.lane] = t.acc[n / T::NT][n % T::NT];
+        }
+        __syncthreads();
+        if (!way) {
+#pragma unroll
+            for (int k = 0; k < SPLIT - 1; ++k)
+#pragma unroll
+                for (int n = 0; n < T::MT * T::NT; ++n) t.acc[n / T::NT][n % T::NT] += sums[((k * T::WAVES + t.wave) * T::MT * T::NT + n) * 64 + t.lane];
+        }
+    }
 
     // The sums' way out: a lane has four columns of 16 rows each; through LDS it gets eight of a row, and eight lanes side by side 64.
     __syncthreads();
+    if (way) return;
     const uint32_t lane = t.lane;
     float* const room = reinterpret_cast<float*>(lds) + t.wave * (SLABS * 16 * PITCH);
     const uint32_t r16 = lane & 15u, quarter = lane >> 4, col = n0 + t.wn() * 64 + (lane & 7u) * 8, row0 = m0 + t.wm() * (BM / WM) + (lane >> 3);
@@ -570,7 +599,7 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
 }
 
 // ---- products of few rows ------------------------------------------------------------
-// Both operands along.  A wavefront has 16 columns and every KWAYS-th block of the depth, straight from memory into registers: it asks for AHEAD
+// Both operands along.  A wavefront has 16 columns and one of KWAYS parts of the depth, straight from memory into registers: it asks for AHEAD
 // blocks before it multiplies the first.  The KWAYS wavefronts' sums of a column are added up in LDS, in their order.
 constexpr int kThinWaves = 8;
 template <int DT, int MT, int KWAYS>
@@ -591,28 +620,31 @@ __global__ void __launch_bounds__(64 * kThinWaves) dense_thin_kernel(DenseArgs a
     const auto load = [&](const uint8_t* row, uint32_t b) MINT_INLINE_LAMBDA {
         return piece_of<SIZE>(row + (int64_t)b * 64, ((int64_t)a.depth - (int64_t)b * K) * SIZE - part * 16);
     };
-    const uint32_t full = a.depth / K;
-    uint32_t b = way;
-    for (; b + (AHEAD - 1) * KWAYS < full; b += AHEAD * KWAYS) {
+    // (a wavefront's are side by side: two of them are a line of memory)
+    const uint32_t share = (steps + KWAYS * 2 - 1) / (KWAYS * 2) * 2, full = a.depth / K, end = min(way * share + share, steps), whole = min(end, full);
+    uint32_t b = way * share;
+    for (; b + AHEAD <= whole; b += AHEAD) {
         u32x4 wv[AHEAD], xv[AHEAD][MT];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            wv[u] = *(MINT_GLOBAL const u32x4_any*)as_global(w + (int64_t)(b + u * KWAYS) * 64);
+            wv[u] = *(MINT_GLOBAL const u32x4_any*)as_global(w + (int64_t)(b + u) * 64);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xv[u][i] = *(MINT_GLOBAL const u32x4_any*)as_global(x[i] + (int64_t)(b + u * KWAYS) * 64);
+            for (int i = 0; i < MT; ++i) xv[u][i] = *(MINT_GLOBAL const u32x4_any*)as_global(x[i] + (int64_t)(b + u) * 64);
         }
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[i] = multiply_add<DT>(wv[u], xv[u][i], acc[i]);
+        for (int u = 0; u < AHEAD; ++u) multiply_add<DT, MT>(xv[u], wv[u], acc);
     }
-    for (; b < steps; b += KWAYS) {
+    for (; b < end; ++b) {
         const u32x4 wv = load(w, b);
+        u32x4 xv[MT];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = multiply_add<DT>(wv, load(x[i], b), acc[i]);
+        for (int i = 0; i < MT; ++i) xv[i] = load(x[i], b);
+        multiply_add<DT, MT>(xv, wv, acc);
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(&sums[wave][i * 16 + r16][part * 4]) = acc[i];
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sums[wave][i * 16 + part * 4 + k][r16] = acc[i][k];
     __syncthreads();
     for (uint32_t at = threadIdx.x; at < BM * BN / 8; at += 64 * WAVES) {
         const uint32_t m = at / (BN / 8), c = at % (BN / 8) * 8;
@@ -689,21 +721,51 @@ bool known(int dtype) { return dtype == MINT_F16 || dtype == MINT_BF16 || dtype 
 constexpr uint64_t kMost = 0x7FFFFFFF - 256;
 uint32_t size_of(int dtype) { return dtype == MINT_F32 ? 4 : 2; }
 
+// Which tiles, and how many thread blocks share one.  What a launch takes by this, us: 2.5, and for each round over the compute units a beginning and an
+// end and so much for a block of the depth (128 bytes); sums that pass through memory take another launch and their bytes. Measured (bf16
+// if not said otherwise, operands used in turn), and the rule's choice behind =:
+//   4096 x 256 x 4096 f32       64 x 64 74, in two sets 76, 128 x 128 134 (two parts)                    = 64 x 64
+//   512 x 4096 x 4096           64 x 64 in two sets 31.7, 128 x 128 in two sets 32.9, in one 37, 128 x 256 47     = 64 x 64 in two sets
+//   1024 x 4096 x 4096          128 x 128 in two sets 35.4, in one 38.4, 128 x 256 47                    = 128 x 128 in two sets
+//   2048 x 4096 x 4096          128 x 256 60, 128 x 128 64, 256 x 256 79                                 = 128 x 256
+//   8192 x 1024 x 512           128 x 128 15.8, 128 x 256 17.2, 256 x 256 22.5                           = 128 x 128
+//   4096 x 4096 x 512 (d_w)     256 x 256 26.4, 128 x 128 28.3, 128 x 256 34                             = 256 x 256
+//   64 x 4096 x 4096            64 x 64 in one part 17.5, two 15.6, four 15.4                            = four
+enum { kThin, k64Four, k64Two, k128, k128Two, k128x256, k256, kHeld64, kHeld128 };
 struct Choice {
-    int tile;                    // 0: few rows; else rows of a tile, and its columns
-    int cols;
+    int tile;
     uint32_t parts;
 };
-Choice choose(const mint_dense_op& op) {
-    const bool along = op.form == MINT_DENSE_PRODUCT;
-    if (along && op.rows <= 32) return {0, 0, 1};
-    const auto tiles = [&](uint64_t bm, uint64_t bn) { return ceil_div(op.rows, bm) * ceil_div(op.cols, bn); };
+struct Cost {
+    int tile;
+    uint32_t rows, cols, round, most;        // tiles of a round; most tiles that it is for
+    float begin, block, block32;             // us; 32-bit operands' (0: not for them)
+};
+constexpr Cost kCosts[] = {{k64Four, 64, 64, 256, 256, 3.5f, 0.22f, 0.53f},   {k64Two, 64, 64, 512, ~0u, 3.5f, 0.42f, 1.02f},
+                           {k128, 128, 128, 256, 256, 4.0f, 0.48f, 1.9f},     {k128, 128, 128, 512, ~0u, 6.0f, 0.89f, 3.65f},
+                           {k128Two, 128, 128, 256, 256, 6.0f, 0.39f, 1.9f},  {k128x256, 128, 256, 256, ~0u, 7.5f, 0.78f, 0.0f},
+                           {k256, 256, 256, 128, 128, 10.5f, 1.03f, 0.0f},    {k256, 256, 256, 256, ~0u, 10.5f, 1.34f, 0.0f}};
+constexpr Cost kHeldCosts[] = {{kHeld64, 64, 64, 512, ~0u, 3.5f, 0.8f, 1.3f}, {kHeld128, 128, 128, 512, ~0u, 6.0f, 1.8f, 4.5f}};
+template <int N>
+Choice cheapest(const Cost (&costs)[N], const mint_dense_op& op) {
     const uint64_t blocks = ceil_div(op.depth * size_of(op.dtype), 128);
-    const auto parts = [&](uint64_t n) { return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(256 / std::max<uint64_t>(n, 1), blocks / 8)); };
-    if (op.dtype != MINT_F32 && tiles(256, 256) >= 200) return {256, 256, 1};
-    if (op.dtype != MINT_F32 && tiles(128, 256) >= 200) return {128, 256, 1};
-    if (tiles(128, 128) >= 100) return {128, 128, parts(tiles(128, 128))};
-    return {64, 64, parts(tiles(64, 64))};
+    Choice best = {costs[0].tile, 1};
+    float least = 1e30f;
+    for (const Cost& c : costs) {
+        const float block = op.dtype == MINT_F32 ? c.block32 : c.block;
+        const uint64_t tiles = ceil_div(op.rows, c.rows) * ceil_div(op.cols, c.cols);
+        if (block == 0.0f || tiles > c.most) continue;
+        const uint64_t most = tiles >= c.round ? 1 : std::min<uint64_t>(c.round / tiles, std::max<uint64_t>(blocks / 8, 1));
+        for (uint64_t parts = 1; parts <= most; ++parts) {
+            float t = (float)ceil_div(tiles * parts, c.round) * (c.begin + (float)ceil_div(blocks, parts) * block);
+            if (parts > 1) t += 2.5f + (float)(op.rows * op.cols) * (float)parts * (8.0f / 4.5e6f);
+            if (t < least) {
+                least = t;
+                best = {c.tile, (uint32_t)parts};
+            }
+        }
+    }
+    return best;
 }
 bool direct(const mint_dense_op& op) {
     const int64_t size = size_of(op.dtype);
@@ -713,27 +775,33 @@ bool direct(const mint_dense_op& op) {
     return op.x % 16 == 0 && op.w % 16 == 0 && (x_rows <= 1 || (op.x_stride * size % 16 == 0 && op.x_stride >= 0 && op.x_stride * size < far)) &&
            (w_rows <= 1 || (op.w_stride * size % 16 == 0 && op.w_stride >= 0 && op.w_stride * size < far));
 }
-template <int DT, int BM, int BN, int WM, int NX, int NW, bool X_ALONG, bool W_ALONG, bool DIRECT>
+Choice choose(const mint_dense_op& op) {
+    if (op.form == MINT_DENSE_PRODUCT && op.rows <= 32) return {kThin, 1};
+    return direct(op) ? cheapest(kCosts, op) : cheapest(kHeldCosts, op);
+}
+template <int DT, int BM, int BN, int WM, int NX, int NW, int SPLIT, bool X_ALONG, bool W_ALONG, bool DIRECT>
 int go_tiles(DenseArgs a, hipStream_t s) {
     a.row_tiles = (uint32_t)ceil_div(a.x.n, BM);
     a.col_tiles = (uint32_t)ceil_div(a.w.n, BN);
     const uint64_t blocks = ceil_div((uint64_t)a.row_tiles * a.col_tiles * a.parts, 8) * 8;
-    if (blocks > 0x7FFFFFFFull / (64 * WM * (BN / 64))) return MINT_ERR_TOO_LARGE;
-    return Launch<&dense_kernel<DT, BM, BN, WM, NX, NW, X_ALONG, W_ALONG, DIRECT>>::go((uint32_t)blocks, 64 * WM * (BN / 64), 0, s, a);
+    if (blocks > 0x7FFFFFFFull / (64 * WM * (BN / 64) * SPLIT)) return MINT_ERR_TOO_LARGE;
+    return Launch<&dense_kernel<DT, BM, BN, WM, NX, NW, SPLIT, X_ALONG, W_ALONG, DIRECT>>::go((uint32_t)blocks, 64 * WM * (BN / 64) * SPLIT, 0, s, a);
 }
-template <int DT, bool X_ALONG, bool W_ALONG>
-int go_form(const DenseArgs& a, const Choice& c, bool is_direct, hipStream_t s) {
-    constexpr bool XA = X_ALONG, WA = W_ALONG;
-    if (!is_direct) {
-        if (c.tile >= 128) return go_tiles<DT, 128, 128, 4, XA ? 2 : 4, WA ? 2 : 4, XA, WA, false>(a, s);
-        return go_tiles<DT, 64, 64, 4, XA ? 2 : 4, WA ? 2 : 4, XA, WA, false>(a, s);
-    }
+template <int DT, bool XA, bool WA>
+int go_form(const DenseArgs& a, int tile, hipStream_t s) {
+    constexpr int X2 = XA ? 2 : 4, X3 = XA ? 3 : 5, W2 = WA ? 2 : 4;
     if constexpr (DT != DT_F32) {
-        if (c.tile == 256) return go_tiles<DT, 256, 256, 2, XA ? 3 : 5, WA ? 2 : XA ? 4 : 5, XA, WA, true>(a, s);
-        if (c.cols == 256) return go_tiles<DT, 128, 256, 2, XA ? 4 : 8, WA ? 3 : 6, XA, WA, true>(a, s);
+        if (tile == k256) return go_tiles<DT, 256, 256, 2, X3, XA == WA && !XA ? 5 : W2, 1, XA, WA, true>(a, s);
+        if (tile == k128x256) return go_tiles<DT, 128, 256, 2, XA ? 4 : 8, WA ? 3 : 6, 1, XA, WA, true>(a, s);
     }
-    if (c.tile == 128) return go_tiles<DT, 128, 128, 4, XA ? 3 : 5, WA ? 2 : 4, XA, WA, true>(a, s);
-    return go_tiles<DT, 64, 64, 4, XA ? 4 : 8, WA ? 3 : 6, XA, WA, true>(a, s);
+    switch (tile) {
+        case kHeld64: return go_tiles<DT, 64, 64, 4, X2, W2, 2, XA, WA, false>(a, s);
+        case kHeld128: return go_tiles<DT, 128, 128, 4, X2, W2, 1, XA, WA, false>(a, s);
+        case k64Four: return go_tiles<DT, 64, 64, 2, X2, W2, 4, XA, WA, true>(a, s);
+        case k64Two: return go_tiles<DT, 64, 64, 2, X2, W2, 2, XA, WA, true>(a, s);
+        case k128Two: return go_tiles<DT, 128, 128, 2, X2, W2, 2, XA, WA, true>(a, s);
+        default: return go_tiles<DT, 128, 128, 4, X3, W2, 1, XA, WA, true>(a, s);
+    }
 }
 template <int DT, int MT, int KWAYS>
 int go_thin(DenseArgs a, hipStream_t s) {
@@ -744,17 +812,16 @@ int go_thin(DenseArgs a, hipStream_t s) {
 }
 template <int DT>
 int go_dense(const mint_dense_op& op, const DenseArgs& a, const Choice& c, hipStream_t s) {
-    if (c.tile == 0) {
+    if (c.tile == kThin) {
         const bool few = ceil_div(op.cols, 16) <= 768;
         if (op.rows <= 16) return few ? go_thin<DT, 1, 8>(a, s) : go_thin<DT, 1, 2>(a, s);
         return few ? go_thin<DT, 2, 8>(a, s) : go_thin<DT, 2, 2>(a, s);
     }
-    const bool is_direct = direct(op);
     int err;
     switch (op.form) {
-        case MINT_DENSE_PRODUCT: err = go_form<DT, true, true>(a, c, is_direct, s); break;
-        case MINT_DENSE_INPUT_GRAD: err = go_form<DT, true, false>(a, c, is_direct, s); break;
-        default: err = go_form<DT, false, false>(a, c, is_direct, s); break;
+        case MINT_DENSE_PRODUCT: err = go_form<DT, true, true>(a, c.tile, s); break;
+        case MINT_DENSE_INPUT_GRAD: err = go_form<DT, true, false>(a, c.tile, s); break;
+        default: err = go_form<DT, false, false>(a, c.tile, s); break;
     }
     if (err != MINT_OK || a.parts == 1) return err;
     const uint64_t blocks = ceil_div((uint64_t)a.x.n * ceil_div(a.w.n, 8), 256);
