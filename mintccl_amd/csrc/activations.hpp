@@ -14,6 +14,12 @@ __device__ __forceinline__ float exponential(float x) {
 }
 __device__ __forceinline__ float reciprocal(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ __forceinline__ float logistic(float x) { return reciprocal(1.0f + exponential(-x)); }
+// Near 0, where 1 - 2 / (1 + e^2x) cancels, the first terms of its series: x^11 is less than 2^-29 of x there.
+__device__ __forceinline__ float tangent(float x) {
+    const float s = x * x, near = x * fmaf(fmaf(fmaf(fmaf(0.0218694885f, s, -0.0539682540f), s, 0.133333333f), s, -0.333333333f), s, 1.0f);
+    const float far = copysignf(1.0f - 2.0f * reciprocal(1.0f + exponential(2.0f * fabsf(x))), x);
+    return fabsf(x) < 0.25f ? near : far;
+}
 // P(N > x) of a normal N for x >= 0: Abramowitz and Stegun, 7.1.26 (1.5e-7 off at most, for twice of it), with e^(-x^2 / 2) as `power`.
 __device__ __forceinline__ float normal_above(float x, float power) {
     const float t = reciprocal(fmaf(0.3275911f * 0.70710678f, x, 1.0f));
@@ -39,7 +45,7 @@ __device__ __forceinline__ void activate(int kind, float (&v)[N]) {
             break;
         case MINT_ACT_TANH:
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = tanhf(v[i]);
+            for (int i = 0; i < N; ++i) v[i] = tangent(v[i]);
             break;
         case MINT_ACT_GELU:
 #pragma unroll
@@ -80,7 +86,7 @@ __device__ __forceinline__ void slopes(int kind, float (&v)[N]) {
         case MINT_ACT_TANH:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float t = tanhf(v[i]);
+                const float t = tangent(v[i]);
                 v[i] = 1.0f - t * t;
             }
             break;
@@ -110,13 +116,13 @@ inline bool activation_known(int kind) { return kind >= MINT_ACT_NONE && kind <=
 // Of a gate: none, sigmoid, tanh or silu, in as little code as that takes (it stands in many kernels).
 __device__ __forceinline__ float gate_value(int kind, float g) {
     if (kind == MINT_ACT_NONE) return g;
-    if (kind == MINT_ACT_TANH) return tanhf(g);
+    if (kind == MINT_ACT_TANH) return tangent(g);
     return logistic(g) * (kind == MINT_ACT_SILU ? g : 1.0f);
 }
 __device__ __forceinline__ float gate_slope(int kind, float g) {
     if (kind == MINT_ACT_NONE) return 1.0f;
     if (kind == MINT_ACT_TANH) {
-        const float t = tanhf(g);
+        const float t = tangent(g);
         return 1.0f - t * t;
     }
     const float e = exponential(-fabsf(g)), r = reciprocal(1.0f + e), s = (g < 0.0f ? e : 1.0f) * r, slope = e * r * r;

@@ -14,27 +14,39 @@ struct ColumnSumsArgs {
     int gate_dtype, gate_by;
     bool block, bias;
 };
-// A thread block has 64 columns, and a wavefront every 16th group's sums of them.
+// A thread block has 16 columns, and 16 lanes every 64th group's sums of them.  512 groups of two sums of 4096: 6 us.
 constexpr int kColumnWaves = 16;
 __global__ void __launch_bounds__(64 * kColumnWaves) column_sums_kernel(ColumnSumsArgs a) {
-    __shared__ float part[4][kColumnWaves][64];
-    const uint32_t col = blockIdx.x * 64 + lane_id(), wave = wave_in_block(), from = min(col, a.width - 1);
+    __shared__ float part[4][kColumnWaves * 4][16];
+    const uint32_t lane = threadIdx.x & 15u, slot = threadIdx.x >> 4, col = blockIdx.x * 16 + lane, from = min(col, a.width - 1);
+    constexpr uint32_t SLOTS = kColumnWaves * 4;
     for (uint32_t k = 0; k < a.n; ++k) {
         float sum = 0.0f;
-        for (uint32_t g0 = wave; g0 < a.groups; g0 += kColumnWaves * 8) {
+        for (uint32_t g0 = slot; g0 < a.groups; g0 += SLOTS * 8) {
             float v[8];
 #pragma unroll
-            for (uint32_t u = 0; u < 8; ++u) v[u] = *as_global(a.sums + ((uint64_t)min(g0 + u * kColumnWaves, a.groups - 1) * a.n + k) * a.width + from);
+            for (uint32_t u = 0; u < 8; ++u) v[u] = *as_global(a.sums + ((uint64_t)min(g0 + u * SLOTS, a.groups - 1) * a.n + k) * a.width + from);
 #pragma unroll
-            for (uint32_t u = 0; u < 8; ++u) sum += g0 + u * kColumnWaves < a.groups ? v[u] : 0.0f;
+            for (uint32_t u = 0; u < 8; ++u) sum += g0 + u * SLOTS < a.groups ? v[u] : 0.0f;
         }
-        part[k][wave][lane_id()] = sum;
+        part[k][slot][lane] = sum;
     }
     __syncthreads();
-    if (wave != 0 || col >= a.width) return;
+    // 64 slots, 16 at a time
+    if (slot < 4) {
+        for (uint32_t k = 0; k < a.n; ++k) {
+            float sum = 0.0f;
+#pragma unroll
+            for (uint32_t u = 0; u < 16; ++u) sum += part[k][slot * 16 + u][lane];
+            part[k][slot * 16][lane] = sum;
+        }
+    }
+    __syncthreads();
+    if (slot != 0 || col >= a.width) return;
     float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t k = 0; k < a.n; ++k)
-        for (int w = 0; w < kColumnWaves; ++w) total[k] += part[k][w][lane_id()];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+        if (k < a.n) total[k] = (part[k][0][lane] + part[k][16][lane]) + (part[k][32][lane] + part[k][48][lane]);
     if (a.before_weight) store_one(a.before_weight, a.before.dtype, col, total[0]);
     if (a.before_bias) store_one(a.before_bias, a.before.dtype, col, total[1]);
     if (!a.block) return;
@@ -49,11 +61,7 @@ __global__ void __launch_bounds__(64 * kColumnWaves) column_sums_kernel(ColumnSu
     }
 }
 
-// groups: as many as are at work together, of not more than a fixed number, so that a sum over rows has the same order everywhere
-uint32_t groups_of(uint64_t rows, uint64_t width) {
-    const uint64_t most = width <= 128 * V ? 2048 : width <= 512 * V ? 1024 : width <= 1024 * V ? 512 : 256;
-    return (uint32_t)std::min(rows, most);
-}
+// ---- the entry points --------------------------------------------------------------
 // the types that go together: the stream is of the block's type, or in 32 bits
 #define MINT_STREAM_TYPES(GO, ...)                                                                                          \
     switch (op->dtype) {                                                                                                    \
@@ -95,8 +103,8 @@ extern "C" int mint_join(const mint_join_op* op, void* stream) {
     if (const int err = join_args(op, a)) return err;
     if (a.rows == 0 || a.width == 0) return MINT_OK;
     if (!a.stream || (a.y && !a.new_stream) || (a.next && !a.before.kind) || (!a.y && !a.next)) return MINT_ERR_ARG;
-    // (a launch has fewer than 2^32 threads)
-    if ((uint64_t)a.rows * (a.width <= 128 * V ? 64 : a.width <= 512 * V ? 256 : 1024) > 0xFFFFFF00ull) return MINT_ERR_TOO_LARGE;
+    // (a launch has fewer than 2^32 threads; the others' thread blocks have many rows)
+    if (a.width > kLongest && (uint64_t)a.rows * kLongThreads > 0xFFFFFF00ull) return MINT_ERR_TOO_LARGE;
     const auto s = static_cast<hipStream_t>(stream);
     MINT_STREAM_TYPES(launch_join, a, s)
 }
@@ -110,7 +118,7 @@ bool grad_sums(const mint_join_grad_op& op) {
 uint64_t grad_workspace(const mint_join_grad_op& op) {
     if (!grad_sums(op) || op.join.rows == 0) return 0;
     const uint64_t n = (op.join.y ? 2 : 1) * (grad_bias(op.join) ? 2 : 1);
-    return groups_of(op.join.rows, op.join.width) * n * op.join.width * 4;
+    return blocks_of(op.join.rows, op.join.width) * n * op.join.width * 4;
 }
 }  // namespace
 
@@ -142,7 +150,7 @@ extern "C" int mint_join_grad(const mint_join_grad_op* op_grad, void* stream) {
     a.to_y_stride = op_grad->to_y_stride;
     a.to_gate_stride = op_grad->to_gate_stride;
     a.sums = need ? reinterpret_cast<float*>(op_grad->workspace) : nullptr;
-    a.groups = groups_of(a.f.rows, a.f.width);
+    a.groups = blocks_of(a.f.rows, a.f.width);
     const bool bias = grad_bias(*op), by_channel = a.f.gate && a.f.gate_form == MINT_GATE_CHANNEL;
     const auto s = static_cast<hipStream_t>(stream);
     const auto rows = [&]() -> int { MINT_STREAM_TYPES(launch_join_grad, a, bias, s) };
@@ -156,5 +164,5 @@ extern "C" int mint_join_grad(const mint_join_grad_op* op_grad, void* stream) {
                               reinterpret_cast<void*>(op_grad->to_after_weight), reinterpret_cast<void*>(op_grad->to_after_bias),
                               by_channel ? a.to_gate : nullptr, by_channel ? a.f.gate : nullptr, a.f.before, a.f.after, a.f.rows ? a.groups : 0u, a.f.width,
                               a.f.rows ? (a.f.y ? 2u : 1u) * (bias ? 2u : 1u) : 0u, a.f.gate_dtype, a.f.gate_by, a.f.y != nullptr || !a.f.rows, bias};
-    return Launch<&column_sums_kernel>::go((uint32_t)ceil_div(a.f.width, 64), 64 * kColumnWaves, 0, s, c);
+    return Launch<&column_sums_kernel>::go((uint32_t)ceil_div(a.f.width, 16), 64 * kColumnWaves, 0, s, c);
 }

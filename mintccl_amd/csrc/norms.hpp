@@ -87,39 +87,35 @@ struct RowSums {
     }
 };
 
-// Of a row in registers: C times V numbers of a lane, LANES lanes side by side.  What lies behind the row's end is zero, and stays.
-template <int LANES, int C>
+// Of a row in registers: V numbers of a lane, LANES lanes side by side.  What lies behind the row's end is zero, and stays.  WHOLE: a lane has all of its
+// numbers or none (ends inside a lane's numbers cost registers, which the kernels that hold most of them do not have).
+template <int LANES, bool WHOLE>
 struct RowOf {
-    uint32_t width, lane;
-    __device__ __forceinline__ uint32_t at(int c) const { return ((uint32_t)c * LANES + lane) * V; }
-    __device__ __forceinline__ int64_t left(int c) const { return (int64_t)width - at(c); }
+    uint32_t width, at;
+    int64_t left;
+    __device__ __forceinline__ RowOf(uint32_t w, uint32_t lane)
+        : width(w), at(lane * V), left(WHOLE ? (lane * V < w ? V : 0) : (int64_t)w - lane * V) {}
     // takes the mean off, but not off what is not there
-    __device__ __forceinline__ void centre(float (&x)[C][V], float mean) const {
+    __device__ __forceinline__ void centre(float (&x)[V], float mean) const {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < V; ++i) x[c][i] = i < left(c) ? x[c][i] - mean : 0.0f;
+        for (int i = 0; i < V; ++i) x[i] = i < left ? x[i] - mean : 0.0f;
     }
-    static __device__ __forceinline__ float sum(const float (&x)[C][V]) {
+    static __device__ __forceinline__ float sum(const float (&x)[V]) {
         float s = 0.0f;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < V; ++i) s += x[c][i];
+        for (int i = 0; i < V; ++i) s += x[i];
         return s;
     }
-    static __device__ __forceinline__ float dot(const float (&x)[C][V], const float (&y)[C][V]) {
+    static __device__ __forceinline__ float dot(const float (&x)[V], const float (&y)[V]) {
         float s = 0.0f;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < V; ++i) s = fmaf(x[c][i], y[c][i], s);
+        for (int i = 0; i < V; ++i) s = fmaf(x[i], y[i], s);
         return s;
     }
 };
 // x becomes (x - m) q; q comes back
-template <int LANES, int C, typename Sums>
-__device__ __forceinline__ float normalise(const RowOf<LANES, C>& row, const NormArgs& n, float (&x)[C][V], Sums& sums) {
+template <int LANES, bool WHOLE, typename Sums>
+__device__ __forceinline__ float normalise(const RowOf<LANES, WHOLE>& row, const NormArgs& n, float (&x)[V], Sums& sums) {
     const float share = 1.0f / (float)row.width;
     if (n.kind == MINT_NORM_LAYER) {
         float mean[1] = {row.sum(x)};
@@ -130,12 +126,10 @@ __device__ __forceinline__ float normalise(const RowOf<LANES, C>& row, const Nor
     sums(square);
     const float q = 1.0f / sqrtf(fmaf(square[0], share, n.eps));
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[c][i] *= q;
+    for (int i = 0; i < V; ++i) x[i] *= q;
     return q;
 }
-// the weight's (or bias's) numbers of chunk c
+// a lane's numbers of the weight, of the bias
 __device__ __forceinline__ void weight_of(const NormArgs& n, uint32_t at, int64_t left, float (&w)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) w[i] = 1.0f;
@@ -146,7 +140,7 @@ __device__ __forceinline__ void bias_of(const NormArgs& n, uint32_t at, int64_t 
     for (int i = 0; i < V; ++i) b[i] = 0.0f;
     if (n.bias) load_any(n.bias, n.dtype, at, left, b);
 }
-// a row's gate for chunk c, as it was given (ones where there is none)
+// a lane's numbers of a row's gate, as it was given (ones where there is none)
 __device__ __forceinline__ void gate_of(const JoinArgs& a, uint64_t row, uint32_t at, int64_t left, float (&g)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) g[i] = 1.0f;
@@ -160,53 +154,107 @@ __device__ __forceinline__ void gate_of(const JoinArgs& a, uint64_t row, uint32_
     }
 }
 
-// S: the stream's type, T: that of y and of h.
-template <int S, int T, int LANES, int C>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) join_kernel(JoinArgs a) {
-    using TS = typename Elem<S>::type;
-    using TT = typename Elem<T>::type;
-    constexpr int WAVES = LANES / 64, ROWS = LANES < 256 ? 256 / LANES : 1;
-    static_assert(WAVES == 1 || ROWS == 1, "wavefronts that meet have the same row");
-    __shared__ float slots[2][WAVES][1];
-    const uint64_t r = (uint64_t)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / LANES : 0u);
-    if (r >= a.rows) return;
-    const RowOf<LANES, C> row = {a.width, threadIdx.x % LANES};
-    RowSums<WAVES, 1> sums = {slots};
-    float s[C][V];
+// V numbers as they are in memory, zeros behind the `left` first: what is on its way while the row before is worked on.
+template <int DT>
+struct Raw {
+    using T = typename Elem<DT>::type;
+    static constexpr int WORDS = V * (int)sizeof(T) / 4;
+    typedef uint32_t words __attribute__((ext_vector_type(WORDS), aligned(sizeof(T))));
+    typedef T numbers __attribute__((ext_vector_type(V)));
+    uint32_t v[WORDS];           // (words: numbers of 16 bits would take a register each)
+    // (where the row is, the same for all, apart from the lane's place in it: the address takes one register)
+    __device__ __forceinline__ void load(const void* p, int64_t row, uint32_t at, int64_t left) {
+        const T* const from = static_cast<const T*>(p) + row + at;
+        if (left >= V) {
+            const words w = *(MINT_GLOBAL const words*)as_global(from);
 #pragma unroll
-    for (int c = 0; c < C; ++c) load_elements<S, V>(static_cast<const TS*>(a.stream) + (int64_t)r * a.stream_stride + row.at(c), row.left(c), s[c]);
-    if (a.y) {
-        float y[C][V];
+            for (int i = 0; i < WORDS; ++i) v[i] = w[i];
+        } else {
 #pragma unroll
-        for (int c = 0; c < C; ++c) load_elements<T, V>(static_cast<const TT*>(a.y) + (int64_t)r * a.y_stride + row.at(c), row.left(c), y[c]);
-        if (a.after.kind) normalise(row, a.after, y, sums);
+            for (int i = 0; i < WORDS; ++i) v[i] = 0u;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (row.left(c) <= 0) continue;
-            float w[V], b[V], g[V];
-            weight_of(a.after, row.at(c), row.left(c), w);
-            bias_of(a.after, row.at(c), row.left(c), b);
-            gate_of(a, r, row.at(c), row.left(c), g);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float u = fmaf(y[c][i], w[i], b[i]) * (a.gate ? gate_value(a.gate_by, g[i]) : 1.0f);
-                // (as it is stored: what the next norm is of)
-                s[c][i] = i < row.left(c) ? Elem<S>::load(Elem<S>::round(fmaf(a.scale, u, a.carry * s[c][i]))) : 0.0f;
-            }
-            store_elements<S, V>(static_cast<TS*>(a.new_stream) + (int64_t)r * a.new_stride + row.at(c), row.left(c), s[c]);
+            for (int i = 0; i < V; ++i)
+                if (i < left) {
+                    if constexpr (sizeof(T) == 4) v[i] = *(MINT_GLOBAL const uint32_t*)as_global(from + i);
+                    else v[i / 2] |= (uint32_t)*(MINT_GLOBAL const uint16_t*)as_global(from + i) << (i % 2 * 16);
+                }
         }
     }
-    if (!a.next) return;
-    normalise(row, a.before, s, sums);
+    __device__ __forceinline__ void get(float (&x)[V]) const {
+        typedef uint32_t whole __attribute__((ext_vector_type(WORDS)));
+        whole w;
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        if (row.left(c) <= 0) continue;
-        float w[V], b[V];
-        weight_of(a.before, row.at(c), row.left(c), w);
-        bias_of(a.before, row.at(c), row.left(c), b);
+        for (int i = 0; i < WORDS; ++i) w[i] = v[i];
+        const numbers n = __builtin_bit_cast(numbers, w);
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[c][i] = fmaf(s[c][i], w[i], b[i]);
-        store_elements<T, V>(static_cast<TT*>(a.next) + (int64_t)r * a.next_stride + row.at(c), row.left(c), s[c]);
+        for (int i = 0; i < V; ++i) x[i] = Elem<DT>::load(n[i]);
+    }
+};
+constexpr int threads_of(int lanes) { return lanes == 64 ? 256 : lanes; }         // four rows to a thread block, or one
+constexpr int rows_of(int lanes) { return lanes == 64 ? 4 : 1; }
+
+// S: the stream's type, T: that of y and of h.  LANES lanes have every groups-th row, of which the next one is on its way while one is worked on;
+// the weights stay in registers.  Bound by memory: 16384 x 4096 bf16 with a gate by channel 104 us
+// (5.2 TB/s; rows one by one, the weights read again for each, 134), 8192 x 8192 with the stream in 32 bits 164 (4.9).
+template <int S, int T, int LANES, bool WHOLE>
+__global__ void __launch_bounds__(threads_of(LANES)) join_kernel(JoinArgs a) {
+    using TS = typename Elem<S>::type;
+    using TT = typename Elem<T>::type;
+    constexpr int WAVES = LANES / 64, ROWS = rows_of(LANES);
+    __shared__ float slots[2][WAVES][1];
+    const uint32_t groups = gridDim.x * ROWS, first = blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / LANES : 0u);
+    if (first >= a.rows) return;
+    const RowOf<LANES, WHOLE> row(a.width, threadIdx.x % LANES);
+    const uint32_t at = row.at;
+    const int64_t left = row.left;
+    RowSums<WAVES, 1> sums = {slots};
+    const bool one_by_one = a.gate && a.gate_form != MINT_GATE_CHANNEL;
+    // u's weight and bias with the scale and a gate by channel in them
+    float wa[V], ba[V], wb[V], bb[V], open[V];
+    weight_of(a.after, at, left, wa);
+    bias_of(a.after, at, left, ba);
+    weight_of(a.before, at, left, wb);
+    bias_of(a.before, at, left, bb);
+    if (!one_by_one) gate_of(a, 0, at, left, open);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float all = a.scale * (a.gate && !one_by_one ? gate_value(a.gate_by, open[i]) : 1.0f);
+        wa[i] *= all;
+        ba[i] *= all;
+    }
+    Raw<S> next_s;
+    Raw<T> next_y;
+    const auto ask = [&](uint32_t r) MINT_INLINE_LAMBDA {
+        next_s.load(a.stream, (int64_t)r * a.stream_stride, at, left);
+        if (a.y) next_y.load(a.y, (int64_t)r * a.y_stride, at, left);
+    };
+    ask(first);
+    for (uint64_t r = first; r < a.rows; r += groups) {
+        float s[V], y[V];
+        next_s.get(s);
+        if (a.y) next_y.get(y);
+        if (r + groups < a.rows) ask((uint32_t)(r + groups));
+        if (a.y) {
+            if (a.after.kind) normalise(row, a.after, y, sums);
+            if (one_by_one) {
+                gate_of(a, r, at, left, open);
+#pragma unroll
+                for (int i = 0; i < V; ++i) open[i] = gate_value(a.gate_by, open[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float u = fmaf(y[i], wa[i], ba[i]);
+                const float sum = one_by_one ? fmaf(open[i], u, a.carry * s[i]) : fmaf(a.carry, s[i], u);
+                // (as it is stored: what the next norm is of)
+                s[i] = i < left ? Elem<S>::load(Elem<S>::round(sum)) : 0.0f;
+            }
+            if (left > 0) store_elements<S, V>(static_cast<TS*>(a.new_stream) + (int64_t)r * a.new_stride + at, left, s);
+        }
+        if (!a.next) continue;
+        normalise(row, a.before, s, sums);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] = fmaf(s[i], wb[i], bb[i]);
+        if (left > 0) store_elements<T, V>(static_cast<TT*>(a.next) + (int64_t)r * a.next_stride + at, left, s);
     }
 }
 
@@ -215,134 +263,223 @@ struct JoinGradArgs {
     const void *d_stream, *d_next;              // either may be 0
     void *to_stream, *to_y, *to_gate;
     int64_t d_stream_stride, d_next_stride, to_stream_stride, to_y_stride, to_gate_stride;
-    float* sums;                                // (groups, SUMS, width): each group's sums over its rows
-    uint32_t groups;
+    float* sums;                                // (groups, SUMS, width): each thread block's sums over its rows
+    uint32_t groups;                            // thread blocks
 };
 // Which of a group's sums over rows are where: before's weight, [its bias,] [after's weight, [its bias]].
 template <bool BLOCK, bool BIAS>
 constexpr int kSums = (BLOCK ? 2 : 1) * (BIAS ? 2 : 1);
 
-// A group of LANES lanes has every groups-th row and keeps its sums over them in registers.
-template <int S, int T, int LANES, int C, bool BLOCK, bool BIAS>
-__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) join_grad_kernel(JoinGradArgs a) {
+// LANES lanes have every groups-th row; the weights stay in registers, and up to 4096 numbers so do the sums over their rows, while the next row is on its
+// way (AHEAD); a thread block of 1024 has the sums in LDS.
+// Bound by memory, and by three meetings for a row: 16384 x 4096 bf16 with a gate by channel 186 us, 4.3 TB/s
+// (twice eight numbers to a lane, half as many wavefronts, nothing held or ahead: 397), 8192 x 8192 with the stream in 32 bits and a gate by row 277, 4.4.
+template <int S, int T, int LANES, bool WHOLE, bool BLOCK, bool BIAS, int GATE>      // GATE: 0 (none, or by channel), MINT_GATE_ROW, MINT_GATE_ALL
+__global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradArgs a) {
     using TS = typename Elem<S>::type;
     using TT = typename Elem<T>::type;
-    constexpr int WAVES = LANES / 64, GROUPS = LANES < 256 ? 256 / LANES : 1, SUMS = kSums<BLOCK, BIAS>;
+    constexpr int WAVES = LANES / 64, ROWS = rows_of(LANES), SUMS = kSums<BLOCK, BIAS>;
+    constexpr bool AHEAD = LANES < 1024;
     __shared__ float slots[2][WAVES][3];
-    const uint32_t group = blockIdx.x * GROUPS + (GROUPS > 1 ? threadIdx.x / LANES : 0u);
-    if (group >= a.groups) return;
+    __shared__ __attribute__((aligned(16))) float joined[!AHEAD ? SUMS * LANES * V : ROWS > 1 ? (ROWS - 1) * SUMS * LANES * V : 1];
+    const uint32_t groups = gridDim.x * ROWS, nth = ROWS > 1 ? threadIdx.x / LANES : 0u;
     const JoinArgs& f = a.f;
-    const RowOf<LANES, C> row = {f.width, threadIdx.x % LANES};
+    const uint32_t lane = threadIdx.x % LANES;
+    const RowOf<LANES, WHOLE> row(f.width, lane);
+    const uint32_t at = row.at;
+    const int64_t left = row.left;
     RowSums<WAVES, 3> sums = {slots};
     const float share = 1.0f / (float)f.width;
-    const bool by_row = f.gate && f.gate_form == MINT_GATE_ROW, by_channel = f.gate && f.gate_form == MINT_GATE_CHANNEL;
-    float total[SUMS][C][V];
+    constexpr bool by_row = GATE == MINT_GATE_ROW;
+    float total[AHEAD ? SUMS : 1][V], wb[V], wa[V], ba[V];
+    // a lane's eight of sum k in LDS: four, and four behind all lanes' first ones
+    const auto in_lds = [&](int k, int half) MINT_INLINE_LAMBDA { return reinterpret_cast<f32x4*>(joined + ((k * 2 + half) * LANES + lane) * 4); };
+    const auto add = [&](int k, const float (&v)[V]) MINT_INLINE_LAMBDA {
+        if constexpr (AHEAD) {
 #pragma unroll
-    for (int k = 0; k < SUMS; ++k)
+            for (int i = 0; i < V; ++i) total[k][i] += v[i];
+        } else {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int i = 0; i < V; ++i) total[k][c][i] = 0.0f;
-    for (uint64_t r = group; r < f.rows; r += a.groups) {
-        float x[C][V], d[C][V], y[C][V];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (a.d_next) {
-                load_elements<S, V>(static_cast<const TS*>(f.stream) + (int64_t)r * f.stream_stride + row.at(c), row.left(c), x[c]);
-                load_elements<T, V>(static_cast<const TT*>(a.d_next) + (int64_t)r * a.d_next_stride + row.at(c), row.left(c), d[c]);
-            }
-            if (BLOCK) load_elements<T, V>(static_cast<const TT*>(f.y) + (int64_t)r * f.y_stride + row.at(c), row.left(c), y[c]);
+            for (int half = 0; half < 2; ++half) *in_lds(k, half) += f32x4{v[half * 4], v[half * 4 + 1], v[half * 4 + 2], v[half * 4 + 3]};
         }
-        float q = 0.0f, mean[2] = {0.0f, 0.0f};
-        if (a.d_next) {
-            q = normalise(row, f.before, x, sums);
+    };
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float w[V];
-                weight_of(f.before, row.at(c), row.left(c), w);
+    for (int k = 0; k < SUMS; ++k) {
+        if constexpr (AHEAD) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    total[0][c][i] = fmaf(d[c][i], x[c][i], total[0][c][i]);
-                    if (BIAS) total[1][c][i] += d[c][i];
-                    d[c][i] *= w[i];
-                }
+            for (int i = 0; i < V; ++i) total[k][i] = 0.0f;
+        } else {
+            *in_lds(k, 0) = *in_lds(k, 1) = f32x4{0, 0, 0, 0};
+        }
+    }
+    constexpr bool HOLD = AHEAD || GATE == 0;
+    if (HOLD) weight_of(f.before, at, left, wb);
+    if (BLOCK && HOLD) {
+        weight_of(f.after, at, left, wa);
+        bias_of(f.after, at, left, ba);
+        if (GATE == 0 && f.gate) {           // (of a gate by channel the sums are without it: column_sums_kernel)
+            float g[V];
+            gate_of(f, 0, at, left, g);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                wa[i] *= gate_value(f.gate_by, g[i]);
+                __builtin_amdgcn_sched_barrier(0);           // (one behind the other: all at once take registers that there are not)
             }
-            mean[0] = row.dot(d, x);
-            mean[1] = row.sum(d);
+        }
+    }
+    Raw<S> next_x, next_d;
+    Raw<T> next_h, next_y;
+    const auto ask = [&](uint32_t r) MINT_INLINE_LAMBDA {
+        if (a.d_next) {
+            next_x.load(f.stream, (int64_t)r * f.stream_stride, at, left);
+            next_h.load(a.d_next, (int64_t)r * a.d_next_stride, at, left);
+        }
+        if (a.d_stream) next_d.load(a.d_stream, (int64_t)r * a.d_stream_stride, at, left);
+        if (BLOCK) next_y.load(f.y, (int64_t)r * f.y_stride, at, left);
+    };
+    const uint32_t first = blockIdx.x * ROWS + nth;
+    if (AHEAD && first < f.rows) ask(first);
+    for (uint64_t r = first; r < f.rows; r += groups) {
+        if constexpr (!AHEAD) {
+            compiler_fence();                                // (or what does not change is read ahead of all rows, into registers that there are not)
+            ask((uint32_t)r);
+        }
+        float row_open = 1.0f, row_slope = 0.0f, g[V];
+        if (AHEAD && GATE == MINT_GATE_ALL) gate_of(f, r, at, left, g);
+        if (by_row) {
+            const float one = load_one(f.gate, f.gate_dtype, (int64_t)r * f.gate_row);
+            row_open = gate_value(f.gate_by, one);
+            row_slope = gate_slope(f.gate_by, one);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float x[V], h[V], d[V], y[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) d[i] = 0.0f;
+        if (a.d_next) {
+            next_x.get(x);
+            next_h.get(h);
+        }
+        if (a.d_stream) next_d.get(d);
+        if (BLOCK && AHEAD) next_y.get(y);
+        if (AHEAD && r + groups < f.rows) ask((uint32_t)(r + groups));
+        if (a.d_next) {
+            const float q = normalise(row, f.before, x, sums);
+            if (!HOLD) weight_of(f.before, at, left, wb);
+            float mean[2], part[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) part[i] = h[i] * x[i];
+            add(0, part);
+            if (BIAS) add(1, h);
+#pragma unroll
+            for (int i = 0; i < V; ++i) h[i] *= wb[i];
+            mean[0] = row.dot(h, x);
+            mean[1] = row.sum(h);
             sums(mean);
             mean[0] *= share;
             mean[1] = f.before.kind == MINT_NORM_LAYER ? mean[1] * share : 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) d[i] += i < left ? q * (h[i] - fmaf(x[i], mean[0], mean[1])) : 0.0f;
         }
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float more[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) more[i] = 0.0f;
-            if (a.d_stream)
-                load_elements<S, V>(static_cast<const TS*>(a.d_stream) + (int64_t)r * a.d_stream_stride + row.at(c), row.left(c), more);
+        if (a.to_stream && left > 0) {
             float to[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float part = a.d_next && i < row.left(c) ? q * (d[c][i] - fmaf(x[c][i], mean[0], mean[1])) : 0.0f;
-                d[c][i] = more[i] + part;
-                to[i] = f.carry * d[c][i];
-            }
-            if (a.to_stream && row.left(c) > 0)
-                store_elements<S, V>(static_cast<TS*>(a.to_stream) + (int64_t)r * a.to_stream_stride + row.at(c), row.left(c), to);
+            for (int i = 0; i < V; ++i) to[i] = f.carry * d[i];
+            store_elements<S, V>(static_cast<TS*>(a.to_stream) + (int64_t)r * a.to_stream_stride + at, left, to);
         }
         if constexpr (BLOCK) {
             constexpr int A = BIAS ? 2 : 1;                  // after's sums
             float yq = 1.0f;
+            if (!AHEAD) {
+                __builtin_amdgcn_sched_barrier(0);
+                next_y.get(y);
+            }
             if (f.after.kind) yq = normalise(row, f.after, y, sums);
-            float of_row[3] = {0.0f, 0.0f, 0.0f};            // of d' yh, of d', of G u (a gate by row)
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                float w[V], b[V], g[V], dg[V];
-                weight_of(f.after, row.at(c), row.left(c), w);
-                bias_of(f.after, row.at(c), row.left(c), b);
-                gate_of(f, r, row.at(c), row.left(c), g);
+            __builtin_amdgcn_sched_barrier(0);               // (what follows would begin further above, in registers that there are not)
+            if (!HOLD) {
+                weight_of(f.after, at, left, wa);
+                bias_of(f.after, at, left, ba);
+            }
+            float of_row[3] = {0.0f, 0.0f, 0.0f};            // of d' yh, of d', of G b; d' without a gate by row
+            if constexpr (GATE == MINT_GATE_ALL) {
+                float dg[V];
+                if (!AHEAD) gate_of(f, r, at, left, g);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float grad = f.scale * d[c][i], u = fmaf(y[c][i], w[i], b[i]), open = f.gate ? gate_value(f.gate_by, g[i]) : 1.0f;
-                    of_row[2] = fmaf(grad, u, of_row[2]);
-                    dg[i] = grad * u * (f.gate ? gate_slope(f.gate_by, g[i]) : 0.0f);
-                    const float inner = grad * open, sum = by_channel ? grad : inner;
-                    total[A][c][i] = fmaf(sum, y[c][i], total[A][c][i]);
-                    if (BIAS) total[A + 1][c][i] += sum;
-                    d[c][i] = inner * w[i];
-                    of_row[0] = fmaf(d[c][i], y[c][i], of_row[0]);
-                    of_row[1] += d[c][i];
+                    const float grad = f.scale * d[i];
+                    dg[i] = grad * fmaf(y[i], wa[i], ba[i]) * gate_slope(f.gate_by, g[i]);
+                    d[i] = grad * gate_value(f.gate_by, g[i]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                if (a.to_gate && !by_row && !by_channel && row.left(c) > 0)
-                    store_any(a.to_gate, f.gate_dtype, (int64_t)r * a.to_gate_stride + row.at(c), row.left(c), dg);
+                if (a.to_gate && left > 0) store_any(a.to_gate, f.gate_dtype, (int64_t)r * a.to_gate_stride + at, left, dg);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) d[i] *= f.scale;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            float part[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) part[i] = row_open * d[i] * y[i];
+            add(A, part);
+            if (BIAS) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    part[i] = row_open * d[i];
+                    if (by_row) of_row[2] = fmaf(d[i], ba[i], of_row[2]);
+                }
+                add(A + 1, part);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                d[i] *= wa[i];
+                of_row[0] = fmaf(d[i], y[i], of_row[0]);
+                of_row[1] += d[i];
             }
             float m0 = 0.0f, m1 = 0.0f;
             if (f.after.kind || by_row) {
                 sums(of_row);
                 if (f.after.kind) m0 = of_row[0] * share;
                 if (f.after.kind == MINT_NORM_LAYER) m1 = of_row[1] * share;
-                if (by_row && a.to_gate && row.lane == 0)
-                    store_one(a.to_gate, f.gate_dtype, (int64_t)r * a.to_gate_stride,
-                              of_row[2] * gate_slope(f.gate_by, load_one(f.gate, f.gate_dtype, (int64_t)r * f.gate_row)));
             }
-            if (a.to_y) {
+            if (a.to_y && left > 0) {
+                float to[V];
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    if (row.left(c) <= 0) continue;
-                    float to[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) to[i] = yq * (d[c][i] - fmaf(y[c][i], m0, m1));
-                    store_elements<T, V>(static_cast<TT*>(a.to_y) + (int64_t)r * a.to_y_stride + row.at(c), row.left(c), to);
-                }
+                for (int i = 0; i < V; ++i) to[i] = yq * row_open * (d[i] - fmaf(y[i], m0, m1));
+                store_elements<T, V>(static_cast<TT*>(a.to_y) + (int64_t)r * a.to_y_stride + at, left, to);
             }
+            if (by_row && a.to_gate && lane == 0)
+                store_one(a.to_gate, f.gate_dtype, (int64_t)r * a.to_gate_stride, (of_row[0] + of_row[2]) * row_slope);
         }
     }
-    if (a.sums) {
+    if (!a.sums) return;
+    if constexpr (ROWS > 1) {                                // a thread block's sums are one group's
+        if (nth) {
 #pragma unroll
-        for (int k = 0; k < SUMS; ++k)
+            for (int k = 0; k < SUMS; ++k)
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-                if (row.left(c) > 0) store_elements<DT_F32, V>(a.sums + ((uint64_t)group * SUMS + k) * f.width + row.at(c), row.left(c), total[k][c]);
+                for (int i = 0; i < V; ++i) joined[(((nth - 1) * SUMS + k) * V + i) * LANES + lane] = total[k][i];
+        }
+        __syncthreads();
+        if (nth) return;
+#pragma unroll
+        for (int n = 0; n < ROWS - 1; ++n)
+#pragma unroll
+            for (int k = 0; k < SUMS; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) total[k][i] += joined[((n * SUMS + k) * V + i) * LANES + lane];
+    }
+    if (left > 0) {
+        if constexpr (!AHEAD) {
+#pragma unroll
+            for (int k = 0; k < SUMS; ++k) {
+                float v[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = (*in_lds(k, i / 4))[i % 4];
+                store_elements<DT_F32, V>(a.sums + ((uint64_t)blockIdx.x * SUMS + k) * f.width + at, left, v);
+            }
+            return;
+        }
+#pragma unroll
+        for (int k = 0; k < (AHEAD ? SUMS : 1); ++k) store_elements<DT_F32, V>(a.sums + ((uint64_t)blockIdx.x * SUMS + k) * f.width + at, left, total[k]);
     }
 }
 
@@ -568,31 +705,54 @@ __global__ void __launch_bounds__(kLongThreads) join_grad_long_kernel(JoinGradAr
 }
 
 // ---- the launches --------------------------------------------------------------------
-// Lanes and numbers of a lane: 64 lanes (four rows to a thread block) up to 512 numbers, then thread blocks of 256 to 1024.
-constexpr uint32_t kLongest = 1024 * V * 2;
+// Lanes of a row: 64 (four rows to a thread block) up to 512 numbers, then a thread block of 128 to 1024.
+constexpr uint32_t kLongest = 1024 * V;
+inline uint32_t threads_for(uint64_t width) {
+    return width <= 64 * V ? 256 : width <= 128 * V ? 128 : width <= 256 * V ? 256 : width <= 512 * V ? 512 : 1024;
+}
+// Thread blocks: as many as are at work together; of a number that does not depend on the device, so that a sum over rows has the same order everywhere.
+inline uint32_t blocks_of(uint64_t rows, uint64_t width, uint32_t threads) {
+    return (uint32_t)std::min<uint64_t>(ceil_div(rows, width <= 64 * V ? 4 : 1), 256 * threads / threads_for(width));
+}
+inline uint32_t blocks_of(uint64_t rows, uint64_t width) { return blocks_of(rows, width, 1024); }      // ... of the gradients
+template <int S, int T, bool WHOLE>
+int go_join_rows(const JoinArgs& a, hipStream_t s) {
+#define MINT_JOIN(LANES) return Launch<&join_kernel<S, T, LANES, WHOLE>>::go(blocks_of(a.rows, a.width, 2048), threads_of(LANES), 0, s, a)
+    if (a.width <= 64 * V) MINT_JOIN(64);
+    if (a.width <= 128 * V) MINT_JOIN(128);
+    if (a.width <= 256 * V) MINT_JOIN(256);
+    if (a.width <= 512 * V) MINT_JOIN(512);
+    MINT_JOIN(1024);
+#undef MINT_JOIN
+}
 template <int S, int T>
 int go_join(const JoinArgs& a, hipStream_t s) {
-#define MINT_JOIN(LANES, C) return Launch<&join_kernel<S, T, LANES, C>>::go((uint32_t)ceil_div(a.rows, LANES < 256 ? 256 / LANES : 1), LANES < 256 ? 256 : LANES, 0, s, a)
-    if (a.width <= 64 * V) MINT_JOIN(64, 1);
-    if (a.width <= 128 * V) MINT_JOIN(64, 2);
-    if (a.width <= 256 * V) MINT_JOIN(256, 1);
-    if (a.width <= 512 * V) MINT_JOIN(256, 2);
-    if (a.width <= 1024 * V) MINT_JOIN(512, 2);
-    if (a.width <= kLongest) MINT_JOIN(1024, 2);
+    if (a.width > kLongest) return Launch<&join_long_kernel<S, T>>::go((uint32_t)a.rows, kLongThreads, 0, s, a);
+    return a.width % V == 0 ? go_join_rows<S, T, true>(a, s) : go_join_rows<S, T, false>(a, s);
+}
+template <int S, int T, bool WHOLE, bool BLOCK, bool BIAS, int GATE>
+int go_join_grad_rows(const JoinGradArgs& a, hipStream_t s) {
+#define MINT_JOIN(LANES) return Launch<&join_grad_kernel<S, T, LANES, WHOLE, BLOCK, BIAS, GATE>>::go(a.groups, threads_of(LANES), 0, s, a)
+    if (a.f.width <= 64 * V) MINT_JOIN(64);
+    if (a.f.width <= 128 * V) MINT_JOIN(128);
+    if (a.f.width <= 256 * V) MINT_JOIN(256);
+    if (a.f.width <= 512 * V) MINT_JOIN(512);
+    // (the registers of a thread block of 1024 do not do for every combination)
+    if constexpr (WHOLE && (GATE != MINT_GATE_ROW || S != DT_F32 || (!BIAS && T != DT_F32))) MINT_JOIN(1024);
+    else return Launch<&join_grad_long_kernel<S, T, BLOCK, BIAS>>::go(a.groups, kLongThreads, 0, s, a);
 #undef MINT_JOIN
-    return Launch<&join_long_kernel<S, T>>::go((uint32_t)a.rows, kLongThreads, 0, s, a);
 }
 template <int S, int T, bool BLOCK, bool BIAS>
 int go_join_grad(const JoinGradArgs& a, hipStream_t s) {
-#define MINT_JOIN(LANES, C) \
-    return Launch<&join_grad_kernel<S, T, LANES, C, BLOCK, BIAS>>::go((uint32_t)ceil_div(a.groups, LANES < 256 ? 256 / LANES : 1), LANES < 256 ? 256 : LANES, 0, s, a)
-    if (a.f.width <= 64 * V) MINT_JOIN(64, 1);
-    if (a.f.width <= 128 * V) MINT_JOIN(64, 2);
-    if (a.f.width <= 256 * V) MINT_JOIN(256, 1);
-    if (a.f.width <= 512 * V) MINT_JOIN(256, 2);
-    if (a.f.width <= 1024 * V) MINT_JOIN(512, 2);
-#undef MINT_JOIN
-    return Launch<&join_grad_long_kernel<S, T, BLOCK, BIAS>>::go(a.groups, kLongThreads, 0, s, a);
+    if (a.f.width > kLongest) return Launch<&join_grad_long_kernel<S, T, BLOCK, BIAS>>::go(a.groups, kLongThreads, 0, s, a);
+    const bool whole = a.f.width % V == 0;
+    if constexpr (BLOCK) {
+        if (a.f.gate && a.f.gate_form == MINT_GATE_ALL)
+            return whole ? go_join_grad_rows<S, T, true, true, BIAS, MINT_GATE_ALL>(a, s) : go_join_grad_rows<S, T, false, true, BIAS, MINT_GATE_ALL>(a, s);
+        if (a.f.gate && a.f.gate_form == MINT_GATE_ROW)
+            return whole ? go_join_grad_rows<S, T, true, true, BIAS, MINT_GATE_ROW>(a, s) : go_join_grad_rows<S, T, false, true, BIAS, MINT_GATE_ROW>(a, s);
+    }
+    return whole ? go_join_grad_rows<S, T, true, BLOCK, BIAS, 0>(a, s) : go_join_grad_rows<S, T, false, BLOCK, BIAS, 0>(a, s);
 }
 template <int S, int T>
 int go_join_grad(const JoinGradArgs& a, bool bias, hipStream_t s) {
