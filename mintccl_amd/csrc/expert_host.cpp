@@ -1005,9 +1005,10 @@ PyObject* host_balance(PyObject*, PyObject* const* list, Py_ssize_t n) {
         const Tensor loss = empty(x, {}, at::kFloat), counts = empty(x, {s, e}, at::kInt), shares = empty(x, {s, e}, at::kFloat),
                      there = empty(x, {s}, at::kInt);
         const size_t need = native.balance_workspace(&op);
-        const Tensor room = empty(x, {(int64_t)need}, at::kByte);
+        Tensor room;
+        if (need) room = empty(x, {(int64_t)need}, at::kByte);
         launch("mint_balance", [&] {
-            return native.balance(&op, address(loss), address(counts), address(shares), address(there), room.data_ptr(), need, on.stream);
+            return native.balance(&op, address(loss), address(counts), address(shares), address(there), need ? room.data_ptr() : nullptr, need, on.stream);
         });
         return pack({wrap(loss), wrap(counts), wrap(shares), wrap(there)});
     });

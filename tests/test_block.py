@@ -77,8 +77,9 @@ def test_join_grad_refuses(code, kw, of_join):
 def test_join_grad_workspace():
     L = _lib.lib()
     room = lambda **kw: L.mint_join_grad_workspace(make(_lib.JoinGradOp, **{**dict(join=join_op(), to_before_weight=4096), **kw}))  # noqa: E731
-    assert room() == 5 * 2 * 64 * 4 and room(to_before_weight=0) == 0 and room(join=join_op(y=0)) == 5 * 64 * 4
-    assert room(join=join_op(rows=0)) == 0 and room(join=join_op(before=spec(bias=4096))) == 5 * 4 * 64 * 4
+    # (four narrow rows a thread block, a line of sums for each of its vectors)
+    assert room() == 2 * 2 * 64 * 4 and room(to_before_weight=0) == 0 and room(join=join_op(y=0)) == 2 * 64 * 4
+    assert room(join=join_op(rows=0)) == 0 and room(join=join_op(before=spec(bias=4096))) == 2 * 4 * 64 * 4
     gated = join_op(gate=4096, gate_form=1, gate_dtype=_lib.F32)
     assert room(join=gated, to_before_weight=0, to_gate=4096) > 0 and room(join=join_op(gate=4096, gate_form=3), to_before_weight=0, to_gate=4096) == 0
     assert L.mint_join_grad_workspace(None) == 0 and L.mint_join(None, None) == L.mint_join_grad(None, None) == _lib.ERR_ARG
@@ -137,12 +138,16 @@ def test_balance_refuses(code, kw):
 
 def test_balance_refuses_results_and_workspaces():
     L = _lib.lib()
-    need = L.mint_balance_workspace(balance_op())
+    assert L.mint_balance_workspace(balance_op(tokens=64)) == L.mint_balance_workspace(balance_op(tokens=0)) == 0           # one launch
+    op = balance_op(tokens=65)
+    need = L.mint_balance_workspace(op)
+    assert need > 0 and L.mint_balance_workspace(balance_op(offsets=4096)) > 0
     for i in range(4):
-        assert L.mint_balance(balance_op(), *(0 if j == i else 4096 for j in range(4)), 1 << 20, need, None) == _lib.ERR_ARG
-    assert L.mint_balance(balance_op(), 4096, 4096, 4096, 4096, 1 << 20, need - 1, None) == _lib.ERR_STAGING
-    assert L.mint_balance(balance_op(), 4096, 4096, 4096, 4096, None, need, None) == _lib.ERR_STAGING
-    assert L.mint_balance(balance_op(), 4096, 4096, 4096, 4096, (1 << 20) + 4, need, None) == _lib.ERR_ALIGN
+        assert L.mint_balance(op, *(0 if j == i else 4096 for j in range(4)), 1 << 20, need, None) == _lib.ERR_ARG
+        assert L.mint_balance(balance_op(), *(0 if j == i else 4096 for j in range(4)), None, 0, None) == _lib.ERR_ARG
+    assert L.mint_balance(op, 4096, 4096, 4096, 4096, 1 << 20, need - 1, None) == _lib.ERR_STAGING
+    assert L.mint_balance(op, 4096, 4096, 4096, 4096, None, need, None) == _lib.ERR_STAGING
+    assert L.mint_balance(op, 4096, 4096, 4096, 4096, (1 << 20) + 4, need, None) == _lib.ERR_ALIGN
     assert L.mint_balance(None, 0, 0, 0, 0, None, 0, None) == L.mint_balance_grad(None, 0, 0, 0, 0, 0, 0, 0, None) == _lib.ERR_ARG
     for i in range(4):
         at = [0 if j == i else 4096 for j in range(4)]
