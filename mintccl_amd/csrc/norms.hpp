@@ -91,6 +91,7 @@ struct RowSums {
 // numbers or none (ends inside a lane's numbers cost registers, which the kernels that hold most of them do not have).
 template <int LANES, bool WHOLE>
 struct RowOf {
+    static constexpr bool whole = WHOLE;
     uint32_t width, at;
     int64_t left;
     __device__ __forceinline__ RowOf(uint32_t w, uint32_t lane)
@@ -154,7 +155,9 @@ __device__ __forceinline__ void gate_of(const JoinArgs& a, uint64_t row, uint32_
     }
 }
 
-// V numbers as they are in memory, zeros behind the `left` first: what is on its way while the row before is worked on.
+// V numbers as they are in memory, zeros behind the `left` first: what is on its way while the row before is worked on.  At a row's end the lane reads the row's
+// last V numbers and moves its own to the front when they are wanted: one by one they would have to be there at once, for what is put together of
+// them, and the other lanes' rows with them (8000 x 2501 f16, rms: 70 us, so 56; 2504 numbers 39).
 template <int DT>
 struct Raw {
     using T = typename Elem<DT>::type;
@@ -163,24 +166,46 @@ struct Raw {
     typedef T numbers __attribute__((ext_vector_type(V)));
     uint32_t v[WORDS];           // (words: numbers of 16 bits would take a register each)
     // (where the row is, the same for all, apart from the lane's place in it: the address takes one register)
-    __device__ __forceinline__ void load(const void* p, int64_t row, uint32_t at, int64_t left) {
-        const T* const from = static_cast<const T*>(p) + row + at;
-        if (left >= V) {
-            const words w = *(MINT_GLOBAL const words*)as_global(from);
+    template <typename Row>
+    __device__ __forceinline__ void load(const void* p, int64_t row, const Row& of) {
+        const T* const first = static_cast<const T*>(p) + row;
+        if (of.whole ? of.left > 0 : of.width >= V) {
+            const words w = *(MINT_GLOBAL const words*)as_global(first + (of.whole ? of.at : min(of.at, of.width - V)));
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) v[i] = w[i];
         } else {
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) v[i] = 0u;
+            if (of.whole) return;
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (i < left) {
-                    if constexpr (sizeof(T) == 4) v[i] = *(MINT_GLOBAL const uint32_t*)as_global(from + i);
-                    else v[i / 2] |= (uint32_t)*(MINT_GLOBAL const uint16_t*)as_global(from + i) << (i % 2 * 16);
+                if (i < of.left) {
+                    if constexpr (sizeof(T) == 4) v[i] = *(MINT_GLOBAL const uint32_t*)as_global(first + i);
+                    else v[i / 2] |= (uint32_t)*(MINT_GLOBAL const uint16_t*)as_global(first + i) << (i % 2 * 16);
                 }
         }
     }
-    __device__ __forceinline__ void get(float (&x)[V]) const {
+    // `of` as it was for load()
+    template <typename Row>
+    __device__ __forceinline__ void place(const Row& of) {
+        if (of.whole || of.left >= V || of.width < V) return;
+        const uint32_t skip = of.left > 0 ? (uint32_t)(V - of.left) : V;         // numbers in front that are another lane's
+        if constexpr (sizeof(T) == 2) {
+            if (skip & 1u) {
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) v[i] = __builtin_amdgcn_alignbit(i + 1 < WORDS ? v[i + 1] : 0u, v[i], 16);
+            }
+        }
+#pragma unroll
+        for (int step = 1; step <= WORDS; step *= 2)
+            if (skip & (uint32_t)(step * V / WORDS)) {
+#pragma unroll
+                for (int i = 0; i < WORDS; ++i) v[i] = i + step < WORDS ? v[i + step] : 0u;
+            }
+    }
+    template <typename Row>
+    __device__ __forceinline__ void get(const Row& of, float (&x)[V]) {
+        place(of);
         typedef uint32_t whole __attribute__((ext_vector_type(WORDS)));
         whole w;
 #pragma unroll
@@ -190,6 +215,18 @@ struct Raw {
         for (int i = 0; i < V; ++i) x[i] = Elem<DT>::load(n[i]);
     }
 };
+// a lane's numbers of a row's gate, as it was given, for rows in registers
+template <typename Row>
+__device__ __forceinline__ void gate_of(const JoinArgs& a, uint64_t r, const Row& of, float (&g)[V]) {
+    const auto all = [&](auto raw) MINT_INLINE_LAMBDA {
+        raw.load(a.gate, (int64_t)r * a.gate_row, of);
+        raw.get(of, g);
+    };
+    if (!a.gate || a.gate_form == MINT_GATE_ROW) gate_of(a, r, of.at, of.left, g);
+    else if (a.gate_dtype == MINT_F32) all(Raw<DT_F32>());
+    else if (a.gate_dtype == MINT_BF16) all(Raw<DT_BF16>());
+    else all(Raw<DT_F16>());
+}
 constexpr int threads_of(int lanes) { return lanes == 64 ? 256 : lanes; }         // four rows to a thread block, or one
 constexpr int rows_of(int lanes) { return lanes == 64 ? 4 : 1; }
 
@@ -215,7 +252,7 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_kernel(JoinArgs a) {
     bias_of(a.after, at, left, ba);
     weight_of(a.before, at, left, wb);
     bias_of(a.before, at, left, bb);
-    if (!one_by_one) gate_of(a, 0, at, left, open);
+    if (!one_by_one) gate_of(a, 0, row, open);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const float all = a.scale * (a.gate && !one_by_one ? gate_value(a.gate_by, open[i]) : 1.0f);
@@ -225,19 +262,19 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_kernel(JoinArgs a) {
     Raw<S> next_s;
     Raw<T> next_y;
     const auto ask = [&](uint32_t r) MINT_INLINE_LAMBDA {
-        next_s.load(a.stream, (int64_t)r * a.stream_stride, at, left);
-        if (a.y) next_y.load(a.y, (int64_t)r * a.y_stride, at, left);
+        next_s.load(a.stream, (int64_t)r * a.stream_stride, row);
+        if (a.y) next_y.load(a.y, (int64_t)r * a.y_stride, row);
     };
     ask(first);
     for (uint64_t r = first; r < a.rows; r += groups) {
         float s[V], y[V];
-        next_s.get(s);
-        if (a.y) next_y.get(y);
+        next_s.get(row, s);
+        if (a.y) next_y.get(row, y);
         if (r + groups < a.rows) ask((uint32_t)(r + groups));
         if (a.y) {
             if (a.after.kind) normalise(row, a.after, y, sums);
             if (one_by_one) {
-                gate_of(a, r, at, left, open);
+                gate_of(a, r, row, open);
 #pragma unroll
                 for (int i = 0; i < V; ++i) open[i] = gate_value(a.gate_by, open[i]);
             }
@@ -319,7 +356,7 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradAr
         bias_of(f.after, at, left, ba);
         if (GATE == 0 && f.gate) {           // (of a gate by channel the sums are without it: column_sums_kernel)
             float g[V];
-            gate_of(f, 0, at, left, g);
+            gate_of(f, 0, row, g);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 wa[i] *= gate_value(f.gate_by, g[i]);
@@ -331,11 +368,11 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradAr
     Raw<T> next_h, next_y;
     const auto ask = [&](uint32_t r) MINT_INLINE_LAMBDA {
         if (a.d_next) {
-            next_x.load(f.stream, (int64_t)r * f.stream_stride, at, left);
-            next_h.load(a.d_next, (int64_t)r * a.d_next_stride, at, left);
+            next_x.load(f.stream, (int64_t)r * f.stream_stride, row);
+            next_h.load(a.d_next, (int64_t)r * a.d_next_stride, row);
         }
-        if (a.d_stream) next_d.load(a.d_stream, (int64_t)r * a.d_stream_stride, at, left);
-        if (BLOCK) next_y.load(f.y, (int64_t)r * f.y_stride, at, left);
+        if (a.d_stream) next_d.load(a.d_stream, (int64_t)r * a.d_stream_stride, row);
+        if (BLOCK) next_y.load(f.y, (int64_t)r * f.y_stride, row);
     };
     const uint32_t first = blockIdx.x * ROWS + nth;
     if (AHEAD && first < f.rows) ask(first);
@@ -345,7 +382,7 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradAr
             ask((uint32_t)r);
         }
         float row_open = 1.0f, row_slope = 0.0f, g[V];
-        if (AHEAD && GATE == MINT_GATE_ALL) gate_of(f, r, at, left, g);
+        if (AHEAD && GATE == MINT_GATE_ALL) gate_of(f, r, row, g);
         if (by_row) {
             const float one = load_one(f.gate, f.gate_dtype, (int64_t)r * f.gate_row);
             row_open = gate_value(f.gate_by, one);
@@ -356,11 +393,11 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradAr
 #pragma unroll
         for (int i = 0; i < V; ++i) d[i] = 0.0f;
         if (a.d_next) {
-            next_x.get(x);
-            next_h.get(h);
+            next_x.get(row, x);
+            next_h.get(row, h);
         }
-        if (a.d_stream) next_d.get(d);
-        if (BLOCK && AHEAD) next_y.get(y);
+        if (a.d_stream) next_d.get(row, d);
+        if (BLOCK && AHEAD) next_y.get(row, y);
         if (AHEAD && r + groups < f.rows) ask((uint32_t)(r + groups));
         if (a.d_next) {
             const float q = normalise(row, f.before, x, sums);
@@ -391,7 +428,7 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradAr
             float yq = 1.0f;
             if (!AHEAD) {
                 __builtin_amdgcn_sched_barrier(0);
-                next_y.get(y);
+                next_y.get(row, y);
             }
             if (f.after.kind) yq = normalise(row, f.after, y, sums);
             __builtin_amdgcn_sched_barrier(0);               // (what follows would begin further above, in registers that there are not)
@@ -402,7 +439,7 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradAr
             float of_row[3] = {0.0f, 0.0f, 0.0f};            // of d' yh, of d', of G b; d' without a gate by row
             if constexpr (GATE == MINT_GATE_ALL) {
                 float dg[V];
-                if (!AHEAD) gate_of(f, r, at, left, g);
+                if (!AHEAD) gate_of(f, r, row, g);
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const float grad = f.scale * d[i];
