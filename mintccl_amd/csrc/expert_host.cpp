@@ -187,6 +187,20 @@ void result(const Tensor& t, int64_t rows, int64_t cols, const char* name) {
         refuse(PyExc_ValueError, "%s must be (%lld, %lld)", name, (long long)rows, (long long)cols);
     if (rows > 1 && cols > 0 && t.stride(0) < cols) refuse(PyExc_ValueError, "the rows of %s overlap", name);
 }
+// ... and that none of the call's rows or vectors lie in, but for one that may be the result itself.  (Rows of one buffer side by side may.)
+void clear_of(const Tensor& out, const Tensor& t, const char* name, bool may_be_it) {
+    if (out.numel() == 0 || t.numel() == 0 || out.get_device() != t.get_device()) return;
+    const auto row = [](const Tensor& x) { return (uint64_t)(x.size(-1) * (int64_t)x.element_size()); };
+    const auto pitch = [](const Tensor& x) { return x.dim() > 1 && x.size(0) > 1 ? (uint64_t)(x.stride(0) * (int64_t)x.element_size()) : 0; };
+    const uint64_t p = (uint64_t)out.data_ptr(), q = (uint64_t)t.data_ptr(), every = pitch(out), also = pitch(t);
+    if (p + (every ? every * (out.size(0) - 1) : 0) + row(out) <= q || q + (also ? also * (t.size(0) - 1) : 0) + row(t) <= p) return;
+    if (may_be_it && p == q && every == also && out.scalar_type() == t.scalar_type()) return;
+    if (every && every == also) {
+        const uint64_t behind = q >= p ? (q - p) % every : (every - (p - q) % every) % every;
+        if (behind >= row(out) && behind + row(t) <= every) return;
+    }
+    refuse(PyExc_ValueError, "out shares memory with %s", name);
+}
 Tensor empty(const Tensor& like, at::IntArrayRef size, at::ScalarType type) {
     return at::empty(size, at::TensorOptions().device(like.device()).dtype(type));
 }
@@ -704,6 +718,10 @@ PyObject* host_join(PyObject*, PyObject* const* list, Py_ssize_t n) {
             same_device(s, out, "out");
             result(out, s.size(0), s.size(1), "out");
             if (code_of(out.scalar_type(), "out") != (block ? op.stream_dtype : op.dtype)) refuse(PyExc_TypeError, "out is of another type than the result");
+            clear_of(out, s, block ? "stream" : "x", true);
+            if (block) clear_of(out, a.tensor(1, "y"), "y", false);
+            for (const auto& [i, name] : {std::pair<int, const char*>{2, "gate"}, {7, "a weight"}, {8, "a bias"}, {11, "a weight"}, {12, "a bias"}})
+                if (!a.none(i)) clear_of(out, a.tensor(i, name), name, false);
         }
         OnDevice on(s.get_device());
         Tensor stream, h;
@@ -868,6 +886,12 @@ PyObject* host_dense_product(PyObject*, PyObject* const* list, Py_ssize_t n) {
             if (code_of(r.scalar_type(), "residual") != op.out_dtype) refuse(PyExc_TypeError, "residual must be of the result's type");
             op.residual = address(r);
             op.residual_stride = r.stride(0);
+        }
+        if (given) {
+            clear_of(out, x, "x", false);
+            clear_of(out, w, "the weight", false);
+            if (!a.none(2)) clear_of(out, a.tensor(2, "bias"), "bias", false);
+            if (!a.none(4)) clear_of(out, a.tensor(4, "residual"), "residual", true);
         }
         Tensor z;
         if (keep) {

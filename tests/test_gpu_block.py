@@ -124,3 +124,41 @@ def test_two_graphs_at_once(dev):
             for k, (a, b) in enumerate(zip(found, want)):
                 assert torch.equal(a, b), k
                 a.zero_() if a.is_floating_point() else a.fill_(-1)
+
+
+def test_results_that_share_memory(dev):
+    """A result may be the stream or the residual itself, and lie beside the other rows of one buffer; else it may share no memory with what the call reads."""
+    g = torch.Generator().manual_seed(9)
+    rand = lambda *s: torch.randn(*s, generator=g).to(dev)  # noqa: E731
+    room = rand(40, 192)
+    x, y, w = room[:, :64], room[:, 64:128], rand(64, 64)
+    n = Norm(rand(64))
+    want = dense.product(x, w, residual=y)
+    for out in (room[:, 128:], torch.empty(40, 64, device=dev)):
+        assert torch.equal(dense.product(x, w, residual=y, out=out), want)
+    assert torch.equal(dense.product(x, w, residual=y, out=y), want) and torch.equal(y, want)
+    for bad in (x, room[:, 1:65], room[:, 60:124]):
+        with pytest.raises(ValueError):
+            dense.product(x, w, out=bad)
+    with pytest.raises(ValueError):
+        dense.product(x, w, residual=y, out=room[:, 65:129])
+    with pytest.raises(ValueError):
+        dense.product(x[:, :64], w, out=w[:40])
+    with pytest.raises(ValueError):
+        dense.product(x, w, bias=w[5], out=w[:40])
+    with pytest.raises(ValueError):
+        join(x, y, out=y)
+    with pytest.raises(ValueError):
+        join(x, y, out=room[:, 32:96])
+    with pytest.raises(ValueError):
+        join(x[:39], y[:39], out=x[1:])                       # (the stream, a row on)
+    with pytest.raises(ValueError):
+        norm(x, n, out=room[:, 8:72])
+    with pytest.raises(ValueError):
+        norm(x, n, dtype=torch.bfloat16, out=room.view(torch.bfloat16)[:, :64])
+    want = norm(x, n)
+    assert torch.equal(norm(x, n, out=room[:, 128:]), want) and torch.equal(norm(x, n, out=x), want)
+    both, of = join(want, y, before=n)
+    s = want.clone()
+    again, also = join(s, y, before=n, out=s)
+    assert torch.equal(again, both) and torch.equal(also, of) and again is s
