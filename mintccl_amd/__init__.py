@@ -17,7 +17,10 @@ plus ``common`` (knobs, ``VirtualComm``), ``primitive``, ``protocol`` and
     routing.route(logits, k) / route_grad / assign      tokens to experts, and their places in the experts' order
     block8.quantise / quantise_weight / product / weight_grad    products in 8 bits with a scale per block of 128
     combine.combine / combine_grad                      a token's rows added up with their weights
-    experts.ExpertLayer                                 all of it over the ranks of a communicator
+    norms.norm / norm_grad / join / join_grad           rms and layer norms, alone or with the residual stream and a gate
+    dense.product / activation_grad / input_grad / weight_grad   products in 16 and 32 bits with bias, activation and residual
+    routing.balance / balance_grad                      the loss that keeps the experts in balance
+    experts.ExpertLayer, ExpertBlock                    all of it over the ranks of a communicator
 
 All compute runs in ``libmintccl.so`` (hand-written HIP); the
 package raises if that library has not been built.

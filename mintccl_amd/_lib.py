@@ -285,8 +285,8 @@ def host_command(out: str, source: str = HOST_SRC) -> list[str]:
 def build(verbose: bool = False, defines: tuple[str, ...] = (), so_path: str | None = None) -> str:
     """Compile the HIP sources for gfx950 into ``libmintccl.so`` (in-tree).
 
-    The ring kernels are one translation unit per element type; the ten
-    compilations run side by side and are linked at the end.  ``defines``
+    The ring kernels are one translation unit per element type, the norms'
+    one per pair of types; all compile side by side and are linked at the end.  ``defines``
     (``-DMINT_RING_STATS``: wait accounting per ring position,
     ``-DMINT_ROW_NOLOAD``: whole blocks of own rows are not loaded - wrong
     results, for timing a collective without its HBM reads) and ``so_path``

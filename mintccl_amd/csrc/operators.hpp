@@ -1,5 +1,5 @@
-// What the expert layer's kernels share (routing.hip, block8.hip, combine.hip): the element
-// types, and reductions over a wavefront.  No counterpart in the reference.
+// What the kernels of the expert layer (routing.hip, block8.hip, combine.hip) and of the block around
+// it (norms.hpp, dense.hip, balance.hip) share: the element types, and reductions over a wavefront.  No counterpart in the reference.
 #pragma once
 #include "ring_launch.hpp"
 
