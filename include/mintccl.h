@@ -743,7 +743,7 @@ typedef struct {
     uint64_t chosen;       /* int32 (tokens, topk); -1: none */
     uint64_t offsets;      /* int32 (sequences + 1), or 0 */
     int64_t row_stride;
-    uint64_t tokens, sequences;
+    uint64_t tokens, sequences;    /* at most 65535 sequences */
     uint32_t experts, topk;
     int32_t dtype;
     int32_t score;         /* mint_score */

@@ -41,49 +41,41 @@ struct BalanceArgs {
     float *out_shares, *out_loss;
 };
 
-// Where tile `t` of `tile` tokens is.  Offsets are device data: whatever they say, tokens stay inside.
+// Where tile `t` of `tile` tokens is.  With offsets the tokens before the first sequence and those behind the last one count as a sequence each: v = 0, 1 ... S,
+// S + 1 begin at tokens b_v, and v has the tiles from b_v / tile + v on, whole numbers, which is room enough for it, and is found by a search.  (Tiles that
+// a sequence has room for and does not need are nobody's.)  Offsets are device data: whatever they say, tokens and tiles stay inside.
 struct Span {
-    uint32_t sequence, begin, end, first;       // tokens [begin, end); the first tile of its sequence
-    bool found;
+    uint32_t sequence, begin, end;              // tokens [begin, end)
+    bool found, outside;                        // outside: tokens of no sequence
 };
-__device__ __forceinline__ uint32_t token_bound(const int32_t* offsets, uint32_t i, uint32_t tokens) { return min((uint32_t)max(offsets[i], 0), tokens); }
-__device__ __forceinline__ uint32_t tiles_in(const int32_t* offsets, uint32_t s, uint32_t sequences, uint32_t tokens, uint32_t tile, uint32_t& begin, uint32_t& end) {
-    begin = end = 0;
-    if (s < sequences) {
-        begin = token_bound(offsets, s, tokens);
-        end = max(begin, token_bound(offsets, s + 1, tokens));
-    }
-    return (end - begin + tile - 1) / tile;
+__device__ __forceinline__ uint32_t begin_of(const BalanceArgs& a, uint32_t v) {
+    return v == 0 ? 0u : v > a.sequences + 1 ? a.tokens : min((uint32_t)max(a.offsets[v - 1], 0), a.tokens);
 }
 __device__ __forceinline__ Span find_span(const BalanceArgs& a, uint32_t t) {
-    if (!a.offsets) return {0, min(t * a.tile, a.tokens), min(t * a.tile + a.tile, a.tokens), 0, t * a.tile < a.tokens};
-    uint32_t base = 0;
-    for (uint32_t s0 = 0; s0 < a.sequences; s0 += 64) {
-        uint32_t begin, end;
-        const uint32_t n = tiles_in(a.offsets, s0 + lane_id(), a.sequences, a.tokens, a.tile, begin, end), sum = sum_below(n);
-        const uint64_t behind = __ballot(base + sum > t);
-        if (behind) {
-            const int at = __builtin_ctzll(behind);
-            const uint32_t first = base + (uint32_t)__builtin_amdgcn_readlane((int)(sum - n), at);
-            const uint32_t b = (uint32_t)__builtin_amdgcn_readlane((int)begin, at), e = (uint32_t)__builtin_amdgcn_readlane((int)end, at);
-            const uint32_t from = b + (t - first) * a.tile;
-            return {s0 + at, from, min(from + a.tile, e), first, true};
-        }
-        base += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    if (!a.offsets) return {0, min(t * a.tile, a.tokens), min(t * a.tile + a.tile, a.tokens), t * a.tile < a.tokens, false};
+    const uint32_t lane = lane_id();
+    uint32_t v = 0, n = a.sequences + 2;
+    for (uint32_t step = 0; step != 1;) {                    // 64 of them at a time
+        step = (n + 63) / 64;
+        const uint32_t at = min(lane * step, n - 1);
+        const uint64_t below = __ballot(lane * step < n && begin_of(a, v + at) / a.tile + (v + at) <= t);
+        const uint32_t skip = (below ? (uint32_t)__popcll(below) - 1u : 0u) * step;
+        v += skip;
+        n = min(step, n - skip);
     }
-    return {a.sequences, 0, 0, base, false};
+    const uint32_t begin = begin_of(a, v), end = max(begin, begin_of(a, v + 1)), nth = t - (begin / a.tile + v);
+    const bool found = nth < (end - begin + a.tile - 1) / a.tile, outside = v == 0 || v > a.sequences;
+    const uint32_t from = found ? begin + nth * a.tile : 0u;
+    return {v - 1, from, found ? min(from + a.tile, end) : 0u, found, outside};
 }
 // the tiles of sequence s
 __device__ __forceinline__ void tiles_of_sequence(const BalanceArgs& a, uint32_t s, uint32_t& first, uint32_t& end) {
-    if (!a.offsets) {
-        first = 0;
-        end = a.tiles;
-        return;
-    }
-    uint32_t before = 0, b, e;
-    for (uint32_t i = lane_id(); i < s; i += 64) before += tiles_in(a.offsets, i, a.sequences, a.tokens, a.tile, b, e);
-    first = min((uint32_t)__builtin_amdgcn_readlane((int)sum_below(before), 63), a.tiles);
-    end = min(first + tiles_in(a.offsets, s, a.sequences, a.tokens, a.tile, b, e), a.tiles);
+    first = 0;
+    end = a.tiles;
+    if (!a.offsets) return;
+    const uint32_t begin = begin_of(a, s + 1), tokens = max(begin, begin_of(a, s + 2)) - begin;
+    first = min(begin / a.tile + s + 1, a.tiles);
+    end = min(first + (tokens + a.tile - 1) / a.tile, a.tiles);
 }
 
 // Of U tokens' logits (V consecutive ones of a lane), side by side so that their steps across lanes overlap: the shares, and what the gradient needs.
@@ -190,7 +182,14 @@ __global__ void __launch_bounds__(64 * kWaves) balance_tiles_kernel(BalanceArgs 
     __shared__ float square[kWaves];
     const Span span = find_span(a, blockIdx.x);
     if (!ALONE && blockIdx.x == 0 && threadIdx.x == 0) *a.arrived = 0u;
-    if (!ALONE && !span.found) return;
+    if (!ALONE && (!span.found || span.outside)) {           // (nobody's: but offsets that descend may have it read)
+        for (uint32_t e = threadIdx.x; e < a.experts; e += 64 * kWaves) {
+            a.shares[(uint64_t)blockIdx.x * a.experts + e] = 0.0f;
+            a.counts[(uint64_t)blockIdx.x * a.experts + e] = 0u;
+        }
+        if (threadIdx.x < 2) a.square[blockIdx.x * 2 + threadIdx.x] = 0.0f;
+        return;
+    }
     for (uint32_t e = threadIdx.x; e < a.experts; e += 64 * kWaves) counts[e] = 0u;
     __syncthreads();
     const uint32_t lane = lane_id(), wave = wave_in_block(), first = lane * V;
@@ -320,25 +319,30 @@ __global__ void __launch_bounds__(kSlots * kOfBlock) balance_join_kernel(Balance
         }
     }
     __syncthreads();
-    if (!last || wave != 0) return;
+    if (!last) return;
     compiler_fence();
-    float total = 0.0f, all_squares = 0.0f;
-    uint32_t sequences = 0, tokens = 0;
-    // (lanes have sequences in turn, and then add each other's up: a fixed order too)
-    for (uint32_t i = lane_id(); i < a.sequences; i += 64) {
+    // (threads have sequences in turn, lanes add theirs up, then wavefronts: a fixed order too)
+    Sums all = {0.0f, 0.0f, 0u, 0u};
+    for (uint32_t i = threadIdx.x; i < a.sequences; i += kSlots * kOfBlock) {
         const uint32_t k = (uint32_t)ld64_agent(a.terms + gridDim.x + i);
-        sequences += k != 0;
-        tokens += k;
+        all.count += k != 0;
+        all.tokens += k;
         float of_one = 0.0f;
         for (uint32_t b = 0; b < blocks; ++b) of_one += __uint_as_float((uint32_t)ld64_agent(a.terms + (uint64_t)i * blocks + b));
-        total += of_one;
-        all_squares += __uint_as_float((uint32_t)(ld64_agent(a.terms + (uint64_t)i * blocks) >> 32));
+        all.share += of_one;
+        all.squares += __uint_as_float((uint32_t)(ld64_agent(a.terms + (uint64_t)i * blocks) >> 32));
     }
-    total = wave_sum(total);
-    all_squares = wave_sum(all_squares);
-    const uint32_t some = (uint32_t)__builtin_amdgcn_readlane((int)sum_below(sequences), 63);
-    const uint32_t every = (uint32_t)__builtin_amdgcn_readlane((int)sum_below(tokens), 63);
-    if (lane_id() == 0) *a.out_loss = loss_of(a, total, all_squares, some, every);
+    all.share = wave_sum(all.share);
+    all.squares = wave_sum(all.squares);
+    all.count = (uint32_t)__builtin_amdgcn_readlane((int)sum_below(all.count), 63);
+    all.tokens = (uint32_t)__builtin_amdgcn_readlane((int)sum_below(all.tokens), 63);
+    if (lane_id() == 0) part[wave][0] = all;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t w = 1; w < kSlots * kOfBlock / 64; ++w)
+            all = {all.share + part[w][0].share, all.squares + part[w][0].squares, all.count + part[w][0].count, all.tokens + part[w][0].tokens};
+        *a.out_loss = loss_of(a, all.share, all.squares, all.count, all.tokens);
+    }
 }
 
 struct BalanceGradArgs {
@@ -356,13 +360,11 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
     const BalanceArgs& f = a.f;
     const uint32_t lane = lane_id(), first = lane * V;
     const int64_t left = (int64_t)f.experts - first;
-    Span span = find_span(f, blockIdx.x);
-    if (!span.found) {
-        // the tokens before the first sequence and behind the last one
-        const uint32_t begin = token_bound(f.offsets, 0, f.tokens), end = max(begin, token_bound(f.offsets, f.sequences, f.tokens));
-        const uint32_t nth = blockIdx.x - span.first, outside = begin + (f.tokens - end);
-        for (uint32_t i = nth * f.tile + wave_in_block(); i < min(outside, (nth + 1) * f.tile); i += kWaves) {
-            const uint32_t t = i < begin ? i : end + (i - begin);
+    __shared__ uint32_t some_of[kWaves], every_of[kWaves];
+    const Span span = find_span(f, blockIdx.x);
+    if (!span.found) return;
+    if (span.outside) {
+        for (uint32_t t = span.begin + wave_in_block(); t < span.end; t += kWaves) {
             float none[V] = {};
             if (a.add) load_elements<DT, V>(static_cast<const T*>(a.add) + (int64_t)t * a.add_stride + first, left, none);
             if (left > 0) store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, none);
@@ -371,13 +373,26 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
     }
     // sequences that have a token, and all tokens
     uint32_t some = 0, every = 0;
-    for (uint32_t s = lane; s < f.sequences; s += 64) {
+    for (uint32_t s = threadIdx.x; s < f.sequences; s += 64 * kWaves) {
         const uint32_t n = (uint32_t)max(a.there[s], 0);
         some += n != 0;
         every += n;
     }
-    some = max((uint32_t)__builtin_amdgcn_readlane((int)sum_below(some), 63), 1u);
-    every = max((uint32_t)__builtin_amdgcn_readlane((int)sum_below(every), 63), 1u);
+    some = sum_below(some);
+    every = sum_below(every);
+    if (lane == 63) {
+        some_of[wave_in_block()] = some;
+        every_of[wave_in_block()] = every;
+    }
+    __syncthreads();
+    some = every = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        some += some_of[w];
+        every += every_of[w];
+    }
+    some = max(some, 1u);
+    every = max(every, 1u);
     const float d = *a.d_loss, n = (float)max(a.there[span.sequence], 1);
     const float by = d * (float)f.experts / ((float)f.topk * n) / ((float)some * n), by_z = f.z != 0.0f ? 2.0f * f.z * d / (float)every : 0.0f;
     float often[V];
@@ -434,8 +449,7 @@ int go_tiles(const BalanceArgs& a, hipStream_t s) {
 }
 template <int DT, int V>
 int go_grad(const BalanceGradArgs& a, hipStream_t s) {
-    // (tokens of no sequence are dealt to the tiles that are left over)
-    return Launch<&balance_grad_kernel<DT, V>>::go(a.f.tiles + (a.f.offsets ? 1u : 0u), 64 * kWaves, 0, s, a);
+    return Launch<&balance_grad_kernel<DT, V>>::go(a.f.tiles, 64 * kWaves, 0, s, a);
 }
 #define MINT_BY_VALUES(GO, DT)                     \
     switch (values_per_lane(op->experts)) {        \
@@ -458,15 +472,16 @@ uint32_t sequences_of(const mint_balance_op& op) { return op.offsets ? (uint32_t
 uint32_t tile_of(uint64_t tokens) { return (uint32_t)std::min<uint64_t>(256, std::max<uint64_t>(16, ceil_div(tokens, 1024))); }
 // So few that one thread block takes less than two launches.
 bool alone(const mint_balance_op& op) { return !op.offsets && op.tokens <= 64; }
-// tiles at most: the last one of each sequence may have a single token, and in the gradient so may those of the tokens of none
+constexpr uint64_t kMostSequences = 0xFFFF;      // (with 64 thread blocks each of 1024 threads: a launch has fewer than 2^32)
+// tiles, those that are nobody's among them
 uint64_t tiles_of(const mint_balance_op& op) {
     const uint64_t tile = tile_of(op.tokens);
-    return std::min<uint64_t>(op.tokens, ceil_div(op.tokens, tile) + (op.offsets ? op.sequences : 0));
+    return op.offsets ? op.tokens / tile + op.sequences + 2 : ceil_div(op.tokens, tile);
 }
 int balance_checks(const mint_balance_op* op) {
     if (!op || !known(op->dtype) || (op->score != MINT_SCORE_SOFTMAX && op->score != MINT_SCORE_SIGMOID)) return MINT_ERR_ARG;
     if (op->experts < 1 || op->experts > kMostExperts || op->topk < 1 || op->topk > kMostExperts) return MINT_ERR_ARG;
-    if (op->tokens > 0x7FFFFFFFull / op->topk || (op->offsets && op->sequences > (1u << 20))) return MINT_ERR_TOO_LARGE;
+    if (op->tokens > 0x7FFFFFFFull / op->topk || (op->offsets && op->sequences > kMostSequences)) return MINT_ERR_TOO_LARGE;
     if (op->offsets && op->sequences == 0) return MINT_ERR_ARG;
     if (op->tokens && (!op->logits || !op->chosen)) return MINT_ERR_ARG;
     return MINT_OK;
@@ -533,13 +548,8 @@ extern "C" int mint_balance(const mint_balance_op* op, uint64_t loss, uint64_t c
     a.square = reinterpret_cast<float*>(at + room.square);
     a.arrived = reinterpret_cast<uint32_t*>(at + room.arrived);
     const uint64_t blocks = a.sequences * ceil_div(a.experts, kOfBlock);
-    if (blocks * kSlots * kOfBlock > 0xFFFFFFFFull) return MINT_ERR_TOO_LARGE;
-    // (of no tokens a block that finds none still clears the count)
-    const uint32_t real = a.tiles;
-    a.tiles = std::max(real, 1u);
     const int err = tiles();
     if (err != MINT_OK) return err;
-    a.tiles = real;
     return Launch<&balance_join_kernel>::go((uint32_t)blocks, kSlots * kOfBlock, 0, s, a);
 }
 

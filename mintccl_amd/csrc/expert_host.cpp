@@ -1011,7 +1011,7 @@ void balance_of(const Args& a, int i, mint_balance_op& op) {
         dims(offsets, 1, "offsets");
         dense(offsets, "offsets");
         if (offsets.size(0) < 2) refuse(PyExc_ValueError, "offsets must have two numbers at least");
-        if (offsets.size(0) - 1 > 1 << 20) refuse(PyExc_ValueError, "at most %d sequences", 1 << 20);
+        if (offsets.size(0) - 1 > 0xFFFF) refuse(PyExc_ValueError, "at most %d sequences", 0xFFFF);
         op.offsets = address(offsets);
         op.sequences = (uint64_t)offsets.size(0) - 1;
     }

@@ -86,7 +86,7 @@ def balance(logits: torch.Tensor, experts: torch.Tensor, *, score: str = "softma
     have an expert left (a logit above -inf), an expert counted c times has the load f = experts * c / (k * n) and the mean
     share P; the loss is the sum of f * P over the experts, its mean over the sequences that have such a token, plus ``z`` times the
     mean over all these tokens of the squared log of their logits' exponentials' sum.  It is 1 where all is even.
-    ``offsets`` (sequences + 1) int32 says where each sequence begins, and the end; tokens outside count nowhere, and
+    ``offsets`` (sequences + 1) int32, at most 65535 sequences, says where each begins, and the end; tokens outside count nowhere, and
     without it all tokens are one sequence.
 
     The counts are whole numbers, and their sum over ranks is that of all ranks' tokens: put into the place of a rank's own

@@ -128,7 +128,7 @@ def balance_op(**kw):
 @pytest.mark.parametrize("code,kw", [
     (_lib.ERR_ARG, {"dtype": _lib.BYTES}), (_lib.ERR_ARG, {"score": 2}), (_lib.ERR_ARG, {"experts": 0}), (_lib.ERR_ARG, {"experts": 1025}), (_lib.ERR_ARG, {"topk": 0}),
     (_lib.ERR_ARG, {"topk": 1025}), (_lib.ERR_ARG, {"logits": 0}), (_lib.ERR_ARG, {"chosen": 0}), (_lib.ERR_ARG, {"offsets": 4096, "sequences": 0}),
-    (_lib.ERR_TOO_LARGE, {"tokens": 1 << 31}), (_lib.ERR_TOO_LARGE, {"offsets": 4096, "sequences": (1 << 20) + 1})])
+    (_lib.ERR_TOO_LARGE, {"tokens": 1 << 31}), (_lib.ERR_TOO_LARGE, {"offsets": 4096, "sequences": 1 << 16})])
 def test_balance_refuses(code, kw):
     L = _lib.lib()
     assert L.mint_balance(balance_op(**kw), 4096, 4096, 4096, 4096, 1 << 20, 1 << 20, None) == code

@@ -100,6 +100,37 @@ def test_tokens_outside_the_sequences(dev):
     assert float(nowhere.loss) == 0 and int(nowhere.counts.sum()) == 0 and int(nowhere.there.sum()) == 0
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_as_many_sequences_as_there_may_be(dev, score):
+    """65535 sequences of one token, of none and of two, tokens before them and behind them: each has a term of its own."""
+    t, e, s, before = 66000, 20, 65535, 311
+    x, _ = inputs(t, e, 1, "f32", dev, masks=False)
+    experts = torch.randint(0, e, (t, 1), generator=torch.Generator().manual_seed(3)).int().to(dev)
+    lengths = torch.ones(s, dtype=torch.int64)
+    lengths[5::64], lengths[6::64] = 0, 2
+    ends = before + torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)])
+    got = balance(x, experts, score=score, offsets=ends.int().to(dev), z=0.0)
+    leaf = x.cpu().double().requires_grad_()
+    p = torch.softmax(leaf, 1) if score == "softmax" else torch.sigmoid(leaf) / torch.sigmoid(leaf).sum(1, keepdim=True)
+    of = torch.repeat_interleave(torch.arange(s), lengths)
+    inside = slice(before, before + len(of))
+    n = lengths.clamp_min(1).double()[:, None]
+    shares = torch.zeros(s, e, dtype=torch.float64).index_add(0, of, p[inside]) / n
+    counts = torch.zeros(s, e, dtype=torch.float64).index_add(0, of, torch.nn.functional.one_hot(experts.cpu()[inside, 0].long(), e).double())
+    loss = (counts * e / n * shares).sum() / (lengths > 0).sum()
+    assert torch.equal(got.counts.cpu().double(), counts) and torch.equal(got.there.cpu().long(), lengths)
+    close(got.shares, shares.detach(), shares.detach(), torch.float32, SHARE + 4 * UNIT)
+    # (a sequence's terms in two blocks of 16 experts, 64 sequences to a thread, lanes and wavefronts)
+    close(got.loss, loss.detach(), loss.detach(), torch.float32, SHARE + (4 + 8 + 64 + 6 + 16) * UNIT)
+    grad = balance_grad(torch.tensor(1e4, device=dev), x, experts, got, score=score, offsets=ends.int().to(dev))
+    want = torch.autograd.grad(loss * 1e4, leaf)[0]
+    load = torch.zeros(t, e, dtype=torch.float64)
+    load[inside] = (counts * e / n / n / (lengths > 0).sum() * 1e4)[of]
+    size = p.detach() * (load + (p.detach() * load).sum(1, keepdim=True))
+    close(grad, want, size, torch.float32, 4 * SHARE)
+    assert not grad[:before].any() and not grad[before + len(of):].any()
+
+
 def test_offsets_that_say_anything(dev):
     """Offsets that descend, are negative or beyond the tokens: nothing outside is read or written, whatever comes out."""
     x, experts = inputs(100, 9, 2, "f32", dev, masks=False)
