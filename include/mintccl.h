@@ -696,7 +696,8 @@ int mint_join_grad(const mint_join_grad_op* op, void* stream);
  * PRODUCT alone takes bias, residual, activation and z (0: not wanted).  Rows
  * may be any distance apart and start at any element; where they start at
  * multiples of 16 bytes a row is read up to the 16 bytes that it ends in.
- * residual may be out itself.  workspace: mint_dense_workspace() bytes, 16-byte aligned. */
+ * residual may be out itself.  workspace: mint_dense_workspace() bytes (of this op: the operands'
+ * addresses and strides count), 16-byte aligned. */
 typedef enum { MINT_DENSE_PRODUCT = 0, MINT_DENSE_INPUT_GRAD = 1, MINT_DENSE_WEIGHT_GRAD = 2 } mint_dense_form;
 typedef struct {
     int32_t form;          /* mint_dense_form */

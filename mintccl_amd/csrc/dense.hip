@@ -274,7 +274,7 @@ struct Ring {
 //   - the rest follows, each operand read some products ahead, and w's for the next step
 //   - units of x NX - 1 on and of w NW on are asked for, into places that are no longer read: w's of a step has been read before it
 // and at its end the wavefronts meet when what the next step reads has come: asked for two steps before and more.  DIRECT: rows in memory
-// begin at multiples of 16 bytes, and their pieces go straight into LDS; else they pass through registers, a block at a time.
+// begin at multiples of 16 bytes (or were copied there), and their pieces go straight into LDS; else they pass through registers, a block at a time.
 template <int DT, int BM, int BN, int WM, int NX, int NW, bool X_ALONG, bool W_ALONG>
 struct Tile {
     static constexpr int WN = BN / 64, WAVES = WM * WN, MT = BM / WM / 16, NT = 4;
@@ -603,6 +603,36 @@ __global__ void __launch_bounds__(256) dense_join_kernel(DenseArgs a) {
     finish8<DT>(a.f, row, col, a.w.n, bias, more, sum);
 }
 
+// ---- operands at any address ------------------------------------------------------------
+// Rows, copied to multiples of 16 bytes, zeros behind their ends.  Both operands of a product in one launch.  Bound by memory: 4096 x 4095 numbers of 16
+// bits each, 134 MB read and written, 26 us, 5.2 TB/s.
+struct Copy {
+    const uint8_t* from;
+    uint8_t* to;
+    int64_t stride;
+    uint32_t bytes, pieces, units;       // of a row: its length, 16 bytes each; all rows' pieces (0: nothing to do)
+};
+constexpr int kCopies = 4;               // pieces of a thread
+template <uint32_t SIZE>
+__global__ void __launch_bounds__(256) copy_kernel(Copy x, Copy w) {
+    u32x4 v[kCopies];
+    uint8_t* to[kCopies];
+#pragma unroll
+    for (int u = 0; u < kCopies; ++u) {
+        const uint64_t unit = (uint64_t)blockIdx.x * (256 * kCopies) + u * 256 + threadIdx.x;
+        const Copy& c = unit < x.units ? x : w;
+        const uint64_t at = unit < x.units ? unit : unit - x.units;
+        to[u] = nullptr;
+        if (at >= c.units) continue;
+        const uint32_t row = (uint32_t)at / c.pieces, piece = (uint32_t)at % c.pieces;
+        v[u] = piece_of<SIZE>(c.from + row * c.stride + (uint64_t)piece * 16, (int64_t)c.bytes - (int64_t)piece * 16);
+        to[u] = c.to + at * 16;
+    }
+#pragma unroll
+    for (int u = 0; u < kCopies; ++u)
+        if (to[u]) *(MINT_GLOBAL u32x4*)as_global(to[u]) = v[u];
+}
+
 // ---- products of few rows ------------------------------------------------------------
 // Both operands along.  A wavefront has 16 columns and one of KWAYS parts of the depth, straight from memory into registers: it asks for AHEAD
 // blocks before it multiplies the first.  The KWAYS wavefronts' sums of a column are added up in LDS, in their order.  Bound by w's bytes: one row,
@@ -741,6 +771,8 @@ enum { kThin, k64Four, k64Two, k128, k128Two, k128x256, k256, kHeld64, kHeld128 
 struct Choice {
     int tile;
     uint32_t parts;
+    float time;
+    bool copies;                             // of the operands that are not at multiples of 16 bytes
 };
 struct Cost {
     int tile;
@@ -751,14 +783,18 @@ constexpr Cost kCosts[] = {{k64Four, 64, 64, 256, 256, 3.5f, 0.22f, 0.53f},   {k
                            {k128, 128, 128, 256, 256, 4.0f, 0.48f, 1.9f},     {k128, 128, 128, 512, ~0u, 6.0f, 0.89f, 3.65f},
                            {k128Two, 128, 128, 256, 256, 6.0f, 0.39f, 1.9f},  {k128x256, 128, 256, 256, ~0u, 7.5f, 0.78f, 0.0f},
                            {k256, 256, 256, 128, 128, 10.5f, 1.03f, 0.0f},    {k256, 256, 256, 256, ~0u, 10.5f, 1.34f, 0.0f}};
-constexpr Cost kHeldCosts[] = {{kHeld64, 64, 64, 512, ~0u, 3.5f, 0.8f, 1.3f}, {kHeld128, 128, 128, 512, ~0u, 6.0f, 1.8f, 4.5f}};
+// Operands that are not at multiples of 16 bytes: through registers, or copied first.  4096 x 4095 x 4095: x w^T 213 through registers, 162 copied, d_z w 351 and
+// 146, d_z^T x 597 and 156; 1000 x 1001 x 1003 f32, x w^T 33 and 39; 300 x 1001 x 701 f16 10.4 and 17.
+constexpr Cost kHeldCosts[] = {{kHeld64, 64, 64, 256, 256, 3.5f, 0.8f, 0.85f}, {kHeld64, 64, 64, 512, ~0u, 3.5f, 0.8f, 1.3f}, {kHeld128, 128, 128, 512, ~0u, 6.0f, 1.8f, 4.5f}};
+constexpr float kHeldForms[] = {1.0f, 1.6f, 2.7f}, kHeldForms32[] = {1.0f, 1.1f, 1.15f};     // ... a block takes, by form
+constexpr float kCopyBegin = 6.0f, kCopyRate = 3.5e6f;       // us; bytes per us, read and written
 template <int N>
-Choice cheapest(const Cost (&costs)[N], const mint_dense_op& op) {
+Choice cheapest(const Cost (&costs)[N], const mint_dense_op& op, float of_block = 1.0f) {
     const uint64_t blocks = ceil_div(op.depth * size_of(op.dtype), 128);
-    Choice best = {costs[0].tile, 1};
+    Choice best = {costs[0].tile, 1, 0.0f, false};
     float least = 1e30f;
     for (const Cost& c : costs) {
-        const float block = op.dtype == MINT_F32 ? c.block32 : c.block;
+        const float block = (op.dtype == MINT_F32 ? c.block32 : c.block) * of_block;
         const uint64_t tiles = ceil_div(op.rows, c.rows) * ceil_div(op.cols, c.cols);
         if (block == 0.0f || tiles > c.most) continue;
         const uint64_t most = tiles >= c.round ? 1 : std::min<uint64_t>(c.round / tiles, std::max<uint64_t>(blocks / 8, 1));
@@ -768,24 +804,52 @@ Choice cheapest(const Cost (&costs)[N], const mint_dense_op& op) {
             if (parts > 1) t += 2.5f + (float)(op.rows * op.cols) * (float)parts * (8.0f / 4.5e6f);
             if (t < least) {
                 least = t;
-                best = {c.tile, (uint32_t)parts};
+                best = {c.tile, (uint32_t)parts, t, false};
             }
         }
     }
     return best;
 }
-bool direct(const mint_dense_op& op) {
-    const int64_t size = size_of(op.dtype);
+// an operand as it lies in memory
+struct Operand {
+    uint64_t p;
+    int64_t stride;                          // bytes
+    uint64_t rows, bytes;                    // ... of a row
+    uint64_t pieces() const { return ceil_div(bytes, 16); }
     // (a stride is looked at only where there is more than one row; a tile's rows have to be in reach of 32 bits)
-    const int64_t far = 1ll << 23;
-    const uint64_t x_rows = op.form == MINT_DENSE_WEIGHT_GRAD ? op.depth : op.rows, w_rows = op.form == MINT_DENSE_PRODUCT ? op.cols : op.depth;
-    return op.x % 16 == 0 && op.w % 16 == 0 && (x_rows <= 1 || (op.x_stride * size % 16 == 0 && op.x_stride >= 0 && op.x_stride * size < far)) &&
-           (w_rows <= 1 || (op.w_stride * size % 16 == 0 && op.w_stride >= 0 && op.w_stride * size < far));
+    static constexpr int64_t kFar = 1ll << 23;
+    bool direct() const { return p % 16 == 0 && (rows <= 1 || (stride % 16 == 0 && stride >= 0 && stride < kFar)); }
+    bool copied() const { return pieces() * 16 < (uint64_t)kFar && rows * pieces() <= 0xFFFFFFFFull; }
+    uint64_t room() const { return direct() ? 0 : rows * pieces() * 16; }
+};
+Operand x_of(const mint_dense_op& op) {
+    const uint64_t size = size_of(op.dtype), across = op.form == MINT_DENSE_WEIGHT_GRAD;
+    return {op.x, op.x_stride * (int64_t)size, across ? op.depth : op.rows, (across ? op.rows : op.depth) * size};
+}
+Operand w_of(const mint_dense_op& op) {
+    const uint64_t size = size_of(op.dtype), across = op.form != MINT_DENSE_PRODUCT;
+    return {op.w, op.w_stride * (int64_t)size, across ? op.depth : op.cols, (across ? op.cols : op.depth) * size};
 }
 Choice choose(const mint_dense_op& op) {
-    if (op.form == MINT_DENSE_PRODUCT && op.rows <= 32) return {kThin, 1};
-    return direct(op) ? cheapest(kCosts, op) : cheapest(kHeldCosts, op);
+    if (op.form == MINT_DENSE_PRODUCT && op.rows <= 32) return {kThin, 1, 0.0f, false};
+    const Operand x = x_of(op), w = w_of(op);
+    const Choice best = cheapest(kCosts, op);
+    if (op.depth == 0 || (x.direct() && w.direct())) return best;
+    const Choice held = cheapest(kHeldCosts, op, (op.dtype == MINT_F32 ? kHeldForms32 : kHeldForms)[op.form]);
+    if ((!x.direct() && !x.copied()) || (!w.direct() && !w.copied())) return held;
+    if (held.time <= best.time + kCopyBegin + 2.0f * (float)(x.room() + w.room()) / kCopyRate) return held;
+    return {best.tile, best.parts, best.time, true};
 }
+// where in the workspace copies and the parts' sums are
+struct Room {
+    uint64_t x, w, sums, bytes;
+    Room(const mint_dense_op& op, const Choice& c) {
+        x = 0;
+        w = x + (c.copies ? x_of(op).room() : 0);
+        sums = w + (c.copies ? w_of(op).room() : 0);
+        bytes = sums + (c.parts > 1 ? (uint64_t)c.parts * op.rows * op.cols * 4 : 0);
+    }
+};
 template <int DT, int BM, int BN, int WM, int NX, int NW, int SPLIT, bool X_ALONG, bool W_ALONG, bool DIRECT>
 int go_tiles(DenseArgs a, hipStream_t s) {
     a.row_tiles = (uint32_t)ceil_div(a.x.n, BM);
@@ -818,11 +882,25 @@ int go_thin(DenseArgs a, hipStream_t s) {
     return Launch<&dense_thin_kernel<DT, MT, KWAYS>>::go((uint32_t)blocks, 64 * kThinWaves, 0, s, a);
 }
 template <int DT>
-int go_dense(const mint_dense_op& op, const DenseArgs& a, const Choice& c, hipStream_t s) {
+int go_dense(const mint_dense_op& op, DenseArgs a, const Choice& c, hipStream_t s) {
     if (c.tile == kThin) {
         const bool few = ceil_div(op.cols, 16) <= 768;
         if (op.rows <= 16) return few ? go_thin<DT, 1, 8>(a, s) : go_thin<DT, 1, 2>(a, s);
         return few ? go_thin<DT, 2, 8>(a, s) : go_thin<DT, 2, 2>(a, s);
+    }
+    if (c.copies) {
+        const auto one = [](const Operand& o, uint8_t* to) {
+            const bool any = !o.direct();
+            return Copy{reinterpret_cast<const uint8_t*>(o.p), to, o.stride, (uint32_t)o.bytes, (uint32_t)o.pieces(), any ? (uint32_t)(o.rows * o.pieces()) : 0u};
+        };
+        const Room room(op, c);
+        auto* const at = reinterpret_cast<uint8_t*>(op.workspace);
+        const Copy x = one(x_of(op), at + room.x), w = one(w_of(op), at + room.w);
+        if (x.units) a.x = {x.to, (int64_t)x.pieces * 16, a.x.n};
+        if (w.units) a.w = {w.to, (int64_t)w.pieces * 16, a.w.n};
+        const uint64_t blocks = ceil_div((uint64_t)x.units + w.units, 256 * kCopies);
+        const int err = Launch<&copy_kernel<kSize<DT>>>::go((uint32_t)blocks, 256, 0, s, x, w);
+        if (err != MINT_OK) return err;
     }
     int err;
     switch (op.form) {
@@ -846,13 +924,11 @@ uint32_t grad_groups(uint64_t rows, uint64_t cols) {
 
 using namespace mint;
 
-namespace {
-size_t room_of(const mint_dense_op& op, const Choice& c) { return c.parts > 1 ? (size_t)c.parts * op.rows * op.cols * 4 : 0; }
-}  // namespace
-
 extern "C" size_t mint_dense_workspace(const mint_dense_op* op) {
-    if (!op || !known(op->dtype) || op->rows == 0 || op->cols == 0 || op->rows > kMost || op->cols > kMost || op->depth > kMost) return 0;
-    return room_of(*op, choose(*op));
+    if (!op || !known(op->dtype) || op->form < MINT_DENSE_PRODUCT || op->form > MINT_DENSE_WEIGHT_GRAD || op->rows == 0 || op->cols == 0 || op->rows > kMost ||
+        op->cols > kMost || op->depth > kMost)
+        return 0;
+    return Room(*op, choose(*op)).bytes;
 }
 
 extern "C" int mint_dense(const mint_dense_op* op, void* stream) {
@@ -864,7 +940,8 @@ extern "C" int mint_dense(const mint_dense_op* op, void* stream) {
     if (op->rows == 0 || op->cols == 0) return MINT_OK;
     if (!op->out || (op->depth && (!op->x || !op->w))) return MINT_ERR_ARG;
     const Choice c = choose(*op);
-    const size_t need = room_of(*op, c);
+    const Room room(*op, c);
+    const size_t need = room.bytes;
     if (need && (!op->workspace || op->workspace_bytes < need)) return MINT_ERR_STAGING;
     if (need && op->workspace % 16) return MINT_ERR_ALIGN;
     const int64_t size = size_of(op->dtype);
@@ -872,7 +949,7 @@ extern "C" int mint_dense(const mint_dense_op* op, void* stream) {
                          {reinterpret_cast<const uint8_t*>(op->w), op->w_stride * size, (uint32_t)op->cols},
                          {reinterpret_cast<const void*>(op->bias), reinterpret_cast<const void*>(op->residual), reinterpret_cast<void*>(op->out),
                           reinterpret_cast<void*>(op->z), op->residual_stride, op->out_stride, op->z_stride, op->out_dtype, op->activation},
-                         (uint32_t)op->depth, 0, 0, c.parts, reinterpret_cast<float*>(op->workspace)};
+                         (uint32_t)op->depth, 0, 0, c.parts, reinterpret_cast<float*>(op->workspace + room.sums)};
     const auto s = static_cast<hipStream_t>(stream);
     switch (op->dtype) {
         case MINT_F16: return go_dense<DT_F16>(*op, a, c, s);

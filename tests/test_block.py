@@ -108,6 +108,11 @@ def test_dense_workspace():
     # (whole copies of the result)
     room = L.mint_dense_workspace(dense_op(rows=64, depth=65536))
     assert room > 0 and room % (64 * 64 * 4) == 0
+    # (copies of operands that are not at multiples of 16 bytes: both, or one)
+    big = dict(rows=1024, cols=1001, depth=1001, x_stride=1001, w_stride=1001, out_stride=1001)
+    assert L.mint_dense_workspace(dense_op(form=2, **{**big, "w_stride": 1008})) == 1001 * 2048
+    assert L.mint_dense_workspace(dense_op(form=2, **{**big, "x_stride": 1024, "x": 4098})) == 1001 * 2048 + 1001 * 2016
+    assert L.mint_dense_workspace(dense_op(form=2, **{**big, "x_stride": 1024, "w_stride": 1008})) == 0
     assert L.mint_activation_grad_workspace(0, 5) == L.mint_activation_grad_workspace(5, 0) == 0 and L.mint_activation_grad_workspace(5, 100) == 5 * 100 * 4
 
 

@@ -119,6 +119,25 @@ def test_rows_any_distance_apart(dev, rows, cols, depth, dt):
             assert same(got, ref) or bool(((got.double() - ref.double()).abs().cpu() <= 2 * (HALF_ULP[DT[dt]] * ref.double().abs().cpu() + sum_units(units, dt) * size)).all())
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("off_x,off_w", [(0, 1), (1, 0), (1, 1), (3, 8)])
+@pytest.mark.parametrize("rows,cols,depth", [(700, 1001, 2051), (1030, 2000, 1992)])
+def test_operands_that_are_copied(dev, rows, cols, depth, off_x, off_w, dt):
+    """Rows that begin at any number of a wider matrix, both operands or one of them, whose surroundings are not read into the result."""
+    def rows_at(t, off):
+        room = torch.full((t.shape[0] + 1, t.shape[1] + 24), float("nan"), dtype=t.dtype, device=dev)
+        room[:-1, off:off + t.shape[1]] = t
+        return room[:-1, off:off + t.shape[1]]
+    x, w = operands(rows, cols, depth, dt, dev)
+    want, size = product64(x, w)
+    close(product(rows_at(x, off_x), rows_at(w, off_w)), want, size, DT[dt], sum_units(depth, dt))
+    d = randn(rows, cols, seed=3, dtype=DT[dt], dev=dev)
+    want, size = product64(d, w.t())
+    close(input_grad(rows_at(d, off_x), rows_at(w, off_w)), want, size, DT[dt], sum_units(cols, dt))
+    want, size = product64(d.t(), x.t())
+    close(weight_grad(rows_at(d, off_x), rows_at(x, off_w)), want, size, DT[dt], sum_units(rows, dt))
+
+
 def test_nothing_to_do(dev):
     z = torch.zeros
     for dt in DT.values():
