@@ -758,15 +758,18 @@ constexpr uint64_t kMost = 0x7FFFFFFF - 256;
 uint32_t size_of(int dtype) { return dtype == MINT_F32 ? 4 : 2; }
 
 // Which tiles, and how many thread blocks share one.  What a launch takes by this, us: 2.5, and for each round over the compute units a beginning and an
-// end and so much for a block of the depth (128 bytes); sums that pass through memory take another launch and their bytes. Measured (bf16
+// end and so much for a block of the depth (128 bytes), less of both in a last round of `few` tiles; sums that pass through memory take another launch and their bytes. Measured (bf16
 // if not said otherwise, operands used in turn), and the rule's choice behind =:
 //   4096 x 256 x 4096 f32       64 x 64 74, in two sets 76, 128 x 128 134 (two parts)                    = 64 x 64
-//   512 x 4096 x 4096           64 x 64 in two sets 31.7, 128 x 128 in two sets 32.9, in one 37, 128 x 256 47     = 64 x 64 in two sets
+//   512 x 4096 x 4096           64 x 64 in two sets 28.5 - 31.7, 128 x 128 in two sets 31.7 - 32.9, in two parts of them 30 = the last of these
 //   1024 x 4096 x 4096          128 x 128 in two sets 35.4, in one 38.4, 128 x 256 47                    = 128 x 128 in two sets
 //   2048 x 4096 x 4096          128 x 256 60, 128 x 128 64, 256 x 256 79                                 = 128 x 256
 //   8192 x 1024 x 512           128 x 128 15.8, 128 x 256 17.2, 256 x 256 22.5                           = 128 x 128
 //   4096 x 4096 x 512 (d_w)     256 x 256 26.4, 128 x 128 28.3, 128 x 256 34                             = 256 x 256
 //   64 x 4096 x 4096            64 x 64 in one part 17.5, two 15.6, four 15.4                            = four
+//   3000 x 2000 x 4000 f32      128 x 128 in two parts 370, 64 x 64 387, 128 x 128 in one 461            = 128 x 128 in two parts
+//   700 x 3000 x 5000           128 x 256 in three parts 45, 128 x 128 in three 48, in two sets 56       = 128 x 128 in two sets (rows that begin inside
+//                               lines of 128 bytes, which the model does not know of)
 enum { kThin, k64Four, k64Two, k128, k128Two, k128x256, k256, kHeld64, kHeld128 };
 struct Choice {
     int tile;
@@ -778,14 +781,19 @@ struct Cost {
     int tile;
     uint32_t rows, cols, round, most;        // tiles of a round; most tiles that it is for
     float begin, block, block32;             // us; 32-bit operands' (0: not for them)
+    uint32_t few;                            // so few tiles have a compute unit (or memory) to themselves, and take
+    float few_begin, few_block, few_block32;
 };
-constexpr Cost kCosts[] = {{k64Four, 64, 64, 256, 256, 3.5f, 0.22f, 0.53f},   {k64Two, 64, 64, 512, ~0u, 3.5f, 0.42f, 1.02f},
-                           {k128, 128, 128, 256, 256, 4.0f, 0.48f, 1.9f},     {k128, 128, 128, 512, ~0u, 6.0f, 0.89f, 3.65f},
-                           {k128Two, 128, 128, 256, 256, 6.0f, 0.39f, 1.9f},  {k128x256, 128, 256, 256, ~0u, 7.5f, 0.78f, 0.0f},
-                           {k256, 256, 256, 128, 128, 10.5f, 1.03f, 0.0f},    {k256, 256, 256, 256, ~0u, 10.5f, 1.34f, 0.0f}};
+constexpr Cost kCosts[] = {{k64Four, 64, 64, 256, 256, 3.5f, 0.22f, 0.53f, 0, 0, 0, 0},
+                           {k64Two, 64, 64, 512, ~0u, 3.5f, 0.42f, 1.02f, 256, 3.5f, 0.25f, 0.55f},
+                           {k128, 128, 128, 512, ~0u, 6.0f, 0.89f, 3.65f, 256, 4.0f, 0.48f, 1.9f},
+                           {k128Two, 128, 128, 256, 256, 6.0f, 0.39f, 1.8f, 0, 0, 0, 0},
+                           {k128x256, 128, 256, 256, ~0u, 7.5f, 0.78f, 0.0f, 0, 0, 0, 0},
+                           {k256, 256, 256, 256, ~0u, 10.5f, 1.34f, 0.0f, 128, 10.5f, 1.03f, 0.0f}};
 // Operands that are not at multiples of 16 bytes: through registers, or copied first.  4096 x 4095 x 4095: x w^T 213 through registers, 162 copied, d_z w 351 and
 // 146, d_z^T x 597 and 156; 1000 x 1001 x 1003 f32, x w^T 33 and 39; 300 x 1001 x 701 f16 10.4 and 17.
-constexpr Cost kHeldCosts[] = {{kHeld64, 64, 64, 256, 256, 3.5f, 0.8f, 0.85f}, {kHeld64, 64, 64, 512, ~0u, 3.5f, 0.8f, 1.3f}, {kHeld128, 128, 128, 512, ~0u, 6.0f, 1.8f, 4.5f}};
+constexpr Cost kHeldCosts[] = {{kHeld64, 64, 64, 512, ~0u, 3.5f, 0.8f, 1.3f, 256, 3.5f, 0.8f, 0.85f},
+                               {kHeld128, 128, 128, 512, ~0u, 6.0f, 1.8f, 4.5f, 0, 0, 0, 0}};
 constexpr float kHeldForms[] = {1.0f, 1.6f, 2.7f}, kHeldForms32[] = {1.0f, 1.1f, 1.15f};     // ... a block takes, by form
 constexpr float kCopyBegin = 6.0f, kCopyRate = 3.5e6f;       // us; bytes per us, read and written
 template <int N>
@@ -794,13 +802,16 @@ Choice cheapest(const Cost (&costs)[N], const mint_dense_op& op, float of_block 
     Choice best = {costs[0].tile, 1, 0.0f, false};
     float least = 1e30f;
     for (const Cost& c : costs) {
-        const float block = (op.dtype == MINT_F32 ? c.block32 : c.block) * of_block;
+        const float block = (op.dtype == MINT_F32 ? c.block32 : c.block) * of_block, few = (op.dtype == MINT_F32 ? c.few_block32 : c.few_block) * of_block;
         const uint64_t tiles = ceil_div(op.rows, c.rows) * ceil_div(op.cols, c.cols);
         if (block == 0.0f || tiles > c.most) continue;
-        const uint64_t most = tiles >= c.round ? 1 : std::min<uint64_t>(c.round / tiles, std::max<uint64_t>(blocks / 8, 1));
+        const uint64_t most = std::max<uint64_t>(std::min<uint64_t>(2 * c.round / tiles, blocks / 8), 1);
         for (uint64_t parts = 1, each; parts <= most; parts = each > 1 ? ceil_div(blocks, each - 1) : most + 1) {
             each = ceil_div(blocks, parts);                  // (more parts of as many blocks only cost more: on to the next ones of fewer)
-            float t = (float)ceil_div(tiles * parts, c.round) * (c.begin + (float)each * block);
+            const uint64_t rounds = tiles * parts / c.round, rest = tiles * parts % c.round;
+            if (tiles * parts > c.most) break;
+            float t = (float)rounds * (c.begin + (float)each * block);
+            if (rest) t += rest <= c.few ? c.few_begin + (float)each * few : c.begin + (float)each * block;
             if (parts > 1) t += 2.5f + (float)(op.rows * op.cols) * (float)parts * (8.0f / 4.5e6f);
             if (t < least) {
                 least = t;
