@@ -770,7 +770,7 @@ uint32_t size_of(int dtype) { return dtype == MINT_F32 ? 4 : 2; }
 //   3000 x 2000 x 4000 f32      128 x 128 in two parts 370, 64 x 64 387, 128 x 128 in one 461            = 128 x 128 in two parts
 //   700 x 3000 x 5000           128 x 256 in three parts 45, 128 x 128 in three 48, in two sets 56       = 128 x 128 in two sets (rows that begin inside
 //                               lines of 128 bytes, which the model does not know of)
-enum { kThin, k64Four, k64Two, k128, k128Two, k128x256, k256, kHeld64, kHeld128 };
+enum { kThin, k64Four, k64Two, k128, k128Two, k128x256, k256, kHeld };
 struct Choice {
     int tile;
     uint32_t parts;
@@ -792,8 +792,7 @@ constexpr Cost kCosts[] = {{k64Four, 64, 64, 256, 256, 3.5f, 0.22f, 0.53f, 0, 0,
                            {k256, 256, 256, 256, ~0u, 10.5f, 1.34f, 0.0f, 128, 10.5f, 1.03f, 0.0f}};
 // Operands that are not at multiples of 16 bytes: through registers, or copied first.  4096 x 4095 x 4095: x w^T 213 through registers, 162 copied, d_z w 351 and
 // 146, d_z^T x 597 and 156; 1000 x 1001 x 1003 f32, x w^T 33 and 39; 300 x 1001 x 701 f16 10.4 and 17.
-constexpr Cost kHeldCosts[] = {{kHeld64, 64, 64, 512, ~0u, 3.5f, 0.8f, 1.3f, 256, 3.5f, 0.8f, 0.85f},
-                               {kHeld128, 128, 128, 512, ~0u, 6.0f, 1.8f, 4.5f, 0, 0, 0, 0}};
+constexpr Cost kHeldCosts[] = {{kHeld, 64, 64, 512, ~0u, 3.5f, 0.8f, 1.3f, 256, 3.5f, 0.8f, 0.85f}};
 constexpr float kHeldForms[] = {1.0f, 1.6f, 2.7f}, kHeldForms32[] = {1.0f, 1.1f, 1.15f};     // ... a block takes, by form
 constexpr float kCopyBegin = 6.0f, kCopyRate = 3.5e6f;       // us; bytes per us, read and written
 template <int N>
@@ -877,8 +876,7 @@ int go_form(const DenseArgs& a, int tile, hipStream_t s) {
         if (tile == k128x256) return go_tiles<DT, 128, 256, 2, XA ? 4 : 8, WA ? 3 : 6, 1, XA, WA, true>(a, s);
     }
     switch (tile) {
-        case kHeld64: return go_tiles<DT, 64, 64, 4, X2, W2, 2, XA, WA, false>(a, s);
-        case kHeld128: return go_tiles<DT, 128, 128, 4, X2, W2, 1, XA, WA, false>(a, s);
+        case kHeld: return go_tiles<DT, 64, 64, 4, X2, W2, 2, XA, WA, false>(a, s);
         case k64Four: return go_tiles<DT, 64, 64, 2, X2, W2, 4, XA, WA, true>(a, s);
         case k64Two: return go_tiles<DT, 64, 64, 2, X2, W2, 2, XA, WA, true>(a, s);
         case k128Two: return go_tiles<DT, 128, 128, 2, X2, W2, 2, XA, WA, true>(a, s);

@@ -41,6 +41,10 @@ def offsets_of(lengths, dev, start=0):
     return None if lengths is None else torch.tensor([start + sum(lengths[:i]) for i in range(len(lengths) + 1)], dtype=torch.int32, device=dev)
 
 
+#: each number of experts of a lane in each type, alone and in tiles
+CASES += [(t, e, 4, ("softmax", "sigmoid")[i % 2], None, 1e-3, dt) for i, e in enumerate((60, 100, 250, 500, 1000)) for t in (50, 90) for dt in ("f32", "bf16", "f16")]
+
+
 @pytest.mark.parametrize("t,e,k,score,lengths,z,dt", CASES)
 def test_balance_and_its_gradient(dev, t, e, k, score, lengths, z, dt):
     x, experts = inputs(t, e, k, dt, dev)

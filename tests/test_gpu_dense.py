@@ -39,6 +39,19 @@ def test_gradients_of_a_product(dev, rows, cols, depth, dt):
     close(weight_grad(d, x, dtype=torch.float32), want, size, torch.float32, sum_units(rows, dt))
 
 
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("rows,cols,depth", [(192, 200, 4000), (1096, 1032, 1000), (2000, 2000, 136), (904, 2200, 1528), (1304, 3000, 1000), (3584, 4096, 128),
+                                             (1704, 600, 2000), (20, 12304, 72), (7, 12304, 72)])
+def test_every_tile(dev, rows, cols, depth, dt):
+    """The result's rows and columns and the sums' length decide about the tiles: each kind of them in each of the three forms."""
+    x, w = operands(rows, cols, depth, dt, dev)
+    want, size = product64(x, w)
+    units = sum_units(depth, dt)
+    close(product(x, w), want, size, DT[dt], units)
+    close(input_grad(x, w.t().contiguous()), want, size, DT[dt], units)
+    close(weight_grad(x.t().contiguous(), w.t().contiguous()), want, size, DT[dt], units)
+
+
 @pytest.mark.parametrize("activation", [None, "relu", "silu", "sigmoid", "tanh", "gelu", "gelu_tanh"])
 @pytest.mark.parametrize("dt,wide", [("bf16", False), ("bf16", True), ("f16", False), ("f32", False)])
 @pytest.mark.parametrize("rows,cols,depth", [(1, 70, 100), (20, 333, 129), (70, 130, 64), (90, 77, 4000), (140, 1700, 96), (300, 2100, 41)])

@@ -92,6 +92,15 @@ def test_join_and_its_gradient(dev, width, s_dt, dt):
         check_join(dev, rows_for(width), width, ("rms", "layer")[i % 2], i % 2 == 1, s_dt, dt, True, True, gate, by)
 
 
+@pytest.mark.parametrize("width", [64, 70, 1024, 1023, 2048, 2047, 4096, 4095, 8192, 8191])
+@pytest.mark.parametrize("s_dt,dt", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32"), ("f32", "bf16"), ("f32", "f16")])
+def test_every_gate_with_and_without_biases(dev, width, s_dt, dt):
+    """All kernels of the gradients: a gate's kind, biases or none, whole lanes or not, each number of lanes."""
+    for gate in ("channel", "row", "all"):
+        for bias in (False, True):
+            check_join(dev, 5, width, "layer", bias, s_dt, dt, True, True, gate, "tanh")
+
+
 @pytest.mark.parametrize("gate,by", GATES)
 @pytest.mark.parametrize("after,before", [(False, False), (True, False), (False, True), (True, True)])
 @pytest.mark.parametrize("width", [130, 1500, 9001])
