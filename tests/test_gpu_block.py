@@ -162,3 +162,41 @@ def test_results_that_share_memory(dev):
     s = want.clone()
     again, also = join(s, y, before=n, out=s)
     assert torch.equal(again, both) and torch.equal(also, of) and again is s
+
+
+@pytest.mark.parametrize("rows,width", [(600_011, 8192), (300_011, 16384)])
+def test_more_numbers_than_32_bits_count(dev, rows, width):
+    """Over 2^32 numbers in an operand or a result: the last rows are what they are alone."""
+    g = torch.Generator(dev).manual_seed(3)
+    x = torch.empty(rows, width, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    n = Norm(torch.empty(width, device=dev).normal_(generator=g))
+    tail = x[-5:].clone()
+    got = norm(x, n)
+    assert torch.equal(got[-5:], norm(tail, n))
+    new, behind = join(x, got, gate=n.weight, before=n)
+    alone = join(tail, got[-5:].clone(), gate=n.weight, before=n)
+    assert torch.equal(new[-5:], alone[0]) and torch.equal(behind[-5:], alone[1])
+    d = join_grad(new, behind, new, got, gate=n.weight, before=n)
+    alone = join_grad(*alone, alone[0], got[-5:].clone(), gate=n.weight, before=n)
+    assert torch.equal(d.stream[-5:], alone.stream) and torch.equal(d.y[-5:], alone.y)
+    del d, new, behind, got
+    # sums are of bf16's exact products, in 32 bits: off by a bf16 rounding, and less than 2^-24 for each of their terms
+    def near(found, want, size, terms):
+        return bool(((found.double() - want).abs() <= want.abs() * 2 ** -8 + size * (terms + 2) * 2 ** -24).all())
+    w = torch.empty(40, width, dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    z = dense.product(x, w)
+    want, size = tail.double() @ w.double().t(), tail.double().abs() @ w.double().abs().t()
+    assert near(z[-5:], want, size, width)
+    d_x = dense.input_grad(z, w)
+    of = z[-5:].double()
+    assert near(d_x[-5:], of @ w.double(), of.abs() @ w.double().abs(), 40)
+    del d_x
+    d_w = dense.weight_grad(z, x, dtype=torch.float32)
+    want, size = torch.zeros(40, width, dtype=torch.float64, device=dev), torch.zeros(40, width, dtype=torch.float64, device=dev)
+    for i in range(0, rows, 20_000):
+        a, b = z[i:i + 20_000].double().t().contiguous(), x[i:i + 20_000].double()
+        want += a @ b
+        size += a.abs() @ b.abs()
+    assert near(d_w, want, size, rows)
+    d_z, _ = dense.activation_grad(x, x, "silu")
+    assert torch.equal(d_z[-5:], dense.activation_grad(tail, tail, "silu")[0])
