@@ -829,7 +829,8 @@ struct Operand {
     // (a stride is looked at only where there is more than one row; a tile's rows have to be in reach of 32 bits)
     static constexpr int64_t kFar = 1ll << 23;
     bool direct() const { return p % 16 == 0 && (rows <= 1 || (stride % 16 == 0 && stride >= 0 && stride < kFar)); }
-    bool copied() const { return pieces() * 16 < (uint64_t)kFar && rows * pieces() <= 0xFFFFFFFFull; }
+    // (a copy is 4 GiB at most: an operand that fills the memory goes through registers)
+    bool copied() const { return pieces() * 16 < (uint64_t)kFar && rows * pieces() <= 1ull << 28; }
     uint64_t room() const { return direct() ? 0 : rows * pieces() * 16; }
 };
 Operand x_of(const mint_dense_op& op) {

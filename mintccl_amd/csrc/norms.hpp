@@ -231,8 +231,8 @@ constexpr int threads_of(int lanes) { return lanes == 64 ? 256 : lanes; }       
 constexpr int rows_of(int lanes) { return lanes == 64 ? 4 : 1; }
 
 // S: the stream's type, T: that of y and of h.  LANES lanes have every groups-th row, of which the next one is on its way while one is worked on;
-// the weights stay in registers.  Bound by memory: 16384 x 4096 bf16 with a gate by channel 104 us
-// (5.2 TB/s; rows one by one, the weights read again for each, 134), 8192 x 8192 with the stream in 32 bits 164 (4.9).
+// the weights stay in registers.  Bound by memory: 16384 x 4096 bf16 with a gate by channel 101 us
+// (5.3 TB/s; rows one by one, the weights read again for each, 134), 8192 x 8192 with the stream in 32 bits 166 (4.9).
 template <int S, int T, int LANES, bool WHOLE>
 __global__ void __launch_bounds__(threads_of(LANES)) join_kernel(JoinArgs a) {
     using TS = typename Elem<S>::type;
@@ -309,8 +309,8 @@ constexpr int kSums = (BLOCK ? 2 : 1) * (BIAS ? 2 : 1);
 
 // LANES lanes have every groups-th row; the weights stay in registers, and up to 4096 numbers so do the sums over their rows, while the next row is on its
 // way (AHEAD); a thread block of 1024 has the sums in LDS.
-// Bound by memory, and by three meetings for a row: 16384 x 4096 bf16 with a gate by channel 186 us, 4.3 TB/s
-// (twice eight numbers to a lane, half as many wavefronts, nothing held or ahead: 397), 8192 x 8192 with the stream in 32 bits and a gate by row 277, 4.4.
+// Bound by memory, and by three meetings for a row: 16384 x 4096 bf16 with a gate by channel 183 us, 4.4 TB/s
+// (twice eight numbers to a lane, half as many wavefronts, nothing held or ahead: 397), 8192 x 8192 with the stream in 32 bits and a gate by row 291, 4.2.
 template <int S, int T, int LANES, bool WHOLE, bool BLOCK, bool BIAS, int GATE>      // GATE: 0 (none, or by channel), MINT_GATE_ROW, MINT_GATE_ALL
 __global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradArgs a) {
     using TS = typename Elem<S>::type;

@@ -113,6 +113,9 @@ def test_dense_workspace():
     assert L.mint_dense_workspace(dense_op(form=2, **{**big, "w_stride": 1008})) == 1001 * 2048
     assert L.mint_dense_workspace(dense_op(form=2, **{**big, "x_stride": 1024, "x": 4098})) == 1001 * 2048 + 1001 * 2016
     assert L.mint_dense_workspace(dense_op(form=2, **{**big, "x_stride": 1024, "w_stride": 1008})) == 0
+    # (none of an operand of more than 4 GiB)
+    far = dict(rows=1 << 20, cols=4104, depth=4097, x_stride=4097, w_stride=4104, out_stride=4104)
+    assert L.mint_dense_workspace(dense_op(form=1, **far)) == 0 and L.mint_dense_workspace(dense_op(form=1, **{**far, "rows": 1 << 17})) == (1 << 17) * 8208
     assert L.mint_activation_grad_workspace(0, 5) == L.mint_activation_grad_workspace(5, 0) == 0 and L.mint_activation_grad_workspace(5, 100) == 5 * 100 * 4
 
 
