@@ -502,13 +502,15 @@ struct Tile {
 //
 // Bound by the matrix instructions where there are tiles enough for all compute units, then by the last round of tiles and its way out.  bf16, 8192 x 8192 x
 // 4096: x w^T 440 us (1.25 PFLOP/s), d_z w 428, d_z^T x 446 (a library's 436, 436, 496); with bias, an activation of the result and z stored 460.
-// 2048 x 4096 x 4096 with a residual and a result in 32 bits 73 (the library's bare product 59): one round of tiles, whose way out no other hides.  f32, 4096 x 256 x 4096: 74 (116 TFLOP/s).
+// 2048 x 4096 x 4096 with a residual and a result in 32 bits 73 (the library's bare product 59): one round of tiles, whose way out no other hides.  f32, 4096 x 256 x
+// 4096: 67 (128 TFLOP/s; its four sets' sums added up and stored by one of them 69.6; the library's 68.5).
 // Not direct, 50 x 5001 x 2500 f16: 13.4, and 5.3 for the parts' sums (a library's 20.2).
 template <int DT, int BM, int BN, int WM, int NX, int NW, int SPLIT, bool X_ALONG, bool W_ALONG, bool DIRECT>
 __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) dense_kernel(DenseArgs a) {
     using T = Tile<DT, BM, BN, WM, NX, NW, X_ALONG, W_ALONG>;
     constexpr uint32_t SLABS = T::SLABS, PITCH = T::PITCH, kRoom = DIRECT ? T::kStages : 2 * T::kHeld;
-    constexpr uint32_t kLds = SPLIT * kRoom > T::kOut ? SPLIT * kRoom : T::kOut;
+    constexpr uint32_t kRows = BM / WM, kAll = SPLIT * T::WAVES * kRows * PITCH * 4, kOut = SPLIT > 1 ? kAll : T::kOut;
+    constexpr uint32_t kLds = SPLIT * kRoom > kOut ? SPLIT * kRoom : kOut;
     static_assert(kLds <= 160 * 1024, "it fits LDS");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
     // The hardware deals thread blocks to the eight XCDs in turn: each takes an eighth of the tiles that lie together, in
@@ -524,25 +526,42 @@ __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) dense_kernel(Dens
     if constexpr (DIRECT) t.run_direct((LdsBytes)lds + way * kRoom);
     else t.run_held((LdsBytes)lds + way * kRoom);
     if constexpr (SPLIT > 1) {
-        static_assert((SPLIT - 1) * BM * BN * 4 <= kLds, "they have room");
-        f32x4* const sums = reinterpret_cast<f32x4*>(lds);
+        // All sets' sums go to LDS, and all of their threads add up eight of a row at a time.
+        constexpr int THREADS = 64 * T::WAVES * SPLIT, UNITS = BM * BN / 8 / THREADS;
+        static_assert(UNITS * THREADS * 8 == BM * BN, "every thread has as many");
+        float* const all = reinterpret_cast<float*>(lds);
         __syncthreads();
-        if (way) {
 #pragma unroll
-            for (int n = 0; n < T::MT * T::NT; ++n) sums[(((way - 1) * T::WAVES + t.wave) * T::MT * T::NT + n) * 64 + t.lane] = t.acc[n / T::NT][n % T::NT];
-        }
+        for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+            for (int j = 0; j < T::NT; ++j)
+                *reinterpret_cast<f32x4*>(all + ((way * T::WAVES + t.wave) * kRows + i * 16 + (t.lane & 15u)) * PITCH + j * 16 + (t.lane >> 4) * 4) = t.acc[i][j];
         __syncthreads();
-        if (!way) {
+        const uint32_t eight = threadIdx.x % (BN / 8), col = n0 + eight * 8;
+        if (col >= a.w.n) return;
+        float bias[8];
+        bias8<DT>(a.f, col, a.w.n, bias);
 #pragma unroll
-            for (int k = 0; k < SPLIT - 1; ++k)
+        for (int u = 0; u < UNITS; ++u) {
+            const uint32_t in = u * (THREADS / (BN / 8)) + threadIdx.x / (BN / 8), row = m0 + in;
+            if (row >= a.x.n) return;
+            float more[8], v[8] = {};
+            if (a.f.residual && a.parts == 1) residual8<DT>(a.f, row, col, a.w.n, more);
 #pragma unroll
-                for (int n = 0; n < T::MT * T::NT; ++n) t.acc[n / T::NT][n % T::NT] += sums[((k * T::WAVES + t.wave) * T::MT * T::NT + n) * 64 + t.lane];
+            for (int k = 0; k < SPLIT; ++k) {
+                const float* const from = all + ((k * T::WAVES + in / kRows * T::WN + eight / 8) * kRows + in % kRows) * PITCH + (eight & 7u) * 8;
+                const f32x4 lo = *reinterpret_cast<const f32x4*>(from), hi = *reinterpret_cast<const f32x4*>(from + 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] += i < 4 ? lo[i & 3] : hi[i & 3];
+            }
+            if (a.parts > 1) store_elements<DT_F32, 8>(a.sums + ((uint64_t)part * a.x.n + row) * a.w.n + col, (int64_t)a.w.n - col, v);
+            else finish8<DT>(a.f, row, col, a.w.n, bias, more, v);
         }
+        return;
     }
 
     // The sums' way out: a lane has four columns of 16 rows each; through LDS it gets eight of a row, and eight lanes side by side 64.
     __syncthreads();
-    if (way) return;
     const uint32_t lane = t.lane;
     float* const room = reinterpret_cast<float*>(lds) + t.wave * (SLABS * 16 * PITCH);
     const uint32_t r16 = lane & 15u, quarter = lane >> 4, col = n0 + t.wn() * 64 + (lane & 7u) * 8, row0 = m0 + t.wm() * (BM / WM) + (lane >> 3);
