@@ -51,18 +51,24 @@ struct Span {
 __device__ __forceinline__ uint32_t begin_of(const BalanceArgs& a, uint32_t v) {
     return v == 0 ? 0u : v > a.sequences + 1 ? a.tokens : min((uint32_t)max(a.offsets[v - 1], 0), a.tokens);
 }
-__device__ __forceinline__ Span find_span(const BalanceArgs& a, uint32_t t) {
-    if (!a.offsets) return {0, min(t * a.tile, a.tokens), min(t * a.tile + a.tile, a.tokens), t * a.tile < a.tokens, false};
+// the last v of `n` of which the first ones, v = 0 among them, are `below`: 64 of them at a time
+template <typename F>
+__device__ __forceinline__ uint32_t last_below(uint32_t n, const F& below) {
     const uint32_t lane = lane_id();
-    uint32_t v = 0, n = a.sequences + 2;
-    for (uint32_t step = 0; step != 1;) {                    // 64 of them at a time
+    uint32_t v = 0;
+    for (uint32_t step = 0; step != 1;) {
         step = (n + 63) / 64;
         const uint32_t at = min(lane * step, n - 1);
-        const uint64_t below = __ballot(lane * step < n && begin_of(a, v + at) / a.tile + (v + at) <= t);
-        const uint32_t skip = (below ? (uint32_t)__popcll(below) - 1u : 0u) * step;
+        const uint64_t found = __ballot(lane * step < n && below(v + at));
+        const uint32_t skip = (found ? (uint32_t)__popcll(found) - 1u : 0u) * step;
         v += skip;
         n = min(step, n - skip);
     }
+    return v;
+}
+__device__ __forceinline__ Span find_span(const BalanceArgs& a, uint32_t t) {
+    if (!a.offsets) return {0, min(t * a.tile, a.tokens), min(t * a.tile + a.tile, a.tokens), t * a.tile < a.tokens, false};
+    const uint32_t v = last_below(a.sequences + 2, [&](uint32_t u) MINT_INLINE_LAMBDA { return begin_of(a, u) / a.tile + u <= t; });
     const uint32_t begin = begin_of(a, v), end = max(begin, begin_of(a, v + 1)), nth = t - (begin / a.tile + v);
     const bool found = nth < (end - begin + a.tile - 1) / a.tile, outside = v == 0 || v > a.sequences;
     const uint32_t from = found ? begin + nth * a.tile : 0u;
@@ -353,24 +359,19 @@ struct BalanceGradArgs {
     void* d_logits;
     int64_t add_stride, d_stride;
 };
-// Tiles as above.  65536 tokens of 256 experts, sigmoids: 29 us for 134 MB (4.7 TB/s; one token at a time, the library's exponential: 56).
+// Tiles lie side by side here, whatever the offsets say, and a token belongs to the last of the sequences that begin at it or before it: so every row is
+// written once, by one thread block, also where the offsets descend.  65536 tokens of 256 experts, sigmoids: 29 us for 134 MB (4.7 TB/s; one token
+// at a time, the library's exponential: 56).
 template <int DT, int V>
 __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradArgs a) {
     using T = typename Elem<DT>::type;
+    constexpr int U = tokens_at_once(V);
     const BalanceArgs& f = a.f;
     const uint32_t lane = lane_id(), first = lane * V;
     const int64_t left = (int64_t)f.experts - first;
     __shared__ uint32_t some_of[kWaves], every_of[kWaves];
-    const Span span = find_span(f, blockIdx.x);
-    if (!span.found) return;
-    if (span.outside) {
-        for (uint32_t t = span.begin + wave_in_block(); t < span.end; t += kWaves) {
-            float none[V] = {};
-            if (a.add) load_elements<DT, V>(static_cast<const T*>(a.add) + (int64_t)t * a.add_stride + first, left, none);
-            if (left > 0) store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, none);
-        }
-        return;
-    }
+    // 64 sequences' beginnings, from `window` on, one to a lane
+    uint32_t window = 0, begins = f.offsets ? begin_of(f, lane) : 0u;
     // sequences that have a token, and all tokens
     uint32_t some = 0, every = 0;
     for (uint32_t s = threadIdx.x; s < f.sequences; s += 64 * kWaves) {
@@ -393,27 +394,44 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
     }
     some = max(some, 1u);
     every = max(every, 1u);
-    const float d = *a.d_loss, n = (float)max(a.there[span.sequence], 1);
-    const float by = d * (float)f.experts / ((float)f.topk * n) / ((float)some * n), by_z = f.z != 0.0f ? 2.0f * f.z * d / (float)every : 0.0f;
-    float often[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) often[i] = first + i < f.experts ? by * (float)a.counts[(uint64_t)span.sequence * f.experts + first + i] : 0.0f;
-    constexpr int U = tokens_at_once(V);
-    for (uint32_t t0 = span.begin + wave_in_block(); t0 < span.end; t0 += kWaves * U) {
-        float x[U][V], mean[U];
-        bool in[U];
+    const float d = *a.d_loss, by_z = f.z != 0.0f ? 2.0f * f.z * d / (float)every : 0.0f;
+    const uint32_t begin = blockIdx.x * f.tile, end = min(begin + f.tile, f.tokens);
+    // a token's sequence, 1 and on (0, and behind the last one: none), and where the next one begins
+    const auto sequence_of = [&](uint32_t t, uint32_t& next) MINT_INLINE_LAMBDA {
+        next = f.tokens;
+        if (!f.offsets) return 1u;
+        // the last lane whose beginning is not behind `t`
+        const auto last = [&]() MINT_INLINE_LAMBDA { return 63u - (uint32_t)__clzll(__ballot(begins <= t) | 1ull); };
+        uint32_t nth = last();
+        if (nth == 63) {                                      // (there may be more behind it)
+            window = last_below(f.sequences + 2, [&](uint32_t u) MINT_INLINE_LAMBDA { return begin_of(f, u) <= t; });
+            begins = begin_of(f, window + lane);
+            nth = last();
+        }
+        // (behind the search lane 63's is behind `t` too, unless the offsets descend)
+        next = nth == 63 ? t : (uint32_t)__builtin_amdgcn_readlane((int)begins, (int)nth + 1);
+        return window + nth;
+    };
+    const auto load_logits = [&](uint32_t t0, float (&x)[U][V], bool (&in)[U]) MINT_INLINE_LAMBDA {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t t = t0 + u * kWaves;
-            in[u] = t < span.end;
+            in[u] = t < end;
             load_elements<DT, V>(static_cast<const T*>(f.logits) + (int64_t)(in[u] ? t : t0) * f.row_stride + first, left, x[u]);
         }
-        const Tokens<V, U> tokens(x, in, first, f.experts, f.sigmoid, f.z != 0.0f);
+    };
+    // what the loss's gradient is by an expert's mean share
+    const auto load_of = [&](float count, float n) MINT_INLINE_LAMBDA { return d * (float)f.experts / ((float)f.topk * n) / ((float)some * n) * count; };
+    // U tokens, of one sequence (W 1) or each of its own; those that are not `inside` count nowhere
+    const auto gradients = [&](uint32_t t0, const float (&x)[U][V], const bool (&in)[U], const bool (&inside)[U], const auto& often) MINT_INLINE_LAMBDA {
+        constexpr int W = sizeof(often) / sizeof(often[0]);
+        float mean[U];
+        const Tokens<V, U> tokens(x, inside, first, f.experts, f.sigmoid, f.z != 0.0f);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             mean[u] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) mean[u] = fmaf(tokens.p[u][i], often[i], mean[u]);
+            for (int i = 0; i < V; ++i) mean[u] = fmaf(tokens.p[u][i], often[u % W][i], mean[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) mean[u] = wave_sum(mean[u]);
@@ -427,12 +445,53 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
             if (a.add) load_elements<DT, V>(static_cast<const T*>(a.add) + (int64_t)t * a.add_stride + first, left, more);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                float dx = tokens.p[u][i] * (often[i] - mean[u]);
+                float dx = tokens.p[u][i] * (often[u % W][i] - mean[u]);
                 if (f.sigmoid) dx *= tokens.rest[u][i];
                 if (f.z != 0.0f) dx = fmaf(by_z * tokens.lse[u], tokens.soft[u][i], dx);
                 more[i] += x[u][i] == -INFINITY || !tokens.there[u] ? 0.0f : dx;
             }
             store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, more);
+        }
+    };
+    uint32_t next;
+    const uint32_t v = sequence_of(begin, next);
+    if (next < end) {
+        // Tokens of several sequences: each has its own load, all of them on their way with the logits.
+        for (uint32_t t0 = begin + wave_in_block(); t0 < end; t0 += kWaves * U) {
+            float x[U][V], often[U][V], n[U];
+            bool in[U], inside[U];
+            load_logits(t0, x, in);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t of = sequence_of(in[u] ? t0 + u * kWaves : t0, next);
+                const uint64_t at = min(max(of, 1u), f.sequences) - 1;
+                inside[u] = in[u] && of != 0 && of <= f.sequences;
+                n[u] = (float)max(a.there[at], 1);
+#pragma unroll
+                for (int i = 0; i < V; ++i) often[u][i] = first + i < f.experts ? (float)a.counts[at * f.experts + first + i] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < V; ++i) often[u][i] = load_of(often[u][i], n[u]);
+            gradients(t0, x, in, inside, often);
+        }
+    } else if (v == 0 || v > f.sequences) {                   // tokens of no sequence
+        for (uint32_t t = begin + wave_in_block(); t < end; t += kWaves) {
+            float none[V] = {};
+            if (a.add) load_elements<DT, V>(static_cast<const T*>(a.add) + (int64_t)t * a.add_stride + first, left, none);
+            if (left > 0) store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, none);
+        }
+    } else {
+        const float n = (float)max(a.there[v - 1], 1);
+        float often[1][V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) often[0][i] = first + i < f.experts ? load_of((float)a.counts[(uint64_t)(v - 1) * f.experts + first + i], n) : 0.0f;
+        for (uint32_t t0 = begin + wave_in_block(); t0 < end; t0 += kWaves * U) {
+            float x[U][V];
+            bool in[U];
+            load_logits(t0, x, in);
+            gradients(t0, x, in, in, often);
         }
     }
 }
@@ -449,7 +508,7 @@ int go_tiles(const BalanceArgs& a, hipStream_t s) {
 }
 template <int DT, int V>
 int go_grad(const BalanceGradArgs& a, hipStream_t s) {
-    return Launch<&balance_grad_kernel<DT, V>>::go(a.f.tiles, 64 * kWaves, 0, s, a);
+    return Launch<&balance_grad_kernel<DT, V>>::go((uint32_t)ceil_div(a.f.tokens, a.f.tile), 64 * kWaves, 0, s, a);
 }
 #define MINT_BY_VALUES(GO, DT)                     \
     switch (values_per_lane(op->experts)) {        \

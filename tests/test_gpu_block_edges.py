@@ -1,0 +1,61 @@
+"""Calls of the operators around an expert layer at the ends of what they take: offsets that descend, infinities, numbers that leave
+the range of 32 bits, rows of no numbers and very many of them, norms with biases and without weights, tensors with tangents."""
+import pytest
+import torch
+
+from mintccl_amd import _lib, block8, combine, dense, experts, routing
+from mintccl_amd.common import DTYPE_CODE
+from mintccl_amd.dense import activation_grad, input_grad, product, weight_grad
+from mintccl_amd.norms import Norm, join, join_grad, norm, norm_grad
+from mintccl_amd.routing import balance, balance_grad
+from tests.block_oracle import DT, EVALUATED, UNIT, balance64, close, norm64
+from tests.expert_oracle import randn
+from tests.test_gpu_balance import SHARE, inputs, tokens_units
+from tests.test_gpu_norms import a_norm, parts
+
+pytestmark = pytest.mark.gpu
+
+
+def gradient_by_the_c_abi(x, experts, offsets, found, add=None, z=0.0):
+    """balance_grad into the middle of memory that is NaN, with the logits in the middle of such memory: (the gradient, whether all around it is as it was)."""
+    (t, e), dev = x.shape, x.device
+    def room(v):
+        all_ = torch.full((t + 6, e + 5), float("nan"), dtype=x.dtype, device=dev)
+        inside = all_[3:3 + t, 2:2 + e]
+        if v is not None:
+            inside.copy_(v)
+        return all_, inside
+    (_, logits), (around, out) = room(x), room(None)
+    more = None if add is None else room(add)[1]
+    op = _lib.BalanceOp(logits=logits.data_ptr(), chosen=experts.data_ptr(), offsets=offsets.data_ptr(), row_stride=logits.stride(0), tokens=t,
+                        sequences=offsets.numel() - 1, experts=e, topk=experts.shape[1], dtype=DTYPE_CODE[x.dtype], z=z)
+    one = torch.ones((), device=dev)
+    _lib.check(_lib.lib().mint_balance_grad(op, one.data_ptr(), found.counts.data_ptr(), found.there.data_ptr(), 0 if more is None else more.data_ptr(),
+                                            0 if more is None else more.stride(0), out.data_ptr(), out.stride(0), torch.cuda.current_stream().cuda_stream), "mint_balance_grad")
+    got = out.clone()
+    out.fill_(float("nan"))
+    return got, bool(around.isnan().all())
+
+
+ANYTHING = [[90, 10, 60], [2 ** 31 - 1, -2 ** 31, 7], [-5, 20, 2000], [0, 100, 0, 100, 0, 100], [100, 0], [60, 60, 20, 20, 80], [-1, -1, -1], "random"]
+
+
+@pytest.mark.parametrize("t", [1, 5, 100, 3000, 40000])
+@pytest.mark.parametrize("list_", ANYTHING, ids=str)
+def test_every_row_of_the_gradient_is_written_whatever_the_offsets_say(dev, t, list_):
+    """Offsets are numbers in device memory: where they descend, are negative or beyond the tokens, every row of the gradient is still some number (and
+    with another gradient added, no less), and nothing around it is written."""
+    x, experts = inputs(t, 9, 2, "f32", dev, masks=False)
+    if list_ == "random":
+        offsets = torch.randint(-t // 8, t + t // 8 + 1, (300,), generator=torch.Generator().manual_seed(t))
+    else:
+        offsets = torch.tensor([v if abs(v) > 2000 else v * t // 100 for v in list_])
+    offsets = offsets.to(torch.int32).to(dev)
+    found = balance(x, experts, offsets=offsets, z=1e-3)
+    assert bool(found.loss.isfinite()) and bool(found.shares.isfinite().all())
+    got, kept = gradient_by_the_c_abi(x, experts, offsets, found, z=1e-3)
+    assert kept and bool(got.isfinite().all())
+    more = randn(t, 9, seed=4, dev=dev)
+    both, kept = gradient_by_the_c_abi(x, experts, offsets, found, more, z=1e-3)
+    # (the same gradient, before the sum with the other one is rounded)
+    assert kept and bool(((both.double() - more.double() - got.double()).abs() <= UNIT * (2 * got.double().abs() + more.double().abs())).all())
