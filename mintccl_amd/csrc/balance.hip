@@ -417,8 +417,17 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
         for (int u = 0; u < U; ++u) {
             const uint32_t t = t0 + u * kWaves;
             in[u] = t < end;
-            load_elements<DT, V>(static_cast<const T*>(f.logits) + (int64_t)(in[u] ? t : t0) * f.row_stride + first, left, x[u]);
+            const T* const row = static_cast<const T*>(f.logits) + (int64_t)(in[u] ? t : t0) * f.row_stride;
+            // (one to a lane: the last one in the place of those behind it, since loads that some lanes have not are waited for one by one)
+            if constexpr (V == 1) x[u][0] = Elem<DT>::load(*as_global(row + min(first, f.experts - 1)));
+            else load_elements<DT, V>(row + first, left, x[u]);
         }
+        __builtin_amdgcn_sched_barrier(0);                    // (all of them, before the first is waited for)
+    };
+    // (clamped where it is one to a lane, as there)
+    const auto count_of = [&](uint64_t sequence, int i) MINT_INLINE_LAMBDA {
+        const int32_t* const row = a.counts + sequence * f.experts;
+        return V == 1 ? (float)row[min(first, f.experts - 1)] : first + i < f.experts ? (float)row[first + i] : 0.0f;
     };
     // what the loss's gradient is by an expert's mean share
     const auto load_of = [&](float count, float n) MINT_INLINE_LAMBDA { return d * (float)f.experts / ((float)f.topk * n) / ((float)some * n) * count; };
@@ -468,7 +477,7 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
                 inside[u] = in[u] && of != 0 && of <= f.sequences;
                 n[u] = (float)max(a.there[at], 1);
 #pragma unroll
-                for (int i = 0; i < V; ++i) often[u][i] = first + i < f.experts ? (float)a.counts[at * f.experts + first + i] : 0.0f;
+                for (int i = 0; i < V; ++i) often[u][i] = count_of(at, i);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -486,7 +495,7 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
         const float n = (float)max(a.there[v - 1], 1);
         float often[1][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) often[0][i] = first + i < f.experts ? load_of((float)a.counts[(uint64_t)(v - 1) * f.experts + first + i], n) : 0.0f;
+        for (int i = 0; i < V; ++i) often[0][i] = load_of(count_of(v - 1, i), n);
         for (uint32_t t0 = begin + wave_in_block(); t0 < end; t0 += kWaves * U) {
             float x[U][V];
             bool in[U];
