@@ -136,10 +136,11 @@ class ExpertBlock:
         stream + gate * y, and after(that)
 
     ``up`` (inner, width) and ``down`` (width, inner) are a shared expert's weights, bfloat16 or float16 (the rows' type); ``gate`` (width,)
-    scales the channels, ``before`` and ``after`` are the norms of this block's and of the next one's rows.  ``z`` is :func:`~mintccl_amd.routing.balance`'s."""
+    scales the channels, ``before`` and ``after`` are the norms of this block's and of the next one's rows, with weights and biases or without.
+    ``z`` is :func:`~mintccl_amd.routing.balance`'s."""
 
     def __init__(self, layer: ExpertLayer, before: Norm, up: torch.Tensor, down: torch.Tensor, after: Norm, gate: torch.Tensor, z: float = 0.0) -> None:
-        bare = lambda n: n._replace(weight=n.weight.detach(), bias=None if n.bias is None else n.bias.detach())  # noqa: E731
+        bare = lambda n: n._replace(**{v: t.detach() for v, t in (("weight", n.weight), ("bias", n.bias)) if t is not None})  # noqa: E731
         self.layer, self.comm, self.z = layer, layer.comm, z
         self.before, self.after, self.up, self.down, self.gate = bare(before), bare(after), up.detach(), down.detach(), gate.detach()
 
@@ -167,7 +168,8 @@ class ExpertBlock:
     def backward(self, d_streams: list[torch.Tensor], d_behind: list[torch.Tensor], d_losses: list[torch.Tensor],
                  kept: list) -> tuple[list[torch.Tensor], list[dict[str, torch.Tensor]]]:
         """From the gradients of :meth:`forward`'s three results (a loss's is a number in float32, the same on every rank): the streams' and the
-        weights' (``before``, ``after``, ``gate``, ``shared_up`` and ``shared_down`` the same on all ranks, and the layer's)."""
+        weights' (``before`` and ``before_bias``, ``after`` and ``after_bias`` where the norms have them, ``gate``, ``shared_up`` and ``shared_down``
+        the same on all ranks, and the layer's)."""
         if len(kept) != 3 or len(kept[1]) != self.comm.world_size:
             raise ValueError("kept must be what a forward pass of this block has left")
         of_layer, of_block, balances = kept
@@ -180,10 +182,12 @@ class ExpertBlock:
             shared = dense.input_grad(d_u, self.up, dtype=torch.float32)
             n = norm_grad((d_x.float() + shared).to(x.dtype), stream, self.before)
             d_in.append(j.stream + n.x)
-            f.update(before=n.weight.float(), after=j.before_weight.float(), gate=j.gate.float(),
-                     shared_up=dense.weight_grad(d_u, x, dtype=torch.float32), shared_down=dense.weight_grad(j.y, h, dtype=torch.float32))
-        for name in ("before", "after", "gate", "shared_up", "shared_down"):
-            self.comm.run(lambda r: allreduce(found[r][name], self.comm))  # noqa: B023
+            own = {"before": n.weight, "before_bias": n.bias, "after": j.before_weight, "after_bias": j.before_bias, "gate": j.gate,
+                   "shared_up": dense.weight_grad(d_u, x, dtype=torch.float32), "shared_down": dense.weight_grad(j.y, h, dtype=torch.float32)}
+            f.update({name: t.float() for name, t in own.items() if t is not None})
+        for name in own:
+            if name in found[0]:
+                self.comm.run(lambda r: allreduce(found[r][name], self.comm))  # noqa: B023
         return d_in, found
 
 
@@ -211,11 +215,14 @@ def small_layer(world: int, device, tokens: int = 96, width: int = 320, inner: i
             "grads": [rand(tokens, width).to(torch.bfloat16).to(device) for _ in range(world)]}
 
 
-def plain_block(stream, before, after, gate, router, up, down, shared_up, shared_down, k, z, dtype, bias=None, score="softmax", renormalise=True):
+def plain_block(stream, before, after, gate, router, up, down, shared_up, shared_down, k, z, dtype, bias=None, score="softmax", renormalise=True,
+                kind="rms", before_bias=0.0, after_bias=0.0):
     """The block on all tokens at once, in elementary operations of the inputs' type: the new stream, the next block's rows and the loss.  What decides
     the choice of experts is rounded as the block rounds it, with the gradient of what is not."""
-    rms = lambda x, w: x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w  # noqa: E731
-    x = rms(stream, before)
+    def normed(x, weight, bias):
+        x = x - x.mean(-1, keepdim=True) if kind == "layer" else x
+        return x * (x.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * weight + bias
+    x = normed(stream, before, before_bias)
     x = x + (x.to(dtype).to(x.dtype) - x).detach()
     y = plain_layer(x, router, up, down, k, bias, score, renormalise) + F.silu(x @ shared_up.t()) @ shared_down.t()
     new = stream + gate * y
@@ -225,11 +232,12 @@ def plain_block(stream, before, after, gate, router, up, down, shared_up, shared
     chosen = (key if bias is None else key + bias).sort(dim=-1, descending=True, stable=True).indices[:, :k]
     often = torch.bincount(chosen.reshape(-1), minlength=len(router)) * (len(router) / chosen.numel())
     loss = (often * (shares / shares.sum(-1, keepdim=True)).mean(0)).sum() + z * torch.logsumexp(logits, -1).square().mean()
-    return new, rms(new, after), loss
+    return new, normed(new, after, after_bias), loss
 
 
-def block_distances(world: int, device, **options) -> dict[str, float]:
-    """How far a small block's results and gradients are from the plain one's in 64 bits (2-norms; the loss's own distance)."""
+def block_distances(world: int, device, kind: str = "rms", weights: bool = True, biases: bool = False, **options) -> dict[str, float]:
+    """How far a small block's results and gradients are from the plain one's in 64 bits (2-norms; the loss's own distance).  Its norms are of
+    a ``kind``, with ``weights`` and ``biases`` or without."""
     s, z = small_layer(world, device), 0.01
     g = torch.Generator().manual_seed(2)
     width, inner = s["up"].shape[2], 184
@@ -239,16 +247,22 @@ def block_distances(world: int, device, **options) -> dict[str, float]:
     own = {n: t.to(torch.bfloat16 if n.startswith("shared") else torch.float32).to(device) for n, t in own.items()}
     streams = [(t.float() * 3).contiguous() for t in s["tokens"]]
     d_streams = [rand(*t.shape).to(device) for t in streams]
+    if biases:
+        own.update({f"{n}_bias": (0.2 * rand(width)).to(device) for n in ("before", "after")})
+    norms = [Norm(own[n] if weights else None, own.get(f"{n}_bias"), kind) for n in ("before", "after")]
     d_loss = torch.tensor(40.0, device=device)                                       # (so that it weighs about as much as the rest)
     layer = ExpertLayer(VirtualComm(world_size=world, device=device), s["router"], s["up"], s["down"], 4, **options)
-    block = ExpertBlock(layer, Norm(own["before"]), own["shared_up"], own["shared_down"], Norm(own["after"]), own["gate"], z)
+    block = ExpertBlock(layer, norms[0], own["shared_up"], own["shared_down"], norms[1], own["gate"], z)
     kept: list = []
     new, behind, balances = block.forward(streams, kept)
     d_in, found = block.backward(d_streams, s["grads"], [d_loss] * world, kept)
     layer.comm.check()
     leaf = {n: t.double().requires_grad_() for n, t in {**own, **{n: s[n] for n in ("router", "up", "down")}}.items()}
     x = torch.cat(streams).double().requires_grad_()
-    want = plain_block(x, **leaf, k=4, z=z, dtype=torch.bfloat16, **options)
+    if not weights:
+        leaf.update(before=1.0, after=1.0)
+        own = {n: t for n, t in own.items() if n not in ("before", "after")}
+    want = plain_block(x, **leaf, k=4, z=z, dtype=torch.bfloat16, kind=kind, **options)
     ((want[0] * torch.cat(d_streams)).sum() + (want[1] * torch.cat(s["grads"]).double()).sum() + want[2] * d_loss).backward()
     off = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
     return {"stream": off(torch.cat(new), want[0].detach()), "rows": off(torch.cat(behind), want[1].detach()),

@@ -59,3 +59,17 @@ def test_every_row_of_the_gradient_is_written_whatever_the_offsets_say(dev, t, l
     both, kept = gradient_by_the_c_abi(x, experts, offsets, found, more, z=1e-3)
     # (the same gradient, before the sum with the other one is rounded)
     assert kept and bool(((both.double() - more.double() - got.double()).abs() <= UNIT * (2 * got.double().abs() + more.double().abs())).all())
+
+
+@pytest.mark.parametrize("world", [1, 4])
+@pytest.mark.parametrize("norms", [{"kind": "layer", "biases": True}, {"kind": "rms", "biases": True}, {"kind": "layer", "weights": False},
+                                   {"kind": "rms", "weights": False, "biases": True}])
+def test_a_blocks_norms_with_biases_and_without_weights(dev, world, norms):
+    """Each norm's weight and bias that there is has its gradient, and one that is not there has none."""
+    found = experts.block_distances(world, dev, **norms)
+    for name in ("before", "after"):
+        for rank in range(world):
+            assert (f"{name} of rank {rank}" in found) == norms.get("weights", True)
+            assert (f"{name}_bias of rank {rank}" in found) == norms.get("biases", False)
+    for name, off in found.items():
+        assert off < (1e-4 if name == "loss" else experts.FAR), (name, off)
