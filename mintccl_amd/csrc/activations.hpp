@@ -3,6 +3,8 @@
 #pragma once
 #include "operators.hpp"
 
+#include <cfloat>
+
 namespace mint {
 
 // e^x: 2^p of the rounded product p = x log2(e), and what the rounding left over to the first order; a few units of 2^-24 off, in
@@ -61,7 +63,9 @@ __device__ __forceinline__ void activate(int kind, float (&v)[N]) {
         default: break;
     }
 }
-// ... v becomes the activation's slope there
+// the largest number of its sign in the place of an infinity: times 0 it is 0
+__device__ __forceinline__ float finite(float x) { return __builtin_amdgcn_fmed3f(x, -FLT_MAX, FLT_MAX); }
+// ... v becomes the activation's slope there, at an infinity its limit (what is kept of a product in 16 bits may have left their range)
 template <int N>
 __device__ __forceinline__ void slopes(int kind, float (&v)[N]) {
     switch (kind) {
@@ -73,7 +77,7 @@ __device__ __forceinline__ void slopes(int kind, float (&v)[N]) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const float s = logistic(v[i]);
-                v[i] = s * fmaf(v[i], 1.0f - s, 1.0f);
+                v[i] = s * fmaf(finite(v[i]), 1.0f - s, 1.0f);
             }
             break;
         case MINT_ACT_SIGMOID:
@@ -93,8 +97,8 @@ __device__ __forceinline__ void slopes(int kind, float (&v)[N]) {
         case MINT_ACT_GELU:
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const float power = exponential(-0.5f * v[i] * v[i]), above = normal_above(fabsf(v[i]), power);
-                v[i] = fmaf(v[i], 0.39894228f * power, v[i] < 0.0f ? above : 1.0f - above);
+                const float power = exponential(-0.5f * v[i] * v[i]), above = normal_above(fabsf(v[i]), power), below = v[i] < 0.0f ? above : 1.0f - above;
+                v[i] = power == 0.0f ? below : fmaf(v[i], 0.39894228f * power, below);
             }
             break;
         case MINT_ACT_GELU_TANH:

@@ -73,3 +73,36 @@ def test_a_blocks_norms_with_biases_and_without_weights(dev, world, norms):
             assert (f"{name}_bias of rank {rank}" in found) == norms.get("biases", False)
     for name, off in found.items():
         assert off < (1e-4 if name == "loss" else experts.FAR), (name, off)
+
+
+#: The slopes' limits at -inf and at +inf.
+LIMITS = {"relu": (0.0, 1.0), "silu": (0.0, 1.0), "sigmoid": (0.0, 0.0), "tanh": (0.0, 0.0), "gelu": (0.0, 1.0), "gelu_tanh": (0.0, 1.0)}
+
+
+@pytest.mark.parametrize("activation", list(LIMITS))
+@pytest.mark.parametrize("dt", list(DT))
+def test_slopes_at_infinities(dev, dt, activation):
+    """What the activation was applied to is kept as an infinity where it leaves its type's range: the slope there is its limit."""
+    inf = float("inf")
+    z = torch.tensor([[-inf, inf, 1.0, -inf, inf, -2.0, 0.5, inf, -inf]], dtype=DT[dt], device=dev)
+    d = torch.full_like(z, 0.5)
+    d_z, d_bias = activation_grad(d, z, activation)
+    low, high = LIMITS[activation]
+    want = torch.where(z == -inf, low / 2, torch.where(z == inf, high / 2, d_z))
+    assert torch.equal(d_z, want) and bool(d_z.isfinite().all()) and bool(d_bias.isfinite().all())
+    nan = torch.full_like(z, float("nan"))
+    assert bool(activation_grad(d, nan, activation)[0].isnan().all())
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+def test_gradients_where_what_is_kept_leaves_its_range(dev, activation):
+    """f16 operands whose products are below -65504: the result is near zero, and so are its gradients."""
+    rows, cols, depth = 40, 24, 64
+    x, w = torch.full((rows, depth), 128.0, dtype=torch.float16, device=dev), torch.full((cols, depth), 0.25, dtype=torch.float16, device=dev)
+    w[3], w[5] = -32.0, 32.0
+    out, z = product(x, w, activation=activation, keep=True, dtype=torch.float32)
+    assert bool((z[:, 3] == -float("inf")).all()) and bool((z[:, 5] == float("inf")).all()) and bool((out[:, 3] == 0).all()) and bool((out[:, 5] == 2.0 ** 18).all())
+    d_z, d_bias = activation_grad(torch.ones_like(out), z, activation)
+    assert bool((d_z[:, 3] == 0).all()) and bool((d_z[:, 5] == 1).all()) and float(d_bias[3]) == 0 and float(d_bias[5]) == rows
+    d_x, d_w = input_grad(d_z, w), weight_grad(d_z, x)
+    assert bool(d_x.isfinite().all()) and bool(d_w.isfinite().all()) and bool((d_w[3] == 0).all())
