@@ -117,11 +117,12 @@ __device__ __forceinline__ void slopes(int kind, float (&v)[N]) {
 }
 inline bool activation_known(int kind) { return kind >= MINT_ACT_NONE && kind <= MINT_ACT_GELU_TANH; }
 
-// Of a gate: none, sigmoid, tanh or silu, in as little code as that takes (it stands in many kernels).
+// Of a gate: none, sigmoid, tanh or silu, in as little code as that takes (it stands in many kernels).  At infinities silu and its slope are their limits: a gate
+// of -inf shuts.
 __device__ __forceinline__ float gate_value(int kind, float g) {
     if (kind == MINT_ACT_NONE) return g;
     if (kind == MINT_ACT_TANH) return tangent(g);
-    return logistic(g) * (kind == MINT_ACT_SILU ? g : 1.0f);
+    return logistic(g) * (kind == MINT_ACT_SILU ? fmaxf(g, -FLT_MAX) : 1.0f);
 }
 __device__ __forceinline__ float gate_slope(int kind, float g) {
     if (kind == MINT_ACT_NONE) return 1.0f;
@@ -130,7 +131,7 @@ __device__ __forceinline__ float gate_slope(int kind, float g) {
         return 1.0f - t * t;
     }
     const float e = exponential(-fabsf(g)), r = reciprocal(1.0f + e), s = (g < 0.0f ? e : 1.0f) * r, slope = e * r * r;
-    return kind == MINT_ACT_SILU ? fmaf(g, slope, s) : slope;
+    return kind == MINT_ACT_SILU ? (slope == 0.0f ? s : fmaf(g, slope, s)) : slope;
 }
 inline bool gate_known(int kind) { return kind == MINT_ACT_NONE || kind == MINT_ACT_SIGMOID || kind == MINT_ACT_TANH || kind == MINT_ACT_SILU; }
 

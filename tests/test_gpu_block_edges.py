@@ -106,3 +106,24 @@ def test_gradients_where_what_is_kept_leaves_its_range(dev, activation):
     assert bool((d_z[:, 3] == 0).all()) and bool((d_z[:, 5] == 1).all()) and float(d_bias[3]) == 0 and float(d_bias[5]) == rows
     d_x, d_w = input_grad(d_z, w), weight_grad(d_z, x)
     assert bool(d_x.isfinite().all()) and bool(d_w.isfinite().all()) and bool((d_w[3] == 0).all())
+
+
+@pytest.mark.parametrize("shape", ["channel", "row", "all"])
+@pytest.mark.parametrize("width", [16, 1500, 4104, 9001])
+def test_gates_by_silu_at_infinities(dev, width, shape):
+    """silu goes to 0 at -inf, and its slope to 0 and, at inf, to 1: a gate of -inf shuts its numbers out, with finite gradients."""
+    rows, inf = 5, float("inf")
+    size = {"channel": (width,), "row": (rows, 1), "all": (rows, width)}[shape]
+    g = randn(*size, seed=1, dev=dev)
+    shut = torch.arange(g.numel(), device=dev).view(size) % 3 == 0
+    g = torch.where(shut, -inf, g)
+    s, y = randn(rows, width, seed=2, dev=dev), randn(rows, width, seed=3, dev=dev)
+    r, _ = join(s, y, gate=g, gate_by="silu")
+    where = shut.expand(rows, width)
+    assert torch.equal(r[where], s[where]) and bool(r.isfinite().all())
+    d = join_grad(s, None, r, y, gate=g, gate_by="silu")
+    assert bool(d.gate.isfinite().all()) and bool((d.gate[shut] == 0).all()) and bool((d.y[where] == 0).all()) and bool(d.y.isfinite().all())
+    # open without end: the gradient is that of the gate's own value (whole numbers, whose sums are exact)
+    ones_ = torch.ones(rows, width, device=dev)
+    wide = join_grad(ones_, None, ones_, 2 * ones_, gate=torch.full(size, inf, device=dev), gate_by="silu").gate
+    assert bool((wide == 2 * {"channel": rows, "row": width, "all": 1}[shape]).all())
