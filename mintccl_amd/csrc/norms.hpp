@@ -245,17 +245,27 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_kernel(JoinArgs a) {
     const uint32_t at = row.at;
     const int64_t left = row.left;
     RowSums<WAVES, 1> sums = {slots};
-    const bool one_by_one = a.gate && a.gate_form != MINT_GATE_CHANNEL;
-    // u's weight and bias with the scale and a gate by channel in them
+    // u's weight and bias with the scale and a gate by channel in them.  (An infinite gate is of the whole u: of the weight and of the bias it would make
+    // infinities whose sum is NaN.  Then the gates are read for every row, as those of every number are.)
+    bool one_by_one = a.gate && a.gate_form != MINT_GATE_CHANNEL;
     float wa[V], ba[V], wb[V], bb[V], open[V];
     weight_of(a.after, at, left, wa);
     bias_of(a.after, at, left, ba);
     weight_of(a.before, at, left, wb);
     bias_of(a.before, at, left, bb);
-    if (!one_by_one) gate_of(a, 0, row, open);
+    if (!one_by_one) {
+        bool infinite = false;
+        gate_of(a, 0, row, open);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            open[i] = a.scale * (a.gate ? gate_value(a.gate_by, open[i]) : 1.0f);
+            infinite |= fabsf(open[i]) == INFINITY;
+        }
+        one_by_one = a.gate && __ballot(infinite) != 0;
+    }
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float all = a.scale * (a.gate && !one_by_one ? gate_value(a.gate_by, open[i]) : 1.0f);
+        const float all = one_by_one ? a.scale : open[i];
         wa[i] *= all;
         ba[i] *= all;
     }
@@ -273,7 +283,11 @@ __global__ void __launch_bounds__(threads_of(LANES)) join_kernel(JoinArgs a) {
         if (r + groups < a.rows) ask((uint32_t)(r + groups));
         if (a.y) {
             if (a.after.kind) normalise(row, a.after, y, sums);
-            if (one_by_one) {
+            if (one_by_one && a.gate_form == MINT_GATE_ROW) {
+                const float one = gate_value(a.gate_by, load_one(a.gate, a.gate_dtype, (int64_t)r * a.gate_row));
+#pragma unroll
+                for (int i = 0; i < V; ++i) open[i] = one;
+            } else if (one_by_one) {
                 gate_of(a, r, row, open);
 #pragma unroll
                 for (int i = 0; i < V; ++i) open[i] = gate_value(a.gate_by, open[i]);

@@ -127,3 +127,20 @@ def test_gates_by_silu_at_infinities(dev, width, shape):
     ones_ = torch.ones(rows, width, device=dev)
     wide = join_grad(ones_, None, ones_, 2 * ones_, gate=torch.full(size, inf, device=dev), gate_by="silu").gate
     assert bool((wide == 2 * {"channel": rows, "row": width, "all": 1}[shape]).all())
+
+
+@pytest.mark.parametrize("bias", [None, False, True])
+@pytest.mark.parametrize("width", [16, 70, 1500, 2501, 4096, 8192, 9001])
+def test_infinite_gates_by_channel(dev, width, bias):
+    """An infinite gate makes infinities of its channel, whether the block's output is normed (with a bias or none) or not, in rows of every length."""
+    rows, inf = 6, float("inf")
+    s, y = randn(rows, width, seed=1, dev=dev), randn(rows, width, seed=2, dev=dev)
+    after = None if bias is None else a_norm(width, "rms", bias, torch.float32, dev, 3)
+    u = y.cpu().double() if after is None else norm64(y.cpu(), *parts(after))
+    g = randn(width, seed=5, dev=dev)
+    at = torch.arange(width, device=dev)
+    g[at % 5 == 1], g[at % 5 == 3] = inf, -inf
+    r, _ = join(s, y, after=after, gate=g, scale=0.5)
+    want = s.cpu().double() + 0.5 * u * g.cpu().double()
+    ends = want.isinf() & (u.abs() > 1e-4)                    # (u is off by less than that: its sign is known)
+    assert int(ends.sum()) > width and torch.equal(r.cpu().double()[ends], want[ends]) and bool(r.cpu()[~want.isinf()].isfinite().all())
