@@ -656,7 +656,7 @@ typedef struct {
  * g: gate by channel (width), by row (gate_row apart) or of every number (rows
  * gate_row apart), a its activation; 0: none.  With y = 0 only h = before(s) is
  * made.  new_stream may be the stream itself.  The stream is of `dtype`
- * (that of y and h) or MINT_F32. */
+ * (that of y and h) or MINT_F32.  Where width is over 8192, rows * width is 2^40 at most. */
 typedef enum { MINT_GATE_CHANNEL = 1, MINT_GATE_ROW = 2, MINT_GATE_ALL = 3 } mint_gate_form;
 typedef struct {
     uint64_t stream, y, gate, new_stream, next;

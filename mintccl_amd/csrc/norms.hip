@@ -103,8 +103,7 @@ extern "C" int mint_join(const mint_join_op* op, void* stream) {
     if (const int err = join_args(op, a)) return err;
     if (a.rows == 0 || a.width == 0) return MINT_OK;
     if (!a.stream || (a.y && !a.new_stream) || (a.next && !a.before.kind) || (!a.y && !a.next)) return MINT_ERR_ARG;
-    // (a launch has fewer than 2^32 threads; the others' thread blocks have many rows)
-    if (a.width > kLongest && (uint64_t)a.rows * kLongThreads > 0xFFFFFF00ull) return MINT_ERR_TOO_LARGE;
+    if (a.width > kLongest && (uint64_t)a.rows * a.width > 1ull << 40) return MINT_ERR_TOO_LARGE;      // (no memory holds the results)
     const auto s = static_cast<hipStream_t>(stream);
     MINT_STREAM_TYPES(launch_join, a, s)
 }

@@ -758,6 +758,7 @@ __global__ void __launch_bounds__(kLongThreads) join_grad_long_kernel(JoinGradAr
 // ---- the launches --------------------------------------------------------------------
 // Lanes of a row: 64 (four rows to a thread block) up to 512 numbers, then a thread block of 128 to 1024.
 constexpr uint32_t kLongest = 1024 * V;
+constexpr uint32_t kMostLong = 1u << 18;         // longer ones of a launch, which has fewer than 2^32 threads
 inline uint32_t threads_for(uint64_t width) {
     return width <= 64 * V ? 256 : width <= 128 * V ? 128 : width <= 256 * V ? 256 : width <= 512 * V ? 512 : 1024;
 }
@@ -778,7 +779,21 @@ int go_join_rows(const JoinArgs& a, hipStream_t s) {
 }
 template <int S, int T>
 int go_join(const JoinArgs& a, hipStream_t s) {
-    if (a.width > kLongest) return Launch<&join_long_kernel<S, T>>::go((uint32_t)a.rows, kLongThreads, 0, s, a);
+    if (a.width > kLongest) {
+        const auto on = [](const void* p, int64_t rows, int64_t stride, size_t size) { return p ? static_cast<const uint8_t*>(p) + rows * stride * (int64_t)size : nullptr; };
+        const size_t of_s = sizeof(typename Elem<S>::type), of_t = sizeof(typename Elem<T>::type), of_gate = a.gate_dtype == MINT_F32 ? 4 : 2;
+        for (uint32_t first = 0; first < a.rows; first += kMostLong) {
+            JoinArgs part = a;
+            part.rows = std::min(a.rows - first, kMostLong);
+            part.stream = on(a.stream, first, a.stream_stride, of_s);
+            part.new_stream = const_cast<uint8_t*>(on(a.new_stream, first, a.new_stride, of_s));
+            part.y = on(a.y, first, a.y_stride, of_t);
+            part.next = const_cast<uint8_t*>(on(a.next, first, a.next_stride, of_t));
+            part.gate = on(a.gate, first, a.gate_row, of_gate);              // (by channel its rows are 0 apart)
+            if (const int err = Launch<&join_long_kernel<S, T>>::go(part.rows, kLongThreads, 0, s, part)) return err;
+        }
+        return MINT_OK;
+    }
     return a.width % V == 0 ? go_join_rows<S, T, true>(a, s) : go_join_rows<S, T, false>(a, s);
 }
 template <int S, int T, bool WHOLE, bool BLOCK, bool BIAS, int GATE>

@@ -144,3 +144,33 @@ def test_infinite_gates_by_channel(dev, width, bias):
     want = s.cpu().double() + 0.5 * u * g.cpu().double()
     ends = want.isinf() & (u.abs() > 1e-4)                    # (u is off by less than that: its sign is known)
     assert int(ends.sum()) > width and torch.equal(r.cpu().double()[ends], want[ends]) and bool(r.cpu()[~want.isinf()].isfinite().all())
+
+
+def test_long_rows_beyond_a_launchs_thread_blocks(dev):
+    """Rows too long for registers, more of them than one launch takes: each is what it is alone."""
+    rows, width = (1 << 18) + 1037, 8200
+    g = torch.Generator(dev).manual_seed(3)
+    s, y = (torch.empty(rows, width, dtype=torch.bfloat16, device=dev).normal_(generator=g) for _ in range(2))
+    n = a_norm(width, "layer", True, torch.bfloat16, dev, 3)
+    row = torch.randn(rows, 1, generator=g, device=dev)
+    for gate in (torch.sigmoid(n.weight), row, y):
+        new, h = join(s, y, after=n, before=n, gate=gate)
+        for part in (slice(0, 5), slice(1030, 1045), slice((1 << 18) - 3, (1 << 18) + 4), slice(rows - 5, rows)):
+            alone = join(s[part].clone(), y[part].clone(), after=n, before=n, gate=gate if gate.dim() == 1 else gate[part].clone())
+            assert torch.equal(new[part], alone[0]) and torch.equal(h[part], alone[1])
+    again = join(s, y, after=n, before=n, gate=y, out=s)
+    assert torch.equal(again[0], new) and torch.equal(again[1], h)
+    del s, y, new, h, again
+    torch.cuda.empty_cache()
+
+
+def test_more_long_rows_than_a_launch_has_threads_for(dev):
+    """2^22 rows of 8200 numbers, all of them one: the results are 69 GB."""
+    rows, width = 1 << 22, 8200
+    x = randn(1, width, seed=1, dtype=torch.bfloat16, dev=dev)
+    n = a_norm(width, "rms", False, torch.bfloat16, dev, 3)
+    want, got = norm(x, n), norm(x.expand(rows, width), n)
+    for i in range(0, rows, 1 << 18):
+        assert bool((got[i:i + (1 << 18)] == want).all())
+    del got
+    torch.cuda.empty_cache()
