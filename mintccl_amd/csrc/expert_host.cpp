@@ -7,6 +7,7 @@
 
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -126,9 +127,11 @@ struct Args {
         if (!THPVariable_Check(list[i])) refuse(PyExc_TypeError, "%s must be a device tensor", name);
         const Tensor& t = THPVariable_Unpack(list[i]);
         if (!t.is_cuda() || t.layout() != at::kStrided) refuse(PyExc_TypeError, "%s must be a device tensor", name);
-        // (a result without a history would end the gradient here without a word)
+        // (a result without a history, or without a tangent, would end the gradient here without a word)
         if (history && t.requires_grad() && c10::GradMode::is_enabled())
             refuse(PyExc_RuntimeError, "%s requires a gradient, and these operators record none: detach it, or call under torch.no_grad()", name);
+        if (history && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+            refuse(PyExc_RuntimeError, "%s has a tangent, and these operators hand none on: unpack it, or call under torch.inference_mode()", name);
         return t;
     }
     int64_t integer(int i, const char* name, int64_t least, int64_t most) const {

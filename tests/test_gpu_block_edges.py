@@ -174,3 +174,38 @@ def test_more_long_rows_than_a_launch_has_threads_for(dev):
         assert bool((got[i:i + (1 << 18)] == want).all())
     del got
     torch.cuda.empty_cache()
+
+
+def test_tensors_with_a_tangent_are_refused(dev):
+    """Results carry no tangent of forward-mode differentiation, so an operand that has one is refused, by each of the operators."""
+    from torch.autograd import forward_ad
+    x, w, d = (torch.randn(8, 128, generator=torch.Generator().manual_seed(i)).to(dev) for i in range(3))
+    n, one = Norm(w[0].contiguous()), torch.ones((), device=dev)
+    weights, chosen = routing.route(x, 2)
+    plan = routing.assign(chosen, 128)
+    found = balance(x, chosen)
+    eight = block8.quantise_weight(w)
+    rows = torch.randn(16, 128, generator=torch.Generator().manual_seed(5)).to(dev)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        of = lambda call, *at: [lambda i=i: call(*(dual(t) if k == i else t for k, t in enumerate(at))) for i in range(len(at))]  # noqa: E731
+        calls = [*of(lambda a: norm(a, n), x), *of(lambda a: norm(x, Norm(a)), n.weight), *of(join, x, w), *of(lambda a: join(x, w, gate=a), d),
+                 *of(lambda a, b: norm_grad(a, b, n), d, x), *of(lambda a, b, c, e: join_grad(a, b, c, e, before=n), d, d, x, w),
+                 *of(dense.product, x, w), *of(lambda a, b: dense.product(x, w, bias=a, residual=b), w[:, 0].contiguous(), d[:, :8].contiguous()),
+                 *of(lambda a, b: dense.activation_grad(a, b, "silu"), d, x), *of(dense.input_grad, d[:, :8].contiguous(), w), *of(dense.weight_grad, d, x),
+                 *of(lambda a: balance(a, chosen), x), *of(lambda a, b: balance_grad(a, b, chosen, found, add=d), one, x), *of(lambda a: balance_grad(one, x, chosen, found, add=a), d),
+                 *of(lambda a: routing.route(a, 2), x), *of(lambda a, b: routing.route_grad(a, b, chosen), weights, x),
+                 *of(lambda a: block8.quantise(a), x), *of(lambda a: block8.quantise_weight(a), w), *of(lambda a: block8.product(a, eight), x),
+                 *of(lambda a, b: combine.combine(a, plan, b), rows, weights), *of(lambda a, b, c: combine.combine_grad(a, b, plan, c), d, rows, weights)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+        # what it was made from is taken, also under no_grad, which leaves tangents alone
+        want = norm(x, n)
+        assert torch.equal(norm(forward_ad.unpack_dual(dual(x)).primal, n), want)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+            norm(dual(x), n)
+        x_dual = dual(x)
+        with torch.inference_mode():
+            assert torch.equal(norm(x_dual, n), want)
+    assert torch.equal(norm(x, n), want)
