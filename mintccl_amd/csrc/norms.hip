@@ -61,6 +61,12 @@ __global__ void __launch_bounds__(64 * kColumnWaves) column_sums_kernel(ColumnSu
     }
 }
 
+// The gradients of gates by row whose rows have no numbers: sums of nothing.
+__global__ void __launch_bounds__(256) clear_gates_kernel(void* to_gate, int dtype, int64_t stride, uint32_t rows) {
+    const uint32_t r = blockIdx.x * 256 + threadIdx.x;
+    if (r < rows) store_one(to_gate, dtype, (int64_t)r * stride, 0.0f);
+}
+
 // ---- the entry points --------------------------------------------------------------
 // the types that go together: the stream is of the block's type, or in 32 bits
 #define MINT_STREAM_TYPES(GO, ...)                                                                                          \
@@ -128,7 +134,11 @@ extern "C" int mint_join_grad(const mint_join_grad_op* op_grad, void* stream) {
     const mint_join_op* const op = &op_grad->join;
     JoinGradArgs a = {};
     if (const int err = join_args(op, a.f)) return err;
-    if (a.f.width == 0) return MINT_OK;
+    if (a.f.width == 0) {
+        if (!op_grad->to_gate || !a.f.gate || op->gate_form != MINT_GATE_ROW || a.f.rows == 0) return MINT_OK;
+        return Launch<&clear_gates_kernel>::go((a.f.rows + 255) / 256, 256, 0, static_cast<hipStream_t>(stream), reinterpret_cast<void*>(op_grad->to_gate),
+                                               op->gate_dtype, op_grad->to_gate_stride, a.f.rows);
+    }
     if (op_grad->to_gate && !a.f.gate) return MINT_ERR_ARG;
     if ((op_grad->to_y || op_grad->to_after_weight || op_grad->to_after_bias) && !a.f.y && a.f.rows) return MINT_ERR_ARG;
     if ((op_grad->to_before_weight && !op->before.weight) || (op_grad->to_before_bias && !op->before.bias) ||

@@ -209,3 +209,17 @@ def test_tensors_with_a_tangent_are_refused(dev):
         with torch.inference_mode():
             assert torch.equal(norm(x_dual, n), want)
     assert torch.equal(norm(x, n), want)
+
+
+def test_gates_by_row_of_rows_without_numbers(dev):
+    """Rows of no numbers have a gate each all the same: its gradient is a sum of nothing."""
+    s, gate = torch.zeros(5, 0, device=dev), randn(5, 1, seed=1, dev=dev)
+    assert torch.equal(join_grad(s, None, s, s, gate=gate, gate_by="silu").gate, torch.zeros(5, 1, device=dev))
+    for dt in DT.values():
+        room = torch.full((700 * 3,), float("nan"), dtype=dt, device=dev)
+        op = _lib.JoinGradOp(to_gate=room.data_ptr(), to_gate_stride=3, d_stream=gate.data_ptr())
+        op.join = _lib.JoinOp(stream=gate.data_ptr(), y=gate.data_ptr(), gate=gate.data_ptr(), rows=699, width=0, stream_dtype=_lib.F32, dtype=_lib.F32,
+                              gate_dtype=DTYPE_CODE[dt], gate_form=2, scale=1.0, carry=1.0)
+        _lib.check(_lib.lib().mint_join_grad(op, torch.cuda.current_stream().cuda_stream), "mint_join_grad")
+        room = room.view(700, 3)
+        assert bool((room[:699, 0] == 0).all()) and bool(room[:, 1:].isnan().all()) and bool(room[699].isnan().all())
