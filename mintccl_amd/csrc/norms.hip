@@ -89,7 +89,7 @@ int join_args(const mint_join_op* op, JoinArgs& a) {
         !norm_known(op->before, true) || !norm_known(op->after, true))
         return MINT_ERR_ARG;
     if (op->gate && (!known(op->gate_dtype) || op->gate_form < MINT_GATE_CHANNEL || op->gate_form > MINT_GATE_ALL)) return MINT_ERR_ARG;
-    if (op->rows && !op->y && (op->gate || op->after.kind)) return MINT_ERR_ARG;
+    if (op->rows && op->width && !op->y && (op->gate || op->after.kind)) return MINT_ERR_ARG;
     if (op->rows > 0x7FFFFFFF / 4 || op->width > 0x7FFFFFFF - kLongThreads * V) return MINT_ERR_TOO_LARGE;
     a = {reinterpret_cast<const void*>(op->stream), reinterpret_cast<const void*>(op->y), reinterpret_cast<const void*>(op->gate),
          reinterpret_cast<void*>(op->new_stream), reinterpret_cast<void*>(op->next),

@@ -214,6 +214,8 @@ def test_tensors_with_a_tangent_are_refused(dev):
 def test_gates_by_row_of_rows_without_numbers(dev):
     """Rows of no numbers have a gate each all the same: its gradient is a sum of nothing."""
     s, gate = torch.zeros(5, 0, device=dev), randn(5, 1, seed=1, dev=dev)
+    for options in ({"gate": gate}, {"after": Norm(None)}, {"before": Norm(None)}, {"gate": s, "after": Norm(s[0])}, {"gate": s[0]}):
+        assert join(s, s, **options)[0].shape == join_grad(s, None, s, s, **options).y.shape == (5, 0)
     assert torch.equal(join_grad(s, None, s, s, gate=gate, gate_by="silu").gate, torch.zeros(5, 1, device=dev))
     for dt in DT.values():
         room = torch.full((700 * 3,), float("nan"), dtype=dt, device=dev)
