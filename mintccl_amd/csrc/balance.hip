@@ -92,8 +92,10 @@ struct Tokens {
     float soft[U][V];            // sigmoids, where z is not 0: the softmax
     float lse[U];                // where z is not 0: the log of the exponentials' sum
     bool there[U];
-    // `in` of the U there are tokens
-    __device__ __forceinline__ Tokens(const float (&x)[U][V], const bool (&in)[U], uint32_t first, uint32_t experts, bool use_sigmoid, bool wants_lse) {
+    bool vanished = false;       // sigmoids: a token's may have left the range, all of them
+    // `in` of the U there are tokens, whose logits have been moved down by `up`
+    __device__ __forceinline__ Tokens(const float (&x)[U][V], const float (&up)[U], const bool (&in)[U], uint32_t first, uint32_t experts, bool use_sigmoid,
+                                      bool wants_lse) {
         float top[U], sum[U], scores[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -124,7 +126,7 @@ struct Tokens {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 sum[u] = wave_sum(sum[u]);
-                lse[u] = there[u] && wants_lse ? top[u] + logf(sum[u]) : 0.0f;
+                lse[u] = there[u] && wants_lse ? top[u] + logf(sum[u]) + up[u] : 0.0f;
                 const float r = there[u] ? 1.0f / sum[u] : 0.0f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) soft[u][i] *= r;
@@ -146,7 +148,7 @@ struct Tokens {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 scores[u] = wave_sum(scores[u]);
-                // (sigmoids that have all vanished have no shares)
+                vanished |= there[u] && scores[u] < 0x1p-60f;
                 const float r = there[u] && scores[u] != 0.0f ? 1.0f / scores[u] : 0.0f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) p[u][i] *= r;
@@ -159,6 +161,21 @@ struct Tokens {
         }
     }
 };
+// Sigmoids far below 1 are e^x to the last bit: where all of a token's are, their quotients are those of its logits moved to -20 and less, and by how much is
+// kept in `up`.  (Seldom: the group is done again, from memory.)
+template <int V, int U>
+__device__ __forceinline__ void move_up(float (&x)[U][V], float (&up)[U], uint32_t first, uint32_t experts) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float top = -FLT_MAX;
+#pragma unroll
+        for (int i = 0; i < V; ++i) top = first + i < experts ? fmaxf(top, x[u][i]) : top;
+        top = wave_max(top);
+        up[u] = top < -40.0f ? top + 20.0f : 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[u][i] -= up[u];
+    }
+}
 constexpr int tokens_at_once(int v) { return v <= 4 ? 4 : v <= 8 ? 2 : 1; }
 
 struct Sums {
@@ -209,21 +226,27 @@ __global__ void __launch_bounds__(64 * kWaves) balance_tiles_kernel(BalanceArgs 
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
     for (uint32_t t0 = span.begin + wave; t0 < span.end; t0 += kWaves * U) {
-        float x[U][V];
-        bool in[U];
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+            float x[U][V], up[U] = {};
+            bool in[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t t = t0 + u * kWaves;
-            in[u] = t < span.end;
-            load_elements<DT, V>(static_cast<const T*>(a.logits) + (int64_t)(in[u] ? t : t0) * a.row_stride + first, (int64_t)a.experts - first, x[u]);
-        }
-        const Tokens<V, U> tokens(x, in, first, a.experts, a.sigmoid, a.z != 0.0f);
+            for (int u = 0; u < U; ++u) {
+                const uint32_t t = t0 + u * kWaves;
+                in[u] = t < span.end;
+                load_elements<DT, V>(static_cast<const T*>(a.logits) + (int64_t)(in[u] ? t : t0) * a.row_stride + first, (int64_t)a.experts - first, x[u]);
+            }
+            if (again) move_up(x, up, first, a.experts);
+            const Tokens<V, U> tokens(x, up, in, first, a.experts, a.sigmoid, a.z != 0.0f);
+            if (tokens.vanished && !again) continue;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum[i] += in[u] ? tokens.p[u][i] : 0.0f;
-            if (a.z != 0.0f) squares = fmaf(tokens.lse[u], tokens.lse[u], squares);
-            n += tokens.there[u];
+                for (int i = 0; i < V; ++i) sum[i] += in[u] ? tokens.p[u][i] : 0.0f;
+                if (a.z != 0.0f) squares = fmaf(tokens.lse[u], tokens.lse[u], squares);
+                n += tokens.there[u];
+            }
+            break;
         }
     }
 #pragma unroll
@@ -408,13 +431,13 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
         next = f.tokens;
         if (!f.offsets) return 1u;
         // the last lane whose beginning is not behind `t`
-        const auto last = [&]() MINT_INLINE_LAMBDA { return 63u - (uint32_t)__clzll(__ballot(begins <= t) | 1ull); };
-        uint32_t nth = last();
-        if (nth == 63) {                                      // (there may be more behind it)
+        uint64_t before = __ballot(begins <= t);
+        if (!(before & 1ull) || before >> 63) {               // (there may be more in front of them, or behind)
             window = last_below(f.sequences + 2, [&](uint32_t u) MINT_INLINE_LAMBDA { return begin_of(f, u) <= t; });
             begins = begin_of(f, window + lane);
-            nth = last();
+            before = __ballot(begins <= t);
         }
+        const uint32_t nth = 63u - (uint32_t)__clzll(before | 1ull);
         // (behind the search lane 63's is behind `t` too, unless the offsets descend)
         next = nth == 63 ? t : (uint32_t)__builtin_amdgcn_readlane((int)begins, (int)nth + 1);
         return window + nth;
@@ -438,11 +461,13 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
     };
     // what the loss's gradient is by an expert's mean share
     const auto load_of = [&](float count, float n) MINT_INLINE_LAMBDA { return d * (float)f.experts / ((float)f.topk * n) / ((float)some * n) * count; };
-    // U tokens, of one sequence (W 1) or each of its own; those that are not `inside` count nowhere
-    const auto gradients = [&](uint32_t t0, const float (&x)[U][V], const bool (&in)[U], const bool (&inside)[U], const auto& often) MINT_INLINE_LAMBDA {
+    // U tokens, of one sequence (W 1) or each of its own; those that are not `inside` count nowhere.  Whether they are done, or have to be loaded again.
+    const auto gradients = [&](uint32_t t0, float (&x)[U][V], bool again, const bool (&in)[U], const bool (&inside)[U], const auto& often) MINT_INLINE_LAMBDA {
         constexpr int W = sizeof(often) / sizeof(often[0]);
-        float mean[U];
-        const Tokens<V, U> tokens(x, inside, first, f.experts, f.sigmoid, f.z != 0.0f);
+        float mean[U], up[U] = {};
+        if (again) move_up(x, up, first, f.experts);
+        const Tokens<V, U> tokens(x, up, inside, first, f.experts, f.sigmoid, f.z != 0.0f);
+        if (tokens.vanished && !again) return false;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             mean[u] = 0.0f;
@@ -468,12 +493,13 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
             }
             store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, more);
         }
+        return true;
     };
     uint32_t next;
     const uint32_t v = sequence_of(begin, next);
     if (next < end) {
         // Tokens of several sequences: each has its own load, all of them on their way with the logits.
-        for (uint32_t t0 = begin + wave_in_block(); t0 < end; t0 += kWaves * U) {
+        for (uint32_t t0 = begin + wave_in_block(), again = 0; t0 < end;) {
             float x[U][V], often[U][V], n[U];
             bool in[U], inside[U];
             load_logits(t0, x, in);
@@ -490,7 +516,8 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < V; ++i) often[u][i] = load_of(often[u][i], n[u]);
-            gradients(t0, x, in, inside, often);
+            again = !gradients(t0, x, again, in, inside, often);
+            if (!again) t0 += kWaves * U;
         }
     } else if (v == 0 || v > f.sequences) {                   // tokens of no sequence
         for (uint32_t t = begin + wave_in_block(); t < end; t += kWaves) {
@@ -503,11 +530,12 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
         float often[1][V];
 #pragma unroll
         for (int i = 0; i < V; ++i) often[0][i] = load_of(count_of(v - 1, i), n);
-        for (uint32_t t0 = begin + wave_in_block(); t0 < end; t0 += kWaves * U) {
+        for (uint32_t t0 = begin + wave_in_block(), again = 0; t0 < end;) {
             float x[U][V];
             bool in[U];
             load_logits(t0, x, in);
-            gradients(t0, x, in, in, often);
+            again = !gradients(t0, x, again, in, in, often);
+            if (!again) t0 += kWaves * U;
         }
     }
 }

@@ -10,7 +10,7 @@ from mintccl_amd.norms import Norm, join, join_grad, norm, norm_grad
 from mintccl_amd.routing import balance, balance_grad
 from tests.block_oracle import DT, EVALUATED, UNIT, balance64, close, norm64
 from tests.expert_oracle import randn
-from tests.test_gpu_balance import SHARE, inputs, tokens_units
+from tests.test_gpu_balance import SHARE, inputs, offsets_of, tokens_units
 from tests.test_gpu_norms import a_norm, parts
 
 pytestmark = pytest.mark.gpu
@@ -225,3 +225,31 @@ def test_gates_by_row_of_rows_without_numbers(dev):
         _lib.check(_lib.lib().mint_join_grad(op, torch.cuda.current_stream().cuda_stream), "mint_join_grad")
         room = room.view(700, 3)
         assert bool((room[:699, 0] == 0).all()) and bool(room[:, 1:].isnan().all()) and bool(room[699].isnan().all())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("t,e,lengths", [(40, 24, None), (700, 200, None), (900, 40, [11] * 81), (1200, 12, [1, 0, 3, 7] * 100), (300, 600, [150, 150])])
+def test_sigmoids_that_are_all_too_small_for_32_bits(dev, t, e, lengths, dt):
+    """Tokens whose logits are all far below zero still have shares: their sigmoids' quotients, which no power of e leaves the range of."""
+    x, experts = inputs(t, e, 3, dt, dev)
+    offsets = offsets_of(lengths, dev, 2 if lengths and sum(lengths) + 2 < t else 0)
+    far = torch.arange(t, device=dev) // 3 % 4
+    x = (x.float() - torch.tensor([0.0, 90.0, 140.0, 400.0], device=dev)[far][:, None]).to(DT[dt])
+    got = balance(x, experts, score="sigmoid", offsets=offsets, z=1e-3)
+    leaf = x.cpu().double().requires_grad_()
+    loss, counts, shares, there = balance64(leaf, experts.cpu(), "sigmoid", None if offsets is None else offsets.cpu(), 1e-3)
+    assert torch.equal(got.counts.cpu(), counts) and torch.equal(got.there.cpu(), there)
+    units = tokens_units(t)
+    close(got.shares, shares, shares, torch.float32, units)
+    close(got.loss, loss.detach(), loss.detach(), torch.float32, 2 * units + (64 + 16 + len(lengths or []) / 64) * UNIT)
+    grad = balance_grad(torch.ones((), device=dev), x, experts, got, score="sigmoid", offsets=offsets, z=1e-3)
+    want = torch.autograd.grad(loss, leaf)[0].masked_fill(torch.isneginf(leaf), 0)
+    v, some, every = leaf.detach(), max(int((there > 0).sum()), 1), max(int(there.sum()), 1)
+    p = (torch.sigmoid(v) / torch.sigmoid(v).sum(1, keepdim=True)).nan_to_num(0)
+    # (the sums' log is rounded at the magnitude of the logits: that is in the first factor of z's part)
+    size = 2e-3 / every * (torch.logsumexp(v, 1, keepdim=True).abs() + 16).nan_to_num(0, 0, 0) * torch.softmax(v, 1).nan_to_num(0)
+    ends = [0, t] if offsets is None else offsets.tolist()
+    for i, (a, b) in enumerate(zip(ends, ends[1:])):
+        load = e * counts[i].double() / (3 * max(int(there[i]), 1)) / (some * max(int(there[i]), 1))
+        size[a:b] += p[a:b] * (load + (p[a:b] * load).sum(1, keepdim=True))
+    close(grad, want, size, DT[dt], 4 * SHARE)
