@@ -22,6 +22,11 @@ __device__ __forceinline__ float tangent(float x) {
     const float far = copysignf(1.0f - 2.0f * reciprocal(1.0f + exponential(2.0f * fabsf(x))), x);
     return fabsf(x) < 0.25f ? near : far;
 }
+// 1 - tanh^2 = 1 / cosh^2, without a difference that cancels where tanh is near 1
+__device__ __forceinline__ float tangent_slope(float x) {
+    const float e = exponential(-2.0f * fabsf(x)), r = reciprocal(1.0f + e);
+    return 4.0f * e * r * r;
+}
 // P(N > x) of a normal N for x >= 0: Abramowitz and Stegun, 7.1.26 (1.5e-7 off at most, for twice of it), with e^(-x^2 / 2) as `power`.
 __device__ __forceinline__ float normal_above(float x, float power) {
     const float t = reciprocal(fmaf(0.3275911f * 0.70710678f, x, 1.0f));
@@ -89,10 +94,7 @@ __device__ __forceinline__ void slopes(int kind, float (&v)[N]) {
             break;
         case MINT_ACT_TANH:
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float t = tangent(v[i]);
-                v[i] = 1.0f - t * t;
-            }
+            for (int i = 0; i < N; ++i) v[i] = tangent_slope(v[i]);
             break;
         case MINT_ACT_GELU:
 #pragma unroll
@@ -126,10 +128,7 @@ __device__ __forceinline__ float gate_value(int kind, float g) {
 }
 __device__ __forceinline__ float gate_slope(int kind, float g) {
     if (kind == MINT_ACT_NONE) return 1.0f;
-    if (kind == MINT_ACT_TANH) {
-        const float t = tangent(g);
-        return 1.0f - t * t;
-    }
+    if (kind == MINT_ACT_TANH) return tangent_slope(g);
     const float e = exponential(-fabsf(g)), r = reciprocal(1.0f + e), s = (g < 0.0f ? e : 1.0f) * r, slope = e * r * r;
     return kind == MINT_ACT_SILU ? (slope == 0.0f ? s : fmaf(g, slope, s)) : slope;
 }

@@ -253,3 +253,25 @@ def test_sigmoids_that_are_all_too_small_for_32_bits(dev, t, e, lengths, dt):
         load = e * counts[i].double() / (3 * max(int(there[i]), 1)) / (some * max(int(there[i]), 1))
         size[a:b] += p[a:b] * (load + (p[a:b] * load).sum(1, keepdim=True))
     close(grad, want, size, DT[dt], 4 * SHARE)
+
+
+def test_slopes_of_the_hyperbolic_tangent_far_out(dev):
+    """1 / cosh^2, relative to itself: its exponential is a few roundings off, two reciprocals and three products are one each or two."""
+    z = torch.linspace(-40, 40, 4001, device=dev)[None]
+    want = 1 / torch.cosh(z.cpu().double()) ** 2
+    close(activation_grad(torch.ones_like(z), z, "tanh")[0], want, want, torch.float32, EVALUATED)
+
+
+@pytest.mark.parametrize("shape", ["channel", "row", "all"])
+@pytest.mark.parametrize("width", [200, 4104, 9001])
+def test_slopes_of_gates_by_a_hyperbolic_tangent_far_out(dev, width, shape):
+    """A gate's gradient by tanh, relative to itself: 1 / cosh^2 has no difference that cancels."""
+    rows = 3
+    size = {"channel": (width,), "row": (rows, 1), "all": (rows, width)}[shape]
+    n = torch.Size(size).numel()
+    g = (torch.arange(n, device=dev) * (40.0 / max(n - 1, 1)) - (20 if shape != "row" else 9)).view(size)
+    ones_ = torch.ones(rows, width, device=dev)
+    got = join_grad(ones_, None, ones_, ones_, gate=g, gate_by="tanh").gate
+    want = (width if shape == "row" else rows if shape == "channel" else 1) / torch.cosh(g.cpu().double()) ** 2
+    # (the sums are of whole numbers; one product and its rounding beside the slope's own 16)
+    close(got, want, want, torch.float32, 18 * UNIT)
