@@ -251,7 +251,7 @@ struct Ring {
 #pragma unroll
             for (int n = 0; n < EACH; ++n) {
                 const uint32_t row = S::row_of(unit(n)), piece = S::piece_of(unit(n)) * 16;
-                const uint32_t back = ALONG ? piece < left * SIZE ? 0u : piece : row < left ? 0u : row * (uint32_t)stride;
+                const uint32_t back = ALONG ? piece < min(left, UNIT) * SIZE ? 0u : piece : row < left ? 0u : row * (uint32_t)stride;
                 to_lds16(from, at[n] - back, to + (wave * EACH + n) * 1024);
             }
         }
