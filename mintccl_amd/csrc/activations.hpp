@@ -8,7 +8,8 @@
 namespace mint {
 
 // e^x: 2^p of the rounded product p = x log2(e), and what the rounding left over to the first order; a few units of 2^-24 off, in
-// eight instructions.  Beyond the range it is infinite, or 0.
+// eight instructions.  From |p| = 126 on (|x| = 87.3) nothing is put right, since 2^p may be infinite: up to |p| = 128 it is off by the rounding of p, 44 units at most.  Beyond
+// the range it is infinite, or 0.
 __device__ __forceinline__ float exponential(float x) {
     constexpr float kLog2e = 0x1.715476p+0f, kRest = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;
     const float p = x * kLog2e, left = fmaf(x, kRest, fmaf(x, kLog2e, -p)), power = __builtin_amdgcn_exp2f(p);

@@ -194,7 +194,7 @@ __device__ __forceinline__ float loss_of(const BalanceArgs& a, float terms, floa
 }
 
 // A wavefront has every kWaves-th token of the tile, a lane V consecutive experts.  ALONE: the tile has all tokens, and the results are made here.
-// Bound by its vector instructions and their steps across lanes: 65536 tokens of 256 experts, sigmoids: 19 us, of which the 67 MB are 14 (one token at a
+// Bound by its vector instructions and their steps across lanes: 65536 tokens of 256 experts, sigmoids: 19.6 us, of which the 67 MB are 12 (one token at a
 // time, the library's exponential: 37).
 template <int DT, int V, bool ALONE>
 __global__ void __launch_bounds__(64 * kWaves) balance_tiles_kernel(BalanceArgs a) {
@@ -382,10 +382,10 @@ struct BalanceGradArgs {
     void* d_logits;
     int64_t add_stride, d_stride;
 };
-// Tiles lie side by side here, whatever the offsets say, and a token belongs to the last of the sequences that begin at it or before it: so every row is
-// written once, by one thread block, also where the offsets descend; and there are no more thread blocks where there are more sequences, whose tokens each of them
-// adds up, eight loads of a thread at a time (66000 tokens of 20 experts in 65535 sequences 39 us; a thread block for each of them 1180).  65536 tokens of 256 experts, sigmoids: 29 us for 134 MB (4.7 TB/s; one token
-// at a time, the library's exponential: 56).
+// Tiles lie side by side here, whatever the offsets say, and a token belongs to the last of the sequences that begin at it or before it: so every row is written once, by
+// one thread block, also where the offsets descend; and there are no more thread blocks where there are more sequences, whose tokens each of them adds up, eight loads
+// of a thread at a time (66000 tokens of 20 experts in 65535 sequences 39 us; a thread block for each of them 1180).  65536 tokens of 256 experts,
+// sigmoids: 30 us for 134 MB (4.5 TB/s; one token at a time, the library's exponential: 56).
 template <int DT, int V>
 __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradArgs a) {
     using T = typename Elem<DT>::type;

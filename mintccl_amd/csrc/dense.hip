@@ -5,7 +5,9 @@
 //
 // The three products are one kernel: the result's rows come from one operand, its columns from the other, and each of them
 // lies in memory either with the depth along its rows ("along": x and w of the first product) or across them ("across": w of d_x, both
-// of d_w).  Sums are in 32 bits in a fixed order; z and d_z are rounded once each to the operands' type, out once to its own.
+// of d_w).  Sums are in 32 bits in a fixed order; out is rounded once to its own type, and z and d_z once each to the operands': d_z is an operand, which the matrix
+// instructions take in 16 bits, and z the largest thing that is kept (in 32 bits it would be twice the bytes, written and read again).  In bf16 gradients are then 2.4e-3
+// off in 2-norm for the 1.7e-3 that their own rounding makes (8192 x 8192 x 4096, silu).
 #include "activations.hpp"
 
 #include <algorithm>
@@ -502,8 +504,9 @@ struct Tile {
 //
 // Bound by the matrix instructions where there are tiles enough for all compute units, then by the last round of tiles and its way out.  bf16, 8192 x 8192 x
 // 4096: x w^T 440 us (1.25 PFLOP/s), d_z w 428, d_z^T x 446 (a library's 436, 436, 496); with bias, an activation of the result and z stored 460.
-// 2048 x 4096 x 4096 with a residual and a result in 32 bits 73 (the library's bare product 59): one round of tiles, whose way out no other hides.  f32, 4096 x 256 x
-// 4096: 67 (128 TFLOP/s; its four sets' sums added up and stored by one of them 69.6; the library's 68.5).
+// 2048 x 4096 x 4096 with a residual and a result in 32 bits 73 (the library's bare product 60): one round of tiles, whose way out no other hides.  f32, 4096 x 256 x
+// 4096: 67 (128 TFLOP/s; its four sets' sums added up and stored by one of them 69.6; the library's 69), in the first milliseconds of work 75 (the library's 80).  f32
+// with the depth across, 4096^3: x w^T 942 us, d_z w 954, d_z^T x 971 (146, 144 and 142 TFLOP/s, the library 915 each): four reads of LDS for one.
 // Not direct, 50 x 5001 x 2500 f16: 13.4, and 5.3 for the parts' sums (a library's 20.2).
 template <int DT, int BM, int BN, int WM, int NX, int NW, int SPLIT, bool X_ALONG, bool W_ALONG, bool DIRECT>
 __global__ void __launch_bounds__(64 * WM * (BN / 64) * SPLIT) dense_kernel(DenseArgs a) {
@@ -724,7 +727,8 @@ struct ActivationGradArgs {
     uint32_t rows, cols, chunks, groups;
     int activation;
 };
-// A wavefront has 512 columns of every groups-th row.  Bound by memory: 8192 x 8192 bf16 80 us for 403 MB, 5.0 TB/s, and 4.9 for the bias's sums.
+// A wavefront has 512 columns of every groups-th row.  Bound by memory: 8192 x 8192 bf16 80 us for 403 MB, 5.0 TB/s, and 4.9 for the bias's sums.  Fewer columns leave
+// lanes without work: 65536 x 256 46 us for 101 MB.
 constexpr int kGradWaves = 4;
 template <int D, int DT>
 __global__ void __launch_bounds__(64 * kGradWaves) activation_grad_kernel(ActivationGradArgs a) {
@@ -779,16 +783,22 @@ uint32_t size_of(int dtype) { return dtype == MINT_F32 ? 4 : 2; }
 // Which tiles, and how many thread blocks share one.  What a launch takes by this, us: 2.5, and for each round over the compute units a beginning and an
 // end and so much for a block of the depth (128 bytes), less of both in a last round of `few` tiles; sums that pass through memory take another launch and their bytes. Measured (bf16
 // if not said otherwise, operands used in turn), and the rule's choice behind =:
-//   4096 x 256 x 4096 f32       64 x 64 74, in two sets 76, 128 x 128 134 (two parts)                    = 64 x 64
-//   512 x 4096 x 4096           64 x 64 in two sets 28.5 - 31.7, 128 x 128 in two sets 31.7 - 32.9, in two parts of them 30 = the last of these
-//   1024 x 4096 x 4096          128 x 128 in two sets 35.4, in one 38.4, 128 x 256 47                    = 128 x 128 in two sets
-//   2048 x 4096 x 4096          128 x 256 60, 128 x 128 64, 256 x 256 79                                 = 128 x 256
-//   8192 x 1024 x 512           128 x 128 15.8, 128 x 256 17.2, 256 x 256 22.5                           = 128 x 128
-//   4096 x 4096 x 512 (d_w)     256 x 256 26.4, 128 x 128 28.3, 128 x 256 34                             = 256 x 256
-//   64 x 4096 x 4096            64 x 64 in one part 17.5, two 15.6, four 15.4                            = four
-//   3000 x 2000 x 4000 f32      128 x 128 in two parts 370, 64 x 64 387, 128 x 128 in one 461            = 128 x 128 in two parts
-//   700 x 3000 x 5000           128 x 256 in three parts 45, 128 x 128 in three 48, in two sets 56       = 128 x 128 in two sets (rows that begin inside
+//   4096 x 256 x 4096 f32       64 x 64 in four sets 67, in two 76, 128 x 128 134 (two parts)            = 64 x 64 in four sets
+//   512 x 4096 x 4096           64 x 64 in two sets 30.0, 128 x 128 in two sets 30.9, in two parts of them 31.1 = the last of these
+//   1024 x 4096 x 4096          128 x 128 in two sets 37.5, in one 40.5, 128 x 256 49                    = 128 x 128 in two sets
+//   2048 x 4096 x 4096          128 x 256 62, 128 x 128 66, 256 x 256 79                                 = 128 x 256
+//   8192 x 1024 x 512           128 x 128 17.4, 128 x 256 18.1, 256 x 256 23.2                           = 128 x 128
+//   4096 x 4096 x 512 (d_w)     256 x 256 27.4, 128 x 128 30.2, 128 x 256 36                             = 256 x 256
+//   64 x 4096 x 4096            64 x 64 in four sets 16.3, two parts of them 15.6, four 15.2             = four
+//   3000 x 2000 x 4000 f32      128 x 128 in two parts 372, 64 x 64 in two sets 389, 128 x 128 in one 463 = 128 x 128 in two parts
+//   700 x 3000 x 5000           128 x 256 in three parts 45, 128 x 128 in three 48, in two sets 54       = 128 x 128 in two sets (rows that begin inside
 //                               lines of 128 bytes, which the model does not know of)
+// The gradients go by the same figures, though 32-bit operands across the depth are read from LDS a number at a time:
+//   4096 x 4096 x 256 f32 (d_x) 128 x 128 77, 64 x 64 in two sets 100                                    = 128 x 128
+//   256 x 4096 x 4096 f32 (d_w) 64 x 64 in four sets 72, in two 86, 128 x 128 139 (two parts)            = 64 x 64 in four sets
+//   8192 x 1024 x 1024 f32 (d_x) 128 x 128 130, 64 x 64 in two sets 150                                  = 128 x 128
+//   1024 x 1024 x 8192 f32 (d_w) 64 x 64 in four sets 136, 128 x 128 in two sets and four parts 140, in four parts 143 = the second of these
+//   128 x 2048 x 4099 f32 (d_w) 64 x 64 in two sets and four parts 32.3, in four sets and four parts 32.9 = the first of these
 enum { kThin, k64Four, k64Two, k128, k128Two, k128x256, k256, kHeld };
 struct Choice {
     int tile;
@@ -860,6 +870,14 @@ Operand w_of(const mint_dense_op& op) {
     const uint64_t size = size_of(op.dtype), across = op.form != MINT_DENSE_PRODUCT;
     return {op.w, op.w_stride * (int64_t)size, across ? op.depth : op.cols, (across ? op.cols : op.depth) * size};
 }
+// Up to 32 rows go to the kernel for few rows.  us, 1, 16 and 32 rows, weights from memory, and what tiles take:
+//   4096 columns of 4096 numbers, bf16   8.8, 11.1, 14.5    tiles 14.0, 15.1, 15.6     (33 rows 20.3, tiles 15.6)
+//   the same in f32                      15.1, 18.0, 27.1   tiles 28.7, 29.3, 29.3     (33 rows 39.6, tiles 28.7)
+//   8192 of 512, bf16                    4.6, 5.3, 6.2      tiles 7.5, 7.6, 7.8
+//   256 of 4096, bf16                    6.7, 9.3, 12.8     tiles 9.8, 10.1, 10.1
+//   11000 of 4096, bf16                  19.6, 28.9, 40.8   tiles 24.4, 24.5, 24.7
+//   1024 of 16384, bf16                  22, 33, 47         tiles 17.8, 17.1, 17.4
+// So from about 16 rows on the rule costs time where there are many columns or much depth: every wavefront reads x again.
 Choice choose(const mint_dense_op& op) {
     if (op.form == MINT_DENSE_PRODUCT && op.rows <= 32) return {kThin, 1, 0.0f, false};
     const Operand x = x_of(op), w = w_of(op);
@@ -913,6 +931,9 @@ int go_thin(DenseArgs a, hipStream_t s) {
 template <int DT>
 int go_dense(const mint_dense_op& op, DenseArgs a, const Choice& c, hipStream_t s) {
     if (c.tile == kThin) {
+        // Eight wavefronts share the depth of 16 columns, or two each of 64, where there are columns enough.  us, 1, 16 and 32 rows, bf16, eight and two:
+        // 4096 columns of 4096 numbers 8.8, 11.1, 14.5 and 22, 31, 45; 16384 of 1024 11.5, 13.1, 16.0 and 8.8, 10.5, 13.9; 14000 of 4096 24, 37, 53
+        // and 28, 35, 48; 12304 of 72 3.9, 4.1, 4.2 and 3.2, 3.3, 3.4; but 50000 of 2048 38, 57, 84 and 44, 66, 95.
         const bool few = ceil_div(op.cols, 16) <= 768;
         if (op.rows <= 16) return few ? go_thin<DT, 1, 8>(a, s) : go_thin<DT, 1, 2>(a, s);
         return few ? go_thin<DT, 2, 8>(a, s) : go_thin<DT, 2, 2>(a, s);

@@ -137,7 +137,8 @@ class ExpertBlock:
 
     ``up`` (inner, width) and ``down`` (width, inner) are a shared expert's weights, bfloat16 or float16 (the rows' type); ``gate`` (width,)
     scales the channels, ``before`` and ``after`` are the norms of this block's and of the next one's rows, with weights and biases or without.
-    ``z`` is :func:`~mintccl_amd.routing.balance`'s."""
+    The layer's sum is rounded to the rows' type when the ranks hand it out, and y once more when the shared expert's is added (a result in 32 bits would
+    need the next block's rows in 32 bits too), and the rows' gradient likewise on the way back.  ``z`` is :func:`~mintccl_amd.routing.balance`'s."""
 
     def __init__(self, layer: ExpertLayer, before: Norm, up: torch.Tensor, down: torch.Tensor, after: Norm, gate: torch.Tensor, z: float = 0.0) -> None:
         bare = lambda n: n._replace(**{v: t.detach() for v, t in (("weight", n.weight), ("bias", n.bias)) if t is not None})  # noqa: E731
