@@ -92,7 +92,7 @@ struct Tokens {
     float soft[U][V];            // sigmoids, where z is not 0: the softmax
     float lse[U];                // where z is not 0: the log of the exponentials' sum
     bool there[U];
-    bool vanished = false;       // sigmoids: a token's may have left the range, all of them
+    uint32_t vanished = 0;       // sigmoids: a bit for each token whose all may have left the range
     // `in` of the U there are tokens, whose logits have been moved down by `up`
     __device__ __forceinline__ Tokens(const float (&x)[U][V], const float (&up)[U], const bool (&in)[U], uint32_t first, uint32_t experts, bool use_sigmoid,
                                       bool wants_lse) {
@@ -148,7 +148,7 @@ struct Tokens {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 scores[u] = wave_sum(scores[u]);
-                vanished |= there[u] && scores[u] < 0x1p-60f;
+                vanished |= there[u] && scores[u] < 0x1p-60f ? 1u << u : 0u;
                 const float r = there[u] && scores[u] != 0.0f ? 1.0f / scores[u] : 0.0f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) p[u][i] *= r;
@@ -162,16 +162,17 @@ struct Tokens {
     }
 };
 // Sigmoids far below 1 are e^x to the last bit: where all of a token's are, their quotients are those of its logits moved to -20 and less, and by how much is
-// kept in `up`.  (Seldom: the group is done again, from memory.)
+// kept in `up`.  `which` have to be moved.  (Seldom: their group is done again, from memory.)
 template <int V, int U>
-__device__ __forceinline__ void move_up(float (&x)[U][V], float (&up)[U], uint32_t first, uint32_t experts) {
+__device__ __forceinline__ void move_up(float (&x)[U][V], float (&up)[U], uint32_t which, uint32_t first, uint32_t experts) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+        if (!(which >> u & 1u)) continue;
         float top = -FLT_MAX;
 #pragma unroll
         for (int i = 0; i < V; ++i) top = first + i < experts ? fmaxf(top, x[u][i]) : top;
         top = wave_max(top);
-        up[u] = top < -40.0f ? top + 20.0f : 0.0f;
+        up[u] = top + 20.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) x[u][i] -= up[u];
     }
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(64 * kWaves) balance_tiles_kernel(BalanceArgs 
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
     for (uint32_t t0 = span.begin + wave; t0 < span.end; t0 += kWaves * U) {
 #pragma unroll 1
-        for (bool again = false;; again = true) {
+        for (uint32_t again = 0;;) {
             float x[U][V], up[U] = {};
             bool in[U];
 #pragma unroll
@@ -236,9 +237,12 @@ __global__ void __launch_bounds__(64 * kWaves) balance_tiles_kernel(BalanceArgs 
                 in[u] = t < span.end;
                 load_elements<DT, V>(static_cast<const T*>(a.logits) + (int64_t)(in[u] ? t : t0) * a.row_stride + first, (int64_t)a.experts - first, x[u]);
             }
-            if (again) move_up(x, up, first, a.experts);
+            if (again) move_up(x, up, again, first, a.experts);
             const Tokens<V, U> tokens(x, up, in, first, a.experts, a.sigmoid, a.z != 0.0f);
-            if (tokens.vanished && !again) continue;
+            if (tokens.vanished && !again) {
+                again = tokens.vanished;
+                continue;
+            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -461,13 +465,14 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
     };
     // what the loss's gradient is by an expert's mean share
     const auto load_of = [&](float count, float n) MINT_INLINE_LAMBDA { return d * (float)f.experts / ((float)f.topk * n) / ((float)some * n) * count; };
-    // U tokens, of one sequence (W 1) or each of its own; those that are not `inside` count nowhere.  Whether they are done, or have to be loaded again.
-    const auto gradients = [&](uint32_t t0, float (&x)[U][V], bool again, const bool (&in)[U], const bool (&inside)[U], const auto& often) MINT_INLINE_LAMBDA {
+    // U tokens, of one sequence (W 1) or each of its own; those that are not `inside` count nowhere.  Which of them have to be moved up first, and the
+    // group loaded again for it; none: they are done.
+    const auto gradients = [&](uint32_t t0, float (&x)[U][V], uint32_t again, const bool (&in)[U], const bool (&inside)[U], const auto& often) MINT_INLINE_LAMBDA -> uint32_t {
         constexpr int W = sizeof(often) / sizeof(often[0]);
         float mean[U], up[U] = {};
-        if (again) move_up(x, up, first, f.experts);
+        if (again) move_up(x, up, again, first, f.experts);
         const Tokens<V, U> tokens(x, up, inside, first, f.experts, f.sigmoid, f.z != 0.0f);
-        if (tokens.vanished && !again) return false;
+        if (tokens.vanished && !again) return tokens.vanished;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             mean[u] = 0.0f;
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
             }
             store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, more);
         }
-        return true;
+        return 0u;
     };
     uint32_t next;
     const uint32_t v = sequence_of(begin, next);
@@ -516,7 +521,7 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int i = 0; i < V; ++i) often[u][i] = load_of(often[u][i], n[u]);
-            again = !gradients(t0, x, again, in, inside, often);
+            again = gradients(t0, x, again, in, inside, often);
             if (!again) t0 += kWaves * U;
         }
     } else if (v == 0 || v > f.sequences) {                   // tokens of no sequence
@@ -534,7 +539,7 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
             float x[U][V];
             bool in[U];
             load_logits(t0, x, in);
-            again = !gradients(t0, x, again, in, in, often);
+            again = gradients(t0, x, again, in, in, often);
             if (!again) t0 += kWaves * U;
         }
     }

@@ -255,6 +255,21 @@ def test_sigmoids_that_are_all_too_small_for_32_bits(dev, t, e, lengths, dt):
     close(grad, want, size, DT[dt], 4 * SHARE)
 
 
+@pytest.mark.parametrize("e", [24, 100, 200, 400, 1000])
+def test_a_tokens_gradient_does_not_depend_on_the_tokens_beside_it(dev, e):
+    """... not even where those are done again: to the last bit."""
+    x, experts = inputs(300, e, 3, "f32", dev, masks=False)
+    x = x - torch.tensor([0.0, 38.0, 41.0, 43.0, 60.0], device=dev)[torch.arange(300, device=dev) % 5][:, None]
+    other = x.clone()
+    other[::3] -= 300.0
+    one = torch.ones((), device=dev)
+    for offsets in (None, torch.tensor([0, 7, 7, 100, 300], dtype=torch.int32, device=dev)):
+        found = balance(x, experts, score="sigmoid", offsets=offsets)
+        a, b = (balance_grad(one, v, experts, found, score="sigmoid", offsets=offsets) for v in (x, other))
+        same = torch.arange(300, device=dev) % 3 != 0
+        assert torch.equal(a[same], b[same]) and bool(a.isfinite().all()) and bool(b.isfinite().all())
+
+
 def test_slopes_of_the_hyperbolic_tangent_far_out(dev):
     """1 / cosh^2, relative to itself: its exponential is a few roundings off, two reciprocals and three products are one each or two."""
     z = torch.linspace(-40, 40, 4001, device=dev)[None]
