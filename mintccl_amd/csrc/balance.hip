@@ -92,7 +92,7 @@ struct Tokens {
     float soft[U][V];            // sigmoids, where z is not 0: the softmax
     float lse[U];                // where z is not 0: the log of the exponentials' sum
     bool there[U];
-    uint32_t vanished = 0;       // sigmoids: a bit for each token whose all may have left the range
+    uint32_t vanished = 0;       // sigmoids: a bit for each token whose all may have left the range; it has no shares
     // `in` of the U there are tokens, whose logits have been moved down by `up`
     __device__ __forceinline__ Tokens(const float (&x)[U][V], const float (&up)[U], const bool (&in)[U], uint32_t first, uint32_t experts, bool use_sigmoid,
                                       bool wants_lse) {
@@ -148,8 +148,9 @@ struct Tokens {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 scores[u] = wave_sum(scores[u]);
-                vanished |= there[u] && scores[u] < 0x1p-60f ? 1u << u : 0u;
-                const float r = there[u] && scores[u] != 0.0f ? 1.0f / scores[u] : 0.0f;
+                const bool far = there[u] && scores[u] < 0x1p-60f;
+                vanished |= far ? 1u << u : 0u;
+                const float r = there[u] && !far ? 1.0f / scores[u] : 0.0f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) p[u][i] *= r;
             }
@@ -161,21 +162,17 @@ struct Tokens {
         }
     }
 };
-// Sigmoids far below 1 are e^x to the last bit: where all of a token's are, their quotients are those of its logits moved to -20 and less, and by how much is
-// kept in `up`.  `which` have to be moved.  (Seldom: their group is done again, from memory.)
-template <int V, int U>
-__device__ __forceinline__ void move_up(float (&x)[U][V], float (&up)[U], uint32_t which, uint32_t first, uint32_t experts) {
+// Sigmoids far below 1 are e^x to the last bit: where all of a token's are, their quotients are those of its logits moved to -20 and less.  By how much comes
+// back.  (Seldom: such tokens are done behind the others, one by one.)
+template <int V>
+__device__ __forceinline__ float move_up(float (&x)[V], uint32_t first, uint32_t experts) {
+    float top = -FLT_MAX;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (!(which >> u & 1u)) continue;
-        float top = -FLT_MAX;
+    for (int i = 0; i < V; ++i) top = first + i < experts ? fmaxf(top, x[i]) : top;
+    const float up = wave_max(top) + 20.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) top = first + i < experts ? fmaxf(top, x[u][i]) : top;
-        top = wave_max(top);
-        up[u] = top + 20.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[u][i] -= up[u];
-    }
+    for (int i = 0; i < V; ++i) x[i] -= up;
+    return up;
 }
 constexpr int tokens_at_once(int v) { return v <= 4 ? 4 : v <= 8 ? 2 : 1; }
 
@@ -223,35 +220,38 @@ __global__ void __launch_bounds__(64 * kWaves) balance_tiles_kernel(BalanceArgs 
         if (e < a.experts) atomicAdd(counts + e, 1u);
     }
     float sum[V], squares = 0.0f;
-    uint32_t n = 0;
+    uint32_t n = 0, vanished = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
     for (uint32_t t0 = span.begin + wave; t0 < span.end; t0 += kWaves * U) {
-#pragma unroll 1
-        for (uint32_t again = 0;;) {
-            float x[U][V], up[U] = {};
-            bool in[U];
+        float x[U][V];
+        const float up[U] = {};
+        bool in[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t t = t0 + u * kWaves;
-                in[u] = t < span.end;
-                load_elements<DT, V>(static_cast<const T*>(a.logits) + (int64_t)(in[u] ? t : t0) * a.row_stride + first, (int64_t)a.experts - first, x[u]);
-            }
-            if (again) move_up(x, up, again, first, a.experts);
-            const Tokens<V, U> tokens(x, up, in, first, a.experts, a.sigmoid, a.z != 0.0f);
-            if (tokens.vanished && !again) {
-                again = tokens.vanished;
-                continue;
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) sum[i] += in[u] ? tokens.p[u][i] : 0.0f;
-                if (a.z != 0.0f) squares = fmaf(tokens.lse[u], tokens.lse[u], squares);
-                n += tokens.there[u];
-            }
-            break;
+        for (int u = 0; u < U; ++u) {
+            const uint32_t t = t0 + u * kWaves;
+            in[u] = t < span.end;
+            load_elements<DT, V>(static_cast<const T*>(a.logits) + (int64_t)(in[u] ? t : t0) * a.row_stride + first, (int64_t)a.experts - first, x[u]);
         }
+        const Tokens<V, U> tokens(x, up, in, first, a.experts, a.sigmoid, a.z != 0.0f);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] += in[u] ? tokens.p[u][i] : 0.0f;
+            if (a.z != 0.0f) squares = fmaf(tokens.lse[u], tokens.lse[u], squares);
+            n += tokens.there[u];
+        }
+        vanished |= tokens.vanished;
+    }
+    for (uint32_t t = vanished ? span.begin + wave : span.end; t < span.end; t += kWaves) {
+        float x[1][V], up[1] = {};
+        const bool in[1] = {true};
+        load_elements<DT, V>(static_cast<const T*>(a.logits) + (int64_t)t * a.row_stride + first, (int64_t)a.experts - first, x[0]);
+        if (!Tokens<V, 1>(x, up, in, first, a.experts, true, false).vanished) continue;
+        up[0] = move_up(x[0], first, a.experts);
+        const Tokens<V, 1> token(x, up, in, first, a.experts, true, false);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum[i] += token.p[0][i];
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) shares[wave][first + i] = sum[i];
@@ -446,9 +446,10 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
         next = nth == 63 ? t : (uint32_t)__builtin_amdgcn_readlane((int)begins, (int)nth + 1);
         return window + nth;
     };
-    const auto load_logits = [&](uint32_t t0, float (&x)[U][V], bool (&in)[U]) MINT_INLINE_LAMBDA {
+    const auto load_logits = [&](uint32_t t0, auto& x, auto& in) MINT_INLINE_LAMBDA {
+        constexpr int N = sizeof(in) / sizeof(in[0]);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < N; ++u) {
             const uint32_t t = t0 + u * kWaves;
             in[u] = t < end;
             const T* const row = static_cast<const T*>(f.logits) + (int64_t)(in[u] ? t : t0) * f.row_stride;
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
             if constexpr (V == 1) x[u][0] = Elem<DT>::load(*as_global(row + min(first, f.experts - 1)));
             else load_elements<DT, V>(row + first, left, x[u]);
         }
-        __builtin_amdgcn_sched_barrier(0);                    // (all of them, before the first is waited for)
+        if constexpr (V <= 2) __builtin_amdgcn_sched_barrier(0);      // (all of them, before the first is waited for)
     };
     // (clamped where it is one to a lane, as there)
     const auto count_of = [&](uint64_t sequence, int i) MINT_INLINE_LAMBDA {
@@ -465,26 +466,24 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
     };
     // what the loss's gradient is by an expert's mean share
     const auto load_of = [&](float count, float n) MINT_INLINE_LAMBDA { return d * (float)f.experts / ((float)f.topk * n) / ((float)some * n) * count; };
-    // U tokens, of one sequence (W 1) or each of its own; those that are not `inside` count nowhere.  Which of them have to be moved up first, and the
-    // group loaded again for it; none: they are done.
-    const auto gradients = [&](uint32_t t0, float (&x)[U][V], uint32_t again, const bool (&in)[U], const bool (&inside)[U], const auto& often) MINT_INLINE_LAMBDA -> uint32_t {
-        constexpr int W = sizeof(often) / sizeof(often[0]);
-        float mean[U], up[U] = {};
-        if (again) move_up(x, up, again, first, f.experts);
-        const Tokens<V, U> tokens(x, up, inside, first, f.experts, f.sigmoid, f.z != 0.0f);
-        if (tokens.vanished && !again) return tokens.vanished;
+    // N tokens, of one sequence (W 1) or each of its own; those that are not `inside` count nowhere.  Whose sigmoids have vanished are left out, and come back,
+    // unless their logits have been `moved`.
+    const auto gradients = [&](uint32_t t0, const auto& x, const auto& up, bool moved, const auto& in, const auto& inside, const auto& often) MINT_INLINE_LAMBDA {
+        constexpr int N = sizeof(in) / sizeof(in[0]), W = sizeof(often) / sizeof(often[0]);
+        float mean[N];
+        const Tokens<V, N> tokens(x, up, inside, first, f.experts, f.sigmoid, f.z != 0.0f);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < N; ++u) {
             mean[u] = 0.0f;
 #pragma unroll
             for (int i = 0; i < V; ++i) mean[u] = fmaf(tokens.p[u][i], often[u % W][i], mean[u]);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) mean[u] = wave_sum(mean[u]);
+        for (int u = 0; u < N; ++u) mean[u] = wave_sum(mean[u]);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
+        for (int u = 0; u < N; ++u) {
             const uint32_t t = t0 + u * kWaves;
-            if (!in[u] || left <= 0) continue;
+            if (!in[u] || left <= 0 || (!moved && tokens.vanished >> u & 1u)) continue;
             float more[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) more[i] = 0.0f;
@@ -498,18 +497,21 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
             }
             store_elements<DT, V>(static_cast<T*>(a.d_logits) + (int64_t)t * a.d_stride + first, left, more);
         }
-        return 0u;
+        return tokens.vanished;
     };
-    uint32_t next;
+    uint32_t next, vanished = 0;
     const uint32_t v = sequence_of(begin, next);
     if (next < end) {
-        // Tokens of several sequences: each has its own load, all of them on their way with the logits.
-        for (uint32_t t0 = begin + wave_in_block(), again = 0; t0 < end;) {
-            float x[U][V], often[U][V], n[U];
-            bool in[U], inside[U];
+        // Tokens of several sequences: each has its own load, all of them on their way with the logits.  (Two at a time: four take registers that
+        // the tokens below then have not either, 2^20 of 128 experts 283 us for 261.)
+        constexpr int N = U < 2 ? U : 2;
+        for (uint32_t t0 = begin + wave_in_block(); t0 < end; t0 += kWaves * N) {
+            float x[N][V], often[N][V], n[N];
+            const float up[N] = {};
+            bool in[N], inside[N];
             load_logits(t0, x, in);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < N; ++u) {
                 const uint32_t of = sequence_of(in[u] ? t0 + u * kWaves : t0, next);
                 const uint64_t at = min(max(of, 1u), f.sequences) - 1;
                 inside[u] = in[u] && of != 0 && of <= f.sequences;
@@ -518,11 +520,10 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
                 for (int i = 0; i < V; ++i) often[u][i] = count_of(at, i);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < N; ++u)
 #pragma unroll
                 for (int i = 0; i < V; ++i) often[u][i] = load_of(often[u][i], n[u]);
-            again = gradients(t0, x, again, in, inside, often);
-            if (!again) t0 += kWaves * U;
+            vanished |= gradients(t0, x, up, false, in, inside, often);
         }
     } else if (v == 0 || v > f.sequences) {                   // tokens of no sequence
         for (uint32_t t = begin + wave_in_block(); t < end; t += kWaves) {
@@ -535,13 +536,26 @@ __global__ void __launch_bounds__(64 * kWaves) balance_grad_kernel(BalanceGradAr
         float often[1][V];
 #pragma unroll
         for (int i = 0; i < V; ++i) often[0][i] = load_of(count_of(v - 1, i), n);
-        for (uint32_t t0 = begin + wave_in_block(), again = 0; t0 < end;) {
+        const float up[U] = {};
+        for (uint32_t t0 = begin + wave_in_block(); t0 < end; t0 += kWaves * U) {
             float x[U][V];
             bool in[U];
             load_logits(t0, x, in);
-            again = gradients(t0, x, again, in, in, often);
-            if (!again) t0 += kWaves * U;
+            vanished |= gradients(t0, x, up, false, in, in, often);
         }
+    }
+    for (uint32_t t = vanished ? begin + wave_in_block() : end; t < end; t += kWaves) {
+        float x[1][V], often[1][V], up[1] = {};
+        bool in[1];
+        const uint32_t of = sequence_of(t, next);
+        if (of == 0 || of > f.sequences) continue;
+        load_logits(t, x, in);
+        if (!Tokens<V, 1>(x, up, in, first, f.experts, true, false).vanished) continue;
+        const float n = (float)max(a.there[of - 1], 1);
+#pragma unroll
+        for (int i = 0; i < V; ++i) often[0][i] = load_of(count_of(of - 1, i), n);
+        up[0] = move_up(x[0], first, f.experts);
+        gradients(t, x, up, true, in, in, often);
     }
 }
 
