@@ -324,8 +324,8 @@ constexpr int kSums = (BLOCK ? 2 : 1) * (BIAS ? 2 : 1);
 
 // LANES lanes have every groups-th row; the weights stay in registers, and up to 4096 numbers so do the sums over their rows, while the next row is on its
 // way (AHEAD); a thread block of 1024 has the sums in LDS.
-// Bound by memory, and by three meetings for a row: 16384 x 4096 bf16 with a gate by channel 181 us, 4.5 TB/s
-// (twice eight numbers to a lane, half as many wavefronts, nothing held or ahead: 397), 8192 x 8192 with the stream in 32 bits and a gate by row 299, 4.1.
+// Bound by memory, and by three meetings for a row: 16384 x 4096 bf16 with a gate by channel 177 us, 4.6 TB/s
+// (twice eight numbers to a lane, half as many wavefronts, nothing held or ahead: 397), 8192 x 8192 with the stream in 32 bits and a gate by row 295, 4.2.
 template <int S, int T, int LANES, bool WHOLE, bool BLOCK, bool BIAS, int GATE>      // GATE: 0 (none, or by channel), MINT_GATE_ROW, MINT_GATE_ALL
 __global__ void __launch_bounds__(threads_of(LANES)) join_grad_kernel(JoinGradArgs a) {
     using TS = typename Elem<S>::type;
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kLongThreads) join_long_kernel(JoinArgs a) {
 
 // A thread block's sums over its rows are kept in its part of the workspace.  Each of the steps (two statistics, their sums, the results) reads x, d, y and the gate
 // again: 8192 x 9000 bf16, both norms, 725 us (1.2 TB/s of what has to pass), 4096 x 16384 514 (1.6), 8192 x 5001, whose ends are inside a lane's numbers, 564 (0.9; 8192 x 5000 in
-// registers 165), 8192 x 8192 with the stream in 32 bits, biases and a gate by row 775 (1.6; without biases 299).
+// registers 165), 8192 x 8192 with the stream in 32 bits, biases and a gate by row 775 (1.6; without biases 295).
 template <int S, int T, bool BLOCK, bool BIAS>
 __global__ void __launch_bounds__(kLongThreads) join_grad_long_kernel(JoinGradArgs a) {
     using TS = typename Elem<S>::type;
