@@ -757,7 +757,7 @@ constexpr int kBiasWaves = 16;
 template <int DT>
 __global__ void __launch_bounds__(64 * kBiasWaves) bias_grad_kernel(const float* sums, void* d_bias, uint32_t cols, uint32_t groups) {
     __shared__ float part[kBiasWaves][64];
-    const uint32_t col = blockIdx.x * 64 + lane_id(), from = min(col, cols - 1), wave = wave_in_block();
+    const uint32_t col = block_in_grid() * 64 + lane_id(), from = min(col, cols - 1), wave = wave_in_block();
     float sum = 0.0f;
     for (uint32_t g0 = wave; g0 < groups; g0 += kBiasWaves * 8) {
         float v[8];
@@ -1042,7 +1042,8 @@ extern "C" int mint_activation_grad(const mint_activation_grad_op* op, void* str
     // (of no rows the sums are zeros)
     const float* const sums = a.sums;
     void* const d_bias = reinterpret_cast<void*>(op->d_bias);
-    const uint32_t n = op->rows ? groups : 0u, grid = (uint32_t)ceil_div(op->cols, 64);
+    const uint32_t n = op->rows ? groups : 0u;
+    const dim3 grid = wide_grid(ceil_div(op->cols, 64));
     switch (op->dtype) {
         case MINT_F16: return Launch<&bias_grad_kernel<DT_F16>>::go(grid, 64 * kBiasWaves, 0, s, sums, d_bias, a.cols, n);
         case MINT_BF16: return Launch<&bias_grad_kernel<DT_BF16>>::go(grid, 64 * kBiasWaves, 0, s, sums, d_bias, a.cols, n);

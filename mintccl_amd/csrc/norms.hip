@@ -18,7 +18,7 @@ struct ColumnSumsArgs {
 constexpr int kColumnWaves = 16;
 __global__ void __launch_bounds__(64 * kColumnWaves) column_sums_kernel(ColumnSumsArgs a) {
     __shared__ float part[4][kColumnWaves * 4][16];
-    const uint32_t lane = threadIdx.x & 15u, slot = threadIdx.x >> 4, col = blockIdx.x * 16 + lane, from = min(col, a.width - 1);
+    const uint32_t lane = threadIdx.x & 15u, slot = threadIdx.x >> 4, col = block_in_grid() * 16 + lane, from = min(col, a.width - 1);
     constexpr uint32_t SLOTS = kColumnWaves * 4;
     for (uint32_t k = 0; k < a.n; ++k) {
         float sum = 0.0f;
@@ -173,5 +173,5 @@ extern "C" int mint_join_grad(const mint_join_grad_op* op_grad, void* stream) {
                               reinterpret_cast<void*>(op_grad->to_after_weight), reinterpret_cast<void*>(op_grad->to_after_bias),
                               by_channel ? a.to_gate : nullptr, by_channel ? a.f.gate : nullptr, a.f.before, a.f.after, a.f.rows ? a.groups : 0u, a.f.width,
                               a.f.rows ? (a.f.y ? 2u : 1u) * (bias ? 2u : 1u) : 0u, a.f.gate_dtype, a.f.gate_by, a.f.y != nullptr || !a.f.rows, bias};
-    return Launch<&column_sums_kernel>::go((uint32_t)ceil_div(a.f.width, 16), 64 * kColumnWaves, 0, s, c);
+    return Launch<&column_sums_kernel>::go(wide_grid(ceil_div(a.f.width, 16)), 64 * kColumnWaves, 0, s, c);
 }

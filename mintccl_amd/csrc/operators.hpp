@@ -110,4 +110,11 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
 inline bool aligned_to(const void* p, uint64_t bytes) { return reinterpret_cast<uint64_t>(p) % bytes == 0; }
 inline uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
+// Thread blocks of up to 1024 threads, more of them than a grid's first dimension takes (fewer than 2^32 threads): those beyond `blocks` have nothing to do.
+inline dim3 wide_grid(uint64_t blocks) {
+    const uint64_t x = blocks < (1u << 20) ? blocks : 1u << 20;
+    return dim3((uint32_t)x, (uint32_t)ceil_div(blocks, x));
+}
+__device__ __forceinline__ uint32_t block_in_grid() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 }  // namespace mint

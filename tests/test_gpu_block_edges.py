@@ -290,3 +290,24 @@ def test_slopes_of_gates_by_a_hyperbolic_tangent_far_out(dev, width, shape):
     want = (width if shape == "row" else rows if shape == "channel" else 1) / torch.cosh(g.cpu().double()) ** 2
     # (the sums are of whole numbers; one product and its rounding beside the slope's own 16)
     close(got, want, want, torch.float32, 18 * UNIT)
+
+
+def test_sums_over_rows_of_very_many_columns(dev):
+    """More columns than a grid's first dimension has threads for: 2^28 of a bias, 2^26 of a norm's weight."""
+    cols = (1 << 28) + 77
+    d = torch.empty(2, cols, dtype=torch.float16, device=dev).normal_(generator=torch.Generator(dev).manual_seed(1))
+    d_bias = activation_grad(d, None)[1]
+    # (two numbers, added in 32 bits and rounded once)
+    assert torch.equal(d_bias, (d[0].float() + d[1].float()).half())
+    del d, d_bias
+    width = (1 << 26) + 24
+    x = torch.ones(2, width, dtype=torch.bfloat16, device=dev)
+    x[1] = -1
+    d = (torch.arange(width, device=dev) % 64).bfloat16().expand(2, width).clone()
+    d[1] *= 3
+    n = Norm(torch.ones(width, dtype=torch.bfloat16, device=dev), torch.zeros(width, dtype=torch.bfloat16, device=dev), "rms", 0.0)
+    got = norm_grad(d, x, n)
+    # (the rows' mean squares are 1: the weight's gradient is d0 - 3 d0, the bias's d0 + 3 d0, whole numbers)
+    assert torch.equal(got.weight, -2 * d[0]) and torch.equal(got.bias, 4 * d[0])
+    del d, x, n, got
+    torch.cuda.empty_cache()
